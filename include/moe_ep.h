@@ -27,6 +27,9 @@
  *                               expert is one GEMM, baseline.py:50)
  *   moe_router                  utils.py:17-25 (router logits einsum, softmax,
  *                               top-k: the step before the reference's path)
+ *   moe_decode_layer            the whole gated layer for a few tokens, its
+ *                               router included (utils.py:17-25, 28-75,
+ *                               baseline.py:18-50 in one kernel)
  *   moe_pack_compact,           the general (unbalanced) all-to-all that
  *   moe_ep_run_compact          alltoall_persistent_gemm.py:221-222 and
  *                               baseline.py:15-16 leave as stubs: unpadded
@@ -363,6 +366,53 @@ int moe_swiglu(const void* a, int64_t rows, int32_t F, void* h, void* stream);
  * 2F % 256 == 0; out is [out_rows, F], same row order as moe_ep_run_compact.
  * Each value equals moe_swiglu applied to moe_ep_run_compact's output. */
 int moe_ep_run_compact_swiglu(const moe_ep_run_params* params, int64_t send_rows, int64_t out_rows, void* stream);
+
+/* ---------------------------------------------------------------- decode
+ * The whole gated layer of one rank's experts for a few tokens, one kernel:
+ *   y[t, :] = sum over k of v[t, k] * (silu(x_t Wg_e) * (x_t Wu_e)) Wd_e,
+ * e = top_idxs[t, k] - first_expert.  Ids outside [first_expert,
+ * first_expert + experts) are skipped and an id repeated within a row counts
+ * once, like the routing's rule; a token with no expert here gets a zero
+ * row, so that ranks holding parts of the experts add their y's.
+ *   w13 [experts, hidden, 2*ffn] bf16: gate columns [0, ffn), up after them
+ *   w2  [experts, ffn, hidden] bf16
+ * Sums are fp32; silu(gate) * up is rounded once to bf16 and y once.
+ * With router_w ([hidden, router_experts] bf16; NULL: none) the call also
+ * chooses the experts: logits = x @ router_w kept in fp32, softmax over
+ * router_experts, the K largest (equal logits: lowest id first), written to
+ * top_idxs and top_vals (fp32), divided by their sum with `renormalize`.
+ * Requires T <= MOE_DECODE_MAX_TOKENS, T * K <= 1024, K <= 32, hidden and ffn
+ * multiples of 8, hidden <= 32768, experts and router_experts <= 1024,
+ * router_experts even; x, w13, w2 and scratch 16-byte aligned.
+ * scratch: moe_decode_scratch_bytes of device memory, not initialised, for
+ * this call alone until it has finished.  Launched cooperatively (one CTA per
+ * SM), so calls on several streams run one after another. */
+#define MOE_DECODE_MAX_TOKENS 64
+typedef struct moe_decode_params {
+  int64_t T;
+  int32_t hidden, ffn;
+  int32_t experts;         /* experts held here (w13, w2)                     */
+  int32_t K;
+  int32_t first_expert;    /* id of the first of them                         */
+  int32_t router_experts;  /* columns of router_w                             */
+  int32_t renormalize;
+  int32_t ids_are_int64, vals_are_bf16;
+  int32_t reserved;
+  const void* x;           /* [T, hidden] bf16                                */
+  const void* w13;
+  const void* w2;
+  const void* router_w;
+  void* top_idxs;          /* [T, K] read, or written with router_w           */
+  void* top_vals;          /* [T, K] read, or written (fp32) with router_w    */
+  void* y;                 /* [T, hidden] bf16                                */
+  void* scratch;
+  size_t scratch_bytes;
+  int32_t* status_host;    /* optional mapped pinned word for device errors   */
+} moe_decode_params;
+
+int moe_decode_scratch_bytes(int64_t T, int32_t hidden, int32_t ffn, int32_t experts, int32_t K,
+                             int32_t router_experts, int32_t device, size_t* out);
+int moe_decode_layer(const moe_decode_params* params, void* stream);
 
 /* Copy the workspace status word to the host (synchronous). */
 int moe_ep_read_status(uint64_t local_base, const moe_ep_layout* layout, uint32_t* out);

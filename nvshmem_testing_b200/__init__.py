@@ -11,6 +11,8 @@ CPU fallback):
   ``pack_compact``), the router (``router``), ``gen_tensor``;
 * ``combine`` — the layer with its return path and top-k combine;
 * ``mlp`` — the full gated expert MLP behind the exchange;
+* ``decode`` — the whole gated layer for a few tokens in one kernel, the
+  router included;
 * ``symm`` — the cuMem symmetric workspaces; ``workloads`` — seeded inputs;
 * ``build`` — compiles the library in-tree.
 """

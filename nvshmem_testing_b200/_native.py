@@ -26,7 +26,7 @@ EXPORTED = ["moe_ep_abi_version", "moe_ep_status_string", "moe_ep_num_sms", "moe
             "moe_symm_alloc", "moe_symm_import", "moe_symm_free", "moe_ep_workspace_layout", "moe_ep_workspace_reset", "moe_ep_run",
             "moe_ep_read_status", "moe_ep_run_noalloc", "moe_route_slots", "moe_ep_workspace_layout_ret",
             "moe_ep_run_combine", "moe_pack_compact", "moe_ep_run_compact", "moe_router", "moe_swiglu",
-            "moe_ep_run_compact_swiglu", "moe_publish_i32"]
+            "moe_ep_run_compact_swiglu", "moe_publish_i32", "moe_decode_scratch_bytes", "moe_decode_layer"]
 
 
 class MoeEpError(RuntimeError):
@@ -64,6 +64,19 @@ class CombineParams(ctypes.Structure):
                 ("ids_are_int64", ctypes.c_int32), ("vals_are_bf16", ctypes.c_int32), ("reserved", ctypes.c_int32)]
 
 
+class DecodeParams(ctypes.Structure):
+    _fields_ = [("T", ctypes.c_int64), ("hidden", ctypes.c_int32), ("ffn", ctypes.c_int32),
+                ("experts", ctypes.c_int32), ("K", ctypes.c_int32), ("first_expert", ctypes.c_int32),
+                ("router_experts", ctypes.c_int32), ("renormalize", ctypes.c_int32),
+                ("ids_are_int64", ctypes.c_int32), ("vals_are_bf16", ctypes.c_int32), ("reserved", ctypes.c_int32),
+                ("x", ctypes.c_void_p), ("w13", ctypes.c_void_p), ("w2", ctypes.c_void_p),
+                ("router_w", ctypes.c_void_p), ("top_idxs", ctypes.c_void_p), ("top_vals", ctypes.c_void_p),
+                ("y", ctypes.c_void_p), ("scratch", ctypes.c_void_p), ("scratch_bytes", ctypes.c_size_t),
+                ("status_host", ctypes.c_void_p)]
+
+
+DECODE_MAX_TOKENS = 64
+DECODE_MAX_ROWS = 1024  # tokens times ids per token
 TRACE_WORDS = 24
 TRACE_FIELDS = ["start", "counts", "sched", "producer_end", "mma_end", "epi_end", "push_end", "zero_end", "end",
                 "tiles", "flag_wait_ns", "full_wait_ns", "push_items", "push_bytes", "empty_wait_ns",
@@ -111,6 +124,8 @@ def lib() -> ctypes.CDLL:
                              ctypes.c_int32, c_vp, c_vp, c_vp]
     L.moe_ep_read_status.argtypes = [c_u64, P(Layout), P(ctypes.c_uint32)]
     L.moe_publish_i32.argtypes = [c_vp, c_i64, c_vp, c_vp]
+    L.moe_decode_scratch_bytes.argtypes = [c_i64] + [ctypes.c_int32] * 6 + [P(c_sz)]
+    L.moe_decode_layer.argtypes = [P(DecodeParams), c_vp]
     for name in EXPORTED:
         if name not in ("moe_ep_status_string",):
             getattr(L, name).restype = c_int

@@ -1,0 +1,150 @@
+"""The gated MoE layer for a few tokens, in one kernel.
+
+``combine.moe_layer`` and ``mlp.moe_mlp`` route, pack, exchange and multiply
+in separate launches and read the largest bucket on the host; with a handful
+of tokens (a decode step) their fixed costs and padded tiles outweigh the
+work, which is one pass over the weights of the experts that were chosen.
+``moe_layer`` is that pass for tokens whose routing is known, and
+``routed_layer`` includes the router (reference: utils.py:17-25 for the
+router, utils.py:28-75 and baseline.py:18-50 for routing and products).
+
+    y[t] = sum_k v[t, k] * (silu(x_t W_gate,e) * (x_t W_up,e)) W_down,e
+
+with e = ids[t, k] - first_expert.  Ids outside the experts held here are
+skipped and a token without any gets a zero row: a rank that holds experts
+[first_expert, first_expert + El) of a replicated batch computes its part of
+the sum, and the ranks' parts add up.  Nothing is read on the host, and a
+call may be captured into a CUDA graph.
+"""
+from __future__ import annotations
+
+import ctypes
+
+import torch
+
+from . import _native as N
+
+
+def _check(x, w13, w2, out, status):
+    if x.dim() != 2 or w13.dim() != 3 or w2.dim() != 3:
+        raise ValueError("x [T, H], w13 [El, H, 2F] and w2 [El, F, H] are required")
+    T, H = x.shape
+    El, _, F2 = w13.shape
+    F = F2 // 2
+    if w13.shape[1] != H or F2 % 2 or tuple(w2.shape) != (El, F, H):
+        raise ValueError(f"x {tuple(x.shape)}, w13 {tuple(w13.shape)} and w2 {tuple(w2.shape)} do not form an MLP")
+    if H % 8 or F % 8 or H == 0 or F == 0:
+        raise ValueError(f"H = {H} and F = {F} must be positive multiples of 8")
+    for name, t in (("x", x), ("w13", w13), ("w2", w2)):
+        if t.dtype != torch.bfloat16:
+            raise TypeError(f"{name} must be bfloat16")
+        if not t.is_cuda or t.device != x.device:
+            raise ValueError(f"{name} must be a CUDA tensor on the tokens' device")
+    for name, t in (("w13", w13), ("w2", w2)):
+        if not t.is_contiguous():
+            raise ValueError(f"{name} must be contiguous")
+    if T > N.DECODE_MAX_TOKENS:
+        raise ValueError(f"{T} tokens: this form takes {N.DECODE_MAX_TOKENS} at most (mlp.moe_mlp has no limit)")
+    if out is not None and (tuple(out.shape) != (T, H) or out.dtype != torch.bfloat16 or out.device != x.device
+                            or not out.is_contiguous()):
+        raise ValueError(f"out must be a contiguous bfloat16 tensor of shape {(T, H)} on the tokens' device")
+    if status is not None and (status.dtype != torch.int32 or status.numel() != 1 or not status.is_pinned()):
+        raise ValueError("status must be one pinned int32")
+    return T, H, F, El
+
+
+def _launch(x, ids, vals, w13, w2, router_w, K, first_expert, renormalize, out, status, dims):
+    T, H, F, El = dims
+    if out is None:
+        out = torch.empty((T, H), dtype=torch.bfloat16, device=x.device)
+    if T == 0:
+        return out
+    dev = x.device.index
+    p = N.DecodeParams()
+    p.T, p.hidden, p.ffn, p.experts, p.K, p.first_expert = T, H, F, El, K, first_expert
+    p.router_experts = 0 if router_w is None else router_w.shape[1]
+    p.renormalize = int(renormalize)
+    p.ids_are_int64 = int(ids.dtype == torch.int64)
+    p.vals_are_bf16 = int(vals.dtype == torch.bfloat16)
+    need = ctypes.c_size_t()
+    lib = N.lib()
+    N.check(lib.moe_decode_scratch_bytes(T, H, F, El, K, p.router_experts, dev, ctypes.byref(need)),
+            "moe_decode_scratch_bytes")
+    scratch = torch.empty(need.value, dtype=torch.uint8, device=x.device)
+    p.x, p.w13, p.w2, p.y = x.data_ptr(), w13.data_ptr(), w2.data_ptr(), out.data_ptr()
+    p.router_w = None if router_w is None else router_w.data_ptr()
+    p.top_idxs, p.top_vals = ids.data_ptr(), vals.data_ptr()
+    p.scratch, p.scratch_bytes = scratch.data_ptr(), need.value
+    p.status_host = None if status is None else status.data_ptr()
+    stream = torch.cuda.current_stream(x.device)
+    with torch.cuda.device(x.device):
+        N.check(lib.moe_decode_layer(ctypes.byref(p), ctypes.c_void_p(stream.cuda_stream)), "moe_decode_layer")
+    return out
+
+
+def moe_layer(x: torch.Tensor, top_idxs: torch.Tensor, top_vals: torch.Tensor, w13: torch.Tensor, w2: torch.Tensor,
+              *, first_expert: int = 0, out: torch.Tensor | None = None,
+              status: torch.Tensor | None = None) -> torch.Tensor:
+    """``y [T, H]`` bf16 for tokens whose routing is known.
+
+    x         [T, H] bf16, T <= 64
+    top_idxs  [T, K] int32/int64 expert ids, T * K <= 1024, K <= 32
+    top_vals  [T, K] float32 or bfloat16 routing weights
+    w13       [El, H, 2F] bf16: gate columns [0, F), up columns [F, 2F)
+    w2        [El, F, H] bf16
+    first_expert: id of the first expert held here.  ``out`` optionally
+    supplies y; ``status`` (one pinned int32) receives a device-side error
+    word, if any."""
+    dims = _check(x, w13, w2, out, status)
+    if top_idxs.dim() == 1:
+        top_idxs = top_idxs[:, None]
+    if top_vals.dim() == 1:
+        top_vals = top_vals[:, None]
+    if top_idxs.dim() != 2 or top_idxs.shape[0] != dims[0] or top_vals.shape != top_idxs.shape:
+        raise ValueError(f"top_idxs {tuple(top_idxs.shape)} and top_vals {tuple(top_vals.shape)} must be [T, K]")
+    if top_idxs.dtype not in (torch.int32, torch.int64):
+        raise TypeError("top_idxs must be int32 or int64")
+    if top_vals.dtype not in (torch.float32, torch.bfloat16):
+        raise TypeError("top_vals must be float32 or bfloat16")
+    if top_idxs.device != x.device or top_vals.device != x.device:
+        raise ValueError("top_idxs and top_vals must be on the tokens' device")
+    K = top_idxs.shape[1]
+    if not 1 <= K <= 32 or dims[0] * K > N.DECODE_MAX_ROWS:
+        raise ValueError(f"{dims[0]} tokens with {K} ids each: 1 to 32 ids, {N.DECODE_MAX_ROWS} in all at most")
+    return _launch(x.contiguous(), top_idxs.contiguous(), top_vals.contiguous(), w13, w2, None, K, int(first_expert),
+                   False, out, status, dims)
+
+
+def routed_layer(x: torch.Tensor, router_w: torch.Tensor, topk: int, w13: torch.Tensor, w2: torch.Tensor, *,
+                 renormalize: bool = False, first_expert: int = 0, ids_dtype=torch.int64,
+                 out: torch.Tensor | None = None,
+                 status: torch.Tensor | None = None) -> tuple[torch.Tensor, torch.Tensor, torch.Tensor]:
+    """The whole layer from activations: ``(y [T, H], top_vals [T, K] float32,
+    top_idxs [T, K])``.
+
+    router_w [H, E] bf16.  The logits ``x @ router_w`` stay in fp32 (unlike
+    ``utils.router``, which rounds logits and probabilities to bf16 as the
+    reference does), top_vals are the K largest of their softmax in
+    descending order, equal ones by ascending id, divided by their sum with
+    ``renormalize``.  The other arguments are those of ``moe_layer``; w13 and
+    w2 may hold a part of the E experts."""
+    dims = _check(x, w13, w2, out, status)
+    T, H = dims[0], dims[1]
+    if router_w.dim() != 2 or router_w.shape[0] != H:
+        raise ValueError(f"router_w {tuple(router_w.shape)} does not match x {tuple(x.shape)}")
+    if router_w.dtype != torch.bfloat16:
+        raise TypeError("router_w must be bfloat16")
+    if router_w.device != x.device:
+        raise ValueError("router_w must be on the tokens' device")
+    if ids_dtype not in (torch.int32, torch.int64):
+        raise TypeError("ids_dtype must be int32 or int64")
+    E = router_w.shape[1]
+    if E % 2 or not 2 <= E <= 1024:
+        raise ValueError(f"{E} experts: an even number of 1024 at most")
+    if not 1 <= topk <= min(32, E) or T * topk > N.DECODE_MAX_ROWS:
+        raise ValueError(f"{T} tokens with {topk} of {E} experts each: 1 to 32, {N.DECODE_MAX_ROWS} in all at most")
+    vals = torch.empty((T, topk), dtype=torch.float32, device=x.device)
+    ids = torch.empty((T, topk), dtype=ids_dtype, device=x.device)
+    y = _launch(x.contiguous(), ids, vals, w13, w2, router_w.contiguous(), topk, int(first_expert), renormalize, out,
+                status, dims)
+    return y, vals, ids

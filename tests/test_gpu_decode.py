@@ -1,0 +1,282 @@
+"""The one-kernel layer for a few tokens (decode.moe_layer, routed_layer)
+against its formula in 64 bits.
+
+Tolerance, elementwise and derived from the arithmetic: the products are
+exact in fp32, a sum of n of them is off by at most n * 2^-23 of the sum of
+their magnitudes; silu has a slope of at most 1.1; h = silu(gate) * up is
+rounded once to bf16 (half a step, 2^-8 of the value) after fp32 arithmetic
+(2^-20 covers expf and the divisions); y is rounded once to bf16.  Over all
+elements two independent roundings of at most 2^-8, uniform within the step,
+leave a relative error of at most sqrt(2/3) * 2^-8 < 2^-8 in the 2-norm."""
+import pytest
+import torch
+
+from nvshmem_testing_b200 import decode
+
+pytestmark = pytest.mark.gpu
+
+HALF = 2.0 ** -8
+
+
+def reference(x, ids, vals, w13, w2, first=0):
+    """(y, bound) in 64 bits; an id counts once per row."""
+    T, H = x.shape
+    El, F, _ = w2.shape
+    y = torch.zeros(T, H, dtype=torch.float64, device=x.device)
+    tol = torch.zeros_like(y)
+    xd = x.double()
+    for t in range(T):
+        seen = set()
+        for k, i in enumerate(ids[t].tolist()):
+            e = i - first
+            if not 0 <= e < El or i in seen:
+                continue
+            seen.add(i)
+            w, d = w13[e].double(), w2[e].double()
+            a, mag = xd[t] @ w, xd[t].abs() @ w.abs()
+            da = mag * H * 2.0 ** -23
+            g, u, dg, du = a[:F], a[F:], da[:F], da[F:]
+            s = g * torch.sigmoid(g)
+            h = s * u
+            dh = 1.1 * dg * u.abs() + (s.abs() + 1.1 * dg) * du + h.abs() * (HALF + 2.0 ** -20)
+            v = float(vals[t, k])
+            y[t] += v * (h @ d)
+            tol[t] += abs(v) * ((dh + (h.abs() + dh) * (F + 4) * 2.0 ** -23) @ d.abs())
+    return y, tol + y.abs() * HALF + 1e-30
+
+
+def check(y, x, ids, vals, w13, w2, first=0):
+    ref, tol = reference(x, ids, vals, w13, w2, first)
+    assert y.shape == x.shape and y.dtype == torch.bfloat16
+    err = (y.double() - ref).abs()
+    assert bool((err <= tol).all()), f"{int((err > tol).sum())} of {err.numel()} beyond the bound, worst {float((err / tol).max()):.2f}x"
+    if ref.numel() >= 1024 and float(ref.norm()) > 0:
+        assert float(err.norm() / ref.norm()) <= HALF
+    return ref
+
+
+def make(T, H, El, K, F, seed, E=None, scale=0.05):
+    g = torch.Generator(device="cuda").manual_seed(seed)
+    E = E or El
+    x = torch.randn(T, H, generator=g, device="cuda").to(torch.bfloat16)
+    w13 = (scale * torch.randn(El, H, 2 * F, generator=g, device="cuda")).to(torch.bfloat16)
+    w2 = (scale * torch.randn(El, F, H, generator=g, device="cuda")).to(torch.bfloat16)
+    ids = torch.rand(T, E, generator=g, device="cuda").topk(K, dim=-1).indices
+    vals = torch.randn(T, K, generator=g, device="cuda").softmax(-1)
+    return x, ids, vals, w13, w2
+
+
+SIZES = [
+    # T, H, E, K, F
+    (1, 8, 1, 1, 8),
+    (1, 64, 4, 1, 64),
+    (1, 2048, 6, 6, 1408),
+    (2, 72, 3, 3, 136),
+    (3, 136, 5, 2, 72),
+    (15, 520, 9, 4, 328),
+    (16, 256, 8, 4, 128),
+    (17, 264, 7, 3, 200),
+    (31, 4096, 2, 2, 64),
+    (33, 512, 16, 8, 384),
+    (48, 64, 200, 5, 2048),
+    (64, 1024, 32, 8, 256),
+    (64, 256, 64, 16, 128),
+    (64, 320, 1, 1, 1000),
+]
+
+
+@pytest.mark.parametrize("T,H,E,K,F", SIZES)
+def test_known_routing(T, H, E, K, F):
+    x, ids, vals, w13, w2 = make(T, H, E, K, F, T * 7 + H + F)
+    y = decode.moe_layer(x, ids, vals, w13, w2)
+    torch.cuda.synchronize()
+    check(y, x, ids, vals, w13, w2)
+    assert torch.equal(y, decode.moe_layer(x, ids, vals, w13, w2))  # sums in a fixed order
+
+
+@pytest.mark.parametrize("ids_dtype", [torch.int32, torch.int64])
+@pytest.mark.parametrize("vals_dtype", [torch.float32, torch.bfloat16])
+def test_types(ids_dtype, vals_dtype):
+    x, ids, vals, w13, w2 = make(9, 256, 8, 3, 192, 5)
+    ids, vals = ids.to(ids_dtype), vals.to(vals_dtype)
+    check(decode.moe_layer(x, ids, vals, w13, w2), x, ids, vals, w13, w2)
+
+
+def test_ids_elsewhere_repeated_and_negative():
+    """A rank that holds experts [4, 9): other ids are skipped, a repeated id
+    counts once with its first weight, a row without any id here is zero."""
+    x, _, _, w13, w2 = make(6, 200, 5, 4, 104, 11)
+    ids = torch.tensor([[4, 4, 5, 4], [0, 3, 9, 100], [8, 7, 6, 5], [-1, -5, 4, 12], [2 ** 31 - 1, 8, 8, 0],
+                        [9, 9, 9, 9]], device="cuda")
+    vals = torch.rand(6, 4, device="cuda") + 0.1
+    for dt in (torch.int64, torch.int32):
+        y = decode.moe_layer(x, ids.to(dt), vals, w13, w2, first_expert=4)
+        check(y, x, ids, vals, w13, w2, first=4)
+        assert not y[1].any() and not y[5].any()
+    big = ids + (1 << 40)  # beyond 32 bits: matches nothing
+    assert not decode.moe_layer(x, big, vals, w13, w2, first_expert=4).any()
+
+
+def test_parts_of_the_experts_add_up():
+    x, ids, vals, w13, w2 = make(12, 256, 8, 4, 128, 3)
+    parts = sum(decode.moe_layer(x, ids, vals, w13[a:a + 2].contiguous(), w2[a:a + 2].contiguous(),
+                                 first_expert=a).double() for a in range(0, 8, 2))
+    ref, tol = reference(x, ids, vals, w13, w2)
+    # four roundings of parts no larger than their magnitudes: the bound's own terms, once per part
+    assert bool(((parts - ref).abs() <= 4 * tol + 4 * HALF * ref.abs() + 0.02 * tol.max()).all())
+
+
+def test_no_expert_here_and_no_token():
+    x, ids, vals, w13, w2 = make(5, 128, 4, 2, 64, 1)
+    out = torch.full_like(x, 3.0)
+    assert decode.moe_layer(x, ids + 4, vals, w13, w2, out=out) is out and not out.any()
+    assert decode.moe_layer(x[:0], ids[:0], vals[:0], w13, w2).shape == (0, 128)
+
+
+def test_a_token_is_touched_by_its_own_experts_only():
+    """Non-finite tokens and experts stay with the rows that use them."""
+    x, ids, vals, w13, w2 = make(8, 192, 4, 1, 96, 21)
+    ids = torch.tensor([[0], [1], [2], [0], [1], [2], [0], [1]], device="cuda")
+    clean = decode.moe_layer(x, ids, vals, w13, w2)
+    x2, w13b, w2b = x.clone(), w13.clone(), w2.clone()
+    x2[3] = float("nan")
+    w13b[3] = float("nan")  # an expert that no token chose
+    w2b[2, 5, 7] = float("inf")
+    y = decode.moe_layer(x2, ids, vals, w13b, w2b)
+    keep = [0, 1, 4, 6, 7]
+    assert torch.equal(y[keep], clean[keep])
+    assert bool(y[3].isnan().all())
+    assert not bool(y[[2, 5]][:, 7].isfinite().any())
+    assert bool(y[[2, 5]][:, :7].isfinite().all())
+
+
+def test_strides_and_given_output():
+    x, ids, vals, w13, w2 = make(7, 256, 6, 2, 128, 4)
+    ref = decode.moe_layer(x, ids, vals, w13, w2)
+    wide = torch.zeros(7, 512, dtype=torch.bfloat16, device="cuda")
+    wide[:, ::2] = x
+    idt = torch.zeros(2, 7, dtype=torch.int64, device="cuda")
+    idt.copy_(ids.t())
+    rows = torch.full((9, 256), 5.0, dtype=torch.bfloat16, device="cuda")
+    y = decode.moe_layer(wide[:, ::2], idt.t(), vals.t().contiguous().t(), w13, w2, out=rows[1:8])
+    assert torch.equal(y, ref)
+    assert bool((rows[0] == 5).all()) and bool((rows[8] == 5).all())
+
+
+def test_captured_and_replayed_beside_eager_calls():
+    x, ids, vals, w13, w2 = make(4, 256, 8, 2, 128, 8)
+    static, sids = x.clone(), ids.clone()
+    decode.moe_layer(static, sids, vals, w13, w2)
+    torch.cuda.synchronize()
+    graphs, outs = [], []
+    for _ in range(2):
+        g = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(g):
+            outs.append(decode.moe_layer(static, sids, vals, w13, w2))
+        graphs.append(g)
+    streams = [torch.cuda.Stream() for _ in range(2)]
+    for i in range(6):
+        x2, ids2, _, _, _ = make(4, 256, 8, 2, 128, 100 + i)
+        static.copy_(x2)
+        sids.copy_(ids2)
+        torch.cuda.synchronize()
+        for g, s in zip(graphs, streams):
+            with torch.cuda.stream(s):
+                g.replay()
+        eager = decode.moe_layer(x2, ids2, vals, w13, w2)
+        torch.cuda.synchronize()
+        assert torch.equal(outs[0], eager) and torch.equal(outs[1], eager)
+
+
+def test_several_streams_at_once():
+    data = [make(3 + 5 * i, 512, 16, 4, 256, 40 + i) for i in range(4)]
+    want = [decode.moe_layer(*d) for d in data]
+    streams = [torch.cuda.Stream() for _ in data]
+    torch.cuda.synchronize()
+    for _ in range(5):
+        got = []
+        for d, s in zip(data, streams):
+            with torch.cuda.stream(s):
+                got.append(decode.moe_layer(*d))
+        torch.cuda.synchronize()
+        for a, b in zip(got, want):
+            assert torch.equal(a, b)
+
+
+ROUTED = [
+    # T, H, E, K, F
+    (1, 64, 2, 1, 64),
+    (1, 2048, 64, 6, 128),
+    (2, 7168, 256, 8, 64),
+    (5, 136, 10, 3, 72),
+    (13, 520, 104, 5, 64),
+    (40, 256, 1024, 4, 16),
+    (64, 1000, 128, 8, 64),
+    (64, 64, 700, 16, 8),
+    (32, 128, 32, 32, 64),
+]
+
+
+@pytest.mark.parametrize("renormalize", [False, True])
+@pytest.mark.parametrize("T,H,E,K,F", ROUTED)
+def test_router(T, H, E, K, F, renormalize):
+    x, _, _, w13, w2 = make(T, H, E, K, F, T + H + E)
+    g = torch.Generator(device="cuda").manual_seed(E)
+    rw = (torch.randn(H, E, generator=g, device="cuda") / H ** 0.5).to(torch.bfloat16)
+    dt = torch.int32 if renormalize else torch.int64
+    y, vals, ids = decode.routed_layer(x, rw, K, w13, w2, renormalize=renormalize, ids_dtype=dt)
+    torch.cuda.synchronize()
+    assert ids.dtype == dt and vals.dtype == torch.float32 and ids.shape == vals.shape == (T, K)
+    logits = x.double() @ rw.double()
+    slack = (x.double().abs() @ rw.double().abs()) * (H + 4) * 2.0 ** -24  # fp32 sums of H products
+    chosen = torch.gather(logits, 1, ids.long())
+    near = 2 * slack.amax(dim=1, keepdim=True)
+    # descending within the slack, distinct, and nothing left out is larger
+    assert bool((chosen[:, 1:] <= chosen[:, :-1] + near).all())
+    assert all(len(set(r)) == K for r in ids.tolist())
+    rest = logits.scatter(1, ids.long(), float("-inf")).amax(dim=1, keepdim=True)
+    assert bool((rest <= chosen[:, -1:] + near).all())
+    prob = torch.softmax(logits, -1).gather(1, ids.long())
+    if renormalize:
+        prob = prob / prob.sum(-1, keepdim=True)
+    # logits off by `slack`, then expf, sum (E terms) and division in fp32
+    rel = torch.expm1(2 * near) + (E + K + 16) * 2.0 ** -23
+    assert bool(((vals.double() - prob).abs() <= prob * rel).all())
+    check(y, x, ids, vals, w13, w2)
+    # the same result as the layer with that routing given
+    assert torch.equal(y, decode.moe_layer(x, ids, vals, w13, w2))
+
+
+def test_router_ties_and_part_of_the_experts():
+    T, H, E, K, F = 6, 128, 32, 4, 64
+    x, _, _, w13, w2 = make(T, H, 8, K, F, 77)
+    rw = torch.zeros(H, E, dtype=torch.bfloat16, device="cuda")
+    _, vals, ids = decode.routed_layer(x, rw, K, w13, w2, first_expert=0)
+    assert ids.tolist() == [list(range(K))] * T  # equal logits: lowest ids
+    assert bool((vals == 1.0 / E).all())
+    rw[:, 20:] = (0.1 * torch.randn(H, 12, device="cuda")).to(torch.bfloat16)
+    y, vals, ids = decode.routed_layer(x, rw, K, w13, w2, first_expert=20)
+    check(y, x, ids, vals, w13, w2, first=20)
+
+
+def test_router_with_non_finite_tokens():
+    """A NaN token keeps to its own row and its ids stay valid."""
+    T, H, E, K, F = 5, 256, 16, 3, 64
+    x, _, _, w13, w2 = make(T, H, E, K, F, 2)
+    rw = (0.1 * torch.randn(H, E, device="cuda")).to(torch.bfloat16)
+    ref, vals0, ids0 = decode.routed_layer(x, rw, K, w13, w2)
+    x2 = x.clone()
+    x2[2, 9] = float("nan")
+    y, vals, ids = decode.routed_layer(x2, rw, K, w13, w2)
+    keep = [0, 1, 3, 4]
+    assert torch.equal(ids[keep], ids0[keep]) and torch.equal(vals[keep], vals0[keep])
+    assert torch.equal(y[keep], ref[keep])
+    assert bool(((ids >= 0) & (ids < E)).all()) and bool(y[2].isnan().all())
+
+
+def test_status_word_stays_clear():
+    x, ids, vals, w13, w2 = make(4, 128, 4, 2, 64, 6)
+    status = torch.zeros(1, dtype=torch.int32, pin_memory=True)
+    decode.moe_layer(x, ids, vals, w13, w2, status=status)
+    torch.cuda.synchronize()
+    assert int(status[0]) == 0
