@@ -19,8 +19,10 @@
 //           outputs meet without leaving the CTA.
 // Each pass splits its list of 32 KB units evenly over the CTAs, at any k:
 // every SM streams the same number of bytes whatever the number of experts
-// or tiles.  A tile that ends up in several CTAs is summed by the last of
-// them, from fp32 partials in CTA order, so results do not depend on timing.
+// or tiles.  A tile that ends up in several CTAs is summed from fp32
+// partials in CTA order, so results do not depend on timing: in pass 1 by the
+// last of its CTAs (few parts, few rows), in pass 2, where 256 features may
+// be spread over all CTAs, by the whole grid after another barrier.
 // The weights' first stages of a pass are requested before the barrier in
 // front of it; only the token rows wait for it.
 #include <cooperative_groups.h>
@@ -28,6 +30,7 @@
 #include <cuda_runtime.h>
 
 #include <climits>
+#include <type_traits>
 
 #include "moe_ep.h"
 #include "moe_ep_internal.h"
@@ -64,7 +67,7 @@ struct DecArgs {
   int ids64, vals_bf16;
   __nv_bfloat16* hs;         // [T*K][F]
   float* part;               // [2 * grid][T][256]
-  uint32_t* ctr;             // [2 * grid]
+  uint32_t* ctr;             // [grid] tickets of pass 1's split tiles
   __nv_bfloat16* y;
   int32_t* status_host;
   // Routed form (router_w != nullptr).
@@ -84,11 +87,14 @@ struct alignas(16) DecSmem {
   uint32_t fills[kDecMaxStages];
   uint32_t tmem_base;
   int err;
-  int nact, rows;
+  int nact;
   int last;
 };
 
-__device__ bool dec_wait(uint64_t* bar, uint32_t parity, DecSmem& sm) {
+// The kernel runs most of its code once per launch, from a cold instruction
+// cache: what is not in a unit's path is kept small (out of line, not
+// unrolled).
+__device__ __noinline__ bool dec_wait_slow(uint64_t* bar, uint32_t parity, DecSmem& sm) {
   uint64_t deadline = 0;
   for (uint32_t spin = 0;; ++spin) {
     if (mbar_try_wait(bar, parity)) return true;
@@ -100,16 +106,47 @@ __device__ bool dec_wait(uint64_t* bar, uint32_t parity, DecSmem& sm) {
     }
   }
 }
+__device__ __forceinline__ bool dec_wait(uint64_t* bar, uint32_t parity, DecSmem& sm) {
+  return mbar_try_wait(bar, parity) || dec_wait_slow(bar, parity, sm);
+}
 
-__device__ void dec_fail(DecSmem& sm, const DecArgs& a, int detail) {
+__device__ __noinline__ void dec_fail(DecSmem& sm, const DecArgs& a, int detail) {
   if (atomicExch(&sm.err, 1) == 0 && a.status_host)
     *reinterpret_cast<volatile int32_t*>(a.status_host) = int32_t(status_word(kTimeout, kSitePipe, detail));
 }
 
-// Share of CTA c of `units`, and the CTA a unit belongs to (g CTAs, g <= units).
-__device__ __forceinline__ int share_lo(int64_t units, int g, int c) { return int(units * c / g); }
-__device__ __forceinline__ int share_owner(int64_t units, int g, int64_t u) {
+// Share of CTA c of `units`, and the CTA a unit belongs to (g CTAs, g <= units;
+// units * g < 2^32).
+__device__ __forceinline__ int share_lo(uint32_t units, uint32_t g, uint32_t c) { return int(units * c / g); }
+__device__ __forceinline__ int share_owner(uint32_t units, uint32_t g, uint32_t u) {
   return int(((u + 1) * g - 1) / units);
+}
+
+// The sum of parts lo..hi in order, `at(q)` giving part q's address: eight
+// loads in flight at a time, the last group's too.
+template <typename V, typename At>
+__device__ __forceinline__ V sum_parts(int lo, int hi, At at) {
+  V sum = {};
+#pragma unroll 1
+  for (int q = lo; q <= hi; q += 8) {
+    V v[8];
+#pragma unroll
+    for (int j = 0; j < 8; ++j) v[j] = q + j <= hi ? __ldcg(at(q + j)) : V{};
+#pragma unroll
+    for (int j = 0; j < 8; ++j) {
+      if constexpr (sizeof(V) == 4) {
+        sum += v[j];
+      } else {
+        sum.x += v[j].x;
+        sum.y += v[j].y;
+        if constexpr (sizeof(V) == 16) {
+          sum.z += v[j].z;
+          sum.w += v[j].w;
+        }
+      }
+    }
+  }
+  return sum;
 }
 
 __device__ __forceinline__ long long load_id(const DecArgs& a, const void* ids, int i) {
@@ -130,34 +167,46 @@ __host__ __device__ inline uint32_t dec_table_bytes(int maxact, int rows) {
 
 // One 64-bit mask of tokens per expert: an id repeated in a row counts once,
 // ids outside [first, first + E) match none, and rows of an expert ascend by
-// token, the same in every CTA.
+// token, the same in every CTA.  The routing is read once, into shared
+// memory.
 __device__ void dec_build(const DecArgs& a, DecSmem& sm, const DecTables& tb, unsigned char* scratch, const void* ids,
                           const void* vals, int vals_bf16) {
   unsigned long long* mask = reinterpret_cast<unsigned long long*>(scratch);  // [E]
-  uint16_t* off_e = reinterpret_cast<uint16_t*>(mask + a.E);                  // [E]
+  float* v = reinterpret_cast<float*>(mask + a.E);                            // [T*K]
+  uint16_t* off_e = reinterpret_cast<uint16_t*>(v + a.T * a.K);               // [E]
+  int16_t* loc = reinterpret_cast<int16_t*>(off_e + a.E);                     // [T*K] expert here, or -1
   const int tid = threadIdx.x, n = a.T * a.K;
-  for (int e = tid; e < a.E; e += kDecThreads) mask[e] = 0;
-  __syncthreads();
+#pragma unroll 1
   for (int i = tid; i < n; i += kDecThreads) {
     const long long e = load_id(a, ids, i) - a.first;
-    if (e >= 0 && e < a.E) atomicOr(&mask[e], 1ull << (i / a.K));
+    v[i] = vals_bf16 ? __bfloat162float(static_cast<const __nv_bfloat16*>(vals)[i])
+                     : __ldcg(static_cast<const float*>(vals) + i);
+    loc[i] = e >= 0 && e < a.E ? int16_t(e) : int16_t(-1);
   }
+#pragma unroll 1
+  for (int e = tid; e < a.E; e += kDecThreads) mask[e] = 0;
+  __syncthreads();
+#pragma unroll 1
+  for (int i = tid; i < n; i += kDecThreads)
+    if (loc[i] >= 0) atomicOr(&mask[loc[i]], 1ull << (i / a.K));
   __syncthreads();
   if (tid < 32) {
     int act = 0, row = 0;
+#pragma unroll 1
     for (int e0 = 0; e0 < a.E; e0 += 32) {
       const int e = e0 + tid;
       const int c = e < a.E ? __popcll(mask[e]) : 0;
+      const uint32_t live = __ballot_sync(0xffffffffu, c > 0);
+      if (live == 0) continue;
       int pre = c;
 #pragma unroll
       for (int o = 1; o < 32; o <<= 1) {
-        const int v = __shfl_up_sync(0xffffffffu, pre, o);
-        if (tid >= o) pre += v;
+        const int u = __shfl_up_sync(0xffffffffu, pre, o);
+        if (tid >= o) pre += u;
       }
-      const uint32_t live = __ballot_sync(0xffffffffu, c > 0);
-      if (e < a.E) off_e[e] = uint16_t(row + pre - c);
       if (c > 0) {
         const int at = act + __popc(live & ((1u << tid) - 1));
+        off_e[e] = uint16_t(row + pre - c);
         tb.act_e[at] = uint16_t(e);
         tb.act_off[at] = uint16_t(row + pre - c);
       }
@@ -167,21 +216,21 @@ __device__ void dec_build(const DecArgs& a, DecSmem& sm, const DecTables& tb, un
     if (tid == 0) {
       tb.act_off[act] = uint16_t(row);
       sm.nact = act;
-      sm.rows = row;
     }
   }
   __syncthreads();
+#pragma unroll 1
   for (int i = tid; i < n; i += kDecThreads) {
+    const int e = loc[i];
+    if (e < 0) continue;
     const int t = i / a.K;
-    const long long id = load_id(a, ids, i), e = id - a.first;
-    if (e < 0 || e >= a.E) continue;
     bool again = false;
-    for (int j = t * a.K; j < i; ++j) again |= load_id(a, ids, j) == id;
+#pragma unroll 1
+    for (int j = t * a.K; j < i; ++j) again |= loc[j] == e;
     if (again) continue;
     const int r = off_e[e] + __popcll(mask[e] & ((1ull << t) - 1));
     tb.tok[r] = uint8_t(t);
-    tb.val[r] = vals_bf16 ? __bfloat162float(static_cast<const __nv_bfloat16*>(vals)[i])
-                          : __ldcg(static_cast<const float*>(vals) + i);
+    tb.val[r] = v[i];
   }
   __syncthreads();
 }
@@ -193,17 +242,22 @@ __device__ void dec_router_partial(const DecArgs& a, unsigned char* stage) {
   const int G = gridDim.x, c = blockIdx.x, tid = threadIdx.x;
   const int h0 = int(int64_t(a.H) * c / G), h1 = int(int64_t(a.H) * (c + 1) / G), nh = h1 - h0;
   float* red = reinterpret_cast<float*>(stage);                       // [groups][chunk][Er]
-  float* xs = red + kDecThreads * 2 * kDecTokChunk;                   // [T][nh]
-  for (int i = tid; i < a.T * nh; i += kDecThreads) {
+  float* xs = red + kDecThreads * 2 * kDecTokChunk;                   // [chunk][nh][kDecTokChunk]
+  const int nt8 = (a.T + kDecTokChunk - 1) / kDecTokChunk * kDecTokChunk;
+#pragma unroll 1
+  for (int i = tid; i < nt8 * nh; i += kDecThreads) {
     const int t = i / nh, h = i - t * nh;
-    xs[i] = __bfloat162float(a.x[int64_t(t) * a.H + h0 + h]);
+    xs[((t / kDecTokChunk) * nh + h) * kDecTokChunk + t % kDecTokChunk] =
+        t < a.T ? __bfloat162float(a.x[int64_t(t) * a.H + h0 + h]) : 0.f;
   }
   __syncthreads();
   const int P = a.Er / 2;
   const int groups = P < kDecThreads ? kDecThreads / P : 1;
   const int grp = tid / P;
+#pragma unroll 1
   for (int t0 = 0; t0 < a.T; t0 += kDecTokChunk) {
     const int nt = min(kDecTokChunk, a.T - t0);
+#pragma unroll 1
     for (int p0 = 0; p0 < P; p0 += kDecThreads) {  // more than one round only for Er > 2 * kDecThreads
       const int p = P < kDecThreads ? tid - grp * P : p0 + tid;
       const bool on = P < kDecThreads ? grp < groups : p < P;
@@ -212,14 +266,29 @@ __device__ void dec_router_partial(const DecArgs& a, unsigned char* stage) {
       for (int j = 0; j < kDecTokChunk; ++j) s[j] = make_float2(0.f, 0.f);
       if (on) {
         const __nv_bfloat162* r = reinterpret_cast<const __nv_bfloat162*>(a.router_w + int64_t(h0) * a.Er) + p;
-#pragma unroll 8
-        for (int h = P < kDecThreads ? grp : 0; h < nh; h += groups) {
-          const float2 w = __bfloat1622float2(r[int64_t(h) * P]);
+        // Eight rows' loads in flight; rows past the slice count as zeros.
+#pragma unroll 1
+        for (int hb = P < kDecThreads ? grp : 0; hb < nh; hb += 8 * groups) {
+          __nv_bfloat162 w8[8];
 #pragma unroll
-          for (int j = 0; j < kDecTokChunk; ++j) {
-            const float xv = j < nt ? xs[(t0 + j) * nh + h] : 0.f;
-            s[j].x = fmaf(xv, w.x, s[j].x);
-            s[j].y = fmaf(xv, w.y, s[j].y);
+          for (int i = 0; i < 8; ++i) {
+            const int h = hb + i * groups;
+            w8[i] = h < nh ? r[int64_t(h) * P] : __nv_bfloat162{};
+          }
+#pragma unroll
+          for (int i = 0; i < 8; ++i) {
+            const int h = min(hb + i * groups, nh - 1);
+            const float2 w = __bfloat1622float2(w8[i]);
+            const float4* xv = reinterpret_cast<const float4*>(xs + t0 * nh + h * kDecTokChunk);
+            float xr[kDecTokChunk];
+#pragma unroll
+            for (int j = 0; j < kDecTokChunk; j += 4) *reinterpret_cast<float4*>(&xr[j]) = xv[j / 4];
+            const bool live = hb + i * groups < nh;
+#pragma unroll
+            for (int j = 0; j < kDecTokChunk; ++j) {
+              s[j].x = live ? fmaf(xr[j], w.x, s[j].x) : s[j].x;
+              s[j].y = live ? fmaf(xr[j], w.y, s[j].y) : s[j].y;
+            }
           }
         }
       }
@@ -230,14 +299,17 @@ __device__ void dec_router_partial(const DecArgs& a, unsigned char* stage) {
             *reinterpret_cast<float2*>(&red[(grp * kDecTokChunk + j) * a.Er + 2 * p]) = s[j];
         }
         __syncthreads();
+#pragma unroll 1
         for (int i = tid; i < nt * a.Er; i += kDecThreads) {
           const int j = i / a.Er, e = i - j * a.Er;
           float v = 0.f;
+#pragma unroll 2
           for (int g = 0; g < groups; ++g) v += red[(g * kDecTokChunk + j) * a.Er + e];
           a.lpart[(int64_t(c) * a.T + t0 + j) * a.Er + e] = v;
         }
         __syncthreads();
       } else if (on) {
+#pragma unroll 1
         for (int j = 0; j < nt; ++j)
           *reinterpret_cast<float2*>(&a.lpart[(int64_t(c) * a.T + t0 + j) * a.Er + 2 * p]) = s[j];
       }
@@ -247,75 +319,63 @@ __device__ void dec_router_partial(const DecArgs& a, unsigned char* stage) {
 
 // Router, step 2: tokens c, c + grid, ...: the slices' sum in CTA order, the
 // softmax over Er in fp32 and the K largest (equal logits: lowest id first).
+// An expert's place is the number of experts before it, counted by one
+// thread per expert: one pass over Er keys instead of K rounds.
 __device__ void dec_router_topk(const DecArgs& a, unsigned char* stage, unsigned char* scratch) {
   const int G = gridDim.x, tid = threadIdx.x, lane = tid & 31;
-  float* red = reinterpret_cast<float*>(stage);       // [parts][Er]
-  float* lg = reinterpret_cast<float*>(scratch);      // [Er]
+  float* red = reinterpret_cast<float*>(stage);              // [parts][Er]
+  float* lg = reinterpret_cast<float*>(scratch);             // [Er]
+  uint32_t* key = reinterpret_cast<uint32_t*>(lg + a.Er);    // [Er]
+  __shared__ int chosen[kMaxRouteK];
   const int parts = a.Er < kDecThreads ? kDecThreads / a.Er : 1;
+#pragma unroll 1
   for (int t = blockIdx.x; t < a.T; t += G) {
+#pragma unroll 1
     for (int i = tid; i < parts * a.Er; i += kDecThreads) {
       const int q = i / a.Er, e = i - q * a.Er;
-      const int c0 = G * q / parts, c1 = G * (q + 1) / parts;
-      float v = 0.f;
-#pragma unroll 16
-      for (int c = c0; c < c1; ++c) v += __ldcg(&a.lpart[(int64_t(c) * a.T + t) * a.Er + e]);
-      red[i] = v;
+      red[i] = sum_parts<float>(G * q / parts, G * (q + 1) / parts - 1,
+                                [&](int c) { return &a.lpart[(int64_t(c) * a.T + t) * a.Er + e]; });
     }
     __syncthreads();
+#pragma unroll 1
     for (int e = tid; e < a.Er; e += kDecThreads) {
       float v = 0.f;
       for (int q = 0; q < parts; ++q) v += red[q * a.Er + e];
       lg[e] = v;
+      // The logit's bits as an unsigned number of the same order (-0 and 0
+      // alike, NaN lowest).
+      const uint32_t b = __float_as_uint(v + 0.f);
+      key[e] = v != v ? 0u : (b >> 31) ? ~b : (b | 0x80000000u);
+    }
+    __syncthreads();
+#pragma unroll 1
+    for (int e = tid; e < a.Er; e += kDecThreads) {
+      const uint32_t mine = key[e];
+      int before = 0;
+#pragma unroll 8
+      for (int i = 0; i < a.Er; ++i) before += key[i] > mine || (key[i] == mine && i < e);
+      if (before < a.K) chosen[before] = e;
     }
     __syncthreads();
     if (tid < 32) {
       float m = -INFINITY;
+#pragma unroll 1
       for (int e = lane; e < a.Er; e += 32) m = fmaxf(m, lg[e]);
 #pragma unroll
       for (int o = 16; o > 0; o >>= 1) m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, o));
       float z = 0.f;
+#pragma unroll 1
       for (int e = lane; e < a.Er; e += 32) z += expf(lg[e] - m);
 #pragma unroll
       for (int o = 16; o > 0; o >>= 1) z += __shfl_xor_sync(0xffffffffu, z, o);
-      uint32_t taken = 0;  // bit i: expert lane + 32 * i
-      float mine = 0.f;    // lane k: the k-th probability
-      int id = 0;
-      float sum = 0.f;
-      for (int k = 0; k < a.K; ++k) {
-        float best = 0.f;
-        int be = INT_MAX;
-        for (int i = 0, e = lane; e < a.Er; ++i, e += 32) {
-          const float v = lg[e];
-          if (!((taken >> i) & 1) && (be == INT_MAX || v > best)) {
-            best = v;
-            be = e;
-          }
-        }
+      const int id = lane < a.K ? chosen[lane] : 0;
+      const float pr = lane < a.K ? expf(lg[id] - m) / z : 0.f;
+      float sum = pr;
 #pragma unroll
-        for (int o = 16; o > 0; o >>= 1) {
-          const float ob = __shfl_xor_sync(0xffffffffu, best, o);
-          const int oe = __shfl_xor_sync(0xffffffffu, be, o);
-          // An empty hand (INT_MAX) loses; equal values, or values that do
-          // not compare (NaN), go to the lower id: every lane agrees.
-          const bool take = be == INT_MAX || (oe != INT_MAX && (ob > best || (!(best > ob) && oe < be)));
-          if (take) {
-            best = ob;
-            be = oe;
-          }
-        }
-        be = __shfl_sync(0xffffffffu, be, 0);
-        best = __shfl_sync(0xffffffffu, best, 0);
-        if ((be & 31) == lane) taken |= 1u << (be >> 5);
-        const float pr = expf(best - m) / z;
-        sum += pr;
-        if (lane == k) {
-          mine = pr;
-          id = be;
-        }
-      }
+      for (int o = 16; o > 0; o >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
       if (lane < a.K) {
         const int64_t o = int64_t(t) * a.K + lane;
-        a.out_vals[o] = a.renorm ? mine / sum : mine;
+        a.out_vals[o] = a.renorm ? pr / sum : pr;
         if (a.ids64) static_cast<long long*>(a.out_ids)[o] = id;
         else static_cast<int*>(a.out_ids)[o] = id;
       }
@@ -324,13 +384,65 @@ __device__ void dec_router_topk(const DecArgs& a, unsigned char* stage, unsigned
   }
 }
 
-// What one pass consists of.
+// One pass: its units in order, and this CTA's share [lo, hi) of them.
+// Pass 1: expert by expert, its tiles of 128 features of F, each over H.
+// Pass 2: tile by tile of 256 features of H, each over the experts' F.
 struct Pass {
-  int units;     // all CTAs
+  int units;     // of all CTAs
   int tile;      // units of one tile (the units whose sums belong together)
   int kb;        // units of one expert's K
+  int nt;        // tiles per expert (pass 1), tiles (pass 2)
   int g;         // CTAs that have units
-  int lo, hi;    // this CTA's
+  int lo, hi;
+};
+
+// A position in a pass, moved on by additions: the loads and the MMAs each
+// run in one thread, whose integer divisions (two per unit and more) took
+// longer than a unit's share of the memory bandwidth.
+struct Cursor {
+  int ai, ft, k;  // active expert, tile of features, K
+};
+template <int PASS>
+__device__ __forceinline__ Cursor cursor_at(const Pass& p, int nact, int u) {
+  Cursor c;
+  const int x = u / p.kb;
+  c.k = u - x * p.kb;
+  const int in = PASS == 1 ? p.nt : nact;
+  const int hi = in > 0 ? x / in : 0;
+  c.ai = PASS == 1 ? hi : x - hi * in;
+  c.ft = PASS == 1 ? x - hi * in : hi;
+  return c;
+}
+template <int PASS>
+__device__ __forceinline__ void cursor_next_k(Cursor& c, const Pass& p, int nact) {  // the next run over K
+  c.k = 0;
+  if (PASS == 1) {
+    if (++c.ft == p.nt) {
+      c.ft = 0;
+      ++c.ai;
+    }
+  } else {
+    if (++c.ai == nact) {
+      c.ai = 0;
+      ++c.ft;
+    }
+  }
+}
+template <int PASS>
+__device__ __forceinline__ void cursor_next(Cursor& c, const Pass& p, int nact) {
+  if (++c.k == p.kb) cursor_next_k<PASS>(c, p, nact);
+}
+
+// The stage a thread has reached, and the parity of its round.
+struct Ring {
+  int st;
+  uint32_t ph;
+  __device__ __forceinline__ void next(int n) {
+    if (++st == n) {
+      st = 0;
+      ph ^= 1;
+    }
+  }
 };
 
 __global__ void __launch_bounds__(kDecThreads, 1)
@@ -382,7 +494,7 @@ __global__ void __launch_bounds__(kDecThreads, 1)
   // The tickets of split tiles start at zero: written here, ordered before
   // their first use by the first grid barrier.
   if (blockIdx.x == 0)
-    for (int i = threadIdx.x; i < 2 * int(gridDim.x); i += kDecThreads) a.ctr[i] = 0;
+    for (int i = threadIdx.x; i < int(gridDim.x); i += kDecThreads) a.ctr[i] = 0;
   tc_fence_before();
   __syncthreads();
   tc_fence_after();
@@ -394,18 +506,17 @@ __global__ void __launch_bounds__(kDecThreads, 1)
     dec_router_topk(a, stage, scratch);
     fence_proxy_async_smem();  // the stages, written by threads so far, belong to the TMA from here
     grid.sync();
-    dec_build(a, sm, tb, scratch, a.out_ids, a.out_vals, 0);
-  } else {
-    dec_build(a, sm, tb, scratch, a.ids, a.vals, a.vals_bf16);
   }
+  dec_build(a, sm, tb, scratch, a.ids, a.vals, a.vals_bf16);
   const int nact = sm.nact;
   const int G = gridDim.x;
 
-  auto make_pass = [&](int tiles, int tile, int kb) {
+  auto make_pass = [&](int tiles, int tile, int kb, int nt) {
     Pass p;
     p.units = tiles * tile;
     p.tile = tile;
     p.kb = kb;
+    p.nt = nt;
     p.g = min(G, p.units);
     const bool on = int(blockIdx.x) < p.g;
     p.lo = on ? share_lo(p.units, p.g, blockIdx.x) : 0;
@@ -414,93 +525,105 @@ __global__ void __launch_bounds__(kDecThreads, 1)
   };
   const int kb1 = (a.H + 63) / 64, nt1 = (a.F + 127) / 128;
   const int kb2 = (a.F + 63) / 64, nt2 = (a.H + 255) / 256;
-  const Pass p1 = make_pass(nact * nt1, kb1, kb1);
-  const Pass p2 = make_pass(nact > 0 ? nt2 : 0, nact * kb2, kb2);
+  const Pass p1 = make_pass(nact * nt1, kb1, kb1, nt1);
+  const Pass p2 = make_pass(nact > 0 ? nt2 : 0, nact * kb2, kb2, nt2);
+  auto act_rows = [&](int ai) { return int(tb.act_off[ai + 1]) - int(tb.act_off[ai]); };
 
   // ---- loads (one thread)
-  uint32_t it = 0;  // stages used so far
-  auto act_rows = [&](int ai) { return int(tb.act_off[ai + 1]) - int(tb.act_off[ai]); };
-  // Weights of unit u of a pass into the next stage; the stage's expected
-  // bytes include the rows that load_rows adds.
-  auto load_weights = [&](int pass, const Pass& p, int u) -> bool {
-    const int st = it % S;
-    if (!dec_wait(&sm.empty[st], ((it / S) & 1) ^ 1, sm)) {
+  Ring lr = {0, 0};  // next stage to fill
+  // A unit's weights into the next stage; the stage's expected bytes include
+  // the rows that load_rows adds.
+  auto load_weights = [&](auto pass, const Cursor& c) -> bool {
+    constexpr int PASS = decltype(pass)::value;
+    uint64_t* full = &sm.full[lr.st];
+    if (!dec_wait(&sm.empty[lr.st], lr.ph ^ 1, sm)) {
       dec_fail(sm, a, 1);
       return false;
     }
-    unsigned char* dst = stage + size_t(st) * a.stage_bytes;
-    const int tile = u / p.tile, k = u % p.kb;
-    if (pass == 1) {
-      const int ai = tile / nt1, f0 = (tile % nt1) * 128;
-      mbar_arrive_expect_tx(&sm.full[st], kDecABytes + uint32_t(a.NB) * 128);
-      tma_load_4d(&tm_w13, &sm.full[st], dst, f0, k * 64, 0, tb.act_e[ai]);
-      tma_load_4d(&tm_w13, &sm.full[st], dst + 16384, f0 + 64, k * 64, 0, tb.act_e[ai]);
+    unsigned char* dst = stage + uint32_t(lr.st) * a.stage_bytes;
+    const int e = tb.act_e[c.ai];
+    if constexpr (PASS == 1) {
+      mbar_arrive_expect_tx(full, kDecABytes + uint32_t(a.NB) * 128);
+      tma_load_4d(&tm_w13, full, dst, c.ft * 128, c.k * 64, 0, e);
+      tma_load_4d(&tm_w13, full, dst + 16384, c.ft * 128 + 64, c.k * 64, 0, e);
     } else {
-      const int ai = (u % p.tile) / p.kb;
-      mbar_arrive_expect_tx(&sm.full[st], kDecABytes + uint32_t((act_rows(ai) + 15) / 16) * 2048);
+      mbar_arrive_expect_tx(full, kDecABytes + uint32_t((act_rows(c.ai) + 15) >> 4) * 2048);
       if (a.w2_atoms) {
-        tma_load_4d(&tm_w2, &sm.full[st], dst, 0, k * 64, tile * 4, tb.act_e[ai]);
+        tma_load_4d(&tm_w2, full, dst, 0, c.k * 64, c.ft * 4, e);
       } else {
-        for (int g = 0; g < 4; ++g)
-          tma_load_3d(&tm_w2, &sm.full[st], dst + g * 8192, tile * 256 + g * 64, k * 64, tb.act_e[ai]);
+        for (int g = 0; g < 4; ++g) tma_load_3d(&tm_w2, full, dst + g * 8192, c.ft * 256 + g * 64, c.k * 64, e);
       }
     }
-    sm.fills[st] += 1;
-    ++it;
+    sm.fills[lr.st] += 1;
+    lr.next(S);
     return true;
   };
-  auto load_rows = [&](int pass, const Pass& p, int u, uint32_t at) {
-    const int st = at % S;
-    unsigned char* dst = stage + size_t(st) * a.stage_bytes + kDecABytes;
-    const int k = u % p.kb;
-    if (pass == 1) {
-      tma_load_2d(&tm_x, &sm.full[st], dst, k * 64, 0);
+  auto load_rows = [&](auto pass, const Cursor& c, int st) {
+    constexpr int PASS = decltype(pass)::value;
+    uint64_t* full = &sm.full[st];
+    unsigned char* dst = stage + uint32_t(st) * a.stage_bytes + kDecABytes;
+    if constexpr (PASS == 1) {
+      tma_load_2d(&tm_x, full, dst, c.k * 64, 0);
     } else {
-      const int ai = (u % p.tile) / p.kb;
-      const int nb = (act_rows(ai) + 15) / 16;
-      for (int b = 0; b < nb; ++b)
-        tma_load_2d(&tm_h, &sm.full[st], dst + b * 2048, k * 64, int(tb.act_off[ai]) + b * 16);
+      const int r0 = tb.act_off[c.ai], nb = (act_rows(c.ai) + 15) >> 4;
+      for (int b = 0; b < nb; ++b) tma_load_2d(&tm_h, full, dst + b * 2048, c.k * 64, r0 + b * 16);
     }
   };
   // The first stages of a pass: weights only, before the barrier.
-  auto preload = [&](int pass, const Pass& p) {
-    int n = 0;
-    while (n < S && p.lo + n < p.hi && load_weights(pass, p, p.lo + n)) ++n;
-    return n;
+  int pre = 0;     // units preloaded
+  Ring pre_at = {0, 0};
+  auto preload = [&](auto pass, const Pass& p) {
+    constexpr int PASS = decltype(pass)::value;
+    pre_at = lr;
+    pre = 0;
+    Cursor c = cursor_at<PASS>(p, nact, p.lo);
+    const int n = min(S, p.hi - p.lo);
+    for (; pre < n && load_weights(pass, c); ++pre) cursor_next<PASS>(c, p, nact);
   };
-  auto produce = [&](int pass, const Pass& p, int pre) {
-    for (int i = 0; i < pre; ++i) load_rows(pass, p, p.lo + i, it - pre + i);
-    for (int u = p.lo + pre; u < p.hi; ++u) {
-      if (!load_weights(pass, p, u)) return;
-      load_rows(pass, p, u, it - 1);
+  auto produce = [&](auto pass, const Pass& p) {
+    constexpr int PASS = decltype(pass)::value;
+    Cursor c = cursor_at<PASS>(p, nact, p.lo);
+    int u = p.lo;
+    for (int i = 0; i < pre; ++i, ++u) {
+      load_rows(pass, c, pre_at.st);
+      pre_at.next(S);
+      cursor_next<PASS>(c, p, nact);
+    }
+    for (; u < p.hi; ++u) {
+      const int st = lr.st;
+      if (!load_weights(pass, c)) return;
+      load_rows(pass, c, st);
+      cursor_next<PASS>(c, p, nact);
     }
   };
 
   // ---- MMA (one thread)
-  uint32_t mi = 0, mseg = 0;  // stages and accumulators used so far
-  auto multiply = [&](int pass, const Pass& p) {
-    for (int u = p.lo; u < p.hi; ++u, ++mi) {
-      const int k = u % p.kb;
-      const bool begin = u == p.lo || k == 0, end = u + 1 == p.hi || k + 1 == p.kb;
-      const uint32_t buf = mseg & 1;
-      if (begin && !dec_wait(&sm.tempty[buf], ((mseg >> 1) & 1) ^ 1, sm)) {
-        dec_fail(sm, a, 2);
-        return;
+  Ring mr = {0, 0};       // next stage to multiply
+  Ring mseg = {0, 0};     // next accumulator (two)
+  auto multiply = [&](auto pass, const Pass& p) {
+    constexpr int PASS = decltype(pass)::value;
+    // Pass 1: box g (64 features of each half) is [gate 64x64][up 64x64];
+    // pass 2: four groups of 64 features in order.
+    constexpr uint32_t half = PASS == 1 ? 8192 : 16384, group = PASS == 1 ? 16384 : 8192;
+    Cursor c = cursor_at<PASS>(p, nact, p.lo);
+    bool begin = true;
+    uint32_t idesc = 0;
+    for (int u = p.lo; u < p.hi; ++u) {
+      if (begin) {
+        if (!dec_wait(&sm.tempty[mseg.st], mseg.ph ^ 1, sm)) {
+          dec_fail(sm, a, 2);
+          return;
+        }
+        const int n = PASS == 1 ? a.NB : (act_rows(c.ai) + 15) / 16 * 16;
+        idesc = make_idesc_mn(/*bf16*/ 1, 128, uint32_t(n), /*A MN-major*/ 1, /*B K-major*/ 0);
       }
-      const int st = mi % S;
-      if (!dec_wait(&sm.full[st], (mi / S) & 1, sm)) {
+      if (!dec_wait(&sm.full[mr.st], mr.ph, sm)) {
         dec_fail(sm, a, 3);
         return;
       }
       tc_fence_after();
-      int n = a.NB;
-      if (pass == 2) n = (act_rows((u % p.tile) / p.kb) + 15) / 16 * 16;
-      const uint32_t idesc = make_idesc_mn(/*bf16*/ 1, 128, uint32_t(n), /*A MN-major*/ 1, /*B K-major*/ 0);
-      const uint32_t aa = smem_u32(stage + size_t(st) * a.stage_bytes), ba = aa + kDecABytes;
-      // Pass 1: box g (64 features of each half) is [gate 64x64][up 64x64];
-      // pass 2: four groups of 64 features in order.
-      const uint32_t half = pass == 1 ? 8192 : 16384, group = pass == 1 ? 16384 : 8192;
-      const uint32_t d = tmem + buf * 2 * uint32_t(a.NB);
+      const uint32_t aa = smem_u32(stage + uint32_t(mr.st) * a.stage_bytes), ba = aa + kDecABytes;
+      const uint32_t d = tmem + uint32_t(mseg.st) * 2 * uint32_t(a.NB);
 #pragma unroll
       for (int kk = 0; kk < 4; ++kk) {
         const uint64_t bd = smem_desc_sw128(ba + kk * 32, 16, 1024);
@@ -510,50 +633,50 @@ __global__ void __launch_bounds__(kDecThreads, 1)
           tc_mma_f16(d + h * uint32_t(a.NB), ad, bd, idesc, (!begin || kk != 0) ? 1u : 0u);
         }
       }
-      tc_commit(&sm.empty[st]);
-      if (end) {
-        tc_commit(&sm.tfull[buf]);
-        ++mseg;
+      tc_commit(&sm.empty[mr.st]);
+      mr.next(S);
+      begin = c.k + 1 == p.kb;
+      if (begin || u + 1 == p.hi) {
+        tc_commit(&sm.tfull[mseg.st]);
+        mseg.next(2);
       }
+      cursor_next<PASS>(c, p, nact);
     }
   };
 
   // ---- epilogue (8 warps: lane quarter = 32 features of 128; two warps each)
-  uint32_t eseg = 0;
+  Ring eseg = {0, 0};
   const int quarter = warp & 3, sub = (warp - kDecEpi0) >> 2;
   const int etid = int(threadIdx.x) - kDecEpi0 * 32;
   const uint32_t tlane = tmem + (uint32_t(quarter * 32) << 16);
-  // This CTA's sums of a split tile are in its slot; true for the CTA whose
-  // ticket is the last of the tile's.
-  auto last_part = [&](uint32_t* ctr, int parts) {
-    __threadfence();
-    named_bar_sync(kBarEpi, kDecEpiWarps * 32);
-    if (etid == 0) {
-      sm.last = atomicAdd(ctr, 1u) == uint32_t(parts - 1);
-      __threadfence();
-    }
-    named_bar_sync(kBarEpi, kDecEpiWarps * 32);
-    return sm.last != 0;
-  };
+  // Of a CTA's split tiles the one it starts goes to its slot 1, the one it
+  // joins to slot 0.
   const size_t slot_floats = size_t(a.T) * 256;
   auto slot = [&](int cta, int which) { return a.part + (size_t(cta) * 2 + which) * slot_floats; };
+  auto seg_full = [&](int site) {
+    if (named_bar_and(kBarEpi, kDecEpiWarps * 32, dec_wait(&sm.tfull[eseg.st], eseg.ph, sm))) return true;
+    dec_fail(sm, a, site);
+    return false;
+  };
+  auto seg_done = [&]() {
+    tc_fence_before();
+    __syncwarp();
+    if (lane == 0) mbar_arrive(&sm.tempty[eseg.st]);
+    eseg.next(2);
+  };
 
   auto epilogue1 = [&](const Pass& p) {
-    for (int u = p.lo; u < p.hi; ++eseg) {
-      const int tile = u / p.kb, ai = tile / nt1;
-      const int seg_end = min(p.hi, (tile + 1) * p.kb);
-      const bool whole = u == tile * p.kb && seg_end == (tile + 1) * p.kb;
-      const uint32_t buf = eseg & 1;
-      if (!named_bar_and(kBarEpi, kDecEpiWarps * 32, dec_wait(&sm.tfull[buf], (eseg >> 1) & 1, sm))) {
-        dec_fail(sm, a, 4);
-        return;
-      }
+    Cursor c = cursor_at<1>(p, nact, p.lo);
+    for (int u = p.lo; u < p.hi;) {
+      const int tile0 = u - c.k, seg_end = min(p.hi, tile0 + p.kb);
+      const bool whole = c.k == 0 && seg_end == tile0 + p.kb;
+      if (!seg_full(4)) return;
       tc_fence_after();
-      const int n = act_rows(ai), r0 = tb.act_off[ai];
+      const int n = act_rows(c.ai), r0 = tb.act_off[c.ai];
       const int fl = quarter * 32 + lane;              // feature within the tile
-      const int f = (tile % nt1) * 128 + fl;
-      const uint32_t d = tlane + buf * 2 * uint32_t(a.NB);
-      float* mine = slot(blockIdx.x, u == tile * p.kb ? 1 : 0);
+      const int f = c.ft * 128 + fl;
+      const uint32_t d = tlane + uint32_t(eseg.st) * 2 * uint32_t(a.NB);
+      float* mine = slot(blockIdx.x, c.k == 0 ? 1 : 0);
       for (int j0 = sub; j0 < n; j0 += 8) {
         uint32_t g[4], w[4];
 #pragma unroll
@@ -577,48 +700,46 @@ __global__ void __launch_bounds__(kDecThreads, 1)
           }
         }
       }
-      tc_fence_before();
-      __syncwarp();
-      if (lane == 0) mbar_arrive(&sm.tempty[buf]);
+      seg_done();
       if (!whole) {
-        const int c0 = share_owner(p.units, p.g, int64_t(tile) * p.kb);
-        const int c1 = share_owner(p.units, p.g, int64_t(tile + 1) * p.kb - 1);
-        if (last_part(&a.ctr[c0], c1 - c0 + 1) && f < a.F) {
+        // The CTA whose ticket is the tile's last adds the parts up.
+        const int c0 = share_owner(p.units, p.g, tile0), c1 = share_owner(p.units, p.g, tile0 + p.kb - 1);
+        __threadfence();
+        named_bar_sync(kBarEpi, kDecEpiWarps * 32);
+        if (etid == 0) {
+          sm.last = atomicAdd(&a.ctr[c0], 1u) == uint32_t(c1 - c0);
+          __threadfence();
+        }
+        named_bar_sync(kBarEpi, kDecEpiWarps * 32);
+        if (sm.last && f < a.F) {
+#pragma unroll 1
           for (int j = sub; j < n; j += 2) {
-            float gv = 0.f, uv = 0.f;
-            for (int c = c0; c <= c1; ++c) {
-              const float* ps = slot(c, c == c0 ? 1 : 0) + j * 256 + fl;
-              gv += __ldcg(ps);
-              uv += __ldcg(ps + 128);
-            }
+            const int at = j * 256 + fl;
+            const float gv = sum_parts<float>(c0, c1, [&](int q) { return slot(q, q == c0 ? 1 : 0) + at; });
+            const float uv = sum_parts<float>(c0, c1, [&](int q) { return slot(q, q == c0 ? 1 : 0) + at + 128; });
             a.hs[size_t(r0 + j) * a.F + f] = __float2bfloat16_rn(gv / (1.f + expf(-gv)) * uv);
           }
         }
       }
       u = seg_end;
+      cursor_next_k<1>(c, p, nact);
     }
   };
 
   auto epilogue2 = [&](const Pass& p) {
     const int fl = sub * 128 + quarter * 32 + lane;  // feature within the tile: this thread's alone
+    Cursor c = cursor_at<2>(p, nact, p.lo);
     for (int u = p.lo; u < p.hi;) {
-      const int tile = u / p.tile;
-      const int tile_end = min(p.hi, (tile + 1) * p.tile);
-      const bool starts = u == tile * p.tile;
-      const bool whole = starts && tile_end == (tile + 1) * p.tile;
-      const int f = tile * 256 + fl;
+      const int tile0 = u - c.ai * p.kb - c.k, tile_end = min(p.hi, tile0 + p.tile);
+      const bool starts = u == tile0, whole = starts && tile_end == tile0 + p.tile;
+      const int f = c.ft * 256 + fl;
+#pragma unroll 4
       for (int t = 0; t < a.T; ++t) acc[t * 256 + fl] = 0.f;
-      for (; u < tile_end; ++eseg) {
-        const int in = u % p.tile, ai = in / p.kb;
-        const int seg_end = min(tile_end, tile * p.tile + (ai + 1) * p.kb);
-        const uint32_t buf = eseg & 1;
-        if (!named_bar_and(kBarEpi, kDecEpiWarps * 32, dec_wait(&sm.tfull[buf], (eseg >> 1) & 1, sm))) {
-          dec_fail(sm, a, 5);
-          return;
-        }
+      while (u < tile_end) {
+        if (!seg_full(5)) return;
         tc_fence_after();
-        const int n = act_rows(ai), r0 = tb.act_off[ai];
-        const uint32_t d = tlane + buf * 2 * uint32_t(a.NB) + uint32_t(sub) * uint32_t(a.NB);
+        const int n = act_rows(c.ai), r0 = tb.act_off[c.ai];
+        const uint32_t d = tlane + (uint32_t(eseg.st) * 2 + uint32_t(sub)) * uint32_t(a.NB);
         for (int j0 = 0; j0 < n; j0 += 4) {
           uint32_t v[4];
 #pragma unroll
@@ -632,54 +753,68 @@ __global__ void __launch_bounds__(kDecThreads, 1)
             *s = fmaf(tb.val[r0 + j0 + q], __uint_as_float(v[q]), *s);
           }
         }
-        tc_fence_before();
-        __syncwarp();
-        if (lane == 0) mbar_arrive(&sm.tempty[buf]);
-        u = seg_end;
+        seg_done();
+        u = min(tile_end, u + p.kb - c.k);
+        cursor_next_k<2>(c, p, nact);
       }
       if (whole) {
         if (f < a.H)
+#pragma unroll 4
           for (int t = 0; t < a.T; ++t) a.y[size_t(t) * a.H + f] = __float2bfloat16_rn(acc[t * 256 + fl]);
       } else {
         float* mine = slot(blockIdx.x, starts ? 1 : 0);
+#pragma unroll 4
         for (int t = 0; t < a.T; ++t) mine[t * 256 + fl] = acc[t * 256 + fl];
-        const int c0 = share_owner(p.units, p.g, int64_t(tile) * p.tile);
-        const int c1 = share_owner(p.units, p.g, int64_t(tile + 1) * p.tile - 1);
-        if (last_part(&a.ctr[G + c0], c1 - c0 + 1) && f < a.H) {
-          for (int t = 0; t < a.T; ++t) {
-            float v = 0.f;
-            for (int c = c0; c <= c1; ++c) v += __ldcg(slot(c, c == c0 ? 1 : 0) + t * 256 + fl);
-            a.y[size_t(t) * a.H + f] = __float2bfloat16_rn(v);
-          }
-        }
       }
     }
   };
 
+  // y of the tiles that several CTAs hold parts of: four features a thread.
+  auto join2 = [&](const Pass& p) {
+    const int per = a.T * 64;
+#pragma unroll 1
+    for (int i = int(blockIdx.x) * kDecThreads + int(threadIdx.x); i < p.nt * per; i += G * kDecThreads) {
+      const int tile = i / per, r = i - tile * per;
+      const int t = r >> 6, fl = (r & 63) * 4, f = tile * 256 + fl;
+      const int u0 = tile * p.tile;
+      const int c0 = share_owner(p.units, p.g, u0), c1 = share_owner(p.units, p.g, u0 + p.tile - 1);
+      if (c0 == c1 || f >= a.H) continue;
+      const float4 v = sum_parts<float4>(c0, c1, [&](int q) {
+        return reinterpret_cast<const float4*>(slot(q, q == c0 ? 1 : 0) + t * 256 + fl);
+      });
+      __nv_bfloat162* o = reinterpret_cast<__nv_bfloat162*>(a.y + size_t(t) * a.H + f);
+      o[0] = __floats2bfloat162_rn(v.x, v.y);
+      o[1] = __floats2bfloat162_rn(v.z, v.w);
+    }
+  };
+
   // ---- the two passes
-  int pre = 0;
-  if (threadIdx.x == 0) pre = preload(1, p1);
+  using Pass1 = std::integral_constant<int, 1>;
+  using Pass2 = std::integral_constant<int, 2>;
+  if (threadIdx.x == 0) preload(Pass1{}, p1);
   __syncwarp();
   if (a.router_w == nullptr) grid.sync();  // (routed: the router's barriers ordered the tickets)
-  if (warp == 0 && lane == 0) produce(1, p1, pre);
-  else if (warp == 1 && lane == 0) multiply(1, p1);
+  if (warp == 0 && lane == 0) produce(Pass1{}, p1);
+  else if (warp == 1 && lane == 0) multiply(Pass1{}, p1);
   else if (warp >= kDecEpi0) epilogue1(p1);
   __syncwarp();
-  if (threadIdx.x == 0 && !*reinterpret_cast<volatile int*>(&sm.err)) pre = preload(2, p2);
+  if (threadIdx.x == 0 && !*reinterpret_cast<volatile int*>(&sm.err)) preload(Pass2{}, p2);
   __syncwarp();
   fence_proxy_async_global();  // h, written by threads, is read by the TMA
   grid.sync();
-  const bool ok = !*reinterpret_cast<volatile int*>(&sm.err);
-  if (ok) {
+  if (!*reinterpret_cast<volatile int*>(&sm.err)) {
     if (warp == 0 && lane == 0) {
       fence_proxy_async_global();
-      produce(2, p2, pre);
+      produce(Pass2{}, p2);
     } else if (warp == 1 && lane == 0) {
-      multiply(2, p2);
+      multiply(Pass2{}, p2);
     } else if (warp >= kDecEpi0) {
       epilogue2(p2);
     }
   }
+  __syncwarp();
+  grid.sync();
+  join2(p2);
   if (nact == 0)  // no token has an expert here
     for (int64_t i = int64_t(blockIdx.x) * kDecThreads + threadIdx.x; i < int64_t(a.T) * a.H;
          i += int64_t(G) * kDecThreads)
@@ -731,7 +866,7 @@ DecScratch dec_scratch(int T, int K, int F, int Er, int sms) {
   s.hs = 0;
   s.part = up256(size_t(T) * K * F * 2);
   s.ctr = s.part + up256(size_t(2) * sms * T * 256 * 4);
-  s.lpart = s.ctr + up256(size_t(2) * sms * 4);
+  s.lpart = s.ctr + up256(size_t(sms) * 4);
   s.total = s.lpart + up256(size_t(sms) * T * Er * 4);
   return s;
 }
@@ -740,10 +875,10 @@ bool dec_sizes_ok(int64_t T, int32_t H, int32_t F, int32_t E, int32_t K, int32_t
   if (T < 0 || T > kDecMaxT || K < 1 || K > kMaxRouteK || T * K > kDecMaxRows) return false;
   if (H <= 0 || H % 8 || H > kDecMaxH || F <= 0 || F % 8 || E < 1 || E > kMaxExperts) return false;
   if (Er < 0 || Er > kMaxExperts || Er % 2 || (Er > 0 && K > Er)) return false;
-  // Unit counts stay within 31 bits.
+  // Unit counts times CTAs stay within 32 bits (2^24 units are 512 GB).
   const int64_t act = E < T * K ? E : T * K;
   const int64_t u1 = act * ((F + 127) / 128) * ((H + 63) / 64), u2 = act * ((H + 255) / 256) * ((F + 63) / 64);
-  return u1 <= INT_MAX && u2 <= INT_MAX;
+  return u1 <= (1 << 24) && u2 <= (1 << 24);
 }
 
 bool misaligned(const void* p) { return (reinterpret_cast<uintptr_t>(p) & 15) != 0; }
@@ -809,7 +944,7 @@ extern "C" int moe_decode_layer(const moe_decode_params* p, void* stream) {
   // Pass 2's sums [T][256] and, before them, the masks and offsets of the
   // routing tables and one token's logits.
   uint32_t scratch = uint32_t(T) * 1024;
-  const uint32_t build = uint32_t(E) * 10 + 16, logits = uint32_t(Er) * 4;
+  const uint32_t build = uint32_t(E) * 10 + uint32_t(T) * K * 6, logits = uint32_t(Er) * 8;
   if (scratch < build) scratch = build;
   if (scratch < logits) scratch = logits;
   a.scratch_bytes = (scratch + 15) / 16 * 16;
@@ -819,7 +954,7 @@ extern "C" int moe_decode_layer(const moe_decode_params* p, void* stream) {
   if (a.stages < 2) return kBadArg;
   const uint32_t smem = fixed + uint32_t(a.stages) * a.stage_bytes;
   // The router's slices use the stage memory.
-  if (Er && uint32_t(a.stages) * a.stage_bytes < kDecThreads * 2 * kDecTokChunk * 4 + uint32_t(T) * ((H + sms - 1) / sms + 1) * 4)
+  if (Er && uint32_t(a.stages) * a.stage_bytes < kDecThreads * 2 * kDecTokChunk * 4 + uint32_t(T + kDecTokChunk - 1) * ((H + sms - 1) / sms + 1) * 4)
     return kBadArg;
 
   CUtensorMap m13, m2, mx, mh;
