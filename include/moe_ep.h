@@ -383,7 +383,7 @@ int moe_ep_run_compact_swiglu(const moe_ep_run_params* params, int64_t send_rows
  * top_idxs and top_vals (fp32), divided by their sum with `renormalize`.
  * Requires T <= MOE_DECODE_MAX_TOKENS, T * K <= 1024, K <= 32, hidden and ffn
  * multiples of 8, hidden <= 32768, experts and router_experts <= 1024,
- * router_experts even; x, w13, w2 and scratch 16-byte aligned.
+ * router_experts a multiple of 4; x, w13, w2 and scratch 16-byte aligned.
  * scratch: moe_decode_scratch_bytes of device memory, not initialised, for
  * this call alone until it has finished.  Launched cooperatively (one CTA per
  * SM), so calls on several streams run one after another. */

@@ -73,7 +73,8 @@ struct DecArgs {
   // Routed form (router_w != nullptr).
   const __nv_bfloat16* router_w;  // [H, Er]
   int Er, renorm;
-  float* lpart;              // [grid][T][Er]
+  int eparts;                // the router's experts in this many slices, H in grid / eparts
+  float* lpart;              // [grid / eparts][T][Er]
   void* out_ids;
   float* out_vals;
 };
@@ -149,8 +150,8 @@ __device__ __forceinline__ V sum_parts(int lo, int hi, At at) {
   return sum;
 }
 
-__device__ __forceinline__ long long load_id(const DecArgs& a, const void* ids, int i) {
-  return a.ids64 ? __ldcg(static_cast<const long long*>(ids) + i) : __ldcg(static_cast<const int*>(ids) + i);
+__device__ __forceinline__ long long load_id(const void* ids, int ids64, int i) {
+  return ids64 ? static_cast<const long long*>(ids)[i] : static_cast<const int*>(ids)[i];
 }
 
 // Tables in shared memory, built alike by every CTA from the routing.
@@ -170,7 +171,7 @@ __host__ __device__ inline uint32_t dec_table_bytes(int maxact, int rows) {
 // token, the same in every CTA.  The routing is read once, into shared
 // memory.
 __device__ void dec_build(const DecArgs& a, DecSmem& sm, const DecTables& tb, unsigned char* scratch, const void* ids,
-                          const void* vals, int vals_bf16) {
+                          int ids64, const void* vals, int vals_bf16) {
   unsigned long long* mask = reinterpret_cast<unsigned long long*>(scratch);  // [E]
   float* v = reinterpret_cast<float*>(mask + a.E);                            // [T*K]
   uint16_t* off_e = reinterpret_cast<uint16_t*>(v + a.T * a.K);               // [E]
@@ -178,9 +179,9 @@ __device__ void dec_build(const DecArgs& a, DecSmem& sm, const DecTables& tb, un
   const int tid = threadIdx.x, n = a.T * a.K;
 #pragma unroll 1
   for (int i = tid; i < n; i += kDecThreads) {
-    const long long e = load_id(a, ids, i) - a.first;
+    const long long e = load_id(ids, ids64, i) - a.first;
     v[i] = vals_bf16 ? __bfloat162float(static_cast<const __nv_bfloat16*>(vals)[i])
-                     : __ldcg(static_cast<const float*>(vals) + i);
+                     : static_cast<const float*>(vals)[i];
     loc[i] = e >= 0 && e < a.E ? int16_t(e) : int16_t(-1);
   }
 #pragma unroll 1
@@ -235,59 +236,66 @@ __device__ void dec_build(const DecArgs& a, DecSmem& sm, const DecTables& tb, un
   __syncthreads();
 }
 
-// Router, step 1: this CTA's slice of H of every token's logits, in fp32.
-// Threads hold two neighbouring experts each; groups of threads take every
-// `groups`-th row of the slice and are summed in group order.
+// Router, step 1: one slice of H of the logits of one slice of the experts,
+// for every token, in fp32.  A thread holds two neighbouring experts and
+// eight tokens; the threads left over take other tokens, then other rows of
+// the slice, whose sums are added in a fixed order.
 __device__ void dec_router_partial(const DecArgs& a, unsigned char* stage) {
-  const int G = gridDim.x, c = blockIdx.x, tid = threadIdx.x;
-  const int h0 = int(int64_t(a.H) * c / G), h1 = int(int64_t(a.H) * (c + 1) / G), nh = h1 - h0;
-  float* red = reinterpret_cast<float*>(stage);                       // [groups][chunk][Er]
-  float* xs = red + kDecThreads * 2 * kDecTokChunk;                   // [chunk][nh][kDecTokChunk]
-  const int nt8 = (a.T + kDecTokChunk - 1) / kDecTokChunk * kDecTokChunk;
+  const int hparts = int(gridDim.x) / a.eparts, hp = int(blockIdx.x) / a.eparts, tid = threadIdx.x;
+  if (hp >= hparts) return;
+  const int Es = a.Er / a.eparts, e0 = (int(blockIdx.x) % a.eparts) * Es;
+  const int h0 = int(int64_t(a.H) * hp / hparts), nh = int(int64_t(a.H) * (hp + 1) / hparts) - h0;
+  float* red = reinterpret_cast<float*>(stage);                       // [groups][cpar][8][Es]
+  float* xs = red + kDecThreads * 2 * kDecTokChunk;                   // [chunk][nh][8]
+  const int chunks = (a.T + kDecTokChunk - 1) / kDecTokChunk;
 #pragma unroll 1
-  for (int i = tid; i < nt8 * nh; i += kDecThreads) {
+  for (int i = tid; i < chunks * kDecTokChunk * nh; i += kDecThreads) {
     const int t = i / nh, h = i - t * nh;
     xs[((t / kDecTokChunk) * nh + h) * kDecTokChunk + t % kDecTokChunk] =
         t < a.T ? __bfloat162float(a.x[int64_t(t) * a.H + h0 + h]) : 0.f;
   }
   __syncthreads();
-  const int P = a.Er / 2;
-  const int groups = P < kDecThreads ? kDecThreads / P : 1;
-  const int grp = tid / P;
+  const int P = Es / 2, rest = tid / P;
+  const bool wide = P >= kDecThreads;  // more experts than threads: rounds over them instead
+  const int cpar = wide ? 1 : min(chunks, kDecThreads / P);
+  const int groups = wide ? 1 : kDecThreads / (P * cpar);
+  const int cc = wide ? 0 : rest % cpar, grp = wide ? 0 : rest / cpar;
 #pragma unroll 1
-  for (int t0 = 0; t0 < a.T; t0 += kDecTokChunk) {
-    const int nt = min(kDecTokChunk, a.T - t0);
+  for (int cb = 0; cb < chunks; cb += cpar) {
+    const int ch = cb + cc;
 #pragma unroll 1
-    for (int p0 = 0; p0 < P; p0 += kDecThreads) {  // more than one round only for Er > 2 * kDecThreads
-      const int p = P < kDecThreads ? tid - grp * P : p0 + tid;
-      const bool on = P < kDecThreads ? grp < groups : p < P;
+    for (int p0 = 0; p0 < P; p0 += kDecThreads) {
+      const int p = wide ? p0 + tid : tid - rest * P;
+      const bool on = ch < chunks && (wide ? p < P : grp < groups);
       float2 s[kDecTokChunk];
 #pragma unroll
       for (int j = 0; j < kDecTokChunk; ++j) s[j] = make_float2(0.f, 0.f);
       if (on) {
-        const __nv_bfloat162* r = reinterpret_cast<const __nv_bfloat162*>(a.router_w + int64_t(h0) * a.Er) + p;
+        const __nv_bfloat162* r =
+            reinterpret_cast<const __nv_bfloat162*>(a.router_w + int64_t(h0) * a.Er + e0) + p;
+        const int P0 = a.Er / 2;
         // Eight rows' loads in flight; rows past the slice count as zeros.
 #pragma unroll 1
-        for (int hb = P < kDecThreads ? grp : 0; hb < nh; hb += 8 * groups) {
+        for (int hb = grp; hb < nh; hb += 8 * groups) {
           __nv_bfloat162 w8[8];
 #pragma unroll
           for (int i = 0; i < 8; ++i) {
             const int h = hb + i * groups;
-            w8[i] = h < nh ? r[int64_t(h) * P] : __nv_bfloat162{};
+            w8[i] = h < nh ? r[int64_t(h) * P0] : __nv_bfloat162{};
           }
 #pragma unroll
           for (int i = 0; i < 8; ++i) {
-            const int h = min(hb + i * groups, nh - 1);
+            const int h = hb + i * groups;
+            if (h >= nh) break;
             const float2 w = __bfloat1622float2(w8[i]);
-            const float4* xv = reinterpret_cast<const float4*>(xs + t0 * nh + h * kDecTokChunk);
+            const float4* xv = reinterpret_cast<const float4*>(xs + (ch * nh + h) * kDecTokChunk);
             float xr[kDecTokChunk];
 #pragma unroll
             for (int j = 0; j < kDecTokChunk; j += 4) *reinterpret_cast<float4*>(&xr[j]) = xv[j / 4];
-            const bool live = hb + i * groups < nh;
 #pragma unroll
             for (int j = 0; j < kDecTokChunk; ++j) {
-              s[j].x = live ? fmaf(xr[j], w.x, s[j].x) : s[j].x;
-              s[j].y = live ? fmaf(xr[j], w.y, s[j].y) : s[j].y;
+              s[j].x = fmaf(xr[j], w.x, s[j].x);
+              s[j].y = fmaf(xr[j], w.y, s[j].y);
             }
           }
         }
@@ -296,50 +304,63 @@ __device__ void dec_router_partial(const DecArgs& a, unsigned char* stage) {
         if (on) {
 #pragma unroll
           for (int j = 0; j < kDecTokChunk; ++j)
-            *reinterpret_cast<float2*>(&red[(grp * kDecTokChunk + j) * a.Er + 2 * p]) = s[j];
+            *reinterpret_cast<float2*>(&red[((grp * cpar + cc) * kDecTokChunk + j) * Es + 2 * p]) = s[j];
         }
         __syncthreads();
 #pragma unroll 1
-        for (int i = tid; i < nt * a.Er; i += kDecThreads) {
-          const int j = i / a.Er, e = i - j * a.Er;
+        for (int i = tid; i < cpar * kDecTokChunk * Es; i += kDecThreads) {
+          const int j = i / Es, t = cb * kDecTokChunk + j, e = i - j * Es;
+          if (t >= a.T) break;
           float v = 0.f;
-#pragma unroll 2
-          for (int g = 0; g < groups; ++g) v += red[(g * kDecTokChunk + j) * a.Er + e];
-          a.lpart[(int64_t(c) * a.T + t0 + j) * a.Er + e] = v;
+#pragma unroll 4
+          for (int g = 0; g < groups; ++g) v += red[(g * cpar * kDecTokChunk + j) * Es + e];
+          a.lpart[(int64_t(hp) * a.T + t) * a.Er + e0 + e] = v;
         }
         __syncthreads();
       } else if (on) {
-#pragma unroll 1
-        for (int j = 0; j < nt; ++j)
-          *reinterpret_cast<float2*>(&a.lpart[(int64_t(c) * a.T + t0 + j) * a.Er + 2 * p]) = s[j];
+#pragma unroll
+        for (int j = 0; j < kDecTokChunk; ++j) {
+          const int t = ch * kDecTokChunk + j;
+          if (t < a.T) *reinterpret_cast<float2*>(&a.lpart[(int64_t(hp) * a.T + t) * a.Er + e0 + 2 * p]) = s[j];
+        }
       }
     }
   }
 }
 
-// Router, step 2: tokens c, c + grid, ...: the slices' sum in CTA order, the
+// Router, step 2: tokens t0, t0 + stride, ...: the slices' sum in order, the
 // softmax over Er in fp32 and the K largest (equal logits: lowest id first).
 // An expert's place is the number of experts before it, counted by one
-// thread per expert: one pass over Er keys instead of K rounds.
-__device__ void dec_router_topk(const DecArgs& a, unsigned char* stage, unsigned char* scratch) {
-  const int G = gridDim.x, tid = threadIdx.x, lane = tid & 31;
+// thread per expert: one pass over Er keys instead of K rounds.  The last
+// token's routing also stays in `keep`.
+struct DecRouted {
+  long long id[kMaxRouteK];
+  float val[kMaxRouteK];
+};
+__device__ void dec_router_topk(const DecArgs& a, unsigned char* stage, unsigned char* scratch, int t0, int stride,
+                                bool store, DecRouted& keep) {
+  const int hparts = int(gridDim.x) / a.eparts, tid = threadIdx.x, lane = tid & 31;
   float* red = reinterpret_cast<float*>(stage);              // [parts][Er]
   float* lg = reinterpret_cast<float*>(scratch);             // [Er]
   uint32_t* key = reinterpret_cast<uint32_t*>(lg + a.Er);    // [Er]
   __shared__ int chosen[kMaxRouteK];
-  const int parts = a.Er < kDecThreads ? kDecThreads / a.Er : 1;
+  const int E4 = a.Er / 4;  // four experts per load
+  const int parts = kDecThreads / E4;
+  float4* red4 = reinterpret_cast<float4*>(red);
 #pragma unroll 1
-  for (int t = blockIdx.x; t < a.T; t += G) {
-#pragma unroll 1
-    for (int i = tid; i < parts * a.Er; i += kDecThreads) {
-      const int q = i / a.Er, e = i - q * a.Er;
-      red[i] = sum_parts<float>(G * q / parts, G * (q + 1) / parts - 1,
-                                [&](int c) { return &a.lpart[(int64_t(c) * a.T + t) * a.Er + e]; });
+  for (int t = t0; t < a.T; t += stride) {
+    if (tid < parts * E4) {
+      const int q = tid / E4, e = tid - q * E4;
+      const float4* at = reinterpret_cast<const float4*>(a.lpart + int64_t(t) * a.Er) + e;
+      const int64_t step = int64_t(a.T) * E4;
+      red4[tid] = sum_parts<float4>(hparts * q / parts, hparts * (q + 1) / parts - 1,
+                                    [&](int c) { return at + c * step; });
     }
     __syncthreads();
 #pragma unroll 1
     for (int e = tid; e < a.Er; e += kDecThreads) {
       float v = 0.f;
+#pragma unroll 4
       for (int q = 0; q < parts; ++q) v += red[q * a.Er + e];
       lg[e] = v;
       // The logit's bits as an unsigned number of the same order (-0 and 0
@@ -351,9 +372,14 @@ __device__ void dec_router_topk(const DecArgs& a, unsigned char* stage, unsigned
 #pragma unroll 1
     for (int e = tid; e < a.Er; e += kDecThreads) {
       const uint32_t mine = key[e];
+      const uint4* keys = reinterpret_cast<const uint4*>(key);
       int before = 0;
-#pragma unroll 8
-      for (int i = 0; i < a.Er; ++i) before += key[i] > mine || (key[i] == mine && i < e);
+#pragma unroll 4
+      for (int i = 0; i < E4; ++i) {  // a key before mine, or the same one at a lower id
+        const uint4 k = keys[i];
+        before += int(k.x >= mine + (4 * i >= e)) + int(k.y >= mine + (4 * i + 1 >= e)) +
+                  int(k.z >= mine + (4 * i + 2 >= e)) + int(k.w >= mine + (4 * i + 3 >= e));
+      }
       if (before < a.K) chosen[before] = e;
     }
     __syncthreads();
@@ -375,9 +401,14 @@ __device__ void dec_router_topk(const DecArgs& a, unsigned char* stage, unsigned
       for (int o = 16; o > 0; o >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
       if (lane < a.K) {
         const int64_t o = int64_t(t) * a.K + lane;
-        a.out_vals[o] = a.renorm ? pr / sum : pr;
-        if (a.ids64) static_cast<long long*>(a.out_ids)[o] = id;
-        else static_cast<int*>(a.out_ids)[o] = id;
+        const float v = a.renorm ? pr / sum : pr;
+        keep.id[lane] = id;
+        keep.val[lane] = v;
+        if (store) {
+          a.out_vals[o] = v;
+          if (a.ids64) static_cast<long long*>(a.out_ids)[o] = id;
+          else static_cast<int*>(a.out_ids)[o] = id;
+        }
       }
     }
     __syncthreads();
@@ -495,19 +526,35 @@ __global__ void __launch_bounds__(kDecThreads, 1)
   // their first use by the first grid barrier.
   if (blockIdx.x == 0)
     for (int i = threadIdx.x; i < int(gridDim.x); i += kDecThreads) a.ctr[i] = 0;
+
+  // (The block meets in each of the following steps before anything of the
+  // above is used.)
+  const void* ids = a.ids;
+  const void* vals = a.vals;
+  int ids64 = a.ids64;
+  if (a.router_w != nullptr) {
+    __shared__ DecRouted routed;
+    dec_router_partial(a, stage);
+    grid.sync();
+    // One token: every CTA finds its experts for itself, which costs less
+    // than handing them round through another barrier.
+    const bool alone = a.T == 1;
+    dec_router_topk(a, stage, scratch, alone ? 0 : blockIdx.x, alone ? 1 : int(gridDim.x), !alone || blockIdx.x == 0,
+                    routed);
+    fence_proxy_async_smem();  // the stages, written by threads so far, belong to the TMA from here
+    if (alone) {
+      ids = routed.id;
+      vals = routed.val;
+      ids64 = 1;
+    } else {
+      grid.sync();
+    }
+  }
+  dec_build(a, sm, tb, scratch, ids, ids64, vals, a.vals_bf16);
   tc_fence_before();
   __syncthreads();
   tc_fence_after();
   const uint32_t tmem = sm.tmem_base;
-
-  if (a.router_w != nullptr) {
-    dec_router_partial(a, stage);
-    grid.sync();
-    dec_router_topk(a, stage, scratch);
-    fence_proxy_async_smem();  // the stages, written by threads so far, belong to the TMA from here
-    grid.sync();
-  }
-  dec_build(a, sm, tb, scratch, a.ids, a.vals, a.vals_bf16);
   const int nact = sm.nact;
   const int G = gridDim.x;
 
@@ -704,12 +751,8 @@ __global__ void __launch_bounds__(kDecThreads, 1)
       if (!whole) {
         // The CTA whose ticket is the tile's last adds the parts up.
         const int c0 = share_owner(p.units, p.g, tile0), c1 = share_owner(p.units, p.g, tile0 + p.kb - 1);
-        __threadfence();
         named_bar_sync(kBarEpi, kDecEpiWarps * 32);
-        if (etid == 0) {
-          sm.last = atomicAdd(&a.ctr[c0], 1u) == uint32_t(c1 - c0);
-          __threadfence();
-        }
+        if (etid == 0) sm.last = atom_add_acq_rel(&a.ctr[c0], 1u) == uint32_t(c1 - c0);
         named_bar_sync(kBarEpi, kDecEpiWarps * 32);
         if (sm.last && f < a.F) {
 #pragma unroll 1
@@ -769,22 +812,39 @@ __global__ void __launch_bounds__(kDecThreads, 1)
     }
   };
 
-  // y of the tiles that several CTAs hold parts of: four features a thread.
+  // y of the tiles that several CTAs hold parts of: four features per four
+  // threads, each of which adds a quarter of the parts.
   auto join2 = [&](const Pass& p) {
-    const int per = a.T * 64;
+    const int per = a.T * 64, total = p.nt * per;
 #pragma unroll 1
-    for (int i = int(blockIdx.x) * kDecThreads + int(threadIdx.x); i < p.nt * per; i += G * kDecThreads) {
+    for (int i0 = (int(blockIdx.x) * kDecThreads + int(threadIdx.x & ~31u)) >> 2; i0 < total;
+         i0 += (G * kDecThreads) >> 2) {
+      const int i = i0 + (lane >> 2), qt = lane & 3;
       const int tile = i / per, r = i - tile * per;
       const int t = r >> 6, fl = (r & 63) * 4, f = tile * 256 + fl;
       const int u0 = tile * p.tile;
-      const int c0 = share_owner(p.units, p.g, u0), c1 = share_owner(p.units, p.g, u0 + p.tile - 1);
-      if (c0 == c1 || f >= a.H) continue;
-      const float4 v = sum_parts<float4>(c0, c1, [&](int q) {
+      int c0 = 0, c1 = 0;
+      if (i < total) {
+        c0 = share_owner(p.units, p.g, u0);
+        c1 = share_owner(p.units, p.g, u0 + p.tile - 1);
+      }
+      const bool split = c0 != c1;
+      const int n = split ? c1 - c0 + 1 : 0;
+      float4 v = sum_parts<float4>(c0 + n * qt / 4, c0 + n * (qt + 1) / 4 - 1, [&](int q) {
         return reinterpret_cast<const float4*>(slot(q, q == c0 ? 1 : 0) + t * 256 + fl);
       });
-      __nv_bfloat162* o = reinterpret_cast<__nv_bfloat162*>(a.y + size_t(t) * a.H + f);
-      o[0] = __floats2bfloat162_rn(v.x, v.y);
-      o[1] = __floats2bfloat162_rn(v.z, v.w);
+#pragma unroll
+      for (int o = 1; o < 4; o <<= 1) {
+        v.x += __shfl_xor_sync(0xffffffffu, v.x, o);
+        v.y += __shfl_xor_sync(0xffffffffu, v.y, o);
+        v.z += __shfl_xor_sync(0xffffffffu, v.z, o);
+        v.w += __shfl_xor_sync(0xffffffffu, v.w, o);
+      }
+      if (split && f < a.H && qt == 0) {
+        __nv_bfloat162* o = reinterpret_cast<__nv_bfloat162*>(a.y + size_t(t) * a.H + f);
+        o[0] = __floats2bfloat162_rn(v.x, v.y);
+        o[1] = __floats2bfloat162_rn(v.z, v.w);
+      }
     }
   };
 
@@ -874,7 +934,7 @@ DecScratch dec_scratch(int T, int K, int F, int Er, int sms) {
 bool dec_sizes_ok(int64_t T, int32_t H, int32_t F, int32_t E, int32_t K, int32_t Er) {
   if (T < 0 || T > kDecMaxT || K < 1 || K > kMaxRouteK || T * K > kDecMaxRows) return false;
   if (H <= 0 || H % 8 || H > kDecMaxH || F <= 0 || F % 8 || E < 1 || E > kMaxExperts) return false;
-  if (Er < 0 || Er > kMaxExperts || Er % 2 || (Er > 0 && K > Er)) return false;
+  if (Er < 0 || Er > kMaxExperts || Er % 4 || (Er > 0 && K > Er)) return false;
   // Unit counts times CTAs stay within 32 bits (2^24 units are 512 GB).
   const int64_t act = E < T * K ? E : T * K;
   const int64_t u1 = act * ((F + 127) / 128) * ((H + 63) / 64), u2 = act * ((H + 255) / 256) * ((F + 63) / 64);
@@ -901,7 +961,7 @@ extern "C" int moe_decode_layer(const moe_decode_params* p, void* stream) {
   if (!p) return kBadArg;
   const int Er = p->router_w ? p->router_experts : 0;
   if (!dec_sizes_ok(p->T, p->hidden, p->ffn, p->experts, p->K, Er)) return kBadArg;
-  if (p->router_w && Er < 2) return kBadArg;
+  if (p->router_w && Er < 4) return kBadArg;
   if (p->T == 0) return kOk;
   if (!p->x || !p->w13 || !p->w2 || !p->y || !p->top_idxs || !p->top_vals || !p->scratch) return kBadArg;
   if (misaligned(p->x) || misaligned(p->w13) || misaligned(p->w2) || misaligned(p->scratch)) return kBadArg;
@@ -953,9 +1013,13 @@ extern "C" int moe_decode_layer(const moe_decode_params* p, void* stream) {
   a.stages = stages > kDecMaxStages ? kDecMaxStages : stages;
   if (a.stages < 2) return kBadArg;
   const uint32_t smem = fixed + uint32_t(a.stages) * a.stage_bytes;
-  // The router's slices use the stage memory.
-  if (Er && uint32_t(a.stages) * a.stage_bytes < kDecThreads * 2 * kDecTokChunk * 4 + uint32_t(T + kDecTokChunk - 1) * ((H + sms - 1) / sms + 1) * 4)
-    return kBadArg;
+  // The router's slices use the stage memory: tokens by H / (slices of H).
+  // Slices of a quarter of the experts leave fewer parts to add per logit,
+  // where a quarter is whole 16-byte pieces of a row and its rows fit.
+  const uint32_t room = uint32_t(a.stages) * a.stage_bytes - kDecThreads * 2 * kDecTokChunk * 4;
+  const uint32_t xrow = uint32_t(T + kDecTokChunk - 1) / kDecTokChunk * kDecTokChunk * 4;
+  a.eparts = Er % 32 == 0 && sms >= 8 && (H / (sms / 4) + 1) * xrow <= room ? 4 : 1;
+  if (Er && (H / (sms / a.eparts) + 1) * xrow > room) return kBadArg;
 
   CUtensorMap m13, m2, mx, mh;
   {

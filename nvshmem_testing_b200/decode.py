@@ -19,10 +19,12 @@ call may be captured into a CUDA graph.
 from __future__ import annotations
 
 import ctypes
+import functools
 
 import torch
 
 from . import _native as N
+from . import utils
 
 
 def _check(x, w13, w2, out, status):
@@ -53,32 +55,33 @@ def _check(x, w13, w2, out, status):
     return T, H, F, El
 
 
+@functools.lru_cache(maxsize=256)
+def _scratch_bytes(*sizes) -> int:
+    need = ctypes.c_size_t()
+    N.check(N.lib().moe_decode_scratch_bytes(*sizes, ctypes.byref(need)), "moe_decode_scratch_bytes")
+    return need.value
+
+
 def _launch(x, ids, vals, w13, w2, router_w, K, first_expert, renormalize, out, status, dims):
     T, H, F, El = dims
     if out is None:
         out = torch.empty((T, H), dtype=torch.bfloat16, device=x.device)
     if T == 0:
         return out
-    dev = x.device.index
     p = N.DecodeParams()
     p.T, p.hidden, p.ffn, p.experts, p.K, p.first_expert = T, H, F, El, K, first_expert
-    p.router_experts = 0 if router_w is None else router_w.shape[1]
-    p.renormalize = int(renormalize)
-    p.ids_are_int64 = int(ids.dtype == torch.int64)
-    p.vals_are_bf16 = int(vals.dtype == torch.bfloat16)
-    need = ctypes.c_size_t()
-    lib = N.lib()
-    N.check(lib.moe_decode_scratch_bytes(T, H, F, El, K, p.router_experts, dev, ctypes.byref(need)),
-            "moe_decode_scratch_bytes")
-    scratch = torch.empty(need.value, dtype=torch.uint8, device=x.device)
+    Er = 0 if router_w is None else router_w.shape[1]
+    p.router_experts, p.renormalize = Er, renormalize
+    p.ids_are_int64, p.vals_are_bf16 = ids.dtype == torch.int64, vals.dtype == torch.bfloat16
+    need = _scratch_bytes(T, H, F, El, K, Er, x.device.index)
+    scratch = torch.empty(need, dtype=torch.uint8, device=x.device)
     p.x, p.w13, p.w2, p.y = x.data_ptr(), w13.data_ptr(), w2.data_ptr(), out.data_ptr()
     p.router_w = None if router_w is None else router_w.data_ptr()
     p.top_idxs, p.top_vals = ids.data_ptr(), vals.data_ptr()
-    p.scratch, p.scratch_bytes = scratch.data_ptr(), need.value
+    p.scratch, p.scratch_bytes = scratch.data_ptr(), need
     p.status_host = None if status is None else status.data_ptr()
-    stream = torch.cuda.current_stream(x.device)
-    with torch.cuda.device(x.device):
-        N.check(lib.moe_decode_layer(ctypes.byref(p), ctypes.c_void_p(stream.cuda_stream)), "moe_decode_layer")
+    with utils.on_device(x.device) as stream:
+        N.check(N.lib().moe_decode_layer(ctypes.byref(p), stream), "moe_decode_layer")
     return out
 
 
@@ -139,8 +142,8 @@ def routed_layer(x: torch.Tensor, router_w: torch.Tensor, topk: int, w13: torch.
     if ids_dtype not in (torch.int32, torch.int64):
         raise TypeError("ids_dtype must be int32 or int64")
     E = router_w.shape[1]
-    if E % 2 or not 2 <= E <= 1024:
-        raise ValueError(f"{E} experts: an even number of 1024 at most")
+    if E % 4 or not 4 <= E <= 1024:
+        raise ValueError(f"{E} experts: a multiple of 4, 1024 at most")
     if not 1 <= topk <= min(32, E) or T * topk > N.DECODE_MAX_ROWS:
         raise ValueError(f"{T} tokens with {topk} of {E} experts each: 1 to 32, {N.DECODE_MAX_ROWS} in all at most")
     vals = torch.empty((T, topk), dtype=torch.float32, device=x.device)

@@ -38,6 +38,24 @@ def _stream_ptr(dev: torch.device) -> ctypes.c_void_p:
     return ctypes.c_void_p(torch.cuda.current_stream(dev).cuda_stream)
 
 
+class on_device:
+    """``with on_device(dev) as stream``: dev is the current device inside, and
+    ``stream`` its current stream (a launch belongs to both)."""
+
+    def __init__(self, dev: torch.device):
+        self.dev = dev
+
+    def __enter__(self) -> ctypes.c_void_p:
+        self.back = torch.cuda.current_device()
+        if self.back != self.dev.index:
+            torch.cuda.set_device(self.dev.index)
+        return _stream_ptr(self.dev)
+
+    def __exit__(self, *exc):
+        if self.back != self.dev.index:
+            torch.cuda.set_device(self.back)
+
+
 def route(top_idxs: torch.Tensor, num_experts: int, with_slots: bool = False) -> Routing:
     """Per-expert counts, offsets and stable token permutation (no host sync).
 

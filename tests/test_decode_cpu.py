@@ -53,7 +53,7 @@ def test_c_entry_refuses_before_any_device_call():
     assert scratch(64, 64, 64, 64, 17, 0, 0) == N.BAD_ARG  # 1088 rows
     assert scratch(4, 64, 64, 4, 33, 0, 0) == N.BAD_ARG
     assert scratch(4, 64, 64, 4, 3, 2, 0) == N.BAD_ARG     # K > router experts
-    assert scratch(4, 64, 64, 4, 1, 7, 0) == N.BAD_ARG     # odd router experts
+    assert scratch(4, 64, 64, 4, 1, 6, 0) == N.BAD_ARG     # router experts not a multiple of 4
     p = N.DecodeParams()
     p.T, p.hidden, p.ffn, p.experts, p.K = 4, 64, 64, 4, 2
     assert lib.moe_decode_layer(ctypes.byref(p), None) == N.BAD_ARG  # null pointers

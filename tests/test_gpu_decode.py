@@ -205,10 +205,10 @@ def test_several_streams_at_once():
 
 ROUTED = [
     # T, H, E, K, F
-    (1, 64, 2, 1, 64),
+    (1, 64, 4, 1, 64),
     (1, 2048, 64, 6, 128),
     (2, 7168, 256, 8, 64),
-    (5, 136, 10, 3, 72),
+    (5, 136, 12, 3, 72),
     (13, 520, 104, 5, 64),
     (40, 256, 1024, 4, 16),
     (64, 1000, 128, 8, 64),
