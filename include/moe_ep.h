@@ -30,6 +30,9 @@
  *   moe_decode_layer            the whole gated layer for a few tokens, its
  *                               router included (utils.py:17-25, 28-75,
  *                               baseline.py:18-50 in one kernel)
+ *   moe_quant_rows,             the expert products in 8-bit integers, beside
+ *   moe_w8a8_gemm,              baseline.py:50's bf16 ones, and the top-k sum
+ *   moe_weighted_sum            of their rows
  *   moe_pack_compact,           the general (unbalanced) all-to-all that
  *   moe_ep_run_compact          alltoall_persistent_gemm.py:221-222 and
  *                               baseline.py:15-16 leave as stubs: unpadded
@@ -413,6 +416,59 @@ typedef struct moe_decode_params {
 int moe_decode_scratch_bytes(int64_t T, int32_t hidden, int32_t ffn, int32_t experts, int32_t K,
                              int32_t router_experts, int32_t device, size_t* out);
 int moe_decode_layer(const moe_decode_params* params, void* stream);
+
+/* ---------------------------------------------------------------- 8-bit products
+ * Rows quantised with one scale each:
+ *   scale[r] = max |x[src(r), :]| / 127 in fp32,
+ *   q[r, i]  = x[src(r), i] / scale[r], the exact quotient rounded half to
+ *              even and held to [-127, 127],
+ * src(r) = perm[r] (the dispatch order of moe_route), or r without perm.
+ * A row of zeros has scale 0 and zeros; a row with an infinity or a NaN has a
+ * NaN scale and zeros, so that its products are NaN.  x is bf16 or
+ * (x_is_f32) fp32, 16-byte aligned, K % 8 == 0.  live_rows (device, optional):
+ * rows from *live_rows on are left as they were. */
+int moe_quant_rows(const void* x, int32_t x_is_f32, int64_t rows, int32_t K, const int32_t* perm,
+                   const int32_t* live_rows, void* q, float* scale, void* stream);
+
+/* One product per expert over rows in expert order:
+ *   out[r, n] = xs[r] * ws[e, n] * sum_k xq[r, k] * wq[e, n, k]
+ * for the counts[e] rows of expert e, with exact integer sums; bf16, or fp32
+ * with out_is_f32.  With swiglu the N channels are gate [0, N/2) and up
+ * [N/2, N), and out [rows, N/2] = silu(gate) * up in fp32 arithmetic.  Rows
+ * behind the sum of the counts are left as they were; counts beyond `rows`
+ * are cut.  counts == NULL: one expert for all rows.
+ * Requires K % 16 == 0, K <= 131056, N % 8 == 0 (16 with swiglu), experts <=
+ * 1024; xq, wq and scratch 16-byte aligned.  scratch:
+ * moe_w8a8_scratch_bytes of device memory (may be 0), not initialised, for
+ * this call alone until it has finished. */
+typedef struct moe_w8a8_params {
+  int64_t rows;
+  int32_t K, N, experts;
+  int32_t swiglu, out_is_f32;
+  int32_t reserved;
+  const void* xq;          /* [rows, K] int8             */
+  const float* xs;         /* [rows]                     */
+  const void* wq;          /* [experts, N, K] int8       */
+  const float* ws;         /* [experts, N]               */
+  const int32_t* counts;   /* [experts] device, or NULL  */
+  void* out;               /* [rows, N] or [rows, N/2]   */
+  void* scratch;
+  size_t scratch_bytes;
+  int32_t* status_host;    /* optional mapped pinned word for device errors */
+} moe_w8a8_params;
+
+int moe_w8a8_scratch_bytes(int64_t rows, int32_t K, int32_t N, int32_t experts, int32_t swiglu, int32_t device,
+                           size_t* out);
+int moe_w8a8_gemm(const moe_w8a8_params* params, void* stream);
+
+/* y[t, :] = sum over k of top_vals[t, k] * rows[offsets[e] + slots[t, k], :],
+ * e = top_idxs[t, k] - first_expert, in fp32 in the order of k, bf16 out; ids
+ * outside [0, experts) after the subtraction and slots of -1 (moe_route_slots)
+ * are skipped.  rows [offsets[experts], H] bf16, H % 8 == 0, rows and y
+ * 16-byte aligned. */
+int moe_weighted_sum(const void* rows, const void* top_idxs, int32_t ids_are_int64, int32_t first_expert,
+                     const void* top_vals, int32_t vals_are_bf16, const int32_t* slots, const int32_t* offsets,
+                     int64_t T, int32_t K, int32_t H, int32_t experts, void* y, void* stream);
 
 /* Copy the workspace status word to the host (synchronous). */
 int moe_ep_read_status(uint64_t local_base, const moe_ep_layout* layout, uint32_t* out);

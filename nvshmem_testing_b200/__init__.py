@@ -13,6 +13,8 @@ CPU fallback):
 * ``mlp`` — the full gated expert MLP behind the exchange;
 * ``decode`` — the whole gated layer for a few tokens in one kernel, the
   router included;
+* ``w8a8`` — expert products in 8-bit integers: quantisation with a scale per
+  row and per channel, the grouped product, the gated layer;
 * ``symm`` — the cuMem symmetric workspaces; ``workloads`` — seeded inputs;
 * ``build`` — compiles the library in-tree.
 """

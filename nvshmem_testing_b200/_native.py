@@ -26,7 +26,8 @@ EXPORTED = ["moe_ep_abi_version", "moe_ep_status_string", "moe_ep_num_sms", "moe
             "moe_symm_alloc", "moe_symm_import", "moe_symm_free", "moe_ep_workspace_layout", "moe_ep_workspace_reset", "moe_ep_run",
             "moe_ep_read_status", "moe_ep_run_noalloc", "moe_route_slots", "moe_ep_workspace_layout_ret",
             "moe_ep_run_combine", "moe_pack_compact", "moe_ep_run_compact", "moe_router", "moe_swiglu",
-            "moe_ep_run_compact_swiglu", "moe_publish_i32", "moe_decode_scratch_bytes", "moe_decode_layer"]
+            "moe_ep_run_compact_swiglu", "moe_publish_i32", "moe_decode_scratch_bytes", "moe_decode_layer",
+            "moe_quant_rows", "moe_w8a8_scratch_bytes", "moe_w8a8_gemm", "moe_weighted_sum"]
 
 
 class MoeEpError(RuntimeError):
@@ -73,6 +74,14 @@ class DecodeParams(ctypes.Structure):
                 ("router_w", ctypes.c_void_p), ("top_idxs", ctypes.c_void_p), ("top_vals", ctypes.c_void_p),
                 ("y", ctypes.c_void_p), ("scratch", ctypes.c_void_p), ("scratch_bytes", ctypes.c_size_t),
                 ("status_host", ctypes.c_void_p)]
+
+
+class W8A8Params(ctypes.Structure):
+    _fields_ = [("rows", ctypes.c_int64), ("K", ctypes.c_int32), ("N", ctypes.c_int32), ("experts", ctypes.c_int32),
+                ("swiglu", ctypes.c_int32), ("out_is_f32", ctypes.c_int32), ("reserved", ctypes.c_int32),
+                ("xq", ctypes.c_void_p), ("xs", ctypes.c_void_p), ("wq", ctypes.c_void_p), ("ws", ctypes.c_void_p),
+                ("counts", ctypes.c_void_p), ("out", ctypes.c_void_p), ("scratch", ctypes.c_void_p),
+                ("scratch_bytes", ctypes.c_size_t), ("status_host", ctypes.c_void_p)]
 
 
 DECODE_MAX_TOKENS = 64
@@ -124,6 +133,12 @@ def lib() -> ctypes.CDLL:
                              ctypes.c_int32, c_vp, c_vp, c_vp]
     L.moe_ep_read_status.argtypes = [c_u64, P(Layout), P(ctypes.c_uint32)]
     L.moe_publish_i32.argtypes = [c_vp, c_i64, c_vp, c_vp]
+    c_i32 = ctypes.c_int32
+    L.moe_quant_rows.argtypes = [c_vp, c_i32, c_i64, c_i32, c_vp, c_vp, c_vp, c_vp, c_vp]
+    L.moe_w8a8_scratch_bytes.argtypes = [c_i64] + [c_i32] * 5 + [P(c_sz)]
+    L.moe_w8a8_gemm.argtypes = [P(W8A8Params), c_vp]
+    L.moe_weighted_sum.argtypes = [c_vp, c_vp, c_i32, c_i32, c_vp, c_i32, c_vp, c_vp, c_i64, c_i32, c_i32, c_i32, c_vp,
+                                   c_vp]
     L.moe_decode_scratch_bytes.argtypes = [c_i64] + [ctypes.c_int32] * 6 + [P(c_sz)]
     L.moe_decode_layer.argtypes = [P(DecodeParams), c_vp]
     for name in EXPORTED:

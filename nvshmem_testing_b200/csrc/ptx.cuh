@@ -204,6 +204,16 @@ __device__ __forceinline__ void tc_mma_f16_pair(uint32_t d_tmem, uint64_t a_desc
       "l"(a_desc), "l"(b_desc), "r"(idesc), "r"(accumulate)
       : "memory");
 }
+// The same for signed 8-bit operands and 32-bit integer sums (kind::i8, K = 32).
+__device__ __forceinline__ void tc_mma_i8_pair(uint32_t d_tmem, uint64_t a_desc, uint64_t b_desc, uint32_t idesc,
+                                               uint32_t accumulate) {
+  asm volatile(
+      "{\n\t.reg .pred p;\n\t"
+      "setp.ne.b32 p, %4, 0;\n\t"
+      "tcgen05.mma.cta_group::2.kind::i8 [%0], %1, %2, %3, p;\n\t}" ::"r"(d_tmem),
+      "l"(a_desc), "l"(b_desc), "r"(idesc), "r"(accumulate)
+      : "memory");
+}
 // Arrive on the barrier at the same offset in every CTA of `mask` once the
 // issuing thread's prior pair MMAs complete.
 __device__ __forceinline__ void tc_commit_pair_mc(uint64_t* bar, uint16_t mask) {
@@ -310,6 +320,12 @@ __host__ __device__ constexpr uint32_t make_idesc_mn(uint32_t ab_fmt, uint32_t m
                                                      uint32_t b_mn_major) {
   return (1u << 4) | (ab_fmt << 7) | (ab_fmt << 10) | (a_mn_major << 15) | (b_mn_major << 16) | ((n >> 3) << 17) |
          ((m >> 4) << 24);
+}
+
+// Instruction descriptor for kind::i8: s8 x s8 -> s32 (wrapping), both
+// operands K-major.
+__host__ __device__ constexpr uint32_t make_idesc_i8(uint32_t m, uint32_t n) {
+  return (2u << 4) | (1u << 7) | (1u << 10) | ((n >> 3) << 17) | ((m >> 4) << 24);
 }
 
 // Instruction descriptor for kind::f16 / kind::tf32 with f32 accumulation.

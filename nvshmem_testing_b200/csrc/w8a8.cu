@@ -1,0 +1,830 @@
+// The expert layer in 8-bit integers (the reference's products are bf16 only,
+// baseline.py:50): rows quantised with a scale each, weights with a scale per
+// output channel,
+//   out[r, n] = xs[r] * ws[e, n] * sum_k xq[r, k] * wq[e, n, k],
+// rows in expert order, one weight matrix per expert.
+//
+// Products (w8a8_kernel).  Transposed like the bf16 layer: channels are the
+// MMA's M, token rows its N, so an expert's ragged row count costs at most 31
+// padded rows, not a 256-row tile.  CTA pairs, tcgen05.mma.cta_group::2
+// kind::i8 (M = 256, N <= 256, K = 32) with exact 32-bit sums in TMEM; both
+// operands are K-major, 128 bytes of K per stage (one swizzle atom), six
+// stages of 32 KB per CTA.  The scales are applied to the sums on the way out.
+// With SwiGLU a CTA's 128 channels are 64 gate and the 64 matching up
+// channels (two boxes of the same matrix, no relayout); the halves sit in
+// different TMEM lanes and are exchanged through shared memory, and
+// silu(gate) * up is written in fp32 for the quantisation that follows.
+//
+// Few tiles (small row counts) leave most SMs without one, although such
+// products wait for the weights' bytes alone.  Then the list of (tile, 128 of
+// K) units is split evenly over the pairs at any k, the partial sums go to
+// scratch and, behind a grid barrier, are added and scaled.  Integer sums do
+// not depend on the split.
+//
+// Quantisation (quant_rows_kernel).  scale = absmax / 127 in fp32, q = the
+// exact quotient x / scale rounded half to even: the product with the
+// reciprocal is corrected by its remainder, which fp32 holds exactly.  One
+// read of the row, kept in registers between maximum and rounding.
+#include <cooperative_groups.h>
+#include <cuda_bf16.h>
+#include <cuda_runtime.h>
+
+#include <algorithm>
+
+#include "moe_ep.h"
+#include "moe_ep_internal.h"
+#include "ptx.cuh"
+
+namespace moe {
+namespace {
+
+namespace cg = cooperative_groups;
+
+constexpr int kQStages = 6;
+constexpr int kQKb = 128;                          // K per stage
+constexpr uint32_t kQABytes = 128 * kQKb;          // 128 channels
+constexpr uint32_t kQStageBytes = 2 * kQABytes;    // + up to 128 rows
+constexpr int kQTileRows = 256;
+constexpr int kQEpiWarps = 8;                      // two per TMEM lane quarter
+constexpr int kQEpi0 = 2;
+constexpr int kQThreads = (kQEpi0 + kQEpiWarps) * 32;
+constexpr uint32_t kQXBytes = kQEpiWarps * 16 * 32 * 4;  // SwiGLU exchange
+constexpr int kQRowMaps = 4;                       // boxes of 16, 32, 64, 128 rows
+constexpr uint64_t kQBoundNs = 2000000000ull;      // bug guard on every pipeline wait
+constexpr int kQMaxK = 131056;                     // 128 * 128 * K < 2^31
+constexpr size_t kQSlotInts = 2 * 128 * kQTileRows;  // one pair's sums of one tile
+
+struct QArgs {
+  int E, K, N;                 // N: channels, both halves with SwiGLU
+  int64_t rows;
+  int F;                       // output columns: N, or N / 2
+  const int32_t* counts;       // [E], or null: one matrix for all rows
+  const float* xs;
+  const float* ws;
+  void* out;
+  int out_f32;
+  int32_t* part;               // split form: [pairs][2] slots
+  int32_t* status_host;
+};
+
+struct QRowMaps {
+  CUtensorMap m[kQRowMaps];
+};
+
+struct alignas(16) QSmem {
+  uint64_t full[kQStages];   // leader: both CTAs' bytes
+  uint64_t empty[kQStages];  // each CTA: the stage has been multiplied
+  uint64_t tfull[2];         // each CTA: sums ready
+  uint64_t tempty[2];        // leader: both CTAs' epilogues are done with them
+  uint64_t drain;
+  uint32_t fills[kQStages], cons[kQStages];
+  uint32_t tmem_base;
+  int err;
+};
+
+__device__ __noinline__ bool q_wait_slow(uint64_t* bar, uint32_t parity, QSmem& sm, bool cluster) {
+  uint64_t deadline = 0;
+  for (uint32_t spin = 0;; ++spin) {
+    if (cluster ? mbar_try_wait_cluster(bar, parity) : mbar_try_wait(bar, parity)) return true;
+    if ((spin & 63) == 63) {
+      if (*reinterpret_cast<volatile int*>(&sm.err)) return false;
+      const uint64_t now = globaltimer_ns();
+      if (deadline == 0) deadline = now + kQBoundNs;
+      else if (now > deadline) return false;
+    }
+  }
+}
+__device__ __forceinline__ bool q_wait(uint64_t* bar, uint32_t parity, QSmem& sm) {
+  return mbar_try_wait(bar, parity) || q_wait_slow(bar, parity, sm, false);
+}
+
+// Stops both CTAs of the pair.
+__device__ __noinline__ void q_fail(QSmem& sm, const QArgs& a, int detail) {
+  if (atomicExch(&sm.err, 1) == 0) {
+    st_shared_cluster_u32(mapa_shared(smem_u32(&sm.err), cluster_ctarank() ^ 1u), 1u);
+    if (a.status_host)
+      *reinterpret_cast<volatile int32_t*>(a.status_host) = int32_t(status_word(kTimeout, kSitePipe, detail));
+  }
+}
+
+// Row offsets and row-tile prefix of the experts.
+struct QSched {
+  int* off;   // [E + 1]
+  int* tpre;  // [E + 1]
+  int E, FT, kb;
+};
+
+struct QTile {
+  int e, f, r0, rows, n;  // expert, channel tile, first row, rows, MMA N
+};
+
+__device__ __forceinline__ QTile q_tile(const QSched& s, int t) {
+  const int x = t / s.FT;
+  int lo = 0, hi = s.E;  // largest e with tpre[e] <= x
+  while (hi - lo > 1) {
+    const int mid = (lo + hi) >> 1;
+    if (s.tpre[mid] <= x) lo = mid;
+    else hi = mid;
+  }
+  QTile q;
+  q.e = lo;
+  const int nrt = s.tpre[lo + 1] - s.tpre[lo], local = t - s.tpre[lo] * s.FT;
+  q.f = local / nrt;
+  const int r = local - q.f * nrt, n = s.off[lo + 1] - s.off[lo];
+  const int tr = ((n + nrt - 1) / nrt + 31) / 32 * 32;  // rows per tile, even among an expert's tiles
+  q.r0 = s.off[lo] + r * tr;
+  q.rows = min(tr, n - r * tr);
+  q.n = (q.rows + 31) / 32 * 32;
+  return q;
+}
+
+// The runs over K that a pair does, in order: whole tiles t0, t0 + step, ...
+// or (split) the tiles of a contiguous share of units.
+template <bool SPLIT>
+struct QWalk {
+  int tile, step, tiles;  // whole tiles
+  int u, hi, kb;          // split
+  int k0, k1;             // current run
+  __device__ __forceinline__ QWalk(const QSched& s, int tiles_, int pair, int pairs) {
+    tiles = tiles_;
+    kb = s.kb;
+    k0 = 0;
+    k1 = kb;
+    if constexpr (SPLIT) {
+      const uint32_t units = uint32_t(tiles_) * uint32_t(kb);
+      const uint32_t g = min(uint32_t(pairs), units);
+      u = uint32_t(pair) < g ? int(uint64_t(units) * pair / g) : 0;
+      hi = uint32_t(pair) < g ? int(uint64_t(units) * (pair + 1) / g) : 0;
+      set();
+    } else {
+      tile = pair;
+      step = pairs;
+    }
+  }
+  __device__ __forceinline__ void set() {
+    tile = u / kb;
+    k0 = u - tile * kb;
+    k1 = min(kb, k0 + hi - u);
+  }
+  __device__ __forceinline__ bool more() const { return SPLIT ? u < hi : tile < tiles; }
+  __device__ __forceinline__ void next() {
+    if constexpr (SPLIT) {
+      u += k1 - k0;
+      set();
+    } else {
+      tile += step;
+    }
+  }
+  __device__ __forceinline__ bool whole() const { return !SPLIT || (k0 == 0 && k1 == kb); }
+};
+
+struct QRing {
+  int st;
+  uint32_t ph;
+  __device__ __forceinline__ void next(int n) {
+    if (++st == n) {
+      st = 0;
+      ph ^= 1;
+    }
+  }
+};
+
+__device__ __forceinline__ void q_store(const QArgs& a, int64_t row, int f, float v) {
+  const int64_t at = row * a.F + f;
+  if (a.out_f32) static_cast<float*>(a.out)[at] = v;
+  else static_cast<__nv_bfloat16*>(a.out)[at] = __float2bfloat16_rn(v);
+}
+
+__device__ __forceinline__ float silu_mul(float g, float u) { return g / (1.f + expf(-g)) * u; }
+
+template <bool GLU, bool SPLIT>
+__global__ void __launch_bounds__(kQThreads, 1)
+    w8a8_kernel(const __grid_constant__ CUtensorMap tm_w, const __grid_constant__ QRowMaps tm_x, const QArgs a) {
+  extern __shared__ unsigned char q_dyn[];
+  unsigned char* stage = reinterpret_cast<unsigned char*>((reinterpret_cast<uintptr_t>(q_dyn) + 1023) & ~uintptr_t(1023));
+  float* xbuf = reinterpret_cast<float*>(stage + kQStages * kQStageBytes);
+  QSmem& sm = *reinterpret_cast<QSmem*>(reinterpret_cast<unsigned char*>(xbuf) + kQXBytes);
+  QSched s;
+  s.off = reinterpret_cast<int*>(&sm + 1);
+  s.tpre = s.off + a.E + 1;
+  s.E = a.E;
+  s.FT = GLU ? (a.F + 127) / 128 : (a.N + 255) / 256;
+  s.kb = (a.K + kQKb - 1) / kQKb;
+
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const uint32_t crank = cluster_ctarank();
+  const bool leader = crank == 0;
+  const int pair = int(blockIdx.x >> 1), pairs = int(gridDim.x >> 1);
+
+  if (threadIdx.x == 0) {
+    for (int i = 0; i < kQStages; ++i) {
+      mbar_init(&sm.full[i], 1);
+      mbar_init(&sm.empty[i], 1);
+      sm.fills[i] = sm.cons[i] = 0;
+    }
+    for (int i = 0; i < 2; ++i) {
+      mbar_init(&sm.tfull[i], 1);
+      mbar_init(&sm.tempty[i], 2 * kQEpiWarps);
+    }
+    mbar_init(&sm.drain, 1);
+    sm.err = 0;
+    fence_mbar_init();
+    prefetch_tensormap(&tm_w);
+  }
+  // Offsets and tile prefix: counts that would pass the last row are cut.
+  if (warp == 2) {
+    int64_t off = 0;
+    int tp = 0;
+    for (int e0 = 0; e0 < a.E; e0 += 32) {
+      const int e = e0 + lane;
+      int64_t c = 0;
+      if (e < a.E) c = a.counts ? max(a.counts[e], 0) : a.rows;
+      int64_t pre = c;
+#pragma unroll
+      for (int o = 1; o < 32; o <<= 1) {
+        const int64_t v = __shfl_up_sync(0xffffffffu, pre, o);
+        if (lane >= o) pre += v;
+      }
+      const int64_t end = min(off + pre, a.rows), begin = min(off + pre - c, a.rows);
+      int nt = int((end - begin + kQTileRows - 1) / kQTileRows), tpre = nt;
+#pragma unroll
+      for (int o = 1; o < 32; o <<= 1) {
+        const int v = __shfl_up_sync(0xffffffffu, tpre, o);
+        if (lane >= o) tpre += v;
+      }
+      if (e < a.E) {
+        s.off[e] = int(begin);
+        s.tpre[e] = tp + tpre - nt;
+        if (e == a.E - 1) {
+          s.off[a.E] = int(end);
+          s.tpre[a.E] = tp + tpre;
+        }
+      }
+      off += __shfl_sync(0xffffffffu, pre, 31);
+      tp += __shfl_sync(0xffffffffu, tpre, 31);
+    }
+  }
+  cluster_sync();  // the peer's barriers exist before any remote arrive
+  if (warp == 1) {
+    __syncwarp();
+    tmem_alloc_pair(&sm.tmem_base, 512);
+    tmem_relinquish_pair();
+  }
+  tc_fence_before();
+  cluster_sync();
+  tc_fence_after();
+  const uint32_t tmem = sm.tmem_base;
+  const int tiles = s.tpre[a.E] * s.FT;
+
+  if (warp == 0 && lane == 0) {
+    // ---- loads: each CTA its 128 channels and half of the tile's rows, all
+    // onto the leader's barrier
+    QRing r = {0, 0};
+    const uint32_t bar0 = mapa_shared(smem_u32(&sm.full[0]), 0);
+    bool stop = false;
+    for (QWalk<SPLIT> w(s, tiles, pair, pairs); w.more() && !stop; w.next()) {
+      const QTile t = q_tile(s, w.tile);
+      const int half = t.n / 2, bm = half <= 16 ? 0 : half <= 32 ? 1 : half <= 64 ? 2 : 3;
+      const uint32_t tx = 2 * (kQABytes + (16u << bm) * kQKb);
+      const int row = t.r0 + int(crank) * half;
+      for (int k = w.k0; k < w.k1; ++k) {
+        if (!q_wait(&sm.empty[r.st], r.ph ^ 1, sm)) {
+          q_fail(sm, a, 1);
+          stop = true;
+          break;
+        }
+        unsigned char* dst = stage + uint32_t(r.st) * kQStageBytes;
+        const uint32_t bar = bar0 + uint32_t(r.st) * sizeof(uint64_t);
+        if (leader) mbar_arrive_expect_tx(&sm.full[r.st], tx);
+        if constexpr (GLU) {
+          const int f = t.f * 128 + int(crank) * 64;
+          tma_load_3d_pair(&tm_w, bar, dst, k * kQKb, f, t.e);
+          tma_load_3d_pair(&tm_w, bar, dst + kQABytes / 2, k * kQKb, a.F + f, t.e);
+        } else {
+          tma_load_3d_pair(&tm_w, bar, dst, k * kQKb, t.f * 256 + int(crank) * 128, t.e);
+        }
+        tma_load_2d_pair(&tm_x.m[bm], bar, dst + kQABytes, k * kQKb, row);
+        sm.fills[r.st] += 1;
+        r.next(kQStages);
+      }
+    }
+  } else if (warp == 1 && lane == 0 && leader) {
+    // ---- MMA
+    QRing r = {0, 0}, acc = {0, 0};
+    bool stop = false;
+    for (QWalk<SPLIT> w(s, tiles, pair, pairs); w.more() && !stop; w.next()) {
+      const QTile t = q_tile(s, w.tile);
+      const uint32_t idesc = make_idesc_i8(256, uint32_t(t.n));
+      if (!mbar_try_wait_cluster(&sm.tempty[acc.st], acc.ph ^ 1) &&
+          !q_wait_slow(&sm.tempty[acc.st], acc.ph ^ 1, sm, true)) {
+        q_fail(sm, a, 2);
+        break;
+      }
+      tc_fence_after();
+      const uint32_t d = tmem + uint32_t(acc.st) * 256;
+      for (int k = w.k0; k < w.k1; ++k) {
+        if (!q_wait(&sm.full[r.st], r.ph, sm)) {
+          q_fail(sm, a, 3);
+          stop = true;
+          break;
+        }
+        tc_fence_after();
+        const uint32_t aa = smem_u32(stage + uint32_t(r.st) * kQStageBytes), ba = aa + kQABytes;
+#pragma unroll
+        for (int kk = 0; kk < kQKb / 32; ++kk)
+          tc_mma_i8_pair(d, smem_desc_sw128(aa + kk * 32, 16, 1024), smem_desc_sw128(ba + kk * 32, 16, 1024), idesc,
+                         (k != w.k0 || kk != 0) ? 1u : 0u);
+        tc_commit_pair_mc(&sm.empty[r.st], 0x3);
+        sm.cons[r.st] += 1;
+        r.next(kQStages);
+      }
+      if (stop) break;
+      tc_commit_pair_mc(&sm.tfull[acc.st], 0x3);
+      acc.next(2);
+    }
+  } else if (warp >= kQEpi0) {
+    // ---- epilogue: chunks of 32 rows, even ones by the first four warps
+    QRing acc = {0, 0};
+    const int quarter = warp & 3, sub = (warp - kQEpi0) >> 2;
+    const uint32_t tempty0 = mapa_shared(smem_u32(&sm.tempty[0]), 0);
+    float* mine = xbuf + (sub * 4 + quarter) * 16 * 32;
+    const float* theirs = xbuf + (sub * 4 + (quarter ^ 2)) * 16 * 32;
+    const int bar_id = 1 + sub * 2 + (quarter & 1);  // this warp and its gate or up partner
+    for (QWalk<SPLIT> w(s, tiles, pair, pairs); w.more(); w.next()) {
+      const QTile t = q_tile(s, w.tile);
+      bool ok = q_wait(&sm.tfull[acc.st], acc.ph, sm);
+      if constexpr (GLU) ok = named_bar_and(bar_id, 64, ok);
+      if (!ok) {
+        q_fail(sm, a, 4);
+        break;
+      }
+      tc_fence_after();
+      const uint32_t d = tmem + uint32_t(acc.st) * 256 + (uint32_t(quarter * 32) << 16);
+      if (!w.whole()) {
+        int32_t* ps = a.part + (size_t(pair) * 2 + (w.k0 == 0 ? 1 : 0)) * kQSlotInts + crank * 128 + quarter * 32 + lane;
+        for (int jc = sub; jc * 32 < t.rows; jc += 2) {
+          uint32_t v[32];
+          tmem_ld_32x32b_x32(d + uint32_t(jc * 32), v);
+          tmem_ld_wait();
+#pragma unroll
+          for (int i = 0; i < 32; ++i)
+            if (jc * 32 + i < t.rows) ps[(jc * 32 + i) * 256] = int32_t(v[i]);
+        }
+      } else if constexpr (GLU) {
+        const int fl = int(crank) * 64 + (quarter & 1) * 32 + lane, f = t.f * 128 + fl;
+        const bool up = quarter >= 2;
+        const float sw = f < a.F ? a.ws[int64_t(t.e) * a.N + (up ? a.F : 0) + f] : 0.f;
+        for (int jc = sub; jc * 32 < t.rows; jc += 2) {
+          uint32_t v[32];
+          tmem_ld_32x32b_x32(d + uint32_t(jc * 32), v);
+          const int left = t.rows - jc * 32;
+          const float xv = lane < left ? a.xs[t.r0 + jc * 32 + lane] : 0.f;
+          tmem_ld_wait();
+          // The gate warp finishes rows 0..15 of the chunk, the up warp rows
+          // 16..31: each hands the other half over.
+          float z[32];
+#pragma unroll
+          for (int i = 0; i < 32; ++i) z[i] = float(int32_t(v[i])) * __shfl_sync(0xffffffffu, xv, i) * sw;
+          named_bar_sync(bar_id, 64);  // the last chunk's have been read
+#pragma unroll
+          for (int i = 0; i < 16; ++i) mine[i * 32 + lane] = up ? z[i] : z[16 + i];
+          named_bar_sync(bar_id, 64);
+#pragma unroll
+          for (int i = 0; i < 16; ++i) {
+            const float o = theirs[i * 32 + lane];
+            const int j = up ? 16 + i : i;
+            const float h = up ? silu_mul(o, z[16 + i]) : silu_mul(z[i], o);
+            if (j < left && f < a.F) q_store(a, t.r0 + jc * 32 + j, f, h);
+          }
+        }
+      } else {
+        const int f = t.f * 256 + int(crank) * 128 + quarter * 32 + lane;
+        const float sw = f < a.N ? a.ws[int64_t(t.e) * a.N + f] : 0.f;
+        for (int jc = sub; jc * 32 < t.rows; jc += 2) {
+          uint32_t v[32];
+          tmem_ld_32x32b_x32(d + uint32_t(jc * 32), v);
+          const int left = t.rows - jc * 32;
+          const float xv = lane < left ? a.xs[t.r0 + jc * 32 + lane] : 0.f;
+          tmem_ld_wait();
+#pragma unroll
+          for (int i = 0; i < 32; ++i) {
+            const float z = float(int32_t(v[i])) * __shfl_sync(0xffffffffu, xv, i) * sw;
+            if (i < left && f < a.N) q_store(a, t.r0 + jc * 32 + i, f, z);
+          }
+        }
+      }
+      tc_fence_before();
+      __syncwarp();
+      if (lane == 0) mbar_arrive_cluster(tempty0 + uint32_t(acc.st) * sizeof(uint64_t));
+      acc.next(2);
+    }
+  }
+  __syncwarp();
+
+  if constexpr (SPLIT) {
+    cg::this_grid().sync();
+    // ---- the tile that this pair started and others went on with: one row
+    // per warp, the parts in flight together
+    const uint32_t units = uint32_t(tiles) * uint32_t(s.kb);
+    const uint32_t g = min(uint32_t(pairs), units);
+    if (uint32_t(pair) < g) {
+      const uint32_t lo = uint64_t(units) * pair / g, hi = uint64_t(units) * (pair + 1) / g;
+      const uint32_t tile = (hi - 1) / s.kb, first = tile * s.kb, end = first + s.kb;
+      if (first >= lo && hi < end) {
+        const int c1 = int((uint64_t(end) * g - 1) / units);
+        const QTile t = q_tile(s, int(tile));
+        auto at = [&](int c, int j) { return a.part + (size_t(c) * 2 + (c == pair ? 1 : 0)) * kQSlotInts + j * 256; };
+        for (int j = int(crank) * (kQThreads / 32) + warp; j < t.rows; j += 2 * (kQThreads / 32)) {
+          const float xv = a.xs[t.r0 + j];
+#pragma unroll 1
+          for (int c = 0; c < 2; ++c) {  // the two CTAs' channels
+            if constexpr (GLU) {
+              const int fl = lane * 2, f = t.f * 128 + c * 64 + fl;
+              int2 gs = {0, 0}, us = {0, 0};
+#pragma unroll 4
+              for (int p = pair; p <= c1; ++p) {
+                const int2 x = __ldcg(reinterpret_cast<const int2*>(at(p, j) + c * 128 + fl));
+                const int2 y = __ldcg(reinterpret_cast<const int2*>(at(p, j) + c * 128 + 64 + fl));
+                gs.x += x.x, gs.y += x.y, us.x += y.x, us.y += y.y;
+              }
+              if (f < a.F) {
+                const float* sg = a.ws + int64_t(t.e) * a.N + f;
+                const float* su = sg + a.F;
+                q_store(a, t.r0 + j, f, silu_mul(float(gs.x) * xv * sg[0], float(us.x) * xv * su[0]));
+                q_store(a, t.r0 + j, f + 1, silu_mul(float(gs.y) * xv * sg[1], float(us.y) * xv * su[1]));
+              }
+            } else {
+              const int fl = c * 128 + lane * 4, f = t.f * 256 + fl;
+              int4 z = {0, 0, 0, 0};
+#pragma unroll 4
+              for (int p = pair; p <= c1; ++p) {
+                const int4 x = __ldcg(reinterpret_cast<const int4*>(at(p, j) + fl));
+                z.x += x.x, z.y += x.y, z.z += x.z, z.w += x.w;
+              }
+              if (f < a.N) {
+                const float* sw = a.ws + int64_t(t.e) * a.N + f;
+                q_store(a, t.r0 + j, f, float(z.x) * xv * sw[0]);
+                q_store(a, t.r0 + j, f + 1, float(z.y) * xv * sw[1]);
+                q_store(a, t.r0 + j, f + 2, float(z.z) * xv * sw[2]);
+                q_store(a, t.r0 + j, f + 3, float(z.w) * xv * sw[3]);
+              }
+            }
+          }
+        }
+      }
+    }
+  }
+
+  // ---- teardown.  After an abort: time for the peer's loads onto the
+  // leader's barriers, then every load and MMA still under way, all bounded.
+  __syncthreads();
+  const bool failed = *reinterpret_cast<volatile int*>(&sm.err) != 0;
+  if (failed && threadIdx.x == 0) {
+    const uint64_t until = globaltimer_ns() + 200000ull;
+    while (globaltimer_ns() < until) {
+    }
+  }
+  cluster_sync();
+  if (leader && threadIdx.x == 0) {
+    for (int i = 0; i < kQStages; ++i) {
+      if (sm.fills[i] == sm.cons[i]) continue;
+      const uint64_t until = globaltimer_ns() + kQBoundNs;
+      while (!mbar_try_wait(&sm.full[i], (sm.fills[i] - 1) & 1) && globaltimer_ns() < until) {
+      }
+    }
+  }
+  if (leader && warp == 1 && lane == 0) {
+    tc_commit_pair(&sm.drain);
+    const uint64_t until = globaltimer_ns() + kQBoundNs;
+    while (!mbar_try_wait(&sm.drain, 0) && globaltimer_ns() < until) {
+    }
+  }
+  tc_fence_before();
+  cluster_sync();
+  tc_fence_after();
+  if (warp == 1) {
+    __syncwarp();
+    tmem_dealloc_pair(tmem, 512);
+  }
+  cluster_sync();  // neither CTA leaves while its peer may still address it
+}
+
+// ---------------------------------------------------------------- quantisation
+constexpr int kQuantThreads = 256;
+
+// Rounds x / s half to even, exactly: |x / s| <= 127.5, inv = 1 / s rounded.
+// t holds the nearest integer of x * inv (within one of the answer) in its
+// low mantissa bits; the remainder x - q*s fits fp32.
+__device__ __forceinline__ int quant_one(float x, float s, float half, float inv) {
+  constexpr float kMagic = 12582912.f;  // 1.5 * 2^23
+  const float t = fmaf(x, inv, kMagic);
+  int q = __float_as_int(t) - __float_as_int(kMagic);
+  const float r = fmaf(-(t - kMagic), s, x);
+  const bool odd = q & 1;
+  if (r > half || (r == half && odd)) ++q;
+  if (r < -half || (r == -half && odd)) --q;
+  return max(-127, min(127, q));
+}
+
+__device__ __forceinline__ void load8(const __nv_bfloat16* p, float (&v)[8]) {
+  const uint4 w = *reinterpret_cast<const uint4*>(p);
+  const __nv_bfloat162* h = reinterpret_cast<const __nv_bfloat162*>(&w);
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    const float2 f = __bfloat1622float2(h[i]);
+    v[2 * i] = f.x;
+    v[2 * i + 1] = f.y;
+  }
+}
+__device__ __forceinline__ void load8(const float* p, float (&v)[8]) {
+  *reinterpret_cast<float4*>(&v[0]) = *reinterpret_cast<const float4*>(p);
+  *reinterpret_cast<float4*>(&v[4]) = *reinterpret_cast<const float4*>(p + 4);
+}
+
+// TPR threads per row, each VPT groups of eight values in registers; rows
+// longer than that are read again for the rounding.
+template <typename In, int VPT>
+__global__ void __launch_bounds__(kQuantThreads)
+    quant_rows_kernel(const In* __restrict__ x, int64_t rows, int K, const int32_t* __restrict__ perm,
+                      const int32_t* __restrict__ live_rows, int tpr, int8_t* __restrict__ q,
+                      float* __restrict__ scale) {
+  __shared__ uint32_t top_s[kQuantThreads / 32];
+  const int per = kQuantThreads / tpr, lr = threadIdx.x / tpr, c = threadIdx.x % tpr;
+  const int64_t live = live_rows ? min(int64_t(max(*live_rows, 0)), rows) : rows;
+  const int groups = K / 8;
+  for (int64_t base = int64_t(blockIdx.x) * per; base < live; base += int64_t(gridDim.x) * per) {
+    const int64_t r = base + lr;
+    const bool on = r < live;
+    const In* src = x + (on ? (perm ? int64_t(perm[r]) : r) : 0) * K;
+    float v[VPT][8];
+    uint32_t top = 0;
+    if (on) {
+#pragma unroll
+      for (int j = 0; j < VPT; ++j)
+        if (c + j * tpr < groups) load8(src + (c + j * tpr) * 8, v[j]);
+#pragma unroll
+      for (int j = 0; j < VPT; ++j)
+        if (c + j * tpr < groups) {
+#pragma unroll
+          for (int i = 0; i < 8; ++i) top = max(top, __float_as_uint(v[j][i]) & 0x7fffffffu);
+        }
+      for (int g = c + VPT * tpr; g < groups; g += tpr) {
+        float w[8];
+        load8(src + g * 8, w);
+#pragma unroll
+        for (int i = 0; i < 8; ++i) top = max(top, __float_as_uint(w[i]) & 0x7fffffffu);
+      }
+    }
+    top = __reduce_max_sync(0xffffffffu, top);
+    if (tpr > 32) {
+      __syncthreads();  // the last round's maxima have been read
+      if ((threadIdx.x & 31) == 0) top_s[threadIdx.x >> 5] = top;
+      __syncthreads();
+      const int w0 = lr * (tpr / 32);
+      for (int w = 0; w < tpr / 32; ++w) top = max(top, top_s[w0 + w]);
+    }
+    if (!on) continue;
+    // Infinities and NaN (largest as numbers): no scale holds the row, and a
+    // NaN scale says so in every output.
+    const bool bad = top >= 0x7f800000u;
+    const float s0 = bad ? __int_as_float(0x7fffffff) : __uint_as_float(top) / 127.f;
+    if (c == 0) scale[r] = s0;
+    const bool zero = bad || s0 == 0.f;
+    // Tiny rows: the reciprocal would overflow; powers of two change nothing.
+    const float up = s0 < 0x1p-90f ? 0x1p100f : 1.f;
+    const float s = zero ? 1.f : s0 * up, half = 0.5f * s, inv = 1.f / s;
+    int8_t* dst = q + r * K;
+    auto put = [&](int g, const float (&w)[8]) {
+      uint32_t b[2] = {0, 0};
+#pragma unroll
+      for (int i = 0; i < 8; ++i) {
+        const int n = zero ? 0 : quant_one(w[i] * up, s, half, inv);
+        b[i >> 2] |= uint32_t(n & 0xff) << (8 * (i & 3));
+      }
+      *reinterpret_cast<uint2*>(dst + g * 8) = make_uint2(b[0], b[1]);
+    };
+#pragma unroll
+    for (int j = 0; j < VPT; ++j)
+      if (c + j * tpr < groups) put(c + j * tpr, v[j]);
+    for (int g = c + VPT * tpr; g < groups; g += tpr) {
+      float w[8];
+      load8(src + g * 8, w);
+      put(g, w);
+    }
+  }
+}
+
+template <typename In>
+int launch_quant(const void* x, int64_t rows, int K, const int32_t* perm, const int32_t* live, void* q, float* scale,
+                 int sms, cudaStream_t stream) {
+  // The fewest threads per row that leave each at most four groups of eight.
+  int tpr = 32;
+  while (tpr < kQuantThreads && K / 8 > 4 * tpr) tpr *= 2;
+  const int per = kQuantThreads / tpr, vpt = (K / 8 + tpr - 1) / tpr;
+  const int64_t blocks = std::min<int64_t>((rows + per - 1) / per, int64_t(sms) * 8);
+  const In* xi = static_cast<const In*>(x);
+  int8_t* qi = static_cast<int8_t*>(q);
+  const unsigned g = unsigned(blocks);
+  if (vpt <= 1) quant_rows_kernel<In, 1><<<g, kQuantThreads, 0, stream>>>(xi, rows, K, perm, live, tpr, qi, scale);
+  else if (vpt <= 2) quant_rows_kernel<In, 2><<<g, kQuantThreads, 0, stream>>>(xi, rows, K, perm, live, tpr, qi, scale);
+  else quant_rows_kernel<In, 4><<<g, kQuantThreads, 0, stream>>>(xi, rows, K, perm, live, tpr, qi, scale);
+  return cudaGetLastError() == cudaSuccess ? kOk : kCudaErr;
+}
+
+// ---------------------------------------------------------------- weighted sum of the experts' rows
+// y[t] = sum over k of v[t, k] * rows[offsets[e] + slots[t, k]], e = ids[t, k];
+// slot -1: not routed here.  fp32 in the order of k, one rounding to bf16.
+constexpr int kSumThreads = 256;
+__global__ void __launch_bounds__(kSumThreads)
+    weighted_sum_kernel(const __nv_bfloat16* __restrict__ src, const void* __restrict__ ids, int ids64, int first,
+                        const void* __restrict__ vals, int vals_bf16, const int32_t* __restrict__ slots,
+                        const int32_t* __restrict__ offsets, int64_t T, int K, int H, int E,
+                        __nv_bfloat16* __restrict__ y) {
+  const int vec = H / 8;
+  const int64_t total = T * vec;
+  for (int64_t i = int64_t(blockIdx.x) * kSumThreads + threadIdx.x; i < total;
+       i += int64_t(gridDim.x) * kSumThreads) {
+    const int64_t t = i / vec;
+    const int f = int(i - t * vec) * 8;
+    float acc[8] = {};
+#pragma unroll 4
+    for (int k = 0; k < K; ++k) {
+      const int64_t o = t * K + k;
+      const int slot = slots[o];
+      const long long e =
+          (ids64 ? static_cast<const long long*>(ids)[o] : static_cast<const int32_t*>(ids)[o]) - (long long)first;
+      if (slot < 0 || e < 0 || e >= E) continue;
+      const float v = vals_bf16 ? __bfloat162float(static_cast<const __nv_bfloat16*>(vals)[o])
+                                : static_cast<const float*>(vals)[o];
+      float w[8];
+      load8(src + (int64_t(offsets[e]) + slot) * H + f, w);
+#pragma unroll
+      for (int j = 0; j < 8; ++j) acc[j] = fmaf(v, w[j], acc[j]);
+    }
+    __nv_bfloat162 o2[4];
+#pragma unroll
+    for (int j = 0; j < 4; ++j) o2[j] = __floats2bfloat162_rn(acc[2 * j], acc[2 * j + 1]);
+    *reinterpret_cast<uint4*>(y + t * H + f) = *reinterpret_cast<uint4*>(o2);
+  }
+}
+
+// ---------------------------------------------------------------- host side
+int sm_count(int* sms) {
+  int dev = 0;
+  if (cudaGetDevice(&dev) != cudaSuccess) return kCudaErr;
+  return cudaDeviceGetAttribute(sms, cudaDevAttrMultiProcessorCount, dev) == cudaSuccess ? kOk : kCudaErr;
+}
+
+bool misaligned16(const void* p) { return (reinterpret_cast<uintptr_t>(p) & 15) != 0; }
+
+size_t q_smem_bytes(int E) {
+  return 1024 + size_t(kQStages) * kQStageBytes + kQXBytes + sizeof(QSmem) + size_t(E + 1) * 8;
+}
+static_assert(1024 + size_t(kQStages) * kQStageBytes + kQXBytes + sizeof(QSmem) + size_t(kMaxExperts + 1) * 8 <=
+                  227 * 1024,
+              "shared memory plan exceeds 227 KB");
+static_assert((kQStages * kQStageBytes + kQXBytes) % 16 == 0, "QSmem must start on a 16-byte boundary");
+
+// Products with fewer tiles than four per pair are split over K.
+bool q_split(int64_t rows, int N, int F, bool glu, int pairs) {
+  const int64_t ft = glu ? (F + 127) / 128 : (N + 255) / 256;
+  return (rows + kQTileRows - 1) / kQTileRows * ft < 4 * int64_t(pairs);
+}
+
+int encode_s8(CUtensorMap* m, int rank, const void* ptr, const cuuint64_t* dims, const cuuint64_t* strides,
+              const cuuint32_t* box) {
+  const cuuint32_t one[3] = {1, 1, 1};
+  return driver().cuTensorMapEncodeTiled(m, CU_TENSOR_MAP_DATA_TYPE_UINT8, cuuint32_t(rank), const_cast<void*>(ptr),
+                                         dims, strides, box, one, CU_TENSOR_MAP_INTERLEAVE_NONE,
+                                         CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
+                                         CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS
+             ? kOk
+             : kCudaErr;
+}
+
+template <bool GLU, bool SPLIT>
+int launch_w8a8(const CUtensorMap& tw, const QRowMaps& tx, const QArgs& a, int pairs, cudaStream_t stream) {
+  const size_t smem = q_smem_bytes(a.E);
+  if (cudaFuncSetAttribute(w8a8_kernel<GLU, SPLIT>, cudaFuncAttributeMaxDynamicSharedMemorySize, int(smem)) !=
+      cudaSuccess)
+    return kCudaErr;
+  cudaLaunchConfig_t cfg = {};
+  cudaLaunchAttribute at[2];
+  at[0].id = cudaLaunchAttributeClusterDimension;
+  at[0].val.clusterDim.x = 2;
+  at[0].val.clusterDim.y = 1;
+  at[0].val.clusterDim.z = 1;
+  at[1].id = cudaLaunchAttributeCooperative;
+  at[1].val.cooperative = 1;
+  cfg.gridDim = dim3(unsigned(2 * pairs));
+  cfg.blockDim = dim3(kQThreads);
+  cfg.dynamicSmemBytes = smem;
+  cfg.stream = stream;
+  cfg.attrs = at;
+  cfg.numAttrs = 1;
+  // The split form's pairs meet at a grid barrier, so no more of them than
+  // can be resident together.
+  int fit = 0;
+  if (cudaOccupancyMaxActiveClusters(&fit, w8a8_kernel<GLU, SPLIT>, &cfg) != cudaSuccess || fit < 1) return kCudaErr;
+  cfg.gridDim = dim3(unsigned(2 * std::min(pairs, fit)));
+  cfg.numAttrs = SPLIT ? 2 : 1;
+  return cudaLaunchKernelEx(&cfg, w8a8_kernel<GLU, SPLIT>, tw, tx, a) == cudaSuccess ? kOk : kCudaErr;
+}
+
+bool q_sizes_ok(int64_t rows, int32_t K, int32_t N, int32_t E, int32_t glu) {
+  if (rows < 0 || rows > (int64_t(1) << 30) || K <= 0 || K % 16 || K > kQMaxK) return false;
+  if (N <= 0 || N % (glu ? 16 : 8) || E < 1 || E > kMaxExperts) return false;
+  const int64_t ft = (N + 255) / 256;
+  const int64_t tiles = ((rows + kQTileRows - 1) / kQTileRows + E) * ft;
+  return tiles * ((K + kQKb - 1) / kQKb) <= (int64_t(1) << 30);
+}
+
+}  // namespace
+}  // namespace moe
+
+using namespace moe;
+
+extern "C" int moe_quant_rows(const void* x, int32_t x_is_f32, int64_t rows, int32_t K, const int32_t* perm,
+                              const int32_t* live_rows, void* q, float* scale, void* stream) {
+  if (rows < 0 || rows > (int64_t(1) << 30) || K <= 0 || K % 8) return kBadArg;
+  if (rows == 0) return kOk;
+  if (!x || !q || !scale || misaligned16(x) || (reinterpret_cast<uintptr_t>(q) & 7)) return kBadArg;
+  int sms = 0;
+  if (sm_count(&sms) != kOk) return kCudaErr;
+  const cudaStream_t s = static_cast<cudaStream_t>(stream);
+  return x_is_f32 ? launch_quant<float>(x, rows, K, perm, live_rows, q, scale, sms, s)
+                  : launch_quant<__nv_bfloat16>(x, rows, K, perm, live_rows, q, scale, sms, s);
+}
+
+extern "C" int moe_w8a8_scratch_bytes(int64_t rows, int32_t K, int32_t N, int32_t E, int32_t swiglu, int32_t device,
+                                      size_t* out) {
+  if (!out || !q_sizes_ok(rows, K, N, E, swiglu)) return kBadArg;
+  int sms = 0;
+  if (cudaDeviceGetAttribute(&sms, cudaDevAttrMultiProcessorCount, device) != cudaSuccess) return kCudaErr;
+  *out = q_split(rows, N, swiglu ? N / 2 : N, swiglu != 0, sms / 2) ? size_t(sms / 2) * 2 * kQSlotInts * 4 : 0;
+  return kOk;
+}
+
+extern "C" int moe_w8a8_gemm(const moe_w8a8_params* p, void* stream) {
+  if (!p || !q_sizes_ok(p->rows, p->K, p->N, p->experts, p->swiglu)) return kBadArg;
+  if (p->rows == 0) return kOk;
+  if (!p->xq || !p->xs || !p->wq || !p->ws || !p->out || (!p->counts && p->experts != 1)) return kBadArg;
+  if (misaligned16(p->xq) || misaligned16(p->wq) || misaligned16(p->scratch)) return kBadArg;
+  if (!driver().ok) return kCudaErr;
+  int sms = 0;
+  if (sm_count(&sms) != kOk) return kCudaErr;
+  const int pairs = sms / 2;
+  const bool glu = p->swiglu != 0;
+  QArgs a = {};
+  a.E = p->experts;
+  a.K = p->K;
+  a.N = p->N;
+  a.rows = p->rows;
+  a.F = glu ? p->N / 2 : p->N;
+  a.counts = p->counts;
+  a.xs = p->xs;
+  a.ws = p->ws;
+  a.out = p->out;
+  a.out_f32 = p->out_is_f32;
+  a.part = static_cast<int32_t*>(p->scratch);
+  a.status_host = p->status_host;
+  const bool split = q_split(a.rows, a.N, a.F, glu, pairs);
+  if (split && (!p->scratch || p->scratch_bytes < size_t(pairs) * 2 * kQSlotInts * 4)) return kBadArg;
+
+  CUtensorMap tw;
+  QRowMaps tx;
+  {
+    const cuuint64_t dims[3] = {cuuint64_t(a.K), cuuint64_t(a.N), cuuint64_t(a.E)};
+    const cuuint64_t str[2] = {cuuint64_t(a.K), cuuint64_t(a.K) * a.N};
+    const cuuint32_t box[3] = {cuuint32_t(kQKb), glu ? 64u : 128u, 1};
+    if (encode_s8(&tw, 3, p->wq, dims, str, box)) return kCudaErr;
+  }
+  for (int i = 0; i < kQRowMaps; ++i) {
+    const cuuint64_t dims[2] = {cuuint64_t(a.K), cuuint64_t(a.rows)};
+    const cuuint64_t str[1] = {cuuint64_t(a.K)};
+    const cuuint32_t box[2] = {cuuint32_t(kQKb), 16u << i};
+    if (encode_s8(&tx.m[i], 2, p->xq, dims, str, box)) return kCudaErr;
+  }
+  const cudaStream_t s = static_cast<cudaStream_t>(stream);
+  if (glu) return split ? launch_w8a8<true, true>(tw, tx, a, pairs, s) : launch_w8a8<true, false>(tw, tx, a, pairs, s);
+  return split ? launch_w8a8<false, true>(tw, tx, a, pairs, s) : launch_w8a8<false, false>(tw, tx, a, pairs, s);
+}
+
+extern "C" int moe_weighted_sum(const void* rows, const void* top_idxs, int32_t ids_are_int64, int32_t first_expert,
+                                const void* top_vals, int32_t vals_are_bf16, const int32_t* slots,
+                                const int32_t* offsets, int64_t T, int32_t K, int32_t H, int32_t experts, void* y,
+                                void* stream) {
+  if (T < 0 || T > (int64_t(1) << 30) || K < 1 || K > kMaxRouteK || H <= 0 || H % 8 || experts < 1 ||
+      experts > kMaxExperts)
+    return kBadArg;
+  if (T == 0) return kOk;
+  if (!rows || !top_idxs || !top_vals || !slots || !offsets || !y || misaligned16(rows) || misaligned16(y))
+    return kBadArg;
+  int sms = 0;
+  if (sm_count(&sms) != kOk) return kCudaErr;
+  const int64_t blocks = std::min<int64_t>((T * (H / 8) + kSumThreads - 1) / kSumThreads, int64_t(sms) * 8);
+  weighted_sum_kernel<<<unsigned(blocks), kSumThreads, 0, static_cast<cudaStream_t>(stream)>>>(
+      static_cast<const __nv_bfloat16*>(rows), top_idxs, ids_are_int64, first_expert, top_vals, vals_are_bf16, slots,
+      offsets, T, K, H, experts, static_cast<__nv_bfloat16*>(y));
+  return cudaGetLastError() == cudaSuccess ? kOk : kCudaErr;
+}

@@ -1,0 +1,228 @@
+"""Expert products in 8-bit integers (8-bit weights, 8-bit activations).
+
+The reference's expert product is bf16 (baseline.py:50).  Here rows are
+quantised with one scale each and weights with one scale per output channel,
+
+    x[r, k] ~ xs[r] * xq[r, k],      w[e, k, n] ~ ws[e, n] * wq[e, n, k]
+    out[r, n] = xs[r] * ws[e, n] * sum_k xq[r, k] * wq[e, n, k]
+
+with the integer sum exact.  Half the bytes of bf16 weights and twice the
+tensor-core rate.
+
+* ``quantize_weights`` — once, when a model is loaded;
+* ``quantize_rows`` — rows of activations, optionally gathered by the
+  dispatch permutation of ``utils.route`` on the way;
+* ``grouped_gemm`` — one product per expert over rows in expert order, with
+  SwiGLU in its epilogue on request; ``linear`` — the dense form from bf16;
+* ``moe_layer`` — the gated layer on one rank's experts, the 8-bit sibling of
+  ``combine.moe_layer`` over ``mlp``: route, gather and quantise, gate/up
+  product with SwiGLU, quantise, down product, weighted sum per token.
+
+Nothing is read on the host and every call may be captured into a CUDA graph.
+"""
+from __future__ import annotations
+
+import ctypes
+import functools
+from dataclasses import dataclass
+
+import torch
+
+from . import _native as N
+from . import utils
+
+
+@dataclass(frozen=True)
+class QuantWeights:
+    """``q [El, N, K]`` int8 (K contiguous) and ``scale [El, N]`` float32."""
+    q: torch.Tensor
+    scale: torch.Tensor
+
+
+def _check_weights(w: QuantWeights, name: str) -> tuple[int, int, int]:
+    if w.q.dim() != 3 or tuple(w.scale.shape) != tuple(w.q.shape[:2]):
+        raise ValueError(f"{name}: q [El, N, K] and scale [El, N] are required, "
+                         f"got {tuple(w.q.shape)} and {tuple(w.scale.shape)}")
+    if w.q.dtype != torch.int8 or w.scale.dtype != torch.float32:
+        raise TypeError(f"{name}: q must be int8 and scale float32")
+    if not w.q.is_contiguous() or not w.scale.is_contiguous():
+        raise ValueError(f"{name}: q and scale must be contiguous")
+    return tuple(w.q.shape)
+
+
+def _on_gpu(device, **tensors):
+    for name, t in tensors.items():
+        if t is not None and (not t.is_cuda or t.device != device):
+            raise ValueError(f"{name} must be a CUDA tensor on {device}")
+
+
+def quantize_rows(x: torch.Tensor, perm: torch.Tensor | None = None,
+                  live_rows: torch.Tensor | None = None) -> tuple[torch.Tensor, torch.Tensor]:
+    """``(q [rows, K] int8, scale [rows] float32)`` of x [n, K], bf16 or fp32.
+
+    scale = max|row| / 127 (fp32) and q the exact quotient, rounded half to
+    even.  With ``perm`` [rows] int32, row r is x[perm[r]] (``Routing.perm``:
+    the send buffer of ``utils.pack_compact``, quantised on the way); rows
+    from ``live_rows`` (one int32 on the device, e.g. ``Routing.offsets[-1:]``)
+    on are not written.  A row of zeros gets scale 0; a row that holds an
+    infinity or a NaN gets a NaN scale and zeros."""
+    if x.dim() != 2 or x.dtype not in (torch.bfloat16, torch.float32):
+        raise TypeError("x [n, K] in bfloat16 or float32 is required")
+    K = x.shape[1]
+    if K % 8 or K == 0:
+        raise ValueError(f"K = {K} must be a positive multiple of 8")
+    if perm is not None and (perm.dtype != torch.int32 or perm.dim() != 1 or not perm.is_contiguous()):
+        raise TypeError("perm must be a contiguous int32 vector")
+    if live_rows is not None and (live_rows.dtype != torch.int32 or live_rows.numel() != 1):
+        raise TypeError("live_rows must be one int32")
+    _on_gpu(x.device, x=x, perm=perm, live_rows=live_rows)
+    x = x.contiguous()
+    rows = x.shape[0] if perm is None else perm.shape[0]
+    q = torch.empty((rows, K), dtype=torch.int8, device=x.device)
+    scale = torch.empty(rows, dtype=torch.float32, device=x.device)
+    with utils.on_device(x.device) as stream:
+        N.check(N.lib().moe_quant_rows(x.data_ptr(), x.dtype == torch.float32, rows, K,
+                                       None if perm is None else perm.data_ptr(),
+                                       None if live_rows is None else live_rows.data_ptr(), q.data_ptr(),
+                                       scale.data_ptr(), stream), "moe_quant_rows")
+    return q, scale
+
+
+def quantize_weights(w: torch.Tensor) -> QuantWeights:
+    """[El, K, N] (bf16 or fp32) -> one scale per output channel, laid out with
+    K contiguous.  One expert's transposed copy at a time."""
+    if w.dim() != 3:
+        raise ValueError("w [El, K, N] is required")
+    El, K, Nout = w.shape
+    _on_gpu(w.device, w=w)
+    q = torch.empty((El, Nout, K), dtype=torch.int8, device=w.device)
+    scale = torch.empty((El, Nout), dtype=torch.float32, device=w.device)
+    for e in range(El):
+        q[e], scale[e] = quantize_rows(w[e].t().contiguous())
+    return QuantWeights(q, scale)
+
+
+@functools.lru_cache(maxsize=256)
+def _scratch_bytes(*sizes) -> int:
+    need = ctypes.c_size_t()
+    N.check(N.lib().moe_w8a8_scratch_bytes(*sizes, ctypes.byref(need)), "moe_w8a8_scratch_bytes")
+    return need.value
+
+
+def grouped_gemm(xq: torch.Tensor, xs: torch.Tensor, w: QuantWeights, counts: torch.Tensor | None = None, *,
+                 swiglu: bool = False, out_dtype=torch.bfloat16, out: torch.Tensor | None = None,
+                 status: torch.Tensor | None = None) -> torch.Tensor:
+    """``out [rows, N]`` of one 8-bit product per expert.
+
+    xq [rows, K] int8 and xs [rows] float32: rows in expert order, counts [El]
+    int32 of them per expert, on the device (None: one expert for all).  K a
+    multiple of 16.  With ``swiglu`` w's channels are gate [0, N/2) and up
+    [N/2, N) and ``out [rows, N/2] = silu(gate) * up``.  Rows behind the last
+    expert's are left as they were (``out`` supplies the buffer).
+    ``out_dtype`` is bfloat16 or float32."""
+    El, Nw, K = _check_weights(w, "w")
+    if xq.dim() != 2 or xq.shape[1] != K or tuple(xs.shape) != (xq.shape[0],):
+        raise ValueError(f"xq {tuple(xq.shape)} and xs {tuple(xs.shape)} do not match w {tuple(w.q.shape)}")
+    if xq.dtype != torch.int8 or xs.dtype != torch.float32:
+        raise TypeError("xq must be int8 and xs float32")
+    if K % 16 or not 0 < K <= 131056:
+        raise ValueError(f"K = {K} must be a multiple of 16, 131056 at most")
+    if Nw % (16 if swiglu else 8) or Nw == 0:
+        raise ValueError(f"{Nw} channels: a multiple of {16 if swiglu else 8} is needed")
+    if El > 1024:
+        raise ValueError(f"{El} experts: 1024 at most")
+    if counts is None:
+        if El != 1:
+            raise ValueError("counts may be left out for one expert only")
+    elif counts.dtype != torch.int32 or tuple(counts.shape) != (El,) or not counts.is_contiguous():
+        raise ValueError(f"counts must be a contiguous int32 vector of {El}")
+    if out_dtype not in (torch.bfloat16, torch.float32):
+        raise TypeError("out_dtype must be bfloat16 or float32")
+    rows, cols = xq.shape[0], Nw // 2 if swiglu else Nw
+    if out is None:
+        out = torch.empty((rows, cols), dtype=out_dtype, device=xq.device)
+    elif tuple(out.shape) != (rows, cols) or out.dtype != out_dtype or not out.is_contiguous():
+        raise ValueError(f"out must be a contiguous {out_dtype} tensor of shape {(rows, cols)}")
+    if status is not None and (status.dtype != torch.int32 or status.numel() != 1 or not status.is_pinned()):
+        raise ValueError("status must be one pinned int32")
+    _on_gpu(xq.device, xq=xq, xs=xs, q=w.q, scale=w.scale, counts=counts, out=out)
+    if rows == 0:
+        return out
+    xq, xs = xq.contiguous(), xs.contiguous()
+    need = _scratch_bytes(rows, K, Nw, El, int(swiglu), xq.device.index)
+    scratch = torch.empty(need, dtype=torch.uint8, device=xq.device) if need else None
+    p = N.W8A8Params()
+    p.rows, p.K, p.N, p.experts, p.swiglu, p.out_is_f32 = rows, K, Nw, El, swiglu, out_dtype == torch.float32
+    p.xq, p.xs, p.wq, p.ws, p.out = (xq.data_ptr(), xs.data_ptr(), w.q.data_ptr(), w.scale.data_ptr(),
+                                     out.data_ptr())
+    p.counts = None if counts is None else counts.data_ptr()
+    p.scratch, p.scratch_bytes = (None, 0) if scratch is None else (scratch.data_ptr(), need)
+    p.status_host = None if status is None else status.data_ptr()
+    with utils.on_device(xq.device) as stream:
+        N.check(N.lib().moe_w8a8_gemm(ctypes.byref(p), stream), "moe_w8a8_gemm")
+    return out
+
+
+def linear(x: torch.Tensor, w: QuantWeights, *, out_dtype=torch.bfloat16) -> torch.Tensor:
+    """``x [rows, K] @ w`` for one weight matrix (w.q [1, N, K]): quantises the
+    rows and multiplies."""
+    if w.q.dim() != 3 or w.q.shape[0] != 1:
+        raise ValueError(f"one weight matrix [1, N, K] is required, got {tuple(w.q.shape)}")
+    q, scale = quantize_rows(x)
+    return grouped_gemm(q, scale, w, out_dtype=out_dtype)
+
+
+def moe_layer(x: torch.Tensor, top_idxs: torch.Tensor, top_vals: torch.Tensor, w13: QuantWeights, w2: QuantWeights,
+              *, first_expert: int = 0, status: torch.Tensor | None = None) -> torch.Tensor:
+    """``y [T, H]`` bf16 of the gated layer on this rank's experts:
+
+        y[t] = sum_k v[t, k] * down_e(silu(gate_e(x_t)) * up_e(x_t))
+
+    with e = top_idxs[t, k] - first_expert; other ids are skipped and an id
+    repeated within a row counts once, so that ranks holding parts of the
+    experts add their y's.
+
+    x [T, H] bf16, top_idxs [T, K] int32/int64, top_vals [T, K] float32 or
+    bfloat16; w13.q [El, 2F, H] (gate channels [0, F), up after them) and w2.q
+    [El, H, F].  H and F multiples of 16."""
+    El, F2, H = _check_weights(w13, "w13")
+    F = F2 // 2
+    _check_weights(w2, "w2")
+    if F2 % 2 or tuple(w2.q.shape) != (El, H, F):
+        raise ValueError(f"w13 {tuple(w13.q.shape)} and w2 {tuple(w2.q.shape)} do not form an MLP")
+    if x.dim() != 2 or x.shape[1] != H:
+        raise ValueError(f"x {tuple(x.shape)} does not match w13 {tuple(w13.q.shape)}")
+    if x.dtype != torch.bfloat16:
+        raise TypeError("x must be bfloat16")
+    if H % 16 or F % 16:
+        raise ValueError(f"H = {H} and F = {F} must be multiples of 16")
+    if top_idxs.dim() == 1:
+        top_idxs = top_idxs[:, None]
+    if top_vals.dim() == 1:
+        top_vals = top_vals[:, None]
+    T = x.shape[0]
+    if top_idxs.dim() != 2 or top_idxs.shape[0] != T or top_vals.shape != top_idxs.shape:
+        raise ValueError(f"top_idxs {tuple(top_idxs.shape)} and top_vals {tuple(top_vals.shape)} must be [T, K]")
+    if top_idxs.dtype not in (torch.int32, torch.int64):
+        raise TypeError("top_idxs must be int32 or int64")
+    if top_vals.dtype not in (torch.float32, torch.bfloat16):
+        raise TypeError("top_vals must be float32 or bfloat16")
+    K = top_idxs.shape[1]
+    if not 1 <= K <= 32:
+        raise ValueError(f"{K} ids per token: 1 to 32")
+    _on_gpu(x.device, x=x, top_idxs=top_idxs, top_vals=top_vals, w13=w13.q, w2=w2.q)
+    y = torch.empty((T, H), dtype=torch.bfloat16, device=x.device)
+    if T == 0:
+        return y
+    ids, vals = top_idxs.contiguous(), top_vals.contiguous()
+    with utils.on_device(x.device) as stream:
+        r = utils.route(ids if first_expert == 0 else ids - first_expert, El, with_slots=True)
+        q, scale = quantize_rows(x, r.perm, r.offsets[El:])
+        h = grouped_gemm(q, scale, w13, r.counts, swiglu=True, out_dtype=torch.float32, status=status)
+        q, scale = quantize_rows(h, live_rows=r.offsets[El:])
+        rows = grouped_gemm(q, scale, w2, r.counts, status=status)
+        N.check(N.lib().moe_weighted_sum(rows.data_ptr(), ids.data_ptr(), ids.dtype == torch.int64, first_expert,
+                                         vals.data_ptr(), vals.dtype == torch.bfloat16, r.slots.data_ptr(),
+                                         r.offsets.data_ptr(), T, K, H, El, y.data_ptr(), stream),
+                "moe_weighted_sum")
+    return y
