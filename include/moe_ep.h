@@ -419,7 +419,7 @@ int moe_decode_layer(const moe_decode_params* params, void* stream);
 
 /* ---------------------------------------------------------------- 8-bit products
  * Rows quantised with one scale each:
- *   scale[r] = max |x[src(r), :]| / 127 in fp32,
+ *   scale[r] = max |x[src(r), :]| * (1/127), both in fp32,
  *   q[r, i]  = x[src(r), i] / scale[r], the exact quotient rounded half to
  *              even and held to [-127, 127],
  * src(r) = perm[r] (the dispatch order of moe_route), or r without perm.
@@ -438,7 +438,7 @@ int moe_quant_rows(const void* x, int32_t x_is_f32, int64_t rows, int32_t K, con
  * behind the sum of the counts are left as they were; counts beyond `rows`
  * are cut.  counts == NULL: one expert for all rows.
  * Requires K % 16 == 0, K <= 131056, N % 8 == 0 (16 with swiglu), experts <=
- * 1024; xq, wq and scratch 16-byte aligned.  scratch:
+ * 1024; xq, wq, ws, out and scratch 16-byte aligned.  scratch:
  * moe_w8a8_scratch_bytes of device memory (may be 0), not initialised, for
  * this call alone until it has finished. */
 typedef struct moe_w8a8_params {
@@ -464,9 +464,9 @@ int moe_w8a8_gemm(const moe_w8a8_params* params, void* stream);
 /* y[t, :] = sum over k of top_vals[t, k] * rows[offsets[e] + slots[t, k], :],
  * e = top_idxs[t, k] - first_expert, in fp32 in the order of k, bf16 out; ids
  * outside [0, experts) after the subtraction and slots of -1 (moe_route_slots)
- * are skipped.  rows [offsets[experts], H] bf16, H % 8 == 0, rows and y
- * 16-byte aligned. */
-int moe_weighted_sum(const void* rows, const void* top_idxs, int32_t ids_are_int64, int32_t first_expert,
+ * are skipped.  rows [offsets[experts], H] bf16 or (rows_are_f32) fp32,
+ * H % 8 == 0, rows and y 16-byte aligned. */
+int moe_weighted_sum(const void* rows, int32_t rows_are_f32, const void* top_idxs, int32_t ids_are_int64, int32_t first_expert,
                      const void* top_vals, int32_t vals_are_bf16, const int32_t* slots, const int32_t* offsets,
                      int64_t T, int32_t K, int32_t H, int32_t experts, void* y, void* stream);
 

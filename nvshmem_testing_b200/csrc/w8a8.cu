@@ -21,7 +21,7 @@
 // scratch and, behind a grid barrier, are added and scaled.  Integer sums do
 // not depend on the split.
 //
-// Quantisation (quant_rows_kernel).  scale = absmax / 127 in fp32, q = the
+// Quantisation (quant_rows_kernel).  scale = absmax * (1/127) in fp32, q = the
 // exact quotient x / scale rounded half to even: the product with the
 // reciprocal is corrected by its remainder, which fp32 holds exactly.  One
 // read of the row, kept in registers between maximum and rounding.
@@ -48,9 +48,10 @@ constexpr int kQTileRows = 256;
 constexpr int kQEpiWarps = 8;                      // two per TMEM lane quarter
 constexpr int kQEpi0 = 2;
 constexpr int kQThreads = (kQEpi0 + kQEpiWarps) * 32;
-constexpr uint32_t kQXBytes = kQEpiWarps * 16 * 32 * 4;  // SwiGLU exchange
+constexpr uint32_t kQXBytes = kQEpiWarps * (16 + 1) * 32 * 4;  // per warp: half a chunk, 32 row scales
 constexpr int kQRowMaps = 4;                       // boxes of 16, 32, 64, 128 rows
 constexpr uint64_t kQBoundNs = 2000000000ull;      // bug guard on every pipeline wait
+constexpr int kQWaves = 4;                         // fewer tiles per pair: split over K
 constexpr int kQMaxK = 131056;                     // 128 * 128 * K < 2^31
 constexpr size_t kQSlotInts = 2 * 128 * kQTileRows;  // one pair's sums of one tile
 
@@ -140,17 +141,19 @@ __device__ __forceinline__ QTile q_tile(const QSched& s, int t) {
 
 // The runs over K that a pair does, in order: whole tiles t0, t0 + step, ...
 // or (split) the tiles of a contiguous share of units.
-template <bool SPLIT>
 struct QWalk {
+  bool split;
   int tile, step, tiles;  // whole tiles
   int u, hi, kb;          // split
   int k0, k1;             // current run
-  __device__ __forceinline__ QWalk(const QSched& s, int tiles_, int pair, int pairs) {
+  __device__ __forceinline__ QWalk(const QSched& s, bool split_, int tiles_, int pair, int pairs) {
+    split = split_;
     tiles = tiles_;
     kb = s.kb;
     k0 = 0;
     k1 = kb;
-    if constexpr (SPLIT) {
+    u = hi = 0;
+    if (split) {
       const uint32_t units = uint32_t(tiles_) * uint32_t(kb);
       const uint32_t g = min(uint32_t(pairs), units);
       u = uint32_t(pair) < g ? int(uint64_t(units) * pair / g) : 0;
@@ -166,16 +169,16 @@ struct QWalk {
     k0 = u - tile * kb;
     k1 = min(kb, k0 + hi - u);
   }
-  __device__ __forceinline__ bool more() const { return SPLIT ? u < hi : tile < tiles; }
+  __device__ __forceinline__ bool more() const { return split ? u < hi : tile < tiles; }
   __device__ __forceinline__ void next() {
-    if constexpr (SPLIT) {
+    if (split) {
       u += k1 - k0;
       set();
     } else {
       tile += step;
     }
   }
-  __device__ __forceinline__ bool whole() const { return !SPLIT || (k0 == 0 && k1 == kb); }
+  __device__ __forceinline__ bool whole() const { return k0 == 0 && k1 == kb; }
 };
 
 struct QRing {
@@ -195,7 +198,18 @@ __device__ __forceinline__ void q_store(const QArgs& a, int64_t row, int f, floa
   else static_cast<__nv_bfloat16*>(a.out)[at] = __float2bfloat16_rn(v);
 }
 
-__device__ __forceinline__ float silu_mul(float g, float u) { return g / (1.f + expf(-g)) * u; }
+__device__ __forceinline__ void q_store4(const QArgs& a, int64_t row, int f, float v0, float v1, float v2, float v3) {
+  const int64_t at = row * a.F + f;
+  if (a.out_f32) {
+    *reinterpret_cast<float4*>(static_cast<float*>(a.out) + at) = make_float4(v0, v1, v2, v3);
+  } else {
+    __nv_bfloat162 o[2] = {__floats2bfloat162_rn(v0, v1), __floats2bfloat162_rn(v2, v3)};
+    *reinterpret_cast<uint2*>(static_cast<__nv_bfloat16*>(a.out) + at) = *reinterpret_cast<uint2*>(o);
+  }
+}
+
+// The quotient within 2 steps of 2^-24 (0 where exp(-g) overflows).
+__device__ __forceinline__ float silu_mul(float g, float u) { return __fdividef(g, 1.f + expf(-g)) * u; }
 
 template <bool GLU, bool SPLIT>
 __global__ void __launch_bounds__(kQThreads, 1)
@@ -275,6 +289,9 @@ __global__ void __launch_bounds__(kQThreads, 1)
   tc_fence_after();
   const uint32_t tmem = sm.tmem_base;
   const int tiles = s.tpre[a.E] * s.FT;
+  // (The host launches the form with a grid barrier where the rows alone
+  // leave it open; ragged experts may make enough tiles all the same.)
+  const bool split = SPLIT && tiles < kQWaves * pairs;
 
   if (warp == 0 && lane == 0) {
     // ---- loads: each CTA its 128 channels and half of the tile's rows, all
@@ -282,7 +299,7 @@ __global__ void __launch_bounds__(kQThreads, 1)
     QRing r = {0, 0};
     const uint32_t bar0 = mapa_shared(smem_u32(&sm.full[0]), 0);
     bool stop = false;
-    for (QWalk<SPLIT> w(s, tiles, pair, pairs); w.more() && !stop; w.next()) {
+    for (QWalk w(s, split, tiles, pair, pairs); w.more() && !stop; w.next()) {
       const QTile t = q_tile(s, w.tile);
       const int half = t.n / 2, bm = half <= 16 ? 0 : half <= 32 ? 1 : half <= 64 ? 2 : 3;
       const uint32_t tx = 2 * (kQABytes + (16u << bm) * kQKb);
@@ -312,7 +329,7 @@ __global__ void __launch_bounds__(kQThreads, 1)
     // ---- MMA
     QRing r = {0, 0}, acc = {0, 0};
     bool stop = false;
-    for (QWalk<SPLIT> w(s, tiles, pair, pairs); w.more() && !stop; w.next()) {
+    for (QWalk w(s, split, tiles, pair, pairs); w.more() && !stop; w.next()) {
       const QTile t = q_tile(s, w.tile);
       const uint32_t idesc = make_idesc_i8(256, uint32_t(t.n));
       if (!mbar_try_wait_cluster(&sm.tempty[acc.st], acc.ph ^ 1) &&
@@ -349,9 +366,16 @@ __global__ void __launch_bounds__(kQThreads, 1)
     const uint32_t tempty0 = mapa_shared(smem_u32(&sm.tempty[0]), 0);
     float* mine = xbuf + (sub * 4 + quarter) * 16 * 32;
     const float* theirs = xbuf + (sub * 4 + (quarter ^ 2)) * 16 * 32;
+    float* xrow = xbuf + kQEpiWarps * 16 * 32 + (warp - kQEpi0) * 32;
     const int bar_id = 1 + sub * 2 + (quarter & 1);  // this warp and its gate or up partner
-    for (QWalk<SPLIT> w(s, tiles, pair, pairs); w.more(); w.next()) {
+    for (QWalk w(s, split, tiles, pair, pairs); w.more(); w.next()) {
       const QTile t = q_tile(s, w.tile);
+      // This lane's channel: within the CTA's 128, then of the output.
+      const int fl = quarter * 32 + lane;
+      const bool up = GLU && quarter >= 2;
+      const int f0 = GLU ? t.f * 128 + int(crank) * 64 + (quarter & 1) * 32 : t.f * 256 + int(crank) * 128 + quarter * 32;
+      const int f = f0 + lane;
+      const float sw = f < a.F ? a.ws[int64_t(t.e) * a.N + (up ? a.F : 0) + f] : 0.f;
       bool ok = q_wait(&sm.tfull[acc.st], acc.ph, sm);
       if constexpr (GLU) ok = named_bar_and(bar_id, 64, ok);
       if (!ok) {
@@ -360,56 +384,79 @@ __global__ void __launch_bounds__(kQThreads, 1)
       }
       tc_fence_after();
       const uint32_t d = tmem + uint32_t(acc.st) * 256 + (uint32_t(quarter * 32) << 16);
-      if (!w.whole()) {
-        int32_t* ps = a.part + (size_t(pair) * 2 + (w.k0 == 0 ? 1 : 0)) * kQSlotInts + crank * 128 + quarter * 32 + lane;
-        for (int jc = sub; jc * 32 < t.rows; jc += 2) {
-          uint32_t v[32];
-          tmem_ld_32x32b_x32(d + uint32_t(jc * 32), v);
-          tmem_ld_wait();
+      int32_t* ps = a.part + (size_t(pair) * 2 + (w.k0 == 0 ? 1 : 0)) * kQSlotInts + crank * 128 + fl;
+      const bool whole = w.whole();
+      // The next chunk's sums are on their way while one is finished.
+      uint32_t v[32];
+      if (sub * 32 < t.rows) tmem_ld_32x32b_x32(d + uint32_t(sub * 32), v);
+#pragma unroll 1
+      for (int jc = sub; jc * 32 < t.rows; jc += 2) {
+        const int left = t.rows - jc * 32;
+        const int64_t row = t.r0 + jc * 32;
+        tmem_ld_wait();
+        if (!whole) {
 #pragma unroll
           for (int i = 0; i < 32; ++i)
-            if (jc * 32 + i < t.rows) ps[(jc * 32 + i) * 256] = int32_t(v[i]);
+            if (i < left) ps[(jc * 32 + i) * 256] = int32_t(v[i]);
+          if ((jc + 2) * 32 < t.rows) tmem_ld_32x32b_x32(d + uint32_t((jc + 2) * 32), v);
+          continue;
         }
-      } else if constexpr (GLU) {
-        const int fl = int(crank) * 64 + (quarter & 1) * 32 + lane, f = t.f * 128 + fl;
-        const bool up = quarter >= 2;
-        const float sw = f < a.F ? a.ws[int64_t(t.e) * a.N + (up ? a.F : 0) + f] : 0.f;
-        for (int jc = sub; jc * 32 < t.rows; jc += 2) {
-          uint32_t v[32];
-          tmem_ld_32x32b_x32(d + uint32_t(jc * 32), v);
-          const int left = t.rows - jc * 32;
-          const float xv = lane < left ? a.xs[t.r0 + jc * 32 + lane] : 0.f;
-          tmem_ld_wait();
+        __syncwarp();
+        xrow[lane] = lane < left ? a.xs[row + lane] : 0.f;
+        __syncwarp();
+        float z[32];
+#pragma unroll
+        for (int i = 0; i < 32; i += 4) {
+          const float4 x4 = *reinterpret_cast<const float4*>(xrow + i);
+          z[i] = float(int32_t(v[i])) * x4.x * sw;
+          z[i + 1] = float(int32_t(v[i + 1])) * x4.y * sw;
+          z[i + 2] = float(int32_t(v[i + 2])) * x4.z * sw;
+          z[i + 3] = float(int32_t(v[i + 3])) * x4.w * sw;
+        }
+        if ((jc + 2) * 32 < t.rows) tmem_ld_32x32b_x32(d + uint32_t((jc + 2) * 32), v);
+        if constexpr (GLU) {
           // The gate warp finishes rows 0..15 of the chunk, the up warp rows
           // 16..31: each hands the other half over.
-          float z[32];
-#pragma unroll
-          for (int i = 0; i < 32; ++i) z[i] = float(int32_t(v[i])) * __shfl_sync(0xffffffffu, xv, i) * sw;
           named_bar_sync(bar_id, 64);  // the last chunk's have been read
 #pragma unroll
           for (int i = 0; i < 16; ++i) mine[i * 32 + lane] = up ? z[i] : z[16 + i];
           named_bar_sync(bar_id, 64);
+          const int first = up ? 16 : 0;
 #pragma unroll
           for (int i = 0; i < 16; ++i) {
             const float o = theirs[i * 32 + lane];
-            const int j = up ? 16 + i : i;
             const float h = up ? silu_mul(o, z[16 + i]) : silu_mul(z[i], o);
-            if (j < left && f < a.F) q_store(a, t.r0 + jc * 32 + j, f, h);
+            if (first + i < left && f < a.F) q_store(a, row + first + i, f, h);
           }
-        }
-      } else {
-        const int f = t.f * 256 + int(crank) * 128 + quarter * 32 + lane;
-        const float sw = f < a.N ? a.ws[int64_t(t.e) * a.N + f] : 0.f;
-        for (int jc = sub; jc * 32 < t.rows; jc += 2) {
-          uint32_t v[32];
-          tmem_ld_32x32b_x32(d + uint32_t(jc * 32), v);
-          const int left = t.rows - jc * 32;
-          const float xv = lane < left ? a.xs[t.r0 + jc * 32 + lane] : 0.f;
-          tmem_ld_wait();
+        } else if (a.out_f32) {
 #pragma unroll
-          for (int i = 0; i < 32; ++i) {
-            const float z = float(int32_t(v[i])) * __shfl_sync(0xffffffffu, xv, i) * sw;
-            if (i < left && f < a.N) q_store(a, t.r0 + jc * 32 + i, f, z);
+          for (int i = 0; i < 32; ++i)
+            if (i < left && f < a.F) static_cast<float*>(a.out)[(row + i) * a.F + f] = z[i];
+        } else {
+          // bf16, two rows to a word, through shared memory: a lane then
+          // holds eight channels of two rows, 16 bytes each.
+          uint32_t* words = reinterpret_cast<uint32_t*>(mine);
+#pragma unroll
+          for (int p = 0; p < 16; ++p) {
+            const __nv_bfloat162 b2 = __floats2bfloat162_rn(z[2 * p], z[2 * p + 1]);
+            words[p * 32 + lane] = *reinterpret_cast<const uint32_t*>(&b2);
+          }
+          __syncwarp();
+          __nv_bfloat16* out = static_cast<__nv_bfloat16*>(a.out);
+#pragma unroll
+          for (int step = 0; step < 2; ++step) {
+            const int p = (lane >> 2) + step * 8, c = (lane & 3) * 8;
+            const uint4 lo = *reinterpret_cast<const uint4*>(words + p * 32 + c);
+            const uint4 hi = *reinterpret_cast<const uint4*>(words + p * 32 + c + 4);
+            if (f0 + c >= a.F) continue;
+            __nv_bfloat16* o = out + (row + 2 * p) * a.F + f0 + c;
+            if (2 * p < left)
+              *reinterpret_cast<uint4*>(o) = make_uint4(__byte_perm(lo.x, lo.y, 0x5410), __byte_perm(lo.z, lo.w, 0x5410),
+                                                        __byte_perm(hi.x, hi.y, 0x5410), __byte_perm(hi.z, hi.w, 0x5410));
+            if (2 * p + 1 < left)
+              *reinterpret_cast<uint4*>(o + a.F) =
+                  make_uint4(__byte_perm(lo.x, lo.y, 0x7632), __byte_perm(lo.z, lo.w, 0x7632),
+                             __byte_perm(hi.x, hi.y, 0x7632), __byte_perm(hi.z, hi.w, 0x7632));
           }
         }
       }
@@ -422,52 +469,54 @@ __global__ void __launch_bounds__(kQThreads, 1)
   __syncwarp();
 
   if constexpr (SPLIT) {
-    cg::this_grid().sync();
-    // ---- the tile that this pair started and others went on with: one row
-    // per warp, the parts in flight together
-    const uint32_t units = uint32_t(tiles) * uint32_t(s.kb);
-    const uint32_t g = min(uint32_t(pairs), units);
-    if (uint32_t(pair) < g) {
+    if (split) {
+      cg::this_grid().sync();
+      // ---- the tile that this pair started and others went on with: four
+      // channels a thread, every part's loads in flight together
+      const uint32_t units = uint32_t(tiles) * uint32_t(s.kb);
+      const uint32_t g = min(uint32_t(pairs), units);
       const uint32_t lo = uint64_t(units) * pair / g, hi = uint64_t(units) * (pair + 1) / g;
       const uint32_t tile = (hi - 1) / s.kb, first = tile * s.kb, end = first + s.kb;
-      if (first >= lo && hi < end) {
+      if (uint32_t(pair) < g && first >= lo && hi < end) {
         const int c1 = int((uint64_t(end) * g - 1) / units);
         const QTile t = q_tile(s, int(tile));
-        auto at = [&](int c, int j) { return a.part + (size_t(c) * 2 + (c == pair ? 1 : 0)) * kQSlotInts + j * 256; };
-        for (int j = int(crank) * (kQThreads / 32) + warp; j < t.rows; j += 2 * (kQThreads / 32)) {
+        const int4* part = reinterpret_cast<const int4*>(a.part);
+        auto sum4 = [&](int at) {  // of int4 `at` of the slots
+          int4 z = __ldcg(part + (size_t(pair) * 2 + 1) * (kQSlotInts / 4) + at);
+#pragma unroll 4
+          for (int p = pair + 1; p <= c1; ++p) {
+            const int4 x = __ldcg(part + size_t(p) * 2 * (kQSlotInts / 4) + at);
+            z.x += x.x, z.y += x.y, z.z += x.z, z.w += x.w;
+          }
+          return z;
+        };
+        // Channels of a row: 64 int4 (both CTAs'); with SwiGLU the first 16
+        // of each CTA's 32 are gate, the others up.
+        constexpr int kPer = GLU ? 32 : 64;
+        const int total = t.rows * kPer;
+#pragma unroll 4
+        for (int i = int(crank) * kQThreads + int(threadIdx.x); i < total; i += 2 * kQThreads) {
+          const int j = i / kPer, c = i % kPer;
           const float xv = a.xs[t.r0 + j];
-#pragma unroll 1
-          for (int c = 0; c < 2; ++c) {  // the two CTAs' channels
-            if constexpr (GLU) {
-              const int fl = lane * 2, f = t.f * 128 + c * 64 + fl;
-              int2 gs = {0, 0}, us = {0, 0};
-#pragma unroll 4
-              for (int p = pair; p <= c1; ++p) {
-                const int2 x = __ldcg(reinterpret_cast<const int2*>(at(p, j) + c * 128 + fl));
-                const int2 y = __ldcg(reinterpret_cast<const int2*>(at(p, j) + c * 128 + 64 + fl));
-                gs.x += x.x, gs.y += x.y, us.x += y.x, us.y += y.y;
-              }
-              if (f < a.F) {
-                const float* sg = a.ws + int64_t(t.e) * a.N + f;
-                const float* su = sg + a.F;
-                q_store(a, t.r0 + j, f, silu_mul(float(gs.x) * xv * sg[0], float(us.x) * xv * su[0]));
-                q_store(a, t.r0 + j, f + 1, silu_mul(float(gs.y) * xv * sg[1], float(us.y) * xv * su[1]));
-              }
-            } else {
-              const int fl = c * 128 + lane * 4, f = t.f * 256 + fl;
-              int4 z = {0, 0, 0, 0};
-#pragma unroll 4
-              for (int p = pair; p <= c1; ++p) {
-                const int4 x = __ldcg(reinterpret_cast<const int4*>(at(p, j) + fl));
-                z.x += x.x, z.y += x.y, z.z += x.z, z.w += x.w;
-              }
-              if (f < a.N) {
-                const float* sw = a.ws + int64_t(t.e) * a.N + f;
-                q_store(a, t.r0 + j, f, float(z.x) * xv * sw[0]);
-                q_store(a, t.r0 + j, f + 1, float(z.y) * xv * sw[1]);
-                q_store(a, t.r0 + j, f + 2, float(z.z) * xv * sw[2]);
-                q_store(a, t.r0 + j, f + 3, float(z.w) * xv * sw[3]);
-              }
+          const float* sw = a.ws + int64_t(t.e) * a.N;
+          if constexpr (GLU) {
+            const int at = j * 64 + (c >> 4) * 32 + (c & 15), f = t.f * 128 + c * 4;
+            const int4 g4 = sum4(at), u4 = sum4(at + 16);
+            if (f < a.F) {
+              const float4 sg = *reinterpret_cast<const float4*>(sw + f);
+              const float4 su = *reinterpret_cast<const float4*>(sw + a.F + f);
+              q_store4(a, t.r0 + j, f, silu_mul(float(g4.x) * xv * sg.x, float(u4.x) * xv * su.x),
+                       silu_mul(float(g4.y) * xv * sg.y, float(u4.y) * xv * su.y),
+                       silu_mul(float(g4.z) * xv * sg.z, float(u4.z) * xv * su.z),
+                       silu_mul(float(g4.w) * xv * sg.w, float(u4.w) * xv * su.w));
+            }
+          } else {
+            const int f = t.f * 256 + c * 4;
+            const int4 z = sum4(j * 64 + c);
+            if (f < a.N) {
+              const float4 s4 = *reinterpret_cast<const float4*>(sw + f);
+              q_store4(a, t.r0 + j, f, float(z.x) * xv * s4.x, float(z.y) * xv * s4.y, float(z.z) * xv * s4.z,
+                       float(z.w) * xv * s4.w);
             }
           }
         }
@@ -515,8 +564,8 @@ constexpr int kQuantThreads = 256;
 // Rounds x / s half to even, exactly: |x / s| <= 127.5, inv = 1 / s rounded.
 // t holds the nearest integer of x * inv (within one of the answer) in its
 // low mantissa bits; the remainder x - q*s fits fp32.
+constexpr float kMagic = 12582912.f;  // 1.5 * 2^23
 __device__ __forceinline__ int quant_one(float x, float s, float half, float inv) {
-  constexpr float kMagic = 12582912.f;  // 1.5 * 2^23
   const float t = fmaf(x, inv, kMagic);
   int q = __float_as_int(t) - __float_as_int(kMagic);
   const float r = fmaf(-(t - kMagic), s, x);
@@ -524,6 +573,28 @@ __device__ __forceinline__ int quant_one(float x, float s, float half, float inv
   if (r > half || (r == half && odd)) ++q;
   if (r < -half || (r == -half && odd)) --q;
   return max(-127, min(127, q));
+}
+
+// Eight values.  x * inv is within 127 * 3 * 2^-24 < 3e-5 of the quotient, so
+// its rounding is the quotient's unless it lies nearer than that to a tie:
+// only then (about 1 value in 4000, more where the values are coarse) the
+// exact form runs.  t's low byte is the integer in two's complement.
+__device__ __forceinline__ uint2 quant8(const float (&x)[8], float s, float inv, bool exact) {
+  uint32_t t[8];
+  float far = 0.f;
+#pragma unroll
+  for (int i = 0; i < 8; ++i) {
+    const float y = fmaf(x[i], inv, kMagic);
+    far = fmaxf(far, fabsf(fmaf(x[i], inv, kMagic - y)));
+    t[i] = __float_as_uint(y);
+  }
+  if (exact || far > 0.49995f) {
+    const float half = 0.5f * s;
+#pragma unroll
+    for (int i = 0; i < 8; ++i) t[i] = uint32_t(quant_one(x[i], s, half, inv));
+  }
+  return make_uint2(__byte_perm(__byte_perm(t[0], t[1], 0x0040), __byte_perm(t[2], t[3], 0x0040), 0x5410),
+                    __byte_perm(__byte_perm(t[4], t[5], 0x0040), __byte_perm(t[6], t[7], 0x0040), 0x5410));
 }
 
 __device__ __forceinline__ void load8(const __nv_bfloat16* p, float (&v)[8]) {
@@ -587,21 +658,20 @@ __global__ void __launch_bounds__(kQuantThreads)
     // Infinities and NaN (largest as numbers): no scale holds the row, and a
     // NaN scale says so in every output.
     const bool bad = top >= 0x7f800000u;
-    const float s0 = bad ? __int_as_float(0x7fffffff) : __uint_as_float(top) / 127.f;
+    const float s0 = bad ? __int_as_float(0x7fffffff) : __uint_as_float(top) * (1.f / 127.f);
     if (c == 0) scale[r] = s0;
     const bool zero = bad || s0 == 0.f;
-    // Tiny rows: the reciprocal would overflow; powers of two change nothing.
-    const float up = s0 < 0x1p-90f ? 0x1p100f : 1.f;
-    const float s = zero ? 1.f : s0 * up, half = 0.5f * s, inv = 1.f / s;
+    // Tiny rows: the reciprocal would overflow (powers of two change
+    // nothing), and a scale below the normal numbers is coarse.
+    const bool tiny = s0 < 0x1p-90f;
+    const float up = tiny ? 0x1p100f : 1.f, s = zero ? 1.f : s0 * up, inv = 1.f / s;
     int8_t* dst = q + r * K;
-    auto put = [&](int g, const float (&w)[8]) {
-      uint32_t b[2] = {0, 0};
+    auto put = [&](int g, float (&w)[8]) {
+      if (tiny) {
 #pragma unroll
-      for (int i = 0; i < 8; ++i) {
-        const int n = zero ? 0 : quant_one(w[i] * up, s, half, inv);
-        b[i >> 2] |= uint32_t(n & 0xff) << (8 * (i & 3));
+        for (int i = 0; i < 8; ++i) w[i] *= up;
       }
-      *reinterpret_cast<uint2*>(dst + g * 8) = make_uint2(b[0], b[1]);
+      *reinterpret_cast<uint2*>(dst + g * 8) = zero ? make_uint2(0u, 0u) : quant8(w, s, inv, tiny);
     };
 #pragma unroll
     for (int j = 0; j < VPT; ++j)
@@ -625,9 +695,11 @@ int launch_quant(const void* x, int64_t rows, int K, const int32_t* perm, const 
   const In* xi = static_cast<const In*>(x);
   int8_t* qi = static_cast<int8_t*>(q);
   const unsigned g = unsigned(blocks);
+  // (Eight groups where even all threads leave more: 16384 values.)
   if (vpt <= 1) quant_rows_kernel<In, 1><<<g, kQuantThreads, 0, stream>>>(xi, rows, K, perm, live, tpr, qi, scale);
   else if (vpt <= 2) quant_rows_kernel<In, 2><<<g, kQuantThreads, 0, stream>>>(xi, rows, K, perm, live, tpr, qi, scale);
-  else quant_rows_kernel<In, 4><<<g, kQuantThreads, 0, stream>>>(xi, rows, K, perm, live, tpr, qi, scale);
+  else if (vpt <= 4) quant_rows_kernel<In, 4><<<g, kQuantThreads, 0, stream>>>(xi, rows, K, perm, live, tpr, qi, scale);
+  else quant_rows_kernel<In, 8><<<g, kQuantThreads, 0, stream>>>(xi, rows, K, perm, live, tpr, qi, scale);
   return cudaGetLastError() == cudaSuccess ? kOk : kCudaErr;
 }
 
@@ -635,8 +707,9 @@ int launch_quant(const void* x, int64_t rows, int K, const int32_t* perm, const 
 // y[t] = sum over k of v[t, k] * rows[offsets[e] + slots[t, k]], e = ids[t, k];
 // slot -1: not routed here.  fp32 in the order of k, one rounding to bf16.
 constexpr int kSumThreads = 256;
+template <typename In>
 __global__ void __launch_bounds__(kSumThreads)
-    weighted_sum_kernel(const __nv_bfloat16* __restrict__ src, const void* __restrict__ ids, int ids64, int first,
+    weighted_sum_kernel(const In* __restrict__ src, const void* __restrict__ ids, int ids64, int first,
                         const void* __restrict__ vals, int vals_bf16, const int32_t* __restrict__ slots,
                         const int32_t* __restrict__ offsets, int64_t T, int K, int H, int E,
                         __nv_bfloat16* __restrict__ y) {
@@ -685,10 +758,10 @@ static_assert(1024 + size_t(kQStages) * kQStageBytes + kQXBytes + sizeof(QSmem) 
               "shared memory plan exceeds 227 KB");
 static_assert((kQStages * kQStageBytes + kQXBytes) % 16 == 0, "QSmem must start on a 16-byte boundary");
 
-// Products with fewer tiles than four per pair are split over K.
+// Whether a product may have fewer tiles than kQWaves per pair.
 bool q_split(int64_t rows, int N, int F, bool glu, int pairs) {
   const int64_t ft = glu ? (F + 127) / 128 : (N + 255) / 256;
-  return (rows + kQTileRows - 1) / kQTileRows * ft < 4 * int64_t(pairs);
+  return (rows + kQTileRows - 1) / kQTileRows * ft < kQWaves * int64_t(pairs);
 }
 
 int encode_s8(CUtensorMap* m, int rank, const void* ptr, const cuuint64_t* dims, const cuuint64_t* strides,
@@ -769,7 +842,9 @@ extern "C" int moe_w8a8_gemm(const moe_w8a8_params* p, void* stream) {
   if (!p || !q_sizes_ok(p->rows, p->K, p->N, p->experts, p->swiglu)) return kBadArg;
   if (p->rows == 0) return kOk;
   if (!p->xq || !p->xs || !p->wq || !p->ws || !p->out || (!p->counts && p->experts != 1)) return kBadArg;
-  if (misaligned16(p->xq) || misaligned16(p->wq) || misaligned16(p->scratch)) return kBadArg;
+  if (misaligned16(p->xq) || misaligned16(p->wq) || misaligned16(p->ws) || misaligned16(p->out) ||
+      misaligned16(p->scratch))
+    return kBadArg;
   if (!driver().ok) return kCudaErr;
   int sms = 0;
   if (sm_count(&sms) != kOk) return kCudaErr;
@@ -810,7 +885,7 @@ extern "C" int moe_w8a8_gemm(const moe_w8a8_params* p, void* stream) {
   return split ? launch_w8a8<false, true>(tw, tx, a, pairs, s) : launch_w8a8<false, false>(tw, tx, a, pairs, s);
 }
 
-extern "C" int moe_weighted_sum(const void* rows, const void* top_idxs, int32_t ids_are_int64, int32_t first_expert,
+extern "C" int moe_weighted_sum(const void* rows, int32_t rows_are_f32, const void* top_idxs, int32_t ids_are_int64, int32_t first_expert,
                                 const void* top_vals, int32_t vals_are_bf16, const int32_t* slots,
                                 const int32_t* offsets, int64_t T, int32_t K, int32_t H, int32_t experts, void* y,
                                 void* stream) {
@@ -823,8 +898,12 @@ extern "C" int moe_weighted_sum(const void* rows, const void* top_idxs, int32_t 
   int sms = 0;
   if (sm_count(&sms) != kOk) return kCudaErr;
   const int64_t blocks = std::min<int64_t>((T * (H / 8) + kSumThreads - 1) / kSumThreads, int64_t(sms) * 8);
-  weighted_sum_kernel<<<unsigned(blocks), kSumThreads, 0, static_cast<cudaStream_t>(stream)>>>(
-      static_cast<const __nv_bfloat16*>(rows), top_idxs, ids_are_int64, first_expert, top_vals, vals_are_bf16, slots,
-      offsets, T, K, H, experts, static_cast<__nv_bfloat16*>(y));
+  const auto launch = [&](auto* src) {
+    weighted_sum_kernel<<<unsigned(blocks), kSumThreads, 0, static_cast<cudaStream_t>(stream)>>>(
+        src, top_idxs, ids_are_int64, first_expert, top_vals, vals_are_bf16, slots, offsets, T, K, H, experts,
+        static_cast<__nv_bfloat16*>(y));
+  };
+  if (rows_are_f32) launch(static_cast<const float*>(rows));
+  else launch(static_cast<const __nv_bfloat16*>(rows));
   return cudaGetLastError() == cudaSuccess ? kOk : kCudaErr;
 }

@@ -60,7 +60,7 @@ def quantize_rows(x: torch.Tensor, perm: torch.Tensor | None = None,
                   live_rows: torch.Tensor | None = None) -> tuple[torch.Tensor, torch.Tensor]:
     """``(q [rows, K] int8, scale [rows] float32)`` of x [n, K], bf16 or fp32.
 
-    scale = max|row| / 127 (fp32) and q the exact quotient, rounded half to
+    scale = max|row| * (1/127) in fp32 and q the exact quotient, rounded half to
     even.  With ``perm`` [rows] int32, row r is x[perm[r]] (``Routing.perm``:
     the send buffer of ``utils.pack_compact``, quantised on the way); rows
     from ``live_rows`` (one int32 on the device, e.g. ``Routing.offsets[-1:]``)
@@ -220,8 +220,9 @@ def moe_layer(x: torch.Tensor, top_idxs: torch.Tensor, top_vals: torch.Tensor, w
         q, scale = quantize_rows(x, r.perm, r.offsets[El:])
         h = grouped_gemm(q, scale, w13, r.counts, swiglu=True, out_dtype=torch.float32, status=status)
         q, scale = quantize_rows(h, live_rows=r.offsets[El:])
-        rows = grouped_gemm(q, scale, w2, r.counts, status=status)
-        N.check(N.lib().moe_weighted_sum(rows.data_ptr(), ids.data_ptr(), ids.dtype == torch.int64, first_expert,
+        # fp32 rows: y is rounded once, like a layer that never splits its sum
+        rows = grouped_gemm(q, scale, w2, r.counts, out_dtype=torch.float32, status=status)
+        N.check(N.lib().moe_weighted_sum(rows.data_ptr(), 1, ids.data_ptr(), ids.dtype == torch.int64, first_expert,
                                          vals.data_ptr(), vals.dtype == torch.bfloat16, r.slots.data_ptr(),
                                          r.offsets.data_ptr(), T, K, H, El, y.data_ptr(), stream),
                 "moe_weighted_sum")

@@ -14,15 +14,15 @@ from nvshmem_testing_b200 import utils, w8a8
 pytestmark = pytest.mark.gpu
 
 HALF = 2.0 ** -8
+RECIP = float(torch.tensor(1.0) / torch.tensor(127.0))  # 1/127 in fp32
 
 
 def quant_ref(x):
     """(q, scale) by definition: the scale in fp32, the quotient in 64 bits
     (24-bit operands: no quotient is nearer to a tie than 2^-48 without being
-    one; and top / 127 in 64 bits, rounded, is the fp32 quotient, where
-    torch's division by a host number multiplies with a rounded reciprocal)."""
+    one)."""
     top = x.float().abs().amax(1)
-    scale = (top.double() / torch.tensor(127.0, dtype=torch.float64, device=x.device)).float()
+    scale = top * RECIP
     q = torch.where(scale[:, None] > 0, x.double() / scale.double()[:, None], 0.0).round().clamp(-127, 127)
     bad = ~torch.isfinite(x.float()).all(1)
     q[bad], scale[bad] = 0, float("nan")
@@ -247,7 +247,7 @@ def layer_ref(x, ids, vals, w13, w2, first):
             h, dh = h[0], dh[0]
             top = h.abs().max()
             rel = float(dh.max() / top) + 2.0 ** -22 if float(top) > 0 else 0.0
-            scale = (top / torch.tensor(127.0, dtype=torch.float64, device=x.device)).float().double()
+            scale = (top.float() * RECIP).double()
             quot = torch.where(scale > 0, h / scale, torch.zeros_like(h))
             hq = quot.round().clamp(-127, 127)
             near = ((quot - quot.floor()) - 0.5).abs() <= quot.abs() * rel + dh / scale.clamp_min(1e-300) + 1e-12
@@ -255,7 +255,7 @@ def layer_ref(x, ids, vals, w13, w2, first):
             o = wd @ (hq * scale)
             v = float(vals[t, k])
             y[t] += v * o
-            tol[t] += abs(v) * (wd.abs() @ ((near.double() + hq.abs() * rel) * scale) + o.abs() * (HALF + 2.0 ** -20))
+            tol[t] += abs(v) * (wd.abs() @ ((near.double() + hq.abs() * rel) * scale) + o.abs() * 2.0 ** -20)
     return y, tol * (1 + HALF) + y.abs() * HALF + 1e-30
 
 
@@ -331,7 +331,7 @@ def test_weighted_sum_uses_the_routing():
     r = utils.route(ids, E, with_slots=True)
     rows = torch.randn(T * K, H, generator=g, device="cuda").to(torch.bfloat16)
     y = torch.empty(T, H, dtype=torch.bfloat16, device="cuda")
-    N.check(N.lib().moe_weighted_sum(rows.data_ptr(), ids.data_ptr(), 1, 0, vals.data_ptr(), 0, r.slots.data_ptr(),
+    N.check(N.lib().moe_weighted_sum(rows.data_ptr(), 0, ids.data_ptr(), 1, 0, vals.data_ptr(), 0, r.slots.data_ptr(),
                                      r.offsets.data_ptr(), T, K, H, E, y.data_ptr(), None), "moe_weighted_sum")
     ref = torch.zeros(T, H, dtype=torch.float64, device="cuda")
     mag = torch.zeros_like(ref)

@@ -71,6 +71,6 @@ def test_c_entries_refuse_before_any_device_call():
     assert lib.moe_quant_rows(None, 0, 4, 64, None, None, None, None, None) == N.BAD_ARG
     assert lib.moe_quant_rows(None, 0, 4, 63, None, None, None, None, None) == N.BAD_ARG
     assert lib.moe_quant_rows(None, 0, 0, 64, None, None, None, None, None) == N.OK
-    assert lib.moe_weighted_sum(None, None, 1, 0, None, 0, None, None, 4, 2, 64, 2, None, None) == N.BAD_ARG
-    assert lib.moe_weighted_sum(None, None, 1, 0, None, 0, None, None, 4, 33, 64, 2, None, None) == N.BAD_ARG
-    assert lib.moe_weighted_sum(None, None, 1, 0, None, 0, None, None, 0, 2, 64, 2, None, None) == N.OK
+    assert lib.moe_weighted_sum(None, 0, None, 1, 0, None, 0, None, None, 4, 2, 64, 2, None, None) == N.BAD_ARG
+    assert lib.moe_weighted_sum(None, 0, None, 1, 0, None, 0, None, None, 4, 33, 64, 2, None, None) == N.BAD_ARG
+    assert lib.moe_weighted_sum(None, 0, None, 1, 0, None, 0, None, None, 0, 2, 64, 2, None, None) == N.OK
