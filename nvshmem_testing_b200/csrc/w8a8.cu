@@ -78,7 +78,7 @@ struct alignas(16) QSmem {
   uint64_t tfull[2];         // each CTA: sums ready
   uint64_t tempty[2];        // leader: both CTAs' epilogues are done with them
   uint64_t drain;
-  uint32_t fills[kQStages], cons[kQStages];
+  uint32_t fills, used;      // stages loaded, multiplied (leader)
   uint32_t tmem_base;
   int err;
 };
@@ -234,13 +234,13 @@ __global__ void __launch_bounds__(kQThreads, 1)
     for (int i = 0; i < kQStages; ++i) {
       mbar_init(&sm.full[i], 1);
       mbar_init(&sm.empty[i], 1);
-      sm.fills[i] = sm.cons[i] = 0;
     }
     for (int i = 0; i < 2; ++i) {
       mbar_init(&sm.tfull[i], 1);
       mbar_init(&sm.tempty[i], 2 * kQEpiWarps);
     }
     mbar_init(&sm.drain, 1);
+    sm.fills = sm.used = 0;
     sm.err = 0;
     fence_mbar_init();
     prefetch_tensormap(&tm_w);
@@ -297,6 +297,7 @@ __global__ void __launch_bounds__(kQThreads, 1)
     // ---- loads: each CTA its 128 channels and half of the tile's rows, all
     // onto the leader's barrier
     QRing r = {0, 0};
+    uint32_t fills = 0;
     const uint32_t bar0 = mapa_shared(smem_u32(&sm.full[0]), 0);
     bool stop = false;
     for (QWalk w(s, split, tiles, pair, pairs); w.more() && !stop; w.next()) {
@@ -321,14 +322,19 @@ __global__ void __launch_bounds__(kQThreads, 1)
           tma_load_3d_pair(&tm_w, bar, dst, k * kQKb, t.f * 256 + int(crank) * 128, t.e);
         }
         tma_load_2d_pair(&tm_x.m[bm], bar, dst + kQABytes, k * kQKb, row);
-        sm.fills[r.st] += 1;
+        ++fills;
         r.next(kQStages);
       }
     }
+    sm.fills = fills;
   } else if (warp == 1 && lane == 0 && leader) {
-    // ---- MMA
+    // ---- MMA.  The tensor pipe takes few instructions ahead, so the issuing
+    // thread's own work per stage must fit beside one MMA: descriptors are
+    // sums.
     QRing r = {0, 0}, acc = {0, 0};
     bool stop = false;
+    uint32_t used = 0;  // stages multiplied
+    const uint64_t desc0 = smem_desc_sw128(smem_u32(stage), 16, 1024);
     for (QWalk w(s, split, tiles, pair, pairs); w.more() && !stop; w.next()) {
       const QTile t = q_tile(s, w.tile);
       const uint32_t idesc = make_idesc_i8(256, uint32_t(t.n));
@@ -339,6 +345,7 @@ __global__ void __launch_bounds__(kQThreads, 1)
       }
       tc_fence_after();
       const uint32_t d = tmem + uint32_t(acc.st) * 256;
+      uint32_t more = 0;  // adds to the sums from the second MMA on
       for (int k = w.k0; k < w.k1; ++k) {
         if (!q_wait(&sm.full[r.st], r.ph, sm)) {
           q_fail(sm, a, 3);
@@ -346,19 +353,21 @@ __global__ void __launch_bounds__(kQThreads, 1)
           break;
         }
         tc_fence_after();
-        const uint32_t aa = smem_u32(stage + uint32_t(r.st) * kQStageBytes), ba = aa + kQABytes;
+        const uint64_t da = desc0 + uint32_t(r.st) * (kQStageBytes >> 4), db = da + (kQABytes >> 4);
 #pragma unroll
-        for (int kk = 0; kk < kQKb / 32; ++kk)
-          tc_mma_i8_pair(d, smem_desc_sw128(aa + kk * 32, 16, 1024), smem_desc_sw128(ba + kk * 32, 16, 1024), idesc,
-                         (k != w.k0 || kk != 0) ? 1u : 0u);
+        for (int kk = 0; kk < kQKb / 32; ++kk) {
+          tc_mma_i8_pair(d, da + kk * 2, db + kk * 2, idesc, more);
+          more = 1;
+        }
         tc_commit_pair_mc(&sm.empty[r.st], 0x3);
-        sm.cons[r.st] += 1;
+        ++used;
         r.next(kQStages);
       }
       if (stop) break;
       tc_commit_pair_mc(&sm.tfull[acc.st], 0x3);
       acc.next(2);
     }
+    sm.used = used;
   } else if (warp >= kQEpi0) {
     // ---- epilogue: chunks of 32 rows, even ones by the first four warps
     QRing acc = {0, 0};
@@ -535,10 +544,9 @@ __global__ void __launch_bounds__(kQThreads, 1)
   }
   cluster_sync();
   if (leader && threadIdx.x == 0) {
-    for (int i = 0; i < kQStages; ++i) {
-      if (sm.fills[i] == sm.cons[i]) continue;
+    for (uint32_t i = sm.used; i < sm.fills; ++i) {  // loaded, never multiplied
       const uint64_t until = globaltimer_ns() + kQBoundNs;
-      while (!mbar_try_wait(&sm.full[i], (sm.fills[i] - 1) & 1) && globaltimer_ns() < until) {
+      while (!mbar_try_wait(&sm.full[i % kQStages], (i / kQStages) & 1) && globaltimer_ns() < until) {
       }
     }
   }
