@@ -29,6 +29,7 @@
 #include <cuda_bf16.h>
 #include <cuda_runtime.h>
 
+#include <atomic>
 #include <climits>
 #include <type_traits>
 
@@ -41,6 +42,7 @@ namespace {
 
 namespace cg = cooperative_groups;
 
+constexpr int kMaxDevices = 64;
 constexpr int kDecMaxT = 64;
 constexpr int kDecMaxRows = 1024;                 // T * K
 constexpr int kDecMaxH = 32768;
@@ -49,7 +51,7 @@ constexpr int kDecEpi0 = 2;                       // warps: 0 loads, 1 MMA, 2.. 
 constexpr int kDecThreads = (kDecEpi0 + kDecEpiWarps) * 32;
 constexpr int kDecMaxStages = 8;
 constexpr uint32_t kDecABytes = 256 * 64 * 2;     // 256 features x 64 K
-constexpr uint32_t kDecMaxSmem = 227 * 1024;
+constexpr uint32_t kDecMaxSmem = 226 * 1024;      // dynamic; under 1 KB is static
 constexpr int kDecTokChunk = 8;                   // router: tokens whose logits a thread sums at a time
 constexpr uint64_t kDecBoundNs = 2000000000ull;   // bug guard on every pipeline wait
 constexpr int kBarEpi = 1;
@@ -1052,8 +1054,15 @@ extern "C" int moe_decode_layer(const moe_decode_params* p, void* stream) {
     const cuuint32_t box[2] = {64, 16};
     if (encode(&mh, 2, a.hs, dims, str, box)) return kCudaErr;
   }
-  if (cudaFuncSetAttribute(decode_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, int(smem)) != cudaSuccess)
-    return kCudaErr;
+  // Once per device: shared memory opted in to.
+  static std::atomic<bool> ready[kMaxDevices];
+  if (dev < 0 || dev >= kMaxDevices) return kCudaErr;
+  if (!ready[dev].load(std::memory_order_acquire)) {
+    if (cudaFuncSetAttribute(decode_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, int(kDecMaxSmem)) !=
+        cudaSuccess)
+      return kCudaErr;
+    ready[dev].store(true, std::memory_order_release);
+  }
   cudaLaunchConfig_t cfg = {};
   cfg.gridDim = dim3(unsigned(sms));
   cfg.blockDim = dim3(kDecThreads);

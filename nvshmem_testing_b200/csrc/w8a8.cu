@@ -30,6 +30,7 @@
 #include <cuda_runtime.h>
 
 #include <algorithm>
+#include <atomic>
 
 #include "moe_ep.h"
 #include "moe_ep_internal.h"
@@ -750,9 +751,10 @@ __global__ void __launch_bounds__(kSumThreads)
 }
 
 // ---------------------------------------------------------------- host side
-int sm_count(int* sms) {
+int sm_count(int* sms, int* device = nullptr) {
   int dev = 0;
   if (cudaGetDevice(&dev) != cudaSuccess) return kCudaErr;
+  if (device) *device = dev;
   return cudaDeviceGetAttribute(sms, cudaDevAttrMultiProcessorCount, dev) == cudaSuccess ? kOk : kCudaErr;
 }
 
@@ -783,12 +785,31 @@ int encode_s8(CUtensorMap* m, int rank, const void* ptr, const cuuint64_t* dims,
              : kCudaErr;
 }
 
+// Once per device and form: shared memory opted in to, and the CTA pairs that
+// can be resident together (the split form's meet at a grid barrier).
+constexpr int kMaxDevices = 64;
 template <bool GLU, bool SPLIT>
-int launch_w8a8(const CUtensorMap& tw, const QRowMaps& tx, const QArgs& a, int pairs, cudaStream_t stream) {
-  const size_t smem = q_smem_bytes(a.E);
-  if (cudaFuncSetAttribute(w8a8_kernel<GLU, SPLIT>, cudaFuncAttributeMaxDynamicSharedMemorySize, int(smem)) !=
-      cudaSuccess)
-    return kCudaErr;
+int w8a8_pairs(int dev, int sms, cudaLaunchConfig_t cfg, int* out) {
+  static std::atomic<int> known[kMaxDevices];
+  if (dev < 0 || dev >= kMaxDevices) return kCudaErr;
+  int n = known[dev].load(std::memory_order_acquire);
+  if (n == 0) {
+    const size_t smem = q_smem_bytes(kMaxExperts);
+    if (cudaFuncSetAttribute(w8a8_kernel<GLU, SPLIT>, cudaFuncAttributeMaxDynamicSharedMemorySize, int(smem)) !=
+        cudaSuccess)
+      return kCudaErr;
+    cfg.gridDim = dim3(unsigned(sms & ~1));
+    cfg.dynamicSmemBytes = smem;
+    if (cudaOccupancyMaxActiveClusters(&n, w8a8_kernel<GLU, SPLIT>, &cfg) != cudaSuccess || n < 1) return kCudaErr;
+    n = std::min(n, sms / 2);
+    known[dev].store(n, std::memory_order_release);
+  }
+  *out = n;
+  return kOk;
+}
+
+template <bool GLU, bool SPLIT>
+int launch_w8a8(const CUtensorMap& tw, const QRowMaps& tx, const QArgs& a, int dev, int sms, cudaStream_t stream) {
   cudaLaunchConfig_t cfg = {};
   cudaLaunchAttribute at[2];
   at[0].id = cudaLaunchAttributeClusterDimension;
@@ -797,17 +818,14 @@ int launch_w8a8(const CUtensorMap& tw, const QRowMaps& tx, const QArgs& a, int p
   at[0].val.clusterDim.z = 1;
   at[1].id = cudaLaunchAttributeCooperative;
   at[1].val.cooperative = 1;
-  cfg.gridDim = dim3(unsigned(2 * pairs));
   cfg.blockDim = dim3(kQThreads);
-  cfg.dynamicSmemBytes = smem;
   cfg.stream = stream;
   cfg.attrs = at;
   cfg.numAttrs = 1;
-  // The split form's pairs meet at a grid barrier, so no more of them than
-  // can be resident together.
-  int fit = 0;
-  if (cudaOccupancyMaxActiveClusters(&fit, w8a8_kernel<GLU, SPLIT>, &cfg) != cudaSuccess || fit < 1) return kCudaErr;
-  cfg.gridDim = dim3(unsigned(2 * std::min(pairs, fit)));
+  int pairs = 0;
+  if (w8a8_pairs<GLU, SPLIT>(dev, sms, cfg, &pairs) != kOk) return kCudaErr;
+  cfg.gridDim = dim3(unsigned(2 * pairs));
+  cfg.dynamicSmemBytes = q_smem_bytes(a.E);
   cfg.numAttrs = SPLIT ? 2 : 1;
   return cudaLaunchKernelEx(&cfg, w8a8_kernel<GLU, SPLIT>, tw, tx, a) == cudaSuccess ? kOk : kCudaErr;
 }
@@ -854,8 +872,8 @@ extern "C" int moe_w8a8_gemm(const moe_w8a8_params* p, void* stream) {
       misaligned16(p->scratch))
     return kBadArg;
   if (!driver().ok) return kCudaErr;
-  int sms = 0;
-  if (sm_count(&sms) != kOk) return kCudaErr;
+  int sms = 0, dev = 0;
+  if (sm_count(&sms, &dev) != kOk) return kCudaErr;
   const int pairs = sms / 2;
   const bool glu = p->swiglu != 0;
   QArgs a = {};
@@ -882,15 +900,17 @@ extern "C" int moe_w8a8_gemm(const moe_w8a8_params* p, void* stream) {
     const cuuint32_t box[3] = {cuuint32_t(kQKb), glu ? 64u : 128u, 1};
     if (encode_s8(&tw, 3, p->wq, dims, str, box)) return kCudaErr;
   }
-  for (int i = 0; i < kQRowMaps; ++i) {
+  // Boxes of 16, 32, ... rows, as far as half a tile's rows may need.
+  for (int i = 0; i < kQRowMaps && (i == 0 || (8 << i) < (a.rows + 31) / 32 * 16); ++i) {
     const cuuint64_t dims[2] = {cuuint64_t(a.K), cuuint64_t(a.rows)};
     const cuuint64_t str[1] = {cuuint64_t(a.K)};
     const cuuint32_t box[2] = {cuuint32_t(kQKb), 16u << i};
     if (encode_s8(&tx.m[i], 2, p->xq, dims, str, box)) return kCudaErr;
   }
   const cudaStream_t s = static_cast<cudaStream_t>(stream);
-  if (glu) return split ? launch_w8a8<true, true>(tw, tx, a, pairs, s) : launch_w8a8<true, false>(tw, tx, a, pairs, s);
-  return split ? launch_w8a8<false, true>(tw, tx, a, pairs, s) : launch_w8a8<false, false>(tw, tx, a, pairs, s);
+  if (glu)
+    return split ? launch_w8a8<true, true>(tw, tx, a, dev, sms, s) : launch_w8a8<true, false>(tw, tx, a, dev, sms, s);
+  return split ? launch_w8a8<false, true>(tw, tx, a, dev, sms, s) : launch_w8a8<false, false>(tw, tx, a, dev, sms, s);
 }
 
 extern "C" int moe_weighted_sum(const void* rows, int32_t rows_are_f32, const void* top_idxs, int32_t ids_are_int64, int32_t first_expert,

@@ -49,7 +49,8 @@ class on_device:
         self.back = torch.cuda.current_device()
         if self.back != self.dev.index:
             torch.cuda.set_device(self.dev.index)
-        return _stream_ptr(self.dev)
+        # the raw handle: a Stream object costs the host as much as the launch
+        return ctypes.c_void_p(torch._C._cuda_getCurrentRawStream(self.dev.index))
 
     def __exit__(self, *exc):
         if self.back != self.dev.index:

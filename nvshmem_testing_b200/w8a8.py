@@ -50,6 +50,15 @@ def _check_weights(w: QuantWeights, name: str) -> tuple[int, int, int]:
     return tuple(w.q.shape)
 
 
+def _check_product(K: int, Nw: int, El: int, swiglu: bool):
+    if K % 16 or not 0 < K <= 131056:
+        raise ValueError(f"K = {K} must be a multiple of 16, 131056 at most")
+    if Nw % (16 if swiglu else 8) or Nw == 0:
+        raise ValueError(f"{Nw} channels: a multiple of {16 if swiglu else 8} is needed")
+    if El > 1024:
+        raise ValueError(f"{El} experts: 1024 at most")
+
+
 def _on_gpu(device, **tensors):
     for name, t in tensors.items():
         if t is not None and (not t.is_cuda or t.device != device):
@@ -76,15 +85,19 @@ def quantize_rows(x: torch.Tensor, perm: torch.Tensor | None = None,
     if live_rows is not None and (live_rows.dtype != torch.int32 or live_rows.numel() != 1):
         raise TypeError("live_rows must be one int32")
     _on_gpu(x.device, x=x, perm=perm, live_rows=live_rows)
-    x = x.contiguous()
     rows = x.shape[0] if perm is None else perm.shape[0]
+    with utils.on_device(x.device) as stream:
+        return _quantize(x.contiguous(), rows, K, perm, live_rows, stream)
+
+
+def _quantize(x, rows, K, perm, live_rows, stream):
+    """The checked call."""
     q = torch.empty((rows, K), dtype=torch.int8, device=x.device)
     scale = torch.empty(rows, dtype=torch.float32, device=x.device)
-    with utils.on_device(x.device) as stream:
-        N.check(N.lib().moe_quant_rows(x.data_ptr(), x.dtype == torch.float32, rows, K,
-                                       None if perm is None else perm.data_ptr(),
-                                       None if live_rows is None else live_rows.data_ptr(), q.data_ptr(),
-                                       scale.data_ptr(), stream), "moe_quant_rows")
+    N.check(N.lib().moe_quant_rows(x.data_ptr(), x.dtype == torch.float32, rows, K,
+                                   None if perm is None else perm.data_ptr(),
+                                   None if live_rows is None else live_rows.data_ptr(), q.data_ptr(),
+                                   scale.data_ptr(), stream), "moe_quant_rows")
     return q, scale
 
 
@@ -125,12 +138,7 @@ def grouped_gemm(xq: torch.Tensor, xs: torch.Tensor, w: QuantWeights, counts: to
         raise ValueError(f"xq {tuple(xq.shape)} and xs {tuple(xs.shape)} do not match w {tuple(w.q.shape)}")
     if xq.dtype != torch.int8 or xs.dtype != torch.float32:
         raise TypeError("xq must be int8 and xs float32")
-    if K % 16 or not 0 < K <= 131056:
-        raise ValueError(f"K = {K} must be a multiple of 16, 131056 at most")
-    if Nw % (16 if swiglu else 8) or Nw == 0:
-        raise ValueError(f"{Nw} channels: a multiple of {16 if swiglu else 8} is needed")
-    if El > 1024:
-        raise ValueError(f"{El} experts: 1024 at most")
+    _check_product(K, Nw, El, swiglu)
     if counts is None:
         if El != 1:
             raise ValueError("counts may be left out for one expert only")
@@ -148,28 +156,41 @@ def grouped_gemm(xq: torch.Tensor, xs: torch.Tensor, w: QuantWeights, counts: to
     _on_gpu(xq.device, xq=xq, xs=xs, q=w.q, scale=w.scale, counts=counts, out=out)
     if rows == 0:
         return out
-    xq, xs = xq.contiguous(), xs.contiguous()
+    with utils.on_device(xq.device) as stream:
+        _gemm(xq.contiguous(), xs.contiguous(), w, counts, rows, K, Nw, El, swiglu, out, status, stream)
+    return out
+
+
+def _gemm(xq, xs, w, counts, rows, K, Nw, El, swiglu, out, status, stream):
+    """The checked call."""
     need = _scratch_bytes(rows, K, Nw, El, int(swiglu), xq.device.index)
     scratch = torch.empty(need, dtype=torch.uint8, device=xq.device) if need else None
-    p = N.W8A8Params()
-    p.rows, p.K, p.N, p.experts, p.swiglu, p.out_is_f32 = rows, K, Nw, El, swiglu, out_dtype == torch.float32
-    p.xq, p.xs, p.wq, p.ws, p.out = (xq.data_ptr(), xs.data_ptr(), w.q.data_ptr(), w.scale.data_ptr(),
-                                     out.data_ptr())
-    p.counts = None if counts is None else counts.data_ptr()
-    p.scratch, p.scratch_bytes = (None, 0) if scratch is None else (scratch.data_ptr(), need)
-    p.status_host = None if status is None else status.data_ptr()
-    with utils.on_device(xq.device) as stream:
-        N.check(N.lib().moe_w8a8_gemm(ctypes.byref(p), stream), "moe_w8a8_gemm")
-    return out
+    p = N.W8A8Params(rows, K, Nw, El, swiglu, out.dtype == torch.float32, 0, xq.data_ptr(), xs.data_ptr(),
+                     w.q.data_ptr(), w.scale.data_ptr(), None if counts is None else counts.data_ptr(),
+                     out.data_ptr(), None if scratch is None else scratch.data_ptr(), need,
+                     None if status is None else status.data_ptr())
+    N.check(N.lib().moe_w8a8_gemm(ctypes.byref(p), stream), "moe_w8a8_gemm")
 
 
 def linear(x: torch.Tensor, w: QuantWeights, *, out_dtype=torch.bfloat16) -> torch.Tensor:
     """``x [rows, K] @ w`` for one weight matrix (w.q [1, N, K]): quantises the
     rows and multiplies."""
-    if w.q.dim() != 3 or w.q.shape[0] != 1:
+    El, Nw, K = _check_weights(w, "w")
+    if El != 1:
         raise ValueError(f"one weight matrix [1, N, K] is required, got {tuple(w.q.shape)}")
-    q, scale = quantize_rows(x)
-    return grouped_gemm(q, scale, w, out_dtype=out_dtype)
+    if x.dim() != 2 or x.shape[1] != K or x.dtype not in (torch.bfloat16, torch.float32):
+        raise TypeError(f"x [rows, {K}] in bfloat16 or float32 is required")
+    _check_product(K, Nw, El, False)
+    if out_dtype not in (torch.bfloat16, torch.float32):
+        raise TypeError("out_dtype must be bfloat16 or float32")
+    _on_gpu(x.device, x=x, q=w.q, scale=w.scale)
+    rows = x.shape[0]
+    out = torch.empty((rows, Nw), dtype=out_dtype, device=x.device)
+    if rows:
+        with utils.on_device(x.device) as stream:
+            q, scale = _quantize(x.contiguous(), rows, K, None, None, stream)
+            _gemm(q, scale, w, None, rows, K, Nw, 1, False, out, None, stream)
+    return out
 
 
 def moe_layer(x: torch.Tensor, top_idxs: torch.Tensor, top_vals: torch.Tensor, w13: QuantWeights, w2: QuantWeights,
@@ -196,6 +217,10 @@ def moe_layer(x: torch.Tensor, top_idxs: torch.Tensor, top_vals: torch.Tensor, w
         raise TypeError("x must be bfloat16")
     if H % 16 or F % 16:
         raise ValueError(f"H = {H} and F = {F} must be multiples of 16")
+    _check_product(H, F2, El, True)
+    _check_product(F, H, El, False)
+    if status is not None and (status.dtype != torch.int32 or status.numel() != 1 or not status.is_pinned()):
+        raise ValueError("status must be one pinned int32")
     if top_idxs.dim() == 1:
         top_idxs = top_idxs[:, None]
     if top_vals.dim() == 1:
@@ -217,11 +242,14 @@ def moe_layer(x: torch.Tensor, top_idxs: torch.Tensor, top_vals: torch.Tensor, w
     ids, vals = top_idxs.contiguous(), top_vals.contiguous()
     with utils.on_device(x.device) as stream:
         r = utils.route(ids if first_expert == 0 else ids - first_expert, El, with_slots=True)
-        q, scale = quantize_rows(x, r.perm, r.offsets[El:])
-        h = grouped_gemm(q, scale, w13, r.counts, swiglu=True, out_dtype=torch.float32, status=status)
-        q, scale = quantize_rows(h, live_rows=r.offsets[El:])
+        n, live = T * K, r.offsets[El:]
+        q, scale = _quantize(x.contiguous(), n, H, r.perm, live, stream)
+        h = torch.empty((n, F), dtype=torch.float32, device=x.device)
+        _gemm(q, scale, w13, r.counts, n, H, F2, El, True, h, status, stream)
+        q, scale = _quantize(h, n, F, None, live, stream)
         # fp32 rows: y is rounded once, like a layer that never splits its sum
-        rows = grouped_gemm(q, scale, w2, r.counts, out_dtype=torch.float32, status=status)
+        rows = torch.empty((n, H), dtype=torch.float32, device=x.device)
+        _gemm(q, scale, w2, r.counts, n, F, H, El, False, rows, status, stream)
         N.check(N.lib().moe_weighted_sum(rows.data_ptr(), 1, ids.data_ptr(), ids.dtype == torch.int64, first_expert,
                                          vals.data_ptr(), vals.dtype == torch.bfloat16, r.slots.data_ptr(),
                                          r.offsets.data_ptr(), T, K, H, El, y.data_ptr(), stream),
