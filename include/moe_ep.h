@@ -445,7 +445,7 @@ typedef struct moe_w8a8_params {
   int64_t rows;
   int32_t K, N, experts;
   int32_t swiglu, out_is_f32;
-  int32_t reserved;
+  int32_t x_is_f32;
   const void* xq;          /* [rows, K] int8             */
   const float* xs;         /* [rows]                     */
   const void* wq;          /* [experts, N, K] int8       */
@@ -455,6 +455,9 @@ typedef struct moe_w8a8_params {
   void* scratch;
   size_t scratch_bytes;
   int32_t* status_host;    /* optional mapped pinned word for device errors */
+  const void* x;           /* NULL, or rows to quantise first, into xq and xs */
+  const int32_t* perm;     /* (both then written), as moe_quant_rows does     */
+  const int32_t* live_rows;
 } moe_w8a8_params;
 
 int moe_w8a8_scratch_bytes(int64_t rows, int32_t K, int32_t N, int32_t experts, int32_t swiglu, int32_t device,

@@ -78,10 +78,11 @@ class DecodeParams(ctypes.Structure):
 
 class W8A8Params(ctypes.Structure):
     _fields_ = [("rows", ctypes.c_int64), ("K", ctypes.c_int32), ("N", ctypes.c_int32), ("experts", ctypes.c_int32),
-                ("swiglu", ctypes.c_int32), ("out_is_f32", ctypes.c_int32), ("reserved", ctypes.c_int32),
+                ("swiglu", ctypes.c_int32), ("out_is_f32", ctypes.c_int32), ("x_is_f32", ctypes.c_int32),
                 ("xq", ctypes.c_void_p), ("xs", ctypes.c_void_p), ("wq", ctypes.c_void_p), ("ws", ctypes.c_void_p),
                 ("counts", ctypes.c_void_p), ("out", ctypes.c_void_p), ("scratch", ctypes.c_void_p),
-                ("scratch_bytes", ctypes.c_size_t), ("status_host", ctypes.c_void_p)]
+                ("scratch_bytes", ctypes.c_size_t), ("status_host", ctypes.c_void_p), ("x", ctypes.c_void_p),
+                ("perm", ctypes.c_void_p), ("live_rows", ctypes.c_void_p)]
 
 
 DECODE_MAX_TOKENS = 64

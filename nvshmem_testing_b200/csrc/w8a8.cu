@@ -67,11 +67,131 @@ struct QArgs {
   int out_f32;
   int32_t* part;               // split form: [pairs][2] slots
   int32_t* status_host;
+  // Split form: rows quantised here first (x != null), into xq and xs.
+  const void* x;
+  int x_f32;
+  const int32_t* perm;
+  const int32_t* live;
+  int8_t* xq_out;
+  float* xs_out;
 };
 
 struct QRowMaps {
   CUtensorMap m[kQRowMaps];
 };
+
+// ---------------------------------------------------------------- quantisation of one row
+// Rounds x / s half to even, exactly: |x / s| <= 127.5, inv = 1 / s rounded.
+// t holds the nearest integer of x * inv (within one of the answer) in its
+// low mantissa bits; the remainder x - q*s fits fp32.
+constexpr float kMagic = 12582912.f;  // 1.5 * 2^23
+__device__ __forceinline__ int quant_one(float x, float s, float half, float inv) {
+  const float t = fmaf(x, inv, kMagic);
+  int q = __float_as_int(t) - __float_as_int(kMagic);
+  const float r = fmaf(-(t - kMagic), s, x);
+  const bool odd = q & 1;
+  if (r > half || (r == half && odd)) ++q;
+  if (r < -half || (r == -half && odd)) --q;
+  return max(-127, min(127, q));
+}
+
+// Eight values.  x * inv is within 127 * 3 * 2^-24 < 3e-5 of the quotient, so
+// its rounding is the quotient's unless it lies nearer than that to a tie:
+// only then (about 1 value in 4000, more where the values are coarse) the
+// exact form runs.  t's low byte is the integer in two's complement.
+__device__ __forceinline__ uint2 quant8(const float (&x)[8], float s, float inv, bool exact) {
+  uint32_t t[8];
+  float far = 0.f;
+#pragma unroll
+  for (int i = 0; i < 8; ++i) {
+    const float y = fmaf(x[i], inv, kMagic);
+    far = fmaxf(far, fabsf(fmaf(x[i], inv, kMagic - y)));
+    t[i] = __float_as_uint(y);
+  }
+  if (exact || far > 0.49995f) {
+    const float half = 0.5f * s;
+#pragma unroll
+    for (int i = 0; i < 8; ++i) t[i] = uint32_t(quant_one(x[i], s, half, inv));
+  }
+  return make_uint2(__byte_perm(__byte_perm(t[0], t[1], 0x0040), __byte_perm(t[2], t[3], 0x0040), 0x5410),
+                    __byte_perm(__byte_perm(t[4], t[5], 0x0040), __byte_perm(t[6], t[7], 0x0040), 0x5410));
+}
+
+__device__ __forceinline__ void load8(const __nv_bfloat16* p, float (&v)[8]) {
+  const uint4 w = *reinterpret_cast<const uint4*>(p);
+  const __nv_bfloat162* h = reinterpret_cast<const __nv_bfloat162*>(&w);
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    const float2 f = __bfloat1622float2(h[i]);
+    v[2 * i] = f.x;
+    v[2 * i + 1] = f.y;
+  }
+}
+__device__ __forceinline__ void load8(const float* p, float (&v)[8]) {
+  *reinterpret_cast<float4*>(&v[0]) = *reinterpret_cast<const float4*>(p);
+  *reinterpret_cast<float4*>(&v[4]) = *reinterpret_cast<const float4*>(p + 4);
+}
+
+// A row's scale and what its values are rounded with, from the largest
+// magnitude's bits.  Infinities and NaN (largest as numbers): no scale holds
+// the row, and a NaN scale says so in every output.  Tiny rows: the
+// reciprocal would overflow (powers of two change nothing), and a scale below
+// the normal numbers is coarse.
+struct RowScale {
+  float scale, s, inv, up;
+  bool zero, tiny;
+  __device__ __forceinline__ explicit RowScale(uint32_t top) {
+    const bool bad = top >= 0x7f800000u;
+    scale = bad ? __int_as_float(0x7fffffff) : __uint_as_float(top) * (1.f / 127.f);
+    zero = bad || scale == 0.f;
+    tiny = scale < 0x1p-90f;
+    up = tiny ? 0x1p100f : 1.f;
+    s = zero ? 1.f : scale * up;
+    inv = 1.f / s;
+  }
+  __device__ __forceinline__ uint2 round8(float (&w)[8]) const {
+    if (zero) return make_uint2(0u, 0u);
+    if (tiny) {
+#pragma unroll
+      for (int i = 0; i < 8; ++i) w[i] *= up;
+    }
+    return quant8(w, s, inv, tiny);
+  }
+};
+
+__device__ __forceinline__ uint32_t top8(const float (&v)[8]) {
+  uint32_t top = 0;
+#pragma unroll
+  for (int i = 0; i < 8; ++i) top = max(top, __float_as_uint(v[i]) & 0x7fffffffu);
+  return top;
+}
+
+// One row by a whole CTA (few rows: the second read comes from L1).
+template <typename In>
+__device__ __noinline__ void quant_row_cta(const In* src, int K, int8_t* q, float* scale, uint32_t* red) {
+  const int tid = threadIdx.x, groups = K / 8;
+  uint32_t top = 0;
+#pragma unroll 2
+  for (int g = tid; g < groups; g += kQThreads) {
+    float v[8];
+    load8(src + g * 8, v);
+    top = max(top, top8(v));
+  }
+  top = __reduce_max_sync(0xffffffffu, top);
+  __syncthreads();  // the last row's maxima have been read
+  if ((tid & 31) == 0) red[tid >> 5] = top;
+  __syncthreads();
+  for (int w = 0; w < kQThreads / 32; ++w) top = max(top, red[w]);
+  const RowScale r(top);
+  if (tid == 0) *scale = r.scale;
+#pragma unroll 1
+  for (int g = tid; g < groups; g += kQThreads) {
+    float v[8];
+    load8(src + g * 8, v);
+    *reinterpret_cast<uint2*>(q + g * 8) = r.round8(v);
+  }
+}
+
 
 struct alignas(16) QSmem {
   uint64_t full[kQStages];   // leader: both CTAs' bytes
@@ -294,37 +414,75 @@ __global__ void __launch_bounds__(kQThreads, 1)
   // leave it open; ragged experts may make enough tiles all the same.)
   const bool split = SPLIT && tiles < kQWaves * pairs;
 
+  // ---- loads (one thread): each CTA its 128 channels and half of the tile's
+  // rows, all onto the leader's barrier
+  QWalk lw(s, split, tiles, pair, pairs);
+  QRing lr = {0, 0};
+  uint32_t fills = 0;
+  const uint32_t bar0 = mapa_shared(smem_u32(&sm.full[0]), 0);
+  auto row_box = [](const QTile& t) { return t.n <= 32 ? 0 : t.n <= 64 ? 1 : t.n <= 128 ? 2 : 3; };
+  // A unit's channels into the next stage, whose expected bytes include the
+  // rows that load_rows adds.
+  auto load_weights = [&](const QTile& t, int k) {
+    if (!q_wait(&sm.empty[lr.st], lr.ph ^ 1, sm)) {
+      q_fail(sm, a, 1);
+      return false;
+    }
+    unsigned char* dst = stage + uint32_t(lr.st) * kQStageBytes;
+    const uint32_t bar = bar0 + uint32_t(lr.st) * sizeof(uint64_t);
+    if (leader) mbar_arrive_expect_tx(&sm.full[lr.st], 2 * (kQABytes + (16u << row_box(t)) * kQKb));
+    if constexpr (GLU) {
+      const int f = t.f * 128 + int(crank) * 64;
+      tma_load_3d_pair(&tm_w, bar, dst, k * kQKb, f, t.e);
+      tma_load_3d_pair(&tm_w, bar, dst + kQABytes / 2, k * kQKb, a.F + f, t.e);
+    } else {
+      tma_load_3d_pair(&tm_w, bar, dst, k * kQKb, t.f * 256 + int(crank) * 128, t.e);
+    }
+    ++fills;
+    lr.next(kQStages);
+    return true;
+  };
+  auto load_rows = [&](const QTile& t, int k, int st) {
+    tma_load_2d_pair(&tm_x.m[row_box(t)], bar0 + uint32_t(st) * sizeof(uint64_t),
+                     stage + uint32_t(st) * kQStageBytes + kQABytes, k * kQKb, t.r0 + int(crank) * (t.n / 2));
+  };
+  int pre = 0;  // units whose channels are under way
+  if constexpr (SPLIT) {
+    if (a.x != nullptr) {
+      // Few rows: quantised by the grid while the first channels arrive.
+      if (threadIdx.x == 0) {
+        for (QWalk w = lw; w.more() && pre < kQStages; w.next()) {
+          const QTile t = q_tile(s, w.tile);
+          for (int k = w.k0; k < w.k1 && pre < kQStages && load_weights(t, k); ++k) ++pre;
+        }
+      }
+      __syncwarp();
+      const int64_t live = a.live ? min(int64_t(max(*a.live, 0)), a.rows) : a.rows;
+      for (int64_t r = blockIdx.x; r < live; r += gridDim.x) {
+        const int64_t from = (a.perm ? int64_t(a.perm[r]) : r) * a.K;
+        uint32_t* red = reinterpret_cast<uint32_t*>(xbuf);
+        if (a.x_f32) quant_row_cta(static_cast<const float*>(a.x) + from, a.K, a.xq_out + r * a.K, a.xs_out + r, red);
+        else quant_row_cta(static_cast<const __nv_bfloat16*>(a.x) + from, a.K, a.xq_out + r * a.K, a.xs_out + r, red);
+      }
+      fence_proxy_async_global();  // written by threads, read by the TMA
+      cg::this_grid().sync();
+      fence_proxy_async_global();
+    }
+  }
+
   if (warp == 0 && lane == 0) {
-    // ---- loads: each CTA its 128 channels and half of the tile's rows, all
-    // onto the leader's barrier
-    QRing r = {0, 0};
-    uint32_t fills = 0;
-    const uint32_t bar0 = mapa_shared(smem_u32(&sm.full[0]), 0);
+    QRing at = {0, 0};
     bool stop = false;
-    for (QWalk w(s, split, tiles, pair, pairs); w.more() && !stop; w.next()) {
+    for (QWalk w = lw; w.more() && !stop; w.next()) {
       const QTile t = q_tile(s, w.tile);
-      const int half = t.n / 2, bm = half <= 16 ? 0 : half <= 32 ? 1 : half <= 64 ? 2 : 3;
-      const uint32_t tx = 2 * (kQABytes + (16u << bm) * kQKb);
-      const int row = t.r0 + int(crank) * half;
       for (int k = w.k0; k < w.k1; ++k) {
-        if (!q_wait(&sm.empty[r.st], r.ph ^ 1, sm)) {
-          q_fail(sm, a, 1);
+        if (pre > 0) --pre;
+        else if (!load_weights(t, k)) {
           stop = true;
           break;
         }
-        unsigned char* dst = stage + uint32_t(r.st) * kQStageBytes;
-        const uint32_t bar = bar0 + uint32_t(r.st) * sizeof(uint64_t);
-        if (leader) mbar_arrive_expect_tx(&sm.full[r.st], tx);
-        if constexpr (GLU) {
-          const int f = t.f * 128 + int(crank) * 64;
-          tma_load_3d_pair(&tm_w, bar, dst, k * kQKb, f, t.e);
-          tma_load_3d_pair(&tm_w, bar, dst + kQABytes / 2, k * kQKb, a.F + f, t.e);
-        } else {
-          tma_load_3d_pair(&tm_w, bar, dst, k * kQKb, t.f * 256 + int(crank) * 128, t.e);
-        }
-        tma_load_2d_pair(&tm_x.m[bm], bar, dst + kQABytes, k * kQKb, row);
-        ++fills;
-        r.next(kQStages);
+        load_rows(t, k, at.st);
+        at.next(kQStages);
       }
     }
     sm.fills = fills;
@@ -570,57 +728,6 @@ __global__ void __launch_bounds__(kQThreads, 1)
 // ---------------------------------------------------------------- quantisation
 constexpr int kQuantThreads = 256;
 
-// Rounds x / s half to even, exactly: |x / s| <= 127.5, inv = 1 / s rounded.
-// t holds the nearest integer of x * inv (within one of the answer) in its
-// low mantissa bits; the remainder x - q*s fits fp32.
-constexpr float kMagic = 12582912.f;  // 1.5 * 2^23
-__device__ __forceinline__ int quant_one(float x, float s, float half, float inv) {
-  const float t = fmaf(x, inv, kMagic);
-  int q = __float_as_int(t) - __float_as_int(kMagic);
-  const float r = fmaf(-(t - kMagic), s, x);
-  const bool odd = q & 1;
-  if (r > half || (r == half && odd)) ++q;
-  if (r < -half || (r == -half && odd)) --q;
-  return max(-127, min(127, q));
-}
-
-// Eight values.  x * inv is within 127 * 3 * 2^-24 < 3e-5 of the quotient, so
-// its rounding is the quotient's unless it lies nearer than that to a tie:
-// only then (about 1 value in 4000, more where the values are coarse) the
-// exact form runs.  t's low byte is the integer in two's complement.
-__device__ __forceinline__ uint2 quant8(const float (&x)[8], float s, float inv, bool exact) {
-  uint32_t t[8];
-  float far = 0.f;
-#pragma unroll
-  for (int i = 0; i < 8; ++i) {
-    const float y = fmaf(x[i], inv, kMagic);
-    far = fmaxf(far, fabsf(fmaf(x[i], inv, kMagic - y)));
-    t[i] = __float_as_uint(y);
-  }
-  if (exact || far > 0.49995f) {
-    const float half = 0.5f * s;
-#pragma unroll
-    for (int i = 0; i < 8; ++i) t[i] = uint32_t(quant_one(x[i], s, half, inv));
-  }
-  return make_uint2(__byte_perm(__byte_perm(t[0], t[1], 0x0040), __byte_perm(t[2], t[3], 0x0040), 0x5410),
-                    __byte_perm(__byte_perm(t[4], t[5], 0x0040), __byte_perm(t[6], t[7], 0x0040), 0x5410));
-}
-
-__device__ __forceinline__ void load8(const __nv_bfloat16* p, float (&v)[8]) {
-  const uint4 w = *reinterpret_cast<const uint4*>(p);
-  const __nv_bfloat162* h = reinterpret_cast<const __nv_bfloat162*>(&w);
-#pragma unroll
-  for (int i = 0; i < 4; ++i) {
-    const float2 f = __bfloat1622float2(h[i]);
-    v[2 * i] = f.x;
-    v[2 * i + 1] = f.y;
-  }
-}
-__device__ __forceinline__ void load8(const float* p, float (&v)[8]) {
-  *reinterpret_cast<float4*>(&v[0]) = *reinterpret_cast<const float4*>(p);
-  *reinterpret_cast<float4*>(&v[4]) = *reinterpret_cast<const float4*>(p + 4);
-}
-
 // TPR threads per row, each VPT groups of eight values in registers; rows
 // longer than that are read again for the rounding.
 template <typename In, int VPT>
@@ -644,15 +751,11 @@ __global__ void __launch_bounds__(kQuantThreads)
         if (c + j * tpr < groups) load8(src + (c + j * tpr) * 8, v[j]);
 #pragma unroll
       for (int j = 0; j < VPT; ++j)
-        if (c + j * tpr < groups) {
-#pragma unroll
-          for (int i = 0; i < 8; ++i) top = max(top, __float_as_uint(v[j][i]) & 0x7fffffffu);
-        }
+        if (c + j * tpr < groups) top = max(top, top8(v[j]));
       for (int g = c + VPT * tpr; g < groups; g += tpr) {
         float w[8];
         load8(src + g * 8, w);
-#pragma unroll
-        for (int i = 0; i < 8; ++i) top = max(top, __float_as_uint(w[i]) & 0x7fffffffu);
+        top = max(top, top8(w));
       }
     }
     top = __reduce_max_sync(0xffffffffu, top);
@@ -664,24 +767,10 @@ __global__ void __launch_bounds__(kQuantThreads)
       for (int w = 0; w < tpr / 32; ++w) top = max(top, top_s[w0 + w]);
     }
     if (!on) continue;
-    // Infinities and NaN (largest as numbers): no scale holds the row, and a
-    // NaN scale says so in every output.
-    const bool bad = top >= 0x7f800000u;
-    const float s0 = bad ? __int_as_float(0x7fffffff) : __uint_as_float(top) * (1.f / 127.f);
-    if (c == 0) scale[r] = s0;
-    const bool zero = bad || s0 == 0.f;
-    // Tiny rows: the reciprocal would overflow (powers of two change
-    // nothing), and a scale below the normal numbers is coarse.
-    const bool tiny = s0 < 0x1p-90f;
-    const float up = tiny ? 0x1p100f : 1.f, s = zero ? 1.f : s0 * up, inv = 1.f / s;
+    const RowScale rs(top);
+    if (c == 0) scale[r] = rs.scale;
     int8_t* dst = q + r * K;
-    auto put = [&](int g, float (&w)[8]) {
-      if (tiny) {
-#pragma unroll
-        for (int i = 0; i < 8; ++i) w[i] *= up;
-      }
-      *reinterpret_cast<uint2*>(dst + g * 8) = zero ? make_uint2(0u, 0u) : quant8(w, s, inv, tiny);
-    };
+    auto put = [&](int g, float (&w)[8]) { *reinterpret_cast<uint2*>(dst + g * 8) = rs.round8(w); };
 #pragma unroll
     for (int j = 0; j < VPT; ++j)
       if (c + j * tpr < groups) put(c + j * tpr, v[j]);
@@ -868,6 +957,7 @@ extern "C" int moe_w8a8_gemm(const moe_w8a8_params* p, void* stream) {
   if (!p || !q_sizes_ok(p->rows, p->K, p->N, p->experts, p->swiglu)) return kBadArg;
   if (p->rows == 0) return kOk;
   if (!p->xq || !p->xs || !p->wq || !p->ws || !p->out || (!p->counts && p->experts != 1)) return kBadArg;
+  if (misaligned16(p->x)) return kBadArg;
   if (misaligned16(p->xq) || misaligned16(p->wq) || misaligned16(p->ws) || misaligned16(p->out) ||
       misaligned16(p->scratch))
     return kBadArg;
@@ -908,6 +998,25 @@ extern "C" int moe_w8a8_gemm(const moe_w8a8_params* p, void* stream) {
     if (encode_s8(&tx.m[i], 2, p->xq, dims, str, box)) return kCudaErr;
   }
   const cudaStream_t s = static_cast<cudaStream_t>(stream);
+  if (p->x) {
+    // Two rows per CTA at most are quantised inside the product (one row
+    // 7168 x 4096: 16.4 us as two launches, see the note at the top);
+    // more by a launch of their own.
+    int8_t* xq = static_cast<int8_t*>(const_cast<void*>(p->xq));
+    float* xs = const_cast<float*>(p->xs);
+    if (split && a.rows <= 2 * sms) {
+      a.x = p->x;
+      a.x_f32 = p->x_is_f32;
+      a.perm = p->perm;
+      a.live = p->live_rows;
+      a.xq_out = xq;
+      a.xs_out = xs;
+    } else {
+      const int rc = p->x_is_f32 ? launch_quant<float>(p->x, a.rows, a.K, p->perm, p->live_rows, xq, xs, sms, s)
+                                 : launch_quant<__nv_bfloat16>(p->x, a.rows, a.K, p->perm, p->live_rows, xq, xs, sms, s);
+      if (rc != kOk) return rc;
+    }
+  }
   if (glu)
     return split ? launch_w8a8<true, true>(tw, tx, a, dev, sms, s) : launch_w8a8<true, false>(tw, tx, a, dev, sms, s);
   return split ? launch_w8a8<false, true>(tw, tx, a, dev, sms, s) : launch_w8a8<false, false>(tw, tx, a, dev, sms, s);

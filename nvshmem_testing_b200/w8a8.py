@@ -162,13 +162,28 @@ def grouped_gemm(xq: torch.Tensor, xs: torch.Tensor, w: QuantWeights, counts: to
 
 
 def _gemm(xq, xs, w, counts, rows, K, Nw, El, swiglu, out, status, stream):
-    """The checked call."""
+    """The checked call for quantised rows."""
     need = _scratch_bytes(rows, K, Nw, El, int(swiglu), xq.device.index)
     scratch = torch.empty(need, dtype=torch.uint8, device=xq.device) if need else None
     p = N.W8A8Params(rows, K, Nw, El, swiglu, out.dtype == torch.float32, 0, xq.data_ptr(), xs.data_ptr(),
                      w.q.data_ptr(), w.scale.data_ptr(), None if counts is None else counts.data_ptr(),
                      out.data_ptr(), None if scratch is None else scratch.data_ptr(), need,
-                     None if status is None else status.data_ptr())
+                     None if status is None else status.data_ptr(), None, None, None)
+    N.check(N.lib().moe_w8a8_gemm(ctypes.byref(p), stream), "moe_w8a8_gemm")
+
+
+def _quantized_gemm(x, w, counts, perm, live_rows, rows, K, Nw, El, swiglu, out, status, stream):
+    """The checked call for rows that are still to be quantised: rows, scales
+    and partial sums in one scratch tensor."""
+    need = _scratch_bytes(rows, K, Nw, El, int(swiglu), x.device.index)
+    s_at = (rows * K + 255) // 256 * 256
+    p_at = (s_at + rows * 4 + 255) // 256 * 256
+    scratch = torch.empty(p_at + need, dtype=torch.uint8, device=x.device)
+    base = scratch.data_ptr()
+    p = N.W8A8Params(rows, K, Nw, El, swiglu, out.dtype == torch.float32, x.dtype == torch.float32, base, base + s_at,
+                     w.q.data_ptr(), w.scale.data_ptr(), None if counts is None else counts.data_ptr(),
+                     out.data_ptr(), base + p_at, need, None if status is None else status.data_ptr(), x.data_ptr(),
+                     None if perm is None else perm.data_ptr(), None if live_rows is None else live_rows.data_ptr())
     N.check(N.lib().moe_w8a8_gemm(ctypes.byref(p), stream), "moe_w8a8_gemm")
 
 
@@ -188,8 +203,7 @@ def linear(x: torch.Tensor, w: QuantWeights, *, out_dtype=torch.bfloat16) -> tor
     out = torch.empty((rows, Nw), dtype=out_dtype, device=x.device)
     if rows:
         with utils.on_device(x.device) as stream:
-            q, scale = _quantize(x.contiguous(), rows, K, None, None, stream)
-            _gemm(q, scale, w, None, rows, K, Nw, 1, False, out, None, stream)
+            _quantized_gemm(x.contiguous(), w, None, None, None, rows, K, Nw, 1, False, out, None, stream)
     return out
 
 
@@ -243,13 +257,11 @@ def moe_layer(x: torch.Tensor, top_idxs: torch.Tensor, top_vals: torch.Tensor, w
     with utils.on_device(x.device) as stream:
         r = utils.route(ids if first_expert == 0 else ids - first_expert, El, with_slots=True)
         n, live = T * K, r.offsets[El:]
-        q, scale = _quantize(x.contiguous(), n, H, r.perm, live, stream)
         h = torch.empty((n, F), dtype=torch.float32, device=x.device)
-        _gemm(q, scale, w13, r.counts, n, H, F2, El, True, h, status, stream)
-        q, scale = _quantize(h, n, F, None, live, stream)
+        _quantized_gemm(x.contiguous(), w13, r.counts, r.perm, live, n, H, F2, El, True, h, status, stream)
         # fp32 rows: y is rounded once, like a layer that never splits its sum
         rows = torch.empty((n, H), dtype=torch.float32, device=x.device)
-        _gemm(q, scale, w2, r.counts, n, F, H, El, False, rows, status, stream)
+        _quantized_gemm(h, w2, r.counts, None, live, n, F, H, El, False, rows, status, stream)
         N.check(N.lib().moe_weighted_sum(rows.data_ptr(), 1, ids.data_ptr(), ids.dtype == torch.int64, first_expert,
                                          vals.data_ptr(), vals.dtype == torch.bfloat16, r.slots.data_ptr(),
                                          r.offsets.data_ptr(), T, K, H, El, y.data_ptr(), stream),
