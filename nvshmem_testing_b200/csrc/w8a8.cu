@@ -67,13 +67,6 @@ struct QArgs {
   int out_f32;
   int32_t* part;               // split form: [pairs][2] slots
   int32_t* status_host;
-  // Split form: rows quantised here first (x != null), into xq and xs.
-  const void* x;
-  int x_f32;
-  const int32_t* perm;
-  const int32_t* live;
-  int8_t* xq_out;
-  float* xs_out;
 };
 
 struct QRowMaps {
@@ -165,33 +158,6 @@ __device__ __forceinline__ uint32_t top8(const float (&v)[8]) {
   for (int i = 0; i < 8; ++i) top = max(top, __float_as_uint(v[i]) & 0x7fffffffu);
   return top;
 }
-
-// One row by a whole CTA (few rows: the second read comes from L1).
-template <typename In>
-__device__ __noinline__ void quant_row_cta(const In* src, int K, int8_t* q, float* scale, uint32_t* red) {
-  const int tid = threadIdx.x, groups = K / 8;
-  uint32_t top = 0;
-#pragma unroll 2
-  for (int g = tid; g < groups; g += kQThreads) {
-    float v[8];
-    load8(src + g * 8, v);
-    top = max(top, top8(v));
-  }
-  top = __reduce_max_sync(0xffffffffu, top);
-  __syncthreads();  // the last row's maxima have been read
-  if ((tid & 31) == 0) red[tid >> 5] = top;
-  __syncthreads();
-  for (int w = 0; w < kQThreads / 32; ++w) top = max(top, red[w]);
-  const RowScale r(top);
-  if (tid == 0) *scale = r.scale;
-#pragma unroll 1
-  for (int g = tid; g < groups; g += kQThreads) {
-    float v[8];
-    load8(src + g * 8, v);
-    *reinterpret_cast<uint2*>(q + g * 8) = r.round8(v);
-  }
-}
-
 
 struct alignas(16) QSmem {
   uint64_t full[kQStages];   // leader: both CTAs' bytes
@@ -414,75 +380,37 @@ __global__ void __launch_bounds__(kQThreads, 1)
   // leave it open; ragged experts may make enough tiles all the same.)
   const bool split = SPLIT && tiles < kQWaves * pairs;
 
-  // ---- loads (one thread): each CTA its 128 channels and half of the tile's
-  // rows, all onto the leader's barrier
-  QWalk lw(s, split, tiles, pair, pairs);
-  QRing lr = {0, 0};
-  uint32_t fills = 0;
-  const uint32_t bar0 = mapa_shared(smem_u32(&sm.full[0]), 0);
-  auto row_box = [](const QTile& t) { return t.n <= 32 ? 0 : t.n <= 64 ? 1 : t.n <= 128 ? 2 : 3; };
-  // A unit's channels into the next stage, whose expected bytes include the
-  // rows that load_rows adds.
-  auto load_weights = [&](const QTile& t, int k) {
-    if (!q_wait(&sm.empty[lr.st], lr.ph ^ 1, sm)) {
-      q_fail(sm, a, 1);
-      return false;
-    }
-    unsigned char* dst = stage + uint32_t(lr.st) * kQStageBytes;
-    const uint32_t bar = bar0 + uint32_t(lr.st) * sizeof(uint64_t);
-    if (leader) mbar_arrive_expect_tx(&sm.full[lr.st], 2 * (kQABytes + (16u << row_box(t)) * kQKb));
-    if constexpr (GLU) {
-      const int f = t.f * 128 + int(crank) * 64;
-      tma_load_3d_pair(&tm_w, bar, dst, k * kQKb, f, t.e);
-      tma_load_3d_pair(&tm_w, bar, dst + kQABytes / 2, k * kQKb, a.F + f, t.e);
-    } else {
-      tma_load_3d_pair(&tm_w, bar, dst, k * kQKb, t.f * 256 + int(crank) * 128, t.e);
-    }
-    ++fills;
-    lr.next(kQStages);
-    return true;
-  };
-  auto load_rows = [&](const QTile& t, int k, int st) {
-    tma_load_2d_pair(&tm_x.m[row_box(t)], bar0 + uint32_t(st) * sizeof(uint64_t),
-                     stage + uint32_t(st) * kQStageBytes + kQABytes, k * kQKb, t.r0 + int(crank) * (t.n / 2));
-  };
-  int pre = 0;  // units whose channels are under way
-  if constexpr (SPLIT) {
-    if (a.x != nullptr) {
-      // Few rows: quantised by the grid while the first channels arrive.
-      if (threadIdx.x == 0) {
-        for (QWalk w = lw; w.more() && pre < kQStages; w.next()) {
-          const QTile t = q_tile(s, w.tile);
-          for (int k = w.k0; k < w.k1 && pre < kQStages && load_weights(t, k); ++k) ++pre;
-        }
-      }
-      __syncwarp();
-      const int64_t live = a.live ? min(int64_t(max(*a.live, 0)), a.rows) : a.rows;
-      for (int64_t r = blockIdx.x; r < live; r += gridDim.x) {
-        const int64_t from = (a.perm ? int64_t(a.perm[r]) : r) * a.K;
-        uint32_t* red = reinterpret_cast<uint32_t*>(xbuf);
-        if (a.x_f32) quant_row_cta(static_cast<const float*>(a.x) + from, a.K, a.xq_out + r * a.K, a.xs_out + r, red);
-        else quant_row_cta(static_cast<const __nv_bfloat16*>(a.x) + from, a.K, a.xq_out + r * a.K, a.xs_out + r, red);
-      }
-      fence_proxy_async_global();  // written by threads, read by the TMA
-      cg::this_grid().sync();
-      fence_proxy_async_global();
-    }
-  }
-
   if (warp == 0 && lane == 0) {
-    QRing at = {0, 0};
+    // ---- loads: each CTA its 128 channels and half of the tile's rows, all
+    // onto the leader's barrier
+    QRing r = {0, 0};
+    uint32_t fills = 0;
+    const uint32_t bar0 = mapa_shared(smem_u32(&sm.full[0]), 0);
     bool stop = false;
-    for (QWalk w = lw; w.more() && !stop; w.next()) {
+    for (QWalk w(s, split, tiles, pair, pairs); w.more() && !stop; w.next()) {
       const QTile t = q_tile(s, w.tile);
+      const int half = t.n / 2, bm = half <= 16 ? 0 : half <= 32 ? 1 : half <= 64 ? 2 : 3;
+      const uint32_t tx = 2 * (kQABytes + (16u << bm) * kQKb);
+      const int row = t.r0 + int(crank) * half;
       for (int k = w.k0; k < w.k1; ++k) {
-        if (pre > 0) --pre;
-        else if (!load_weights(t, k)) {
+        if (!q_wait(&sm.empty[r.st], r.ph ^ 1, sm)) {
+          q_fail(sm, a, 1);
           stop = true;
           break;
         }
-        load_rows(t, k, at.st);
-        at.next(kQStages);
+        unsigned char* dst = stage + uint32_t(r.st) * kQStageBytes;
+        const uint32_t bar = bar0 + uint32_t(r.st) * sizeof(uint64_t);
+        if (leader) mbar_arrive_expect_tx(&sm.full[r.st], tx);
+        if constexpr (GLU) {
+          const int f = t.f * 128 + int(crank) * 64;
+          tma_load_3d_pair(&tm_w, bar, dst, k * kQKb, f, t.e);
+          tma_load_3d_pair(&tm_w, bar, dst + kQABytes / 2, k * kQKb, a.F + f, t.e);
+        } else {
+          tma_load_3d_pair(&tm_w, bar, dst, k * kQKb, t.f * 256 + int(crank) * 128, t.e);
+        }
+        tma_load_2d_pair(&tm_x.m[bm], bar, dst + kQABytes, k * kQKb, row);
+        ++fills;
+        r.next(kQStages);
       }
     }
     sm.fills = fills;
@@ -725,6 +653,214 @@ __global__ void __launch_bounds__(kQThreads, 1)
   cluster_sync();  // neither CTA leaves while its peer may still address it
 }
 
+// ---------------------------------------------------------------- a handful of rows
+// Up to kRwMaxRows rows (a decode step's): no tile to fill, so a warp takes a
+// channel (its gate and its up channel with SwiGLU) of up to four rows,
+// streams the channel's K contiguous bytes once, 16 per lane, against the
+// rows in shared memory with 4-way 8-bit dot products, and adds its lanes up.
+// No partial sums, barriers or tensor maps: the launch and one pass over the
+// weights.  Rows given in bf16 or fp32 are quantised by every CTA for itself
+// (four rows at most) behind the first loads of weights.
+constexpr int kRwThreads = 512;
+constexpr int kRwMaxRows = 16;
+constexpr int kRwMaxFresh = 4;   // rows quantised here
+constexpr int kRwRows = 4;       // rows of a channel's pass
+constexpr uint32_t kRwMaxSmem = 96 * 1024;  // of rows: two CTAs per SM
+
+struct RwArgs {
+  int E, K, N, F, rows;
+  const int32_t* counts;
+  const int8_t* xq;
+  const float* xs;
+  const void* x;  // or null: xq and xs
+  int x_f32;
+  const int32_t* perm;
+  const int32_t* live;
+  const int8_t* wq;
+  const float* ws;
+  void* out;
+  int out_f32;
+};
+
+struct RwSmem {
+  float scale[kRwMaxRows];
+  uint32_t top[kRwThreads / 32];
+  int e[kRwMaxRows], r0[kRwMaxRows], n[kRwMaxRows];  // an expert's rows, four at a time
+  int chunks;
+};
+
+__device__ __forceinline__ int dot16(uint4 a, uint4 b, int c) {
+  c = __dp4a(int(a.x), int(b.x), c);
+  c = __dp4a(int(a.y), int(b.y), c);
+  c = __dp4a(int(a.z), int(b.z), c);
+  return __dp4a(int(a.w), int(b.w), c);
+}
+
+__device__ __forceinline__ void rw_store(const RwArgs& a, int row, int f, float v) {
+  const int64_t at = int64_t(row) * a.F + f;
+  if (a.out_f32) static_cast<float*>(a.out)[at] = v;
+  else static_cast<__nv_bfloat16*>(a.out)[at] = __float2bfloat16_rn(v);
+}
+
+// The loads of one round: kRwLoads vectors of 16 bytes per lane in all.
+constexpr int kRwLoads = 4;
+template <bool GLU>
+__device__ __forceinline__ void rw_load(const uint4* w, const uint4* w2, int v0, int V, int lane,
+                                        uint4 (&buf)[kRwLoads]) {
+  constexpr int U = GLU ? kRwLoads / 2 : kRwLoads;
+#pragma unroll
+  for (int j = 0; j < U; ++j) {
+    const int v = v0 + j * 32 + lane;
+    const bool in = v < V;
+    buf[j] = in ? ld_nc_v4(w + v) : make_uint4(0, 0, 0, 0);
+    if constexpr (GLU) buf[U + j] = in ? ld_nc_v4(w2 + v) : make_uint4(0, 0, 0, 0);
+  }
+}
+
+template <bool GLU, int NR>
+__device__ __forceinline__ void rw_channel(const RwArgs& a, const RwSmem& sm, const uint4* rows, int c, int f,
+                                           const uint4* w, const uint4* w2, uint4 (&buf)[kRwLoads]) {
+  constexpr int U = GLU ? kRwLoads / 2 : kRwLoads;
+  const int V = a.K / 16, lane = threadIdx.x & 31, r0 = sm.r0[c], last = sm.n[c] - 1;  // NR > n: the last row again
+  int s[NR] = {}, s2[NR] = {};
+#pragma unroll 1
+  for (int v0 = 0; v0 < V; v0 += 32 * U) {
+    uint4 next[kRwLoads];
+    rw_load<GLU>(w, w2, v0 + 32 * U, V, lane, next);
+#pragma unroll
+    for (int j = 0; j < U; ++j) {
+      const int v = min(v0 + j * 32 + lane, V - 1);  // (past the end the weights are zeros)
+#pragma unroll
+      for (int r = 0; r < NR; ++r) {
+        const uint4 x = rows[(r0 + min(r, last)) * V + v];
+        s[r] = dot16(buf[j], x, s[r]);
+        if constexpr (GLU) s2[r] = dot16(buf[U + j], x, s2[r]);
+      }
+    }
+#pragma unroll
+    for (int j = 0; j < kRwLoads; ++j) buf[j] = next[j];
+  }
+  const float* sw = a.ws + int64_t(sm.e[c]) * a.N + f;
+  const float g = sw[0], u = GLU ? sw[a.F] : 0.f;
+#pragma unroll
+  for (int r = 0; r < NR; ++r) {
+    const int t = __reduce_add_sync(0xffffffffu, s[r]);
+    const int t2 = GLU ? __reduce_add_sync(0xffffffffu, s2[r]) : 0;
+    if (lane == r && r <= last) {
+      const float x = sm.scale[r0 + r];
+      const float z = float(t) * x * g;
+      rw_store(a, r0 + r, f, GLU ? silu_mul(z, float(t2) * x * u) : z);
+    }
+  }
+}
+
+template <typename In>
+__device__ __forceinline__ void rw_quantize(const RwArgs& a, RwSmem& sm, unsigned char* rows) {
+  // All, half or a quarter of the warps for each of up to four rows.
+  const int per = a.rows == 1 ? kRwThreads : a.rows == 2 ? kRwThreads / 2 : kRwThreads / 4;
+  const int r = int(threadIdx.x) / per, c = int(threadIdx.x) % per, groups = a.K / 8;
+  const int live = a.live ? min(max(*a.live, 0), a.rows) : a.rows;
+  const bool on = r < live;
+  const In* src = static_cast<const In*>(a.x) + int64_t(on ? (a.perm ? a.perm[r] : r) : 0) * a.K;
+  uint32_t top = 0;
+#pragma unroll 4
+  for (int g = c; g < groups && on; g += per) {
+    float v[8];
+    load8(src + g * 8, v);
+    top = max(top, top8(v));
+  }
+  top = __reduce_max_sync(0xffffffffu, top);
+  if ((threadIdx.x & 31) == 0) sm.top[threadIdx.x >> 5] = top;
+  __syncthreads();
+#pragma unroll 4
+  for (int w = 0; w < per / 32; ++w) top = max(top, sm.top[r * (per / 32) + w]);
+  const RowScale rs(top);
+  if (c == 0 && on) sm.scale[r] = rs.scale;
+#pragma unroll 1
+  for (int g = c; g < groups && on; g += per) {
+    float v[8];
+    load8(src + g * 8, v);
+    *reinterpret_cast<uint2*>(rows + r * a.K + g * 8) = rs.round8(v);
+  }
+}
+
+template <bool GLU>
+__global__ void __launch_bounds__(kRwThreads, 2) w8a8_rows_kernel(const RwArgs a) {
+  extern __shared__ __align__(16) unsigned char rw_rows[];
+  __shared__ RwSmem sm;
+  const int warp = int(threadIdx.x) >> 5, lane = threadIdx.x & 31;
+  if (warp == 0) {
+    // Experts with rows, in order; counts that would pass the last row are cut.
+    int row = 0, chunks = 0;
+#pragma unroll 1
+    for (int e0 = 0; e0 < a.E && row < a.rows; e0 += 32) {
+      const int e = e0 + lane;
+      int c = e < a.E ? (a.counts ? min(max(a.counts[e], 0), a.rows) : a.rows) : 0;
+      int pre = c;
+#pragma unroll
+      for (int o = 1; o < 32; o <<= 1) {
+        const int v = __shfl_up_sync(0xffffffffu, pre, o);
+        if (lane >= o) pre += v;
+      }
+      const int begin = min(row + pre - c, a.rows);
+      c = min(row + pre, a.rows) - begin;
+      const int mine = (c + kRwRows - 1) / kRwRows;
+      int at = mine;
+#pragma unroll
+      for (int o = 1; o < 32; o <<= 1) {
+        const int v = __shfl_up_sync(0xffffffffu, at, o);
+        if (lane >= o) at += v;
+      }
+      for (int i = 0; i < mine; ++i) {
+        const int k = chunks + at - mine + i;
+        sm.e[k] = e;
+        sm.r0[k] = begin + i * kRwRows;
+        sm.n[k] = min(kRwRows, c - i * kRwRows);
+      }
+      row = min(row + __shfl_sync(0xffffffffu, pre, 31), a.rows);
+      chunks += __shfl_sync(0xffffffffu, at, 31);
+    }
+    if (lane == 0) sm.chunks = chunks;
+  }
+  __syncthreads();
+  const int V = a.K / 16, items = sm.chunks * a.F, warps = int(gridDim.x) * (kRwThreads / 32);
+  auto channel = [&](int item, int& c, int& f, const uint4*& w, const uint4*& w2) {
+    c = item / a.F;
+    f = item - c * a.F;
+    w = reinterpret_cast<const uint4*>(a.wq) + (int64_t(sm.e[c]) * a.N + f) * V;
+    w2 = w + int64_t(a.F) * V;
+  };
+  int item = int(blockIdx.x) * (kRwThreads / 32) + warp;
+  int c = 0, f = 0;
+  const uint4 *w = nullptr, *w2 = nullptr;
+  uint4 buf[kRwLoads];
+  if (item < items) {
+    channel(item, c, f, w, w2);
+    rw_load<GLU>(w, w2, 0, V, lane, buf);
+  }
+  if (a.x != nullptr) {
+    if (a.x_f32) rw_quantize<float>(a, sm, rw_rows);
+    else rw_quantize<__nv_bfloat16>(a, sm, rw_rows);
+  } else {
+    for (int i = threadIdx.x; i < a.rows * V; i += kRwThreads)
+      reinterpret_cast<uint4*>(rw_rows)[i] = reinterpret_cast<const uint4*>(a.xq)[i];
+    if (int(threadIdx.x) < a.rows) sm.scale[threadIdx.x] = a.xs[threadIdx.x];
+  }
+  __syncthreads();
+  const uint4* rows = reinterpret_cast<const uint4*>(rw_rows);
+  while (item < items) {
+    const int n = sm.n[c];
+    if (n == 1) rw_channel<GLU, 1>(a, sm, rows, c, f, w, w2, buf);
+    else if (n == 2) rw_channel<GLU, 2>(a, sm, rows, c, f, w, w2, buf);
+    else rw_channel<GLU, 4>(a, sm, rows, c, f, w, w2, buf);
+    item += warps;
+    if (item < items) {
+      channel(item, c, f, w, w2);
+      rw_load<GLU>(w, w2, 0, V, lane, buf);
+    }
+  }
+}
+
 // ---------------------------------------------------------------- quantisation
 constexpr int kQuantThreads = 256;
 
@@ -897,6 +1033,25 @@ int w8a8_pairs(int dev, int sms, cudaLaunchConfig_t cfg, int* out) {
   return kOk;
 }
 
+// The form for a handful of rows: they have to fit shared memory twice per SM.
+bool rows_form(int64_t rows, int K) { return rows <= kRwMaxRows && rows * K <= int64_t(kRwMaxSmem); }
+
+template <bool GLU>
+int launch_rows(const RwArgs& a, int dev, int sms, cudaStream_t stream) {
+  static std::atomic<bool> ready[kMaxDevices];
+  if (dev < 0 || dev >= kMaxDevices) return kCudaErr;
+  if (!ready[dev].load(std::memory_order_acquire)) {
+    if (cudaFuncSetAttribute(w8a8_rows_kernel<GLU>, cudaFuncAttributeMaxDynamicSharedMemorySize, int(kRwMaxSmem)) !=
+        cudaSuccess)
+      return kCudaErr;
+    ready[dev].store(true, std::memory_order_release);
+  }
+  const int64_t warps = int64_t(a.F) * std::min(a.rows, a.E);  // at least one chunk per expert with rows
+  const int64_t blocks = std::min<int64_t>((warps + kRwThreads / 32 - 1) / (kRwThreads / 32), 2 * int64_t(sms));
+  w8a8_rows_kernel<GLU><<<unsigned(blocks), kRwThreads, size_t(a.rows) * a.K, stream>>>(a);
+  return cudaGetLastError() == cudaSuccess ? kOk : kCudaErr;
+}
+
 template <bool GLU, bool SPLIT>
 int launch_w8a8(const CUtensorMap& tw, const QRowMaps& tx, const QArgs& a, int dev, int sms, cudaStream_t stream) {
   cudaLaunchConfig_t cfg = {};
@@ -949,7 +1104,8 @@ extern "C" int moe_w8a8_scratch_bytes(int64_t rows, int32_t K, int32_t N, int32_
   if (!out || !q_sizes_ok(rows, K, N, E, swiglu)) return kBadArg;
   int sms = 0;
   if (cudaDeviceGetAttribute(&sms, cudaDevAttrMultiProcessorCount, device) != cudaSuccess) return kCudaErr;
-  *out = q_split(rows, N, swiglu ? N / 2 : N, swiglu != 0, sms / 2) ? size_t(sms / 2) * 2 * kQSlotInts * 4 : 0;
+  const bool split = !rows_form(rows, K) && q_split(rows, N, swiglu ? N / 2 : N, swiglu != 0, sms / 2);
+  *out = split ? size_t(sms / 2) * 2 * kQSlotInts * 4 : 0;
   return kOk;
 }
 
@@ -979,6 +1135,35 @@ extern "C" int moe_w8a8_gemm(const moe_w8a8_params* p, void* stream) {
   a.out_f32 = p->out_is_f32;
   a.part = static_cast<int32_t*>(p->scratch);
   a.status_host = p->status_host;
+  const cudaStream_t s = static_cast<cudaStream_t>(stream);
+  const bool few = rows_form(a.rows, a.K);
+  if (p->x && !(few && a.rows <= kRwMaxFresh)) {
+    int8_t* xq = static_cast<int8_t*>(const_cast<void*>(p->xq));
+    float* xs = const_cast<float*>(p->xs);
+    const int rc = p->x_is_f32 ? launch_quant<float>(p->x, a.rows, a.K, p->perm, p->live_rows, xq, xs, sms, s)
+                               : launch_quant<__nv_bfloat16>(p->x, a.rows, a.K, p->perm, p->live_rows, xq, xs, sms, s);
+    if (rc != kOk) return rc;
+  }
+  if (few) {
+    RwArgs w = {};
+    w.E = a.E;
+    w.K = a.K;
+    w.N = a.N;
+    w.F = a.F;
+    w.rows = int(a.rows);
+    w.counts = a.counts;
+    w.xq = static_cast<const int8_t*>(p->xq);
+    w.xs = p->xs;
+    w.x = a.rows <= kRwMaxFresh ? p->x : nullptr;
+    w.x_f32 = p->x_is_f32;
+    w.perm = p->perm;
+    w.live = p->live_rows;
+    w.wq = static_cast<const int8_t*>(p->wq);
+    w.ws = p->ws;
+    w.out = p->out;
+    w.out_f32 = p->out_is_f32;
+    return glu ? launch_rows<true>(w, dev, sms, s) : launch_rows<false>(w, dev, sms, s);
+  }
   const bool split = q_split(a.rows, a.N, a.F, glu, pairs);
   if (split && (!p->scratch || p->scratch_bytes < size_t(pairs) * 2 * kQSlotInts * 4)) return kBadArg;
 
@@ -996,26 +1181,6 @@ extern "C" int moe_w8a8_gemm(const moe_w8a8_params* p, void* stream) {
     const cuuint64_t str[1] = {cuuint64_t(a.K)};
     const cuuint32_t box[2] = {cuuint32_t(kQKb), 16u << i};
     if (encode_s8(&tx.m[i], 2, p->xq, dims, str, box)) return kCudaErr;
-  }
-  const cudaStream_t s = static_cast<cudaStream_t>(stream);
-  if (p->x) {
-    // Two rows per CTA at most are quantised inside the product (one row
-    // 7168 x 4096: 16.4 us as two launches, see the note at the top);
-    // more by a launch of their own.
-    int8_t* xq = static_cast<int8_t*>(const_cast<void*>(p->xq));
-    float* xs = const_cast<float*>(p->xs);
-    if (split && a.rows <= 2 * sms) {
-      a.x = p->x;
-      a.x_f32 = p->x_is_f32;
-      a.perm = p->perm;
-      a.live = p->live_rows;
-      a.xq_out = xq;
-      a.xs_out = xs;
-    } else {
-      const int rc = p->x_is_f32 ? launch_quant<float>(p->x, a.rows, a.K, p->perm, p->live_rows, xq, xs, sms, s)
-                                 : launch_quant<__nv_bfloat16>(p->x, a.rows, a.K, p->perm, p->live_rows, xq, xs, sms, s);
-      if (rc != kOk) return rc;
-    }
   }
   if (glu)
     return split ? launch_w8a8<true, true>(tw, tx, a, dev, sms, s) : launch_w8a8<true, false>(tw, tx, a, dev, sms, s);

@@ -126,6 +126,11 @@ PRODUCTS = [
     (2048, 2816, [600, 0, 7, 1]),
     (7168, 320, [1]),
     (7168, 4096, [1, 2]),
+    (7168, 512, [17]),
+    (528, 72, [3]),
+    (1040, 328, [2, 0, 4, 1, 5, 0, 4]),
+    (6128, 256, [4, 0, 0, 12]),
+    (6160, 256, [16]),
     (256, 4096, [1500, 2000, 1300]),   # whole tiles
     (512, 1536, [4090, 3841]),
 ]
@@ -216,7 +221,8 @@ def test_non_finite_rows_stay_apart():
     assert not w8a8.linear(x2, w)[7].any()
 
 
-@pytest.mark.parametrize("rows,K,Nn", [(1, 64, 40), (5, 7168, 128), (130, 512, 264), (3000, 256, 4096)])
+@pytest.mark.parametrize("rows,K,Nn", [(1, 64, 40), (1, 7168, 4096), (2, 2048, 264), (3, 1424, 136), (4, 7168, 264),
+                                       (5, 7168, 128), (17, 512, 128), (130, 512, 264), (3000, 256, 4096)])
 def test_linear(rows, K, Nn):
     g = torch.Generator(device="cuda").manual_seed(rows)
     x = torch.randn(rows, K, generator=g, device="cuda").to(torch.bfloat16)
