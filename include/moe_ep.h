@@ -438,16 +438,18 @@ int moe_quant_rows(const void* x, int32_t x_is_f32, int64_t rows, int32_t K, con
  * behind the sum of the counts are left as they were; counts beyond `rows`
  * are cut.  counts == NULL: one expert for all rows.
  * Requires K % 16 == 0, K <= 131056, N % 8 == 0 (16 with swiglu), experts <=
- * 1024; xq, wq, ws, out and scratch 16-byte aligned.  scratch:
+ * 1024; xq, wq, ws, out, x and scratch 16-byte aligned.  scratch:
  * moe_w8a8_scratch_bytes of device memory (may be 0), not initialised, for
- * this call alone until it has finished. */
+ * this call alone until it has finished.
+ * With x the rows are quantised first, as moe_quant_rows does (x_is_f32,
+ * perm, live_rows); xq and xs are then not used. */
 typedef struct moe_w8a8_params {
   int64_t rows;
   int32_t K, N, experts;
   int32_t swiglu, out_is_f32;
   int32_t x_is_f32;
-  const void* xq;          /* [rows, K] int8             */
-  const float* xs;         /* [rows]                     */
+  const void* xq;          /* [rows, K] int8 (no x)      */
+  const float* xs;         /* [rows] (no x)              */
   const void* wq;          /* [experts, N, K] int8       */
   const float* ws;         /* [experts, N]               */
   const int32_t* counts;   /* [experts] device, or NULL  */
@@ -455,13 +457,13 @@ typedef struct moe_w8a8_params {
   void* scratch;
   size_t scratch_bytes;
   int32_t* status_host;    /* optional mapped pinned word for device errors */
-  const void* x;           /* NULL, or rows to quantise first, into xq and xs */
-  const int32_t* perm;     /* (both then written), as moe_quant_rows does     */
+  const void* x;           /* [.., K] bf16 or fp32, or NULL                 */
+  const int32_t* perm;
   const int32_t* live_rows;
 } moe_w8a8_params;
 
-int moe_w8a8_scratch_bytes(int64_t rows, int32_t K, int32_t N, int32_t experts, int32_t swiglu, int32_t device,
-                           size_t* out);
+int moe_w8a8_scratch_bytes(int64_t rows, int32_t K, int32_t N, int32_t experts, int32_t swiglu, int32_t with_x,
+                           int32_t device, size_t* out);
 int moe_w8a8_gemm(const moe_w8a8_params* params, void* stream);
 
 /* y[t, :] = sum over k of top_vals[t, k] * rows[offsets[e] + slots[t, k], :],

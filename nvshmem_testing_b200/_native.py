@@ -136,7 +136,7 @@ def lib() -> ctypes.CDLL:
     L.moe_publish_i32.argtypes = [c_vp, c_i64, c_vp, c_vp]
     c_i32 = ctypes.c_int32
     L.moe_quant_rows.argtypes = [c_vp, c_i32, c_i64, c_i32, c_vp, c_vp, c_vp, c_vp, c_vp]
-    L.moe_w8a8_scratch_bytes.argtypes = [c_i64] + [c_i32] * 5 + [P(c_sz)]
+    L.moe_w8a8_scratch_bytes.argtypes = [c_i64] + [c_i32] * 6 + [P(c_sz)]
     L.moe_w8a8_gemm.argtypes = [P(W8A8Params), c_vp]
     L.moe_weighted_sum.argtypes = [c_vp, c_i32, c_vp, c_i32, c_i32, c_vp, c_i32, c_vp, c_vp, c_i64, c_i32, c_i32, c_i32,
                                    c_vp, c_vp]

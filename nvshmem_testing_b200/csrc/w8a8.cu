@@ -1099,20 +1099,38 @@ extern "C" int moe_quant_rows(const void* x, int32_t x_is_f32, int64_t rows, int
                   : launch_quant<__nv_bfloat16>(x, rows, K, perm, live_rows, q, scale, sms, s);
 }
 
-extern "C" int moe_w8a8_scratch_bytes(int64_t rows, int32_t K, int32_t N, int32_t E, int32_t swiglu, int32_t device,
-                                      size_t* out) {
+namespace {
+// scratch: partial sums of the split form, then (x given, quantised by a
+// launch of its own) the quantised rows and their scales.
+struct QScratch {
+  bool few, split, rows_outside;
+  size_t xq, xs, total;
+};
+QScratch q_scratch(int64_t rows, int K, int N, bool glu, bool with_x, int sms) {
+  QScratch q;
+  q.few = rows_form(rows, K);
+  q.split = !q.few && q_split(rows, N, glu ? N / 2 : N, glu, sms / 2);
+  q.rows_outside = with_x && !(q.few && rows <= kRwMaxFresh);
+  q.xq = q.split ? size_t(sms / 2) * 2 * kQSlotInts * 4 : 0;
+  q.xs = q.xq + (q.rows_outside ? (size_t(rows) * K + 255) / 256 * 256 : 0);
+  q.total = q.xs + (q.rows_outside ? size_t(rows) * 4 : 0);
+  return q;
+}
+}  // namespace
+
+extern "C" int moe_w8a8_scratch_bytes(int64_t rows, int32_t K, int32_t N, int32_t E, int32_t swiglu, int32_t with_x,
+                                      int32_t device, size_t* out) {
   if (!out || !q_sizes_ok(rows, K, N, E, swiglu)) return kBadArg;
   int sms = 0;
   if (cudaDeviceGetAttribute(&sms, cudaDevAttrMultiProcessorCount, device) != cudaSuccess) return kCudaErr;
-  const bool split = !rows_form(rows, K) && q_split(rows, N, swiglu ? N / 2 : N, swiglu != 0, sms / 2);
-  *out = split ? size_t(sms / 2) * 2 * kQSlotInts * 4 : 0;
+  *out = q_scratch(rows, K, N, swiglu != 0, with_x != 0, sms).total;
   return kOk;
 }
 
 extern "C" int moe_w8a8_gemm(const moe_w8a8_params* p, void* stream) {
   if (!p || !q_sizes_ok(p->rows, p->K, p->N, p->experts, p->swiglu)) return kBadArg;
   if (p->rows == 0) return kOk;
-  if (!p->xq || !p->xs || !p->wq || !p->ws || !p->out || (!p->counts && p->experts != 1)) return kBadArg;
+  if ((!p->x && (!p->xq || !p->xs)) || !p->wq || !p->ws || !p->out || (!p->counts && p->experts != 1)) return kBadArg;
   if (misaligned16(p->x)) return kBadArg;
   if (misaligned16(p->xq) || misaligned16(p->wq) || misaligned16(p->ws) || misaligned16(p->out) ||
       misaligned16(p->scratch))
@@ -1120,8 +1138,12 @@ extern "C" int moe_w8a8_gemm(const moe_w8a8_params* p, void* stream) {
   if (!driver().ok) return kCudaErr;
   int sms = 0, dev = 0;
   if (sm_count(&sms, &dev) != kOk) return kCudaErr;
-  const int pairs = sms / 2;
   const bool glu = p->swiglu != 0;
+  const QScratch sc = q_scratch(p->rows, p->K, p->N, glu, p->x != nullptr, sms);
+  unsigned char* scratch = static_cast<unsigned char*>(p->scratch);
+  if (sc.total > 0 && (!scratch || p->scratch_bytes < sc.total)) return kBadArg;
+  const int8_t* xq = static_cast<const int8_t*>(p->xq);
+  const float* xs = p->xs;
   QArgs a = {};
   a.E = p->experts;
   a.K = p->K;
@@ -1129,22 +1151,24 @@ extern "C" int moe_w8a8_gemm(const moe_w8a8_params* p, void* stream) {
   a.rows = p->rows;
   a.F = glu ? p->N / 2 : p->N;
   a.counts = p->counts;
-  a.xs = p->xs;
   a.ws = p->ws;
   a.out = p->out;
   a.out_f32 = p->out_is_f32;
-  a.part = static_cast<int32_t*>(p->scratch);
+  a.part = reinterpret_cast<int32_t*>(scratch);
   a.status_host = p->status_host;
   const cudaStream_t s = static_cast<cudaStream_t>(stream);
-  const bool few = rows_form(a.rows, a.K);
-  if (p->x && !(few && a.rows <= kRwMaxFresh)) {
-    int8_t* xq = static_cast<int8_t*>(const_cast<void*>(p->xq));
-    float* xs = const_cast<float*>(p->xs);
-    const int rc = p->x_is_f32 ? launch_quant<float>(p->x, a.rows, a.K, p->perm, p->live_rows, xq, xs, sms, s)
-                               : launch_quant<__nv_bfloat16>(p->x, a.rows, a.K, p->perm, p->live_rows, xq, xs, sms, s);
+  if (sc.rows_outside) {
+    int8_t* q = reinterpret_cast<int8_t*>(scratch + sc.xq);
+    float* scale = reinterpret_cast<float*>(scratch + sc.xs);
+    const int rc = p->x_is_f32
+                       ? launch_quant<float>(p->x, a.rows, a.K, p->perm, p->live_rows, q, scale, sms, s)
+                       : launch_quant<__nv_bfloat16>(p->x, a.rows, a.K, p->perm, p->live_rows, q, scale, sms, s);
     if (rc != kOk) return rc;
+    xq = q;
+    xs = scale;
   }
-  if (few) {
+  a.xs = xs;
+  if (sc.few) {
     RwArgs w = {};
     w.E = a.E;
     w.K = a.K;
@@ -1152,9 +1176,9 @@ extern "C" int moe_w8a8_gemm(const moe_w8a8_params* p, void* stream) {
     w.F = a.F;
     w.rows = int(a.rows);
     w.counts = a.counts;
-    w.xq = static_cast<const int8_t*>(p->xq);
-    w.xs = p->xs;
-    w.x = a.rows <= kRwMaxFresh ? p->x : nullptr;
+    w.xq = xq;
+    w.xs = xs;
+    w.x = sc.rows_outside ? nullptr : p->x;
     w.x_f32 = p->x_is_f32;
     w.perm = p->perm;
     w.live = p->live_rows;
@@ -1164,9 +1188,7 @@ extern "C" int moe_w8a8_gemm(const moe_w8a8_params* p, void* stream) {
     w.out_f32 = p->out_is_f32;
     return glu ? launch_rows<true>(w, dev, sms, s) : launch_rows<false>(w, dev, sms, s);
   }
-  const bool split = q_split(a.rows, a.N, a.F, glu, pairs);
-  if (split && (!p->scratch || p->scratch_bytes < size_t(pairs) * 2 * kQSlotInts * 4)) return kBadArg;
-
+  const bool split = sc.split;
   CUtensorMap tw;
   QRowMaps tx;
   {
@@ -1180,7 +1202,7 @@ extern "C" int moe_w8a8_gemm(const moe_w8a8_params* p, void* stream) {
     const cuuint64_t dims[2] = {cuuint64_t(a.K), cuuint64_t(a.rows)};
     const cuuint64_t str[1] = {cuuint64_t(a.K)};
     const cuuint32_t box[2] = {cuuint32_t(kQKb), 16u << i};
-    if (encode_s8(&tx.m[i], 2, p->xq, dims, str, box)) return kCudaErr;
+    if (encode_s8(&tx.m[i], 2, xq, dims, str, box)) return kCudaErr;
   }
   if (glu)
     return split ? launch_w8a8<true, true>(tw, tx, a, dev, sms, s) : launch_w8a8<true, false>(tw, tx, a, dev, sms, s);

@@ -37,14 +37,12 @@ def _check(x, w13, w2, out, status):
         raise ValueError(f"x {tuple(x.shape)}, w13 {tuple(w13.shape)} and w2 {tuple(w2.shape)} do not form an MLP")
     if H % 8 or F % 8 or H == 0 or F == 0:
         raise ValueError(f"H = {H} and F = {F} must be positive multiples of 8")
-    for name, t in (("x", x), ("w13", w13), ("w2", w2)):
-        if t.dtype != torch.bfloat16:
-            raise TypeError(f"{name} must be bfloat16")
-        if not t.is_cuda or t.device != x.device:
-            raise ValueError(f"{name} must be a CUDA tensor on the tokens' device")
-    for name, t in (("w13", w13), ("w2", w2)):
-        if not t.is_contiguous():
-            raise ValueError(f"{name} must be contiguous")
+    if not (x.dtype == w13.dtype == w2.dtype == torch.bfloat16):
+        raise TypeError("x, w13 and w2 must be bfloat16")
+    if not x.is_cuda or w13.device != x.device or w2.device != x.device:
+        raise ValueError("x, w13 and w2 must be CUDA tensors on one device")
+    if not w13.is_contiguous() or not w2.is_contiguous():
+        raise ValueError("w13 and w2 must be contiguous")
     if T > N.DECODE_MAX_TOKENS:
         raise ValueError(f"{T} tokens: this form takes {N.DECODE_MAX_TOKENS} at most (mlp.moe_mlp has no limit)")
     if out is not None and (tuple(out.shape) != (T, H) or out.dtype != torch.bfloat16 or out.device != x.device
@@ -68,18 +66,13 @@ def _launch(x, ids, vals, w13, w2, router_w, K, first_expert, renormalize, out, 
         out = torch.empty((T, H), dtype=torch.bfloat16, device=x.device)
     if T == 0:
         return out
-    p = N.DecodeParams()
-    p.T, p.hidden, p.ffn, p.experts, p.K, p.first_expert = T, H, F, El, K, first_expert
     Er = 0 if router_w is None else router_w.shape[1]
-    p.router_experts, p.renormalize = Er, renormalize
-    p.ids_are_int64, p.vals_are_bf16 = ids.dtype == torch.int64, vals.dtype == torch.bfloat16
     need = _scratch_bytes(T, H, F, El, K, Er, x.device.index)
     scratch = torch.empty(need, dtype=torch.uint8, device=x.device)
-    p.x, p.w13, p.w2, p.y = x.data_ptr(), w13.data_ptr(), w2.data_ptr(), out.data_ptr()
-    p.router_w = None if router_w is None else router_w.data_ptr()
-    p.top_idxs, p.top_vals = ids.data_ptr(), vals.data_ptr()
-    p.scratch, p.scratch_bytes = scratch.data_ptr(), need
-    p.status_host = None if status is None else status.data_ptr()
+    p = N.DecodeParams(T, H, F, El, K, first_expert, Er, renormalize, ids.dtype == torch.int64,
+                       vals.dtype == torch.bfloat16, 0, x.data_ptr(), w13.data_ptr(), w2.data_ptr(),
+                       None if router_w is None else router_w.data_ptr(), ids.data_ptr(), vals.data_ptr(),
+                       out.data_ptr(), scratch.data_ptr(), need, None if status is None else status.data_ptr())
     with utils.on_device(x.device) as stream:
         N.check(N.lib().moe_decode_layer(ctypes.byref(p), stream), "moe_decode_layer")
     return out

@@ -86,18 +86,14 @@ def quantize_rows(x: torch.Tensor, perm: torch.Tensor | None = None,
         raise TypeError("live_rows must be one int32")
     _on_gpu(x.device, x=x, perm=perm, live_rows=live_rows)
     rows = x.shape[0] if perm is None else perm.shape[0]
-    with utils.on_device(x.device) as stream:
-        return _quantize(x.contiguous(), rows, K, perm, live_rows, stream)
-
-
-def _quantize(x, rows, K, perm, live_rows, stream):
-    """The checked call."""
+    x = x.contiguous()
     q = torch.empty((rows, K), dtype=torch.int8, device=x.device)
     scale = torch.empty(rows, dtype=torch.float32, device=x.device)
-    N.check(N.lib().moe_quant_rows(x.data_ptr(), x.dtype == torch.float32, rows, K,
-                                   None if perm is None else perm.data_ptr(),
-                                   None if live_rows is None else live_rows.data_ptr(), q.data_ptr(),
-                                   scale.data_ptr(), stream), "moe_quant_rows")
+    with utils.on_device(x.device) as stream:
+        N.check(N.lib().moe_quant_rows(x.data_ptr(), x.dtype == torch.float32, rows, K,
+                                       None if perm is None else perm.data_ptr(),
+                                       None if live_rows is None else live_rows.data_ptr(), q.data_ptr(),
+                                       scale.data_ptr(), stream), "moe_quant_rows")
     return q, scale
 
 
@@ -157,32 +153,20 @@ def grouped_gemm(xq: torch.Tensor, xs: torch.Tensor, w: QuantWeights, counts: to
     if rows == 0:
         return out
     with utils.on_device(xq.device) as stream:
-        _gemm(xq.contiguous(), xs.contiguous(), w, counts, rows, K, Nw, El, swiglu, out, status, stream)
+        _gemm(xq.contiguous(), xs.contiguous(), None, w, counts, None, None, rows, K, Nw, El, swiglu, out, status,
+              stream)
     return out
 
 
-def _gemm(xq, xs, w, counts, rows, K, Nw, El, swiglu, out, status, stream):
-    """The checked call for quantised rows."""
-    need = _scratch_bytes(rows, K, Nw, El, int(swiglu), xq.device.index)
-    scratch = torch.empty(need, dtype=torch.uint8, device=xq.device) if need else None
-    p = N.W8A8Params(rows, K, Nw, El, swiglu, out.dtype == torch.float32, 0, xq.data_ptr(), xs.data_ptr(),
-                     w.q.data_ptr(), w.scale.data_ptr(), None if counts is None else counts.data_ptr(),
-                     out.data_ptr(), None if scratch is None else scratch.data_ptr(), need,
-                     None if status is None else status.data_ptr(), None, None, None)
-    N.check(N.lib().moe_w8a8_gemm(ctypes.byref(p), stream), "moe_w8a8_gemm")
-
-
-def _quantized_gemm(x, w, counts, perm, live_rows, rows, K, Nw, El, swiglu, out, status, stream):
-    """The checked call for rows that are still to be quantised: rows, scales
-    and partial sums in one scratch tensor."""
-    need = _scratch_bytes(rows, K, Nw, El, int(swiglu), x.device.index)
-    s_at = (rows * K + 255) // 256 * 256
-    p_at = (s_at + rows * 4 + 255) // 256 * 256
-    scratch = torch.empty(p_at + need, dtype=torch.uint8, device=x.device)
-    base = scratch.data_ptr()
-    p = N.W8A8Params(rows, K, Nw, El, swiglu, out.dtype == torch.float32, x.dtype == torch.float32, base, base + s_at,
-                     w.q.data_ptr(), w.scale.data_ptr(), None if counts is None else counts.data_ptr(),
-                     out.data_ptr(), base + p_at, need, None if status is None else status.data_ptr(), x.data_ptr(),
+def _gemm(xq, xs, x, w, counts, perm, live_rows, rows, K, Nw, El, swiglu, out, status, stream):
+    """The checked call, for quantised rows (xq, xs) or rows x that are still
+    to be."""
+    need = _scratch_bytes(rows, K, Nw, El, int(swiglu), int(x is not None), out.device.index)
+    scratch = torch.empty(need, dtype=torch.uint8, device=out.device).data_ptr() if need else None
+    p = N.W8A8Params(rows, K, Nw, El, swiglu, out.dtype == torch.float32, x is not None and x.dtype == torch.float32,
+                     None if xq is None else xq.data_ptr(), None if xs is None else xs.data_ptr(), w.q.data_ptr(),
+                     w.scale.data_ptr(), None if counts is None else counts.data_ptr(), out.data_ptr(), scratch, need,
+                     None if status is None else status.data_ptr(), None if x is None else x.data_ptr(),
                      None if perm is None else perm.data_ptr(), None if live_rows is None else live_rows.data_ptr())
     N.check(N.lib().moe_w8a8_gemm(ctypes.byref(p), stream), "moe_w8a8_gemm")
 
@@ -203,7 +187,7 @@ def linear(x: torch.Tensor, w: QuantWeights, *, out_dtype=torch.bfloat16) -> tor
     out = torch.empty((rows, Nw), dtype=out_dtype, device=x.device)
     if rows:
         with utils.on_device(x.device) as stream:
-            _quantized_gemm(x.contiguous(), w, None, None, None, rows, K, Nw, 1, False, out, None, stream)
+            _gemm(None, None, x.contiguous(), w, None, None, None, rows, K, Nw, 1, False, out, None, stream)
     return out
 
 
@@ -258,10 +242,10 @@ def moe_layer(x: torch.Tensor, top_idxs: torch.Tensor, top_vals: torch.Tensor, w
         r = utils.route(ids if first_expert == 0 else ids - first_expert, El, with_slots=True)
         n, live = T * K, r.offsets[El:]
         h = torch.empty((n, F), dtype=torch.float32, device=x.device)
-        _quantized_gemm(x.contiguous(), w13, r.counts, r.perm, live, n, H, F2, El, True, h, status, stream)
+        _gemm(None, None, x.contiguous(), w13, r.counts, r.perm, live, n, H, F2, El, True, h, status, stream)
         # fp32 rows: y is rounded once, like a layer that never splits its sum
         rows = torch.empty((n, H), dtype=torch.float32, device=x.device)
-        _quantized_gemm(h, w2, r.counts, None, live, n, F, H, El, False, rows, status, stream)
+        _gemm(None, None, h, w2, r.counts, None, live, n, F, H, El, False, rows, status, stream)
         N.check(N.lib().moe_weighted_sum(rows.data_ptr(), 1, ids.data_ptr(), ids.dtype == torch.int64, first_expert,
                                          vals.data_ptr(), vals.dtype == torch.bfloat16, r.slots.data_ptr(),
                                          r.offsets.data_ptr(), T, K, H, El, y.data_ptr(), stream),

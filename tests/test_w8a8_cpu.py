@@ -56,13 +56,13 @@ def test_c_entries_refuse_before_any_device_call():
     def scratch(*a):
         return lib.moe_w8a8_scratch_bytes(*a, ctypes.byref(need))
 
-    #              rows, K, N, E, swiglu, device
-    assert scratch(-1, 64, 64, 1, 0, 0) == N.BAD_ARG
-    assert scratch(4, 60, 64, 1, 0, 0) == N.BAD_ARG
-    assert scratch(4, 131072, 64, 1, 0, 0) == N.BAD_ARG
-    assert scratch(4, 64, 60, 1, 0, 0) == N.BAD_ARG
-    assert scratch(4, 64, 24, 1, 1, 0) == N.BAD_ARG
-    assert scratch(4, 64, 64, 1025, 0, 0) == N.BAD_ARG
+    #              rows, K, N, E, swiglu, with_x, device
+    assert scratch(-1, 64, 64, 1, 0, 0, 0) == N.BAD_ARG
+    assert scratch(4, 60, 64, 1, 0, 0, 0) == N.BAD_ARG
+    assert scratch(4, 131072, 64, 1, 0, 0, 0) == N.BAD_ARG
+    assert scratch(4, 64, 60, 1, 0, 0, 0) == N.BAD_ARG
+    assert scratch(4, 64, 24, 1, 1, 0, 0) == N.BAD_ARG
+    assert scratch(4, 64, 64, 1025, 0, 0, 0) == N.BAD_ARG
     p = N.W8A8Params()
     p.rows, p.K, p.N, p.experts = 4, 64, 64, 2
     assert lib.moe_w8a8_gemm(ctypes.byref(p), None) == N.BAD_ARG  # null pointers
