@@ -174,6 +174,52 @@ __host__ __device__ inline uint32_t dec_table_bytes(int maxact, int rows) {
 // memory.
 __device__ void dec_build(const DecArgs& a, DecSmem& sm, const DecTables& tb, unsigned char* scratch, const void* ids,
                           int ids64, const void* vals, int vals_bf16) {
+  if (a.T * a.K <= 32) {
+    // Few rows: one warp sorts them by expert, then token, by counting.
+    const int lane = threadIdx.x;
+    if (lane < 32) {
+      const int n = a.T * a.K, t = lane / a.K;
+      long long e = -1;
+      float v = 0.f;
+      if (lane < n) {
+        e = load_id(ids, ids64, lane) - a.first;
+        v = vals_bf16 ? __bfloat162float(static_cast<const __nv_bfloat16*>(vals)[lane])
+                      : static_cast<const float*>(vals)[lane];
+      }
+      // The order of a row: expert, token, and (an id repeated within a
+      // token's row counts once) its first place; what is not held here last.
+      const uint32_t key = e >= 0 && e < a.E ? uint32_t(e) * 32 + uint32_t(t) : 0xffffffffu;
+      const uint32_t same = __match_any_sync(0xffffffffu, key);
+      const bool on = key != 0xffffffffu && (same & ((1u << lane) - 1)) == 0;
+      const uint32_t expert = on ? key >> 5 : 0xffffffffu;
+      const uint32_t peers = __match_any_sync(0xffffffffu, expert);  // rows of the same expert
+      const bool head = on && (peers & ((1u << lane) - 1)) == 0;
+      int row = 0, at = 0;
+#pragma unroll 4
+      for (int j = 0; j < 32; ++j) {
+        const uint32_t kj = __shfl_sync(0xffffffffu, on ? key : 0xffffffffu, j);
+        const uint32_t hj = __shfl_sync(0xffffffffu, head ? expert : 0xffffffffu, j);
+        row += on && kj < key;
+        at += on && hj < expert;
+      }
+      if (on) {
+        tb.tok[row] = uint8_t(t);
+        tb.val[row] = v;
+      }
+      // Rows of an expert are ascending by token: its head is the first.
+      if (head) {
+        tb.act_e[at] = uint16_t(expert);
+        tb.act_off[at] = uint16_t(row);
+      }
+      const uint32_t ons = __ballot_sync(0xffffffffu, on), heads = __ballot_sync(0xffffffffu, head);
+      if (lane == 0) {
+        tb.act_off[__popc(heads)] = uint16_t(__popc(ons));
+        sm.nact = __popc(heads);
+      }
+    }
+    __syncthreads();
+    return;
+  }
   unsigned long long* mask = reinterpret_cast<unsigned long long*>(scratch);  // [E]
   float* v = reinterpret_cast<float*>(mask + a.E);                            // [T*K]
   uint16_t* off_e = reinterpret_cast<uint16_t*>(v + a.T * a.K);               // [E]
@@ -288,12 +334,12 @@ __device__ void dec_router_partial(const DecArgs& a, unsigned char* stage) {
 #pragma unroll
           for (int i = 0; i < 8; ++i) {
             const int h = hb + i * groups;
-            if (h >= nh) break;
             const float2 w = __bfloat1622float2(w8[i]);
-            const float4* xv = reinterpret_cast<const float4*>(xs + (ch * nh + h) * kDecTokChunk);
+            const float4* xv = reinterpret_cast<const float4*>(xs + (ch * nh + min(h, nh - 1)) * kDecTokChunk);
             float xr[kDecTokChunk];
 #pragma unroll
-            for (int j = 0; j < kDecTokChunk; j += 4) *reinterpret_cast<float4*>(&xr[j]) = xv[j / 4];
+            for (int j = 0; j < kDecTokChunk; j += 4)
+              *reinterpret_cast<float4*>(&xr[j]) = h < nh ? xv[j / 4] : make_float4(0.f, 0.f, 0.f, 0.f);
 #pragma unroll
             for (int j = 0; j < kDecTokChunk; ++j) {
               s[j].x = fmaf(xr[j], w.x, s[j].x);
@@ -580,6 +626,9 @@ __global__ void __launch_bounds__(kDecThreads, 1)
 
   // ---- loads (one thread)
   Ring lr = {0, 0};  // next stage to fill
+  // Weights are read once: they leave L2 first, so that activations, partial
+  // sums and the kernel's own code stay.
+  const uint64_t once = l2_policy_evict_first();
   // A unit's weights into the next stage; the stage's expected bytes include
   // the rows that load_rows adds.
   auto load_weights = [&](auto pass, const Cursor& c) -> bool {
@@ -593,14 +642,15 @@ __global__ void __launch_bounds__(kDecThreads, 1)
     const int e = tb.act_e[c.ai];
     if constexpr (PASS == 1) {
       mbar_arrive_expect_tx(full, kDecABytes + uint32_t(a.NB) * 128);
-      tma_load_4d(&tm_w13, full, dst, c.ft * 128, c.k * 64, 0, e);
-      tma_load_4d(&tm_w13, full, dst + 16384, c.ft * 128 + 64, c.k * 64, 0, e);
+      tma_load_4d_hint(&tm_w13, full, dst, c.ft * 128, c.k * 64, 0, e, once);
+      tma_load_4d_hint(&tm_w13, full, dst + 16384, c.ft * 128 + 64, c.k * 64, 0, e, once);
     } else {
       mbar_arrive_expect_tx(full, kDecABytes + uint32_t((act_rows(c.ai) + 15) >> 4) * 2048);
       if (a.w2_atoms) {
-        tma_load_4d(&tm_w2, full, dst, 0, c.k * 64, c.ft * 4, e);
+        tma_load_4d_hint(&tm_w2, full, dst, 0, c.k * 64, c.ft * 4, e, once);
       } else {
-        for (int g = 0; g < 4; ++g) tma_load_3d(&tm_w2, full, dst + g * 8192, c.ft * 256 + g * 64, c.k * 64, e);
+        for (int g = 0; g < 4; ++g)
+          tma_load_3d_hint(&tm_w2, full, dst + g * 8192, c.ft * 256 + g * 64, c.k * 64, e, once);
       }
     }
     sm.fills[lr.st] += 1;
