@@ -19,8 +19,12 @@
 //           outputs meet without leaving the CTA.
 // Each pass splits its list of 32 KB units evenly over the CTAs, at any k:
 // every SM streams the same number of bytes whatever the number of experts
-// or tiles.  A tile that ends up in several CTAs is summed from fp32
-// partials in CTA order, so results do not depend on timing: in pass 1 by the
+// or tiles.  SMs do not get the same bandwidth, though (those of the fuller
+// GPCs up to 14 % less, always the same ones), so of a long list the last
+// eighth is left in small chunks for whoever is done first (7 tokens, 8
+// experts of 352 MB: 410 -> 392 us; 705 MB in all: no gain).  A tile that ends
+// up in several parts is summed from fp32 partials in the order of the list,
+// so results depend neither on timing nor on who did what: in pass 1 by the
 // last of its CTAs (few parts, few rows), in pass 2, where 256 features may
 // be spread over all CTAs, by the whole grid after another barrier.
 // The weights' first stages of a pass are requested before the barrier in
@@ -53,6 +57,9 @@ constexpr int kDecMaxStages = 8;
 constexpr uint32_t kDecABytes = 256 * 64 * 2;     // 256 features x 64 K
 constexpr uint32_t kDecMaxSmem = 226 * 1024;      // dynamic; under 1 KB is static
 constexpr int kDecTokChunk = 8;                   // router: tokens whose logits a thread sums at a time
+constexpr int kDecMaxChunks = 640;                // handed out as CTAs get done
+constexpr int kDecChunkTokens = 32;               // most tokens of a call that uses them (partials grow with T)
+constexpr int kDecRunSlots = 16;                  // > stages + 2 accumulators: runs under way in a CTA
 constexpr uint64_t kDecBoundNs = 2000000000ull;   // bug guard on every pipeline wait
 constexpr int kBarEpi = 1;
 
@@ -68,8 +75,8 @@ struct DecArgs {
   const void* vals;
   int ids64, vals_bf16;
   __nv_bfloat16* hs;         // [T*K][F]
-  float* part;               // [2 * grid][T][256]
-  uint32_t* ctr;             // [grid] tickets of pass 1's split tiles
+  float* part;               // [2 * (grid + kDecMaxChunks)][T][256]
+  uint32_t* ctr;             // [grid + kDecMaxChunks] tickets of pass 1's split tiles, [2] chunks handed out
   __nv_bfloat16* y;
   int32_t* status_host;
   // Routed form (router_w != nullptr).
@@ -87,6 +94,8 @@ struct alignas(16) DecSmem {
   uint64_t tfull[2];
   uint64_t tempty[2];
   uint64_t drain;
+  uint64_t run[kDecRunSlots];   // a chunk (or the end) has been taken
+  int chunk[kDecRunSlots];
   uint32_t fills[kDecMaxStages];
   uint32_t tmem_base;
   int err;
@@ -376,10 +385,17 @@ __device__ void dec_router_partial(const DecArgs& a, unsigned char* stage) {
   }
 }
 
+// A logit's bits as an unsigned number of the same order (-0 and 0 alike, NaN
+// lowest).
+__device__ __forceinline__ uint32_t order_key(float v) {
+  const uint32_t bits = __float_as_uint(v + 0.f);
+  return v != v ? 0u : (bits >> 31) ? ~bits : (bits | 0x80000000u);
+}
+constexpr int kDecCountExperts = 128;
+
 // Router, step 2: tokens t0, t0 + stride, ...: the slices' sum in order, the
 // softmax over Er in fp32 and the K largest (equal logits: lowest id first).
-// An expert's place is the number of experts before it, counted by one
-// thread per expert: one pass over Er keys instead of K rounds.  The last
+// The last
 // token's routing also stays in `keep`.
 struct DecRouted {
   long long id[kMaxRouteK];
@@ -390,8 +406,9 @@ __device__ void dec_router_topk(const DecArgs& a, unsigned char* stage, unsigned
   const int hparts = int(gridDim.x) / a.eparts, tid = threadIdx.x, lane = tid & 31;
   float* red = reinterpret_cast<float*>(stage);              // [parts][Er]
   float* lg = reinterpret_cast<float*>(scratch);             // [Er]
-  uint32_t* key = reinterpret_cast<uint32_t*>(lg + a.Er);    // [Er]
+  uint2* cand = reinterpret_cast<uint2*>(lg + a.Er);         // [groups][K] (key, id)
   __shared__ int chosen[kMaxRouteK];
+  __shared__ float norm[2];
   const int E4 = a.Er / 4;  // four experts per load
   const int parts = kDecThreads / E4;
   float4* red4 = reinterpret_cast<float4*>(red);
@@ -411,27 +428,64 @@ __device__ void dec_router_topk(const DecArgs& a, unsigned char* stage, unsigned
 #pragma unroll 4
       for (int q = 0; q < parts; ++q) v += red[q * a.Er + e];
       lg[e] = v;
-      // The logit's bits as an unsigned number of the same order (-0 and 0
-      // alike, NaN lowest).
-      const uint32_t b = __float_as_uint(v + 0.f);
-      key[e] = v != v ? 0u : (b >> 31) ? ~b : (b | 0x80000000u);
     }
     __syncthreads();
-#pragma unroll 1
-    for (int e = tid; e < a.Er; e += kDecThreads) {
-      const uint32_t mine = key[e];
-      const uint4* keys = reinterpret_cast<const uint4*>(key);
+    // Few experts: an expert's place is the number of those before it,
+    // counted by one thread each.  More (256: 5.3 us against 4.0): the K
+    // largest of every 32, a warp each, then K times the largest of those.
+    const int warp = tid >> 5, warps = kDecThreads / 32, groups = a.Er <= kDecCountExperts ? 0 : (a.Er + 31) / 32;
+    if (groups == 0 && tid < a.Er) {
+      const uint32_t mine = order_key(lg[tid]);
       int before = 0;
 #pragma unroll 4
       for (int i = 0; i < E4; ++i) {  // a key before mine, or the same one at a lower id
-        const uint4 k = keys[i];
-        before += int(k.x >= mine + (4 * i >= e)) + int(k.y >= mine + (4 * i + 1 >= e)) +
-                  int(k.z >= mine + (4 * i + 2 >= e)) + int(k.w >= mine + (4 * i + 3 >= e));
+        const float4 k = reinterpret_cast<const float4*>(lg)[i];
+        before += int(order_key(k.x) >= mine + (4 * i >= tid)) + int(order_key(k.y) >= mine + (4 * i + 1 >= tid)) +
+                  int(order_key(k.z) >= mine + (4 * i + 2 >= tid)) + int(order_key(k.w) >= mine + (4 * i + 3 >= tid));
       }
-      if (before < a.K) chosen[before] = e;
+      if (before < a.K) chosen[before] = tid;
     }
-    __syncthreads();
+#pragma unroll 1
+    for (int g = warp; g < groups; g += warps) {
+      const int e = g * 32 + lane;
+      bool open = e < a.Er;
+      const uint32_t key = order_key(open ? lg[e] : 0.f);
+#pragma unroll 1
+      for (int k = 0; k < a.K; ++k) {
+        const uint32_t top = __reduce_max_sync(0xffffffffu, open ? key : 0u);
+        const uint32_t have = __ballot_sync(0xffffffffu, open && key == top);
+        if (have == 0) {  // fewer than K in the group
+          if (lane == 0) cand[g * a.K + k] = make_uint2(0u, INT_MAX);
+        } else if (lane == __ffs(have) - 1) {  // equal logits: the lowest id
+          cand[g * a.K + k] = make_uint2(key, uint32_t(e));
+          open = false;
+        }
+      }
+    }
+    if (groups > 0) __syncthreads();
     if (tid < 32) {
+      // (An id of INT_MAX: taken, or none.)
+      const int n = groups * a.K;
+#pragma unroll 1
+      for (int k = 0; k < a.K && groups > 0; ++k) {
+        uint32_t best = 0, be = INT_MAX;
+        int at = 0;
+#pragma unroll 1
+        for (int i = lane; i < n; i += 32) {
+          const uint2 c = cand[i];
+          if (c.y != INT_MAX && (be == INT_MAX || c.x > best || (c.x == best && c.y < be))) {
+            best = c.x;
+            be = c.y;
+            at = i;
+          }
+        }
+        const uint32_t top = __reduce_max_sync(0xffffffffu, best);
+        const uint32_t pick = __reduce_min_sync(0xffffffffu, best == top ? be : INT_MAX);
+        if (best == top && be == pick) cand[at].y = INT_MAX;
+        if (lane == 0) chosen[k] = int(pick);
+      }
+      __syncwarp();
+    } else if (tid < 64) {
       float m = -INFINITY;
 #pragma unroll 1
       for (int e = lane; e < a.Er; e += 32) m = fmaxf(m, lg[e]);
@@ -442,6 +496,14 @@ __device__ void dec_router_topk(const DecArgs& a, unsigned char* stage, unsigned
       for (int e = lane; e < a.Er; e += 32) z += expf(lg[e] - m);
 #pragma unroll
       for (int o = 16; o > 0; o >>= 1) z += __shfl_xor_sync(0xffffffffu, z, o);
+      if (lane == 0) {
+        norm[0] = m;
+        norm[1] = z;
+      }
+    }
+    __syncthreads();
+    if (tid < 32) {
+      const float m = norm[0], z = norm[1];
       const int id = lane < a.K ? chosen[lane] : 0;
       const float pr = lane < a.K ? expf(lg[id] - m) / z : 0.f;
       float sum = pr;
@@ -463,7 +525,9 @@ __device__ void dec_router_topk(const DecArgs& a, unsigned char* stage, unsigned
   }
 }
 
-// One pass: its units in order, and this CTA's share [lo, hi) of them.
+// One pass: its units in order.  The first `fixed` are shared out evenly, the
+// rest lies in `chunks` chunks of `cz`; a CTA's share and every chunk is a
+// part.
 // Pass 1: expert by expert, its tiles of 128 features of F, each over H.
 // Pass 2: tile by tile of 256 features of H, each over the experts' F.
 struct Pass {
@@ -471,8 +535,12 @@ struct Pass {
   int tile;      // units of one tile (the units whose sums belong together)
   int kb;        // units of one expert's K
   int nt;        // tiles per expert (pass 1), tiles (pass 2)
-  int g;         // CTAs that have units
-  int lo, hi;
+  int g;         // CTAs that have a share
+  int fixed, chunks, cz;
+  int lo, hi;    // this CTA's share
+  __device__ __forceinline__ int part_of(int u) const {
+    return u < fixed ? share_owner(uint32_t(fixed), uint32_t(g), uint32_t(u)) : g + (u - fixed) / cz;
+  }
 };
 
 // A position in a pass, moved on by additions: the loads and the MMAs each
@@ -527,7 +595,7 @@ struct Ring {
 __global__ void __launch_bounds__(kDecThreads, 1)
     decode_kernel(const __grid_constant__ CUtensorMap tm_w13, const __grid_constant__ CUtensorMap tm_w2,
                   const __grid_constant__ CUtensorMap tm_x, const __grid_constant__ CUtensorMap tm_h,
-                  const DecArgs a) {
+                  const __grid_constant__ DecArgs a) {
   extern __shared__ unsigned char dec_dyn[];
   unsigned char* stage =
       reinterpret_cast<unsigned char*>((reinterpret_cast<uintptr_t>(dec_dyn) + 1023) & ~uintptr_t(1023));
@@ -557,6 +625,7 @@ __global__ void __launch_bounds__(kDecThreads, 1)
       mbar_init(&sm.tempty[i], kDecEpiWarps);
     }
     mbar_init(&sm.drain, 1);
+    for (int i = 0; i < kDecRunSlots; ++i) mbar_init(&sm.run[i], 1);
     sm.err = 0;
     fence_mbar_init();
     prefetch_tensormap(&tm_w13);
@@ -573,7 +642,7 @@ __global__ void __launch_bounds__(kDecThreads, 1)
   // The tickets of split tiles start at zero: written here, ordered before
   // their first use by the first grid barrier.
   if (blockIdx.x == 0)
-    for (int i = threadIdx.x; i < int(gridDim.x); i += kDecThreads) a.ctr[i] = 0;
+    for (int i = threadIdx.x; i < int(gridDim.x) + kDecMaxChunks + 2; i += kDecThreads) a.ctr[i] = 0;
 
   // (The block meets in each of the following steps before anything of the
   // above is used.)
@@ -612,16 +681,58 @@ __global__ void __launch_bounds__(kDecThreads, 1)
     p.tile = tile;
     p.kb = kb;
     p.nt = nt;
-    p.g = min(G, p.units);
+    p.chunks = 0;
+    p.cz = 1;
+    if (a.T <= kDecChunkTokens && p.units >= 128 * G) {  // shorter lists: the chunks' sums cost more than they gain
+      const int rest = p.units / 8;
+      p.cz = max(16, (rest + kDecMaxChunks - 1) / kDecMaxChunks);
+      p.chunks = rest / p.cz;
+    }
+    p.fixed = p.units - p.chunks * p.cz;
+    p.g = min(G, p.fixed);
     const bool on = int(blockIdx.x) < p.g;
-    p.lo = on ? share_lo(p.units, p.g, blockIdx.x) : 0;
-    p.hi = on ? share_lo(p.units, p.g, blockIdx.x + 1) : 0;
+    p.lo = on ? share_lo(p.fixed, p.g, blockIdx.x) : 0;
+    p.hi = on ? share_lo(p.fixed, p.g, blockIdx.x + 1) : 0;
     return p;
   };
   const int kb1 = (a.H + 63) / 64, nt1 = (a.F + 127) / 128;
   const int kb2 = (a.F + 63) / 64, nt2 = (a.H + 255) / 256;
   const Pass p1 = make_pass(nact * nt1, kb1, kb1, nt1);
   const Pass p2 = make_pass(nact > 0 ? nt2 : 0, nact * kb2, kb2, nt2);
+  // The runs of units that a CTA does in a pass: its share, then chunks until
+  // none is left.  One thread takes them and the other roles follow through
+  // a ring in shared memory; `n` counts a role's chunks over both passes.
+  struct Runs {
+    int n;          // chunks seen by this role
+    int lo, hi;     // current run
+    int part;
+  };
+  auto first_run = [&](Runs& r, const Pass& p) {
+    r.lo = p.lo;
+    r.hi = p.hi;
+    r.part = blockIdx.x;
+  };
+  auto set_run = [&](Runs& r, const Pass& p, int chunk) {
+    r.lo = p.fixed + chunk * p.cz;
+    r.hi = r.lo + p.cz;
+    r.part = p.g + chunk;
+    return chunk >= 0;
+  };
+  auto take_run = [&](Runs& r, const Pass& p, int pass) {
+    if (p.chunks == 0) return false;
+    int chunk = int(atomicAdd(&a.ctr[G + kDecMaxChunks + pass - 1], 1u));
+    if (chunk >= p.chunks) chunk = -1;
+    sm.chunk[r.n % kDecRunSlots] = chunk;
+    mbar_arrive(&sm.run[r.n % kDecRunSlots]);
+    ++r.n;
+    return set_run(r, p, chunk);
+  };
+  auto follow_run = [&](Runs& r, const Pass& p) {
+    if (p.chunks == 0 || !dec_wait(&sm.run[r.n % kDecRunSlots], (r.n / kDecRunSlots) & 1, sm)) return false;
+    const int chunk = *reinterpret_cast<volatile int*>(&sm.chunk[r.n % kDecRunSlots]);
+    ++r.n;
+    return set_run(r, p, chunk);
+  };
   auto act_rows = [&](int ai) { return int(tb.act_off[ai + 1]) - int(tb.act_off[ai]); };
 
   // ---- loads (one thread)
@@ -679,68 +790,78 @@ __global__ void __launch_bounds__(kDecThreads, 1)
     const int n = min(S, p.hi - p.lo);
     for (; pre < n && load_weights(pass, c); ++pre) cursor_next<PASS>(c, p, nact);
   };
+  Runs lruns = {0, 0, 0, 0};
   auto produce = [&](auto pass, const Pass& p) {
     constexpr int PASS = decltype(pass)::value;
-    Cursor c = cursor_at<PASS>(p, nact, p.lo);
-    int u = p.lo;
-    for (int i = 0; i < pre; ++i, ++u) {
-      load_rows(pass, c, pre_at.st);
-      pre_at.next(S);
-      cursor_next<PASS>(c, p, nact);
-    }
-    for (; u < p.hi; ++u) {
-      const int st = lr.st;
-      if (!load_weights(pass, c)) return;
-      load_rows(pass, c, st);
-      cursor_next<PASS>(c, p, nact);
-    }
+    Runs& r = lruns;
+    first_run(r, p);
+    do {
+      Cursor c = cursor_at<PASS>(p, nact, r.lo);
+      for (int u = r.lo; u < r.hi; ++u) {
+        if (pre > 0) {
+          --pre;
+          load_rows(pass, c, pre_at.st);
+          pre_at.next(S);
+        } else {
+          const int st = lr.st;
+          if (!load_weights(pass, c)) return;
+          load_rows(pass, c, st);
+        }
+        cursor_next<PASS>(c, p, nact);
+      }
+    } while (take_run(r, p, PASS));
   };
 
   // ---- MMA (one thread)
   Ring mr = {0, 0};       // next stage to multiply
   Ring mseg = {0, 0};     // next accumulator (two)
+  Runs mruns = {0, 0, 0, 0};
   auto multiply = [&](auto pass, const Pass& p) {
     constexpr int PASS = decltype(pass)::value;
     // Pass 1: box g (64 features of each half) is [gate 64x64][up 64x64];
     // pass 2: four groups of 64 features in order.
     constexpr uint32_t half = PASS == 1 ? 8192 : 16384, group = PASS == 1 ? 16384 : 8192;
-    Cursor c = cursor_at<PASS>(p, nact, p.lo);
-    bool begin = true;
-    uint32_t idesc = 0;
-    for (int u = p.lo; u < p.hi; ++u) {
-      if (begin) {
-        if (!dec_wait(&sm.tempty[mseg.st], mseg.ph ^ 1, sm)) {
-          dec_fail(sm, a, 2);
+    Runs& r = mruns;
+    first_run(r, p);
+    do {
+      Cursor c = cursor_at<PASS>(p, nact, r.lo);
+      bool begin = true;
+      uint32_t idesc = 0;
+      for (int u = r.lo; u < r.hi; ++u) {
+        if (begin) {
+          if (!dec_wait(&sm.tempty[mseg.st], mseg.ph ^ 1, sm)) {
+            dec_fail(sm, a, 2);
+            return;
+          }
+          const int n = PASS == 1 ? a.NB : (act_rows(c.ai) + 15) / 16 * 16;
+          idesc = make_idesc_mn(/*bf16*/ 1, 128, uint32_t(n), /*A MN-major*/ 1, /*B K-major*/ 0);
+        }
+        if (!dec_wait(&sm.full[mr.st], mr.ph, sm)) {
+          dec_fail(sm, a, 3);
           return;
         }
-        const int n = PASS == 1 ? a.NB : (act_rows(c.ai) + 15) / 16 * 16;
-        idesc = make_idesc_mn(/*bf16*/ 1, 128, uint32_t(n), /*A MN-major*/ 1, /*B K-major*/ 0);
-      }
-      if (!dec_wait(&sm.full[mr.st], mr.ph, sm)) {
-        dec_fail(sm, a, 3);
-        return;
-      }
-      tc_fence_after();
-      const uint32_t aa = smem_u32(stage + uint32_t(mr.st) * a.stage_bytes), ba = aa + kDecABytes;
-      const uint32_t d = tmem + uint32_t(mseg.st) * 2 * uint32_t(a.NB);
+        tc_fence_after();
+        const uint32_t aa = smem_u32(stage + uint32_t(mr.st) * a.stage_bytes), ba = aa + kDecABytes;
+        const uint32_t d = tmem + uint32_t(mseg.st) * 2 * uint32_t(a.NB);
 #pragma unroll
-      for (int kk = 0; kk < 4; ++kk) {
-        const uint64_t bd = smem_desc_sw128(ba + kk * 32, 16, 1024);
+        for (int kk = 0; kk < 4; ++kk) {
+          const uint64_t bd = smem_desc_sw128(ba + kk * 32, 16, 1024);
 #pragma unroll
-        for (int h = 0; h < 2; ++h) {
-          const uint64_t ad = smem_desc_sw128(aa + h * half + kk * 2048, group, 1024);
-          tc_mma_f16(d + h * uint32_t(a.NB), ad, bd, idesc, (!begin || kk != 0) ? 1u : 0u);
+          for (int h = 0; h < 2; ++h) {
+            const uint64_t ad = smem_desc_sw128(aa + h * half + kk * 2048, group, 1024);
+            tc_mma_f16(d + h * uint32_t(a.NB), ad, bd, idesc, (!begin || kk != 0) ? 1u : 0u);
+          }
         }
+        tc_commit(&sm.empty[mr.st]);
+        mr.next(S);
+        begin = c.k + 1 == p.kb;
+        if (begin || u + 1 == r.hi) {
+          tc_commit(&sm.tfull[mseg.st]);
+          mseg.next(2);
+        }
+        cursor_next<PASS>(c, p, nact);
       }
-      tc_commit(&sm.empty[mr.st]);
-      mr.next(S);
-      begin = c.k + 1 == p.kb;
-      if (begin || u + 1 == p.hi) {
-        tc_commit(&sm.tfull[mseg.st]);
-        mseg.next(2);
-      }
-      cursor_next<PASS>(c, p, nact);
-    }
+    } while (follow_run(r, p));
   };
 
   // ---- epilogue (8 warps: lane quarter = 32 features of 128; two warps each)
@@ -748,10 +869,16 @@ __global__ void __launch_bounds__(kDecThreads, 1)
   const int quarter = warp & 3, sub = (warp - kDecEpi0) >> 2;
   const int etid = int(threadIdx.x) - kDecEpi0 * 32;
   const uint32_t tlane = tmem + (uint32_t(quarter * 32) << 16);
-  // Of a CTA's split tiles the one it starts goes to its slot 1, the one it
+  // Of a part's split tiles the one it starts goes to its slot 1, the one it
   // joins to slot 0.
   const size_t slot_floats = size_t(a.T) * 256;
-  auto slot = [&](int cta, int which) { return a.part + (size_t(cta) * 2 + which) * slot_floats; };
+  auto slot = [&](int part, int which) { return a.part + (size_t(part) * 2 + which) * slot_floats; };
+  Runs eruns = {0, 0, 0, 0};
+  // Every epilogue warp follows the same runs.
+  auto next_run = [&](const Pass& p) {
+    const bool more = follow_run(eruns, p);
+    return p.chunks != 0 && named_bar_and(kBarEpi, kDecEpiWarps * 32, more);
+  };
   auto seg_full = [&](int site) {
     if (named_bar_and(kBarEpi, kDecEpiWarps * 32, dec_wait(&sm.tfull[eseg.st], eseg.ph, sm))) return true;
     dec_fail(sm, a, site);
@@ -765,106 +892,112 @@ __global__ void __launch_bounds__(kDecThreads, 1)
   };
 
   auto epilogue1 = [&](const Pass& p) {
-    Cursor c = cursor_at<1>(p, nact, p.lo);
-    for (int u = p.lo; u < p.hi;) {
-      const int tile0 = u - c.k, seg_end = min(p.hi, tile0 + p.kb);
-      const bool whole = c.k == 0 && seg_end == tile0 + p.kb;
-      if (!seg_full(4)) return;
-      tc_fence_after();
-      const int n = act_rows(c.ai), r0 = tb.act_off[c.ai];
-      const int fl = quarter * 32 + lane;              // feature within the tile
-      const int f = c.ft * 128 + fl;
-      const uint32_t d = tlane + uint32_t(eseg.st) * 2 * uint32_t(a.NB);
-      float* mine = slot(blockIdx.x, c.k == 0 ? 1 : 0);
-      for (int j0 = sub; j0 < n; j0 += 8) {
-        uint32_t g[4], w[4];
+    first_run(eruns, p);
+    do {
+      Cursor c = cursor_at<1>(p, nact, eruns.lo);
+      for (int u = eruns.lo; u < eruns.hi;) {
+        const int tile0 = u - c.k, seg_end = min(eruns.hi, tile0 + p.kb);
+        const bool whole = c.k == 0 && seg_end == tile0 + p.kb;
+        if (!seg_full(4)) return;
+        tc_fence_after();
+        const int n = act_rows(c.ai), r0 = tb.act_off[c.ai];
+        const int fl = quarter * 32 + lane;              // feature within the tile
+        const int f = c.ft * 128 + fl;
+        const uint32_t d = tlane + uint32_t(eseg.st) * 2 * uint32_t(a.NB);
+        float* mine = slot(eruns.part, c.k == 0 ? 1 : 0);
+        for (int j0 = sub; j0 < n; j0 += 8) {
+          uint32_t g[4], w[4];
 #pragma unroll
-        for (int q = 0; q < 4; ++q)
-          if (j0 + 2 * q < n) {
-            const uint32_t t = tb.tok[r0 + j0 + 2 * q];
-            g[q] = tmem_ld_32x32b_x1(d + t);
-            w[q] = tmem_ld_32x32b_x1(d + uint32_t(a.NB) + t);
-          }
-        tmem_ld_wait();
+          for (int q = 0; q < 4; ++q)
+            if (j0 + 2 * q < n) {
+              const uint32_t t = tb.tok[r0 + j0 + 2 * q];
+              g[q] = tmem_ld_32x32b_x1(d + t);
+              w[q] = tmem_ld_32x32b_x1(d + uint32_t(a.NB) + t);
+            }
+          tmem_ld_wait();
 #pragma unroll
-        for (int q = 0; q < 4; ++q) {
-          const int j = j0 + 2 * q;
-          if (j >= n) break;
-          const float gv = __uint_as_float(g[q]), uv = __uint_as_float(w[q]);
-          if (whole) {
-            if (f < a.F) a.hs[size_t(r0 + j) * a.F + f] = __float2bfloat16_rn(gv / (1.f + expf(-gv)) * uv);
-          } else {
-            mine[j * 256 + fl] = gv;
-            mine[j * 256 + 128 + fl] = uv;
+          for (int q = 0; q < 4; ++q) {
+            const int j = j0 + 2 * q;
+            if (j >= n) break;
+            const float gv = __uint_as_float(g[q]), uv = __uint_as_float(w[q]);
+            if (whole) {
+              if (f < a.F) a.hs[size_t(r0 + j) * a.F + f] = __float2bfloat16_rn(gv / (1.f + expf(-gv)) * uv);
+            } else {
+              mine[j * 256 + fl] = gv;
+              mine[j * 256 + 128 + fl] = uv;
+            }
           }
         }
-      }
-      seg_done();
-      if (!whole) {
-        // The CTA whose ticket is the tile's last adds the parts up.
-        const int c0 = share_owner(p.units, p.g, tile0), c1 = share_owner(p.units, p.g, tile0 + p.kb - 1);
-        named_bar_sync(kBarEpi, kDecEpiWarps * 32);
-        if (etid == 0) sm.last = atom_add_acq_rel(&a.ctr[c0], 1u) == uint32_t(c1 - c0);
-        named_bar_sync(kBarEpi, kDecEpiWarps * 32);
-        if (sm.last && f < a.F) {
+        seg_done();
+        if (!whole) {
+          // The part whose ticket is the tile's last adds them all up.
+          const int c0 = p.part_of(tile0), c1 = p.part_of(tile0 + p.kb - 1);
+          named_bar_sync(kBarEpi, kDecEpiWarps * 32);
+          if (etid == 0) sm.last = atom_add_acq_rel(&a.ctr[c0], 1u) == uint32_t(c1 - c0);
+          named_bar_sync(kBarEpi, kDecEpiWarps * 32);
+          if (sm.last && f < a.F) {
 #pragma unroll 1
-          for (int j = sub; j < n; j += 2) {
-            const int at = j * 256 + fl;
-            const float gv = sum_parts<float>(c0, c1, [&](int q) { return slot(q, q == c0 ? 1 : 0) + at; });
-            const float uv = sum_parts<float>(c0, c1, [&](int q) { return slot(q, q == c0 ? 1 : 0) + at + 128; });
-            a.hs[size_t(r0 + j) * a.F + f] = __float2bfloat16_rn(gv / (1.f + expf(-gv)) * uv);
+            for (int j = sub; j < n; j += 2) {
+              const int at = j * 256 + fl;
+              const float gv = sum_parts<float>(c0, c1, [&](int q) { return slot(q, q == c0 ? 1 : 0) + at; });
+              const float uv = sum_parts<float>(c0, c1, [&](int q) { return slot(q, q == c0 ? 1 : 0) + at + 128; });
+              a.hs[size_t(r0 + j) * a.F + f] = __float2bfloat16_rn(gv / (1.f + expf(-gv)) * uv);
+            }
           }
         }
+        u = seg_end;
+        cursor_next_k<1>(c, p, nact);
       }
-      u = seg_end;
-      cursor_next_k<1>(c, p, nact);
-    }
+    } while (next_run(p));
   };
 
   auto epilogue2 = [&](const Pass& p) {
     const int fl = sub * 128 + quarter * 32 + lane;  // feature within the tile: this thread's alone
-    Cursor c = cursor_at<2>(p, nact, p.lo);
-    for (int u = p.lo; u < p.hi;) {
-      const int tile0 = u - c.ai * p.kb - c.k, tile_end = min(p.hi, tile0 + p.tile);
-      const bool starts = u == tile0, whole = starts && tile_end == tile0 + p.tile;
-      const int f = c.ft * 256 + fl;
+    first_run(eruns, p);
+    do {
+      Cursor c = cursor_at<2>(p, nact, eruns.lo);
+      for (int u = eruns.lo; u < eruns.hi;) {
+        const int tile0 = u - c.ai * p.kb - c.k, tile_end = min(eruns.hi, tile0 + p.tile);
+        const bool starts = u == tile0, whole = starts && tile_end == tile0 + p.tile;
+        const int f = c.ft * 256 + fl;
 #pragma unroll 4
-      for (int t = 0; t < a.T; ++t) acc[t * 256 + fl] = 0.f;
-      while (u < tile_end) {
-        if (!seg_full(5)) return;
-        tc_fence_after();
-        const int n = act_rows(c.ai), r0 = tb.act_off[c.ai];
-        const uint32_t d = tlane + (uint32_t(eseg.st) * 2 + uint32_t(sub)) * uint32_t(a.NB);
-        for (int j0 = 0; j0 < n; j0 += 4) {
-          uint32_t v[4];
+        for (int t = 0; t < a.T; ++t) acc[t * 256 + fl] = 0.f;
+        while (u < tile_end) {
+          if (!seg_full(5)) return;
+          tc_fence_after();
+          const int n = act_rows(c.ai), r0 = tb.act_off[c.ai];
+          const uint32_t d = tlane + (uint32_t(eseg.st) * 2 + uint32_t(sub)) * uint32_t(a.NB);
+          for (int j0 = 0; j0 < n; j0 += 4) {
+            uint32_t v[4];
 #pragma unroll
-          for (int q = 0; q < 4; ++q)
-            if (j0 + q < n) v[q] = tmem_ld_32x32b_x1(d + uint32_t(j0 + q));
-          tmem_ld_wait();
+            for (int q = 0; q < 4; ++q)
+              if (j0 + q < n) v[q] = tmem_ld_32x32b_x1(d + uint32_t(j0 + q));
+            tmem_ld_wait();
 #pragma unroll
-          for (int q = 0; q < 4; ++q) {
-            if (j0 + q >= n) break;
-            float* s = &acc[int(tb.tok[r0 + j0 + q]) * 256 + fl];
-            *s = fmaf(tb.val[r0 + j0 + q], __uint_as_float(v[q]), *s);
+            for (int q = 0; q < 4; ++q) {
+              if (j0 + q >= n) break;
+              float* s = &acc[int(tb.tok[r0 + j0 + q]) * 256 + fl];
+              *s = fmaf(tb.val[r0 + j0 + q], __uint_as_float(v[q]), *s);
+            }
           }
+          seg_done();
+          u = min(tile_end, u + p.kb - c.k);
+          cursor_next_k<2>(c, p, nact);
         }
-        seg_done();
-        u = min(tile_end, u + p.kb - c.k);
-        cursor_next_k<2>(c, p, nact);
-      }
-      if (whole) {
-        if (f < a.H)
+        if (whole) {
+          if (f < a.H)
 #pragma unroll 4
-          for (int t = 0; t < a.T; ++t) a.y[size_t(t) * a.H + f] = __float2bfloat16_rn(acc[t * 256 + fl]);
-      } else {
-        float* mine = slot(blockIdx.x, starts ? 1 : 0);
+            for (int t = 0; t < a.T; ++t) a.y[size_t(t) * a.H + f] = __float2bfloat16_rn(acc[t * 256 + fl]);
+        } else {
+          float* mine = slot(eruns.part, starts ? 1 : 0);
 #pragma unroll 4
-        for (int t = 0; t < a.T; ++t) mine[t * 256 + fl] = acc[t * 256 + fl];
+          for (int t = 0; t < a.T; ++t) mine[t * 256 + fl] = acc[t * 256 + fl];
+        }
       }
-    }
+    } while (next_run(p));
   };
 
-  // y of the tiles that several CTAs hold parts of: four features per four
+  // y of the tiles that lie in several parts: four features per four
   // threads, each of which adds a quarter of the parts.
   auto join2 = [&](const Pass& p) {
     const int per = a.T * 64, total = p.nt * per;
@@ -877,8 +1010,8 @@ __global__ void __launch_bounds__(kDecThreads, 1)
       const int u0 = tile * p.tile;
       int c0 = 0, c1 = 0;
       if (i < total) {
-        c0 = share_owner(p.units, p.g, u0);
-        c1 = share_owner(p.units, p.g, u0 + p.tile - 1);
+        c0 = p.part_of(u0);
+        c1 = p.part_of(u0 + p.tile - 1);
       }
       const bool split = c0 != c1;
       const int n = split ? c1 - c0 + 1 : 0;
@@ -977,8 +1110,9 @@ DecScratch dec_scratch(int T, int K, int F, int Er, int sms) {
   DecScratch s;
   s.hs = 0;
   s.part = up256(size_t(T) * K * F * 2);
-  s.ctr = s.part + up256(size_t(2) * sms * T * 256 * 4);
-  s.lpart = s.ctr + up256(size_t(sms) * 4);
+  const size_t parts = size_t(sms) + (T <= kDecChunkTokens ? kDecMaxChunks : 0);
+  s.ctr = s.part + up256(2 * parts * T * 256 * 4);
+  s.lpart = s.ctr + up256((size_t(sms) + kDecMaxChunks + 2) * 4);
   s.total = s.lpart + up256(size_t(sms) * T * Er * 4);
   return s;
 }
@@ -1056,7 +1190,7 @@ extern "C" int moe_decode_layer(const moe_decode_params* p, void* stream) {
   // Pass 2's sums [T][256] and, before them, the masks and offsets of the
   // routing tables and one token's logits.
   uint32_t scratch = uint32_t(T) * 1024;
-  const uint32_t build = uint32_t(E) * 10 + uint32_t(T) * K * 6, logits = uint32_t(Er) * 8;
+  const uint32_t build = uint32_t(E) * 10 + uint32_t(T) * K * 6, logits = uint32_t(Er) * 4 + uint32_t((Er + 31) / 32 * K) * 8;
   if (scratch < build) scratch = build;
   if (scratch < logits) scratch = logits;
   a.scratch_bytes = (scratch + 15) / 16 * 16;

@@ -300,7 +300,8 @@ __device__ __forceinline__ float silu_mul(float g, float u) { return __fdividef(
 
 template <bool GLU, bool SPLIT>
 __global__ void __launch_bounds__(kQThreads, 1)
-    w8a8_kernel(const __grid_constant__ CUtensorMap tm_w, const __grid_constant__ QRowMaps tm_x, const QArgs a) {
+    w8a8_kernel(const __grid_constant__ CUtensorMap tm_w, const __grid_constant__ QRowMaps tm_x,
+                const __grid_constant__ QArgs a) {
   extern __shared__ unsigned char q_dyn[];
   unsigned char* stage = reinterpret_cast<unsigned char*>((reinterpret_cast<uintptr_t>(q_dyn) + 1023) & ~uintptr_t(1023));
   float* xbuf = reinterpret_cast<float*>(stage + kQStages * kQStageBytes);

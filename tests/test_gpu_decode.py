@@ -94,6 +94,17 @@ def test_known_routing(T, H, E, K, F):
     assert torch.equal(y, decode.moe_layer(x, ids, vals, w13, w2))  # sums in a fixed order
 
 
+@pytest.mark.parametrize("T,H,E,K,F", [(5, 4096, 6, 2, 14344), (17, 4104, 7, 3, 12296), (33, 4096, 6, 2, 14344)])
+def test_long_lists(T, H, E, K, F):
+    """Enough weights that their last part is handed out in chunks (33 tokens:
+    the same size without)."""
+    x, ids, vals, w13, w2 = make(T, H, E, K, F, T, scale=0.02)
+    y = decode.moe_layer(x, ids, vals, w13, w2)
+    check(y, x, ids, vals, w13, w2)
+    for _ in range(3):  # whoever takes a chunk, the sums are the same
+        assert torch.equal(y, decode.moe_layer(x, ids, vals, w13, w2))
+
+
 @pytest.mark.parametrize("ids_dtype", [torch.int32, torch.int64])
 @pytest.mark.parametrize("vals_dtype", [torch.float32, torch.bfloat16])
 def test_types(ids_dtype, vals_dtype):
