@@ -31,6 +31,7 @@
 
 #include <algorithm>
 #include <atomic>
+#include <type_traits>
 
 #include "moe_ep.h"
 #include "moe_ep_internal.h"
@@ -49,7 +50,8 @@ constexpr int kQTileRows = 256;
 constexpr int kQEpiWarps = 8;                      // two per TMEM lane quarter
 constexpr int kQEpi0 = 2;
 constexpr int kQThreads = (kQEpi0 + kQEpiWarps) * 32;
-constexpr uint32_t kQXBytes = kQEpiWarps * (16 + 1) * 32 * 4;  // per warp: half a chunk, 32 row scales
+constexpr int kQXFloats = 32 * 20;                 // half a chunk of a warp, padded
+constexpr uint32_t kQXBytes = kQEpiWarps * (kQXFloats + 32) * 4;  // and 32 row scales
 constexpr int kQRowMaps = 4;                       // boxes of 16, 32, 64, 128 rows
 constexpr uint64_t kQBoundNs = 2000000000ull;      // bug guard on every pipeline wait
 constexpr int kQWaves = 4;                         // fewer tiles per pair: split over K
@@ -88,20 +90,22 @@ __device__ __forceinline__ int quant_one(float x, float s, float half, float inv
   return max(-127, min(127, q));
 }
 
-// Eight values.  x * inv is within 127 * 3 * 2^-24 < 3e-5 of the quotient, so
-// its rounding is the quotient's unless it lies nearer than that to a tie:
-// only then (about 1 value in 4000, more where the values are coarse) the
-// exact form runs.  t's low byte is the integer in two's complement.
+// Eight values.  x * inv is within 127 * 2^-24 < 1e-5 of the quotient, so its
+// rounding is the quotient's unless it lies nearer than that to a tie: only
+// then (bf16 rows: about 1 value in 1000, half the row's maximum, is one) the
+// exact form runs, behind a branch that the whole warp takes together so that
+// its instructions are not issued otherwise.  t's low byte is the integer in
+// two's complement.
 __device__ __forceinline__ uint2 quant8(const float (&x)[8], float s, float inv, bool exact) {
   uint32_t t[8];
-  float far = 0.f;
+  float far = exact ? 1.f : 0.f;
 #pragma unroll
   for (int i = 0; i < 8; ++i) {
     const float y = fmaf(x[i], inv, kMagic);
     far = fmaxf(far, fabsf(fmaf(x[i], inv, kMagic - y)));
     t[i] = __float_as_uint(y);
   }
-  if (exact || far > 0.49995f) {
+  if (__any_sync(__activemask(), far > 0.49999f)) {
     const float half = 0.5f * s;
 #pragma unroll
     for (int i = 0; i < 8; ++i) t[i] = uint32_t(quant_one(x[i], s, half, inv));
@@ -149,6 +153,44 @@ struct RowScale {
       for (int i = 0; i < 8; ++i) w[i] *= up;
     }
     return quant8(w, s, inv, tiny);
+  }
+};
+
+// Eight values as they lie in memory, and their largest magnitude's fp32 bits.
+template <typename In>
+struct Raw8 {
+  uint4 r[sizeof(In) / 2];
+  __device__ __forceinline__ void load(const In* p) {
+#pragma unroll
+    for (int i = 0; i < int(sizeof(In) / 2); ++i) r[i] = ld_nc_v4(reinterpret_cast<const uint4*>(p) + i);
+  }
+  __device__ __forceinline__ uint32_t top() const {
+    uint32_t t = 0;
+#pragma unroll
+    for (int i = 0; i < int(sizeof(In) / 2); ++i) {
+      const uint32_t w[4] = {r[i].x, r[i].y, r[i].z, r[i].w};
+#pragma unroll
+      for (int j = 0; j < 4; ++j) {
+        if constexpr (sizeof(In) == 2) t = max(t, max(w[j] & 0x7fff0000u, (w[j] << 16) & 0x7fffffffu));
+        else t = max(t, w[j] & 0x7fffffffu);
+      }
+    }
+    return t;
+  }
+  __device__ __forceinline__ void values(float (&v)[8]) const {
+#pragma unroll
+    for (int i = 0; i < int(sizeof(In) / 2); ++i) {
+      const uint32_t w[4] = {r[i].x, r[i].y, r[i].z, r[i].w};
+#pragma unroll
+      for (int j = 0; j < 4; ++j) {
+        if constexpr (sizeof(In) == 2) {
+          v[2 * j] = __uint_as_float(w[j] << 16);
+          v[2 * j + 1] = __uint_as_float(w[j] & 0xffff0000u);
+        } else {
+          v[4 * i + j] = __uint_as_float(w[j]);
+        }
+      }
+    }
   }
 };
 
@@ -279,12 +321,6 @@ struct QRing {
   }
 };
 
-__device__ __forceinline__ void q_store(const QArgs& a, int64_t row, int f, float v) {
-  const int64_t at = row * a.F + f;
-  if (a.out_f32) static_cast<float*>(a.out)[at] = v;
-  else static_cast<__nv_bfloat16*>(a.out)[at] = __float2bfloat16_rn(v);
-}
-
 __device__ __forceinline__ void q_store4(const QArgs& a, int64_t row, int f, float v0, float v1, float v2, float v3) {
   const int64_t at = row * a.F + f;
   if (a.out_f32) {
@@ -375,7 +411,7 @@ __global__ void __launch_bounds__(kQThreads, 1)
   tc_fence_before();
   cluster_sync();
   tc_fence_after();
-  const uint32_t tmem = sm.tmem_base;
+  const uint32_t tmem = __shfl_sync(0xffffffffu, sm.tmem_base, 0);
   const int tiles = s.tpre[a.E] * s.FT;
   // (The host launches the form with a grid barrier where the rows alone
   // leave it open; ragged experts may make enough tiles all the same.)
@@ -415,55 +451,58 @@ __global__ void __launch_bounds__(kQThreads, 1)
       }
     }
     sm.fills = fills;
-  } else if (warp == 1 && lane == 0 && leader) {
-    // ---- MMA.  The tensor pipe takes few instructions ahead, so the issuing
-    // thread's own work per stage must fit beside one MMA: descriptors are
-    // sums.
+  } else if (warp == 1 && leader) {
+    // ---- MMA.  The whole warp walks the list, so that what an instruction
+    // needs (descriptors, sums of constants) is known to be the same in all
+    // lanes and stays in uniform registers; one lane issues.
     QRing r = {0, 0}, acc = {0, 0};
     bool stop = false;
     uint32_t used = 0;  // stages multiplied
     const uint64_t desc0 = smem_desc_sw128(smem_u32(stage), 16, 1024);
+    const bool issuer = elect_one();
     for (QWalk w(s, split, tiles, pair, pairs); w.more() && !stop; w.next()) {
       const QTile t = q_tile(s, w.tile);
-      const uint32_t idesc = make_idesc_i8(256, uint32_t(t.n));
-      if (!mbar_try_wait_cluster(&sm.tempty[acc.st], acc.ph ^ 1) &&
-          !q_wait_slow(&sm.tempty[acc.st], acc.ph ^ 1, sm, true)) {
+      const uint32_t idesc = make_idesc_i8(256, uint32_t(__shfl_sync(0xffffffffu, t.n, 0)));
+      bool ok = mbar_try_wait_cluster(&sm.tempty[acc.st], acc.ph ^ 1) ||
+                q_wait_slow(&sm.tempty[acc.st], acc.ph ^ 1, sm, true);
+      if (!__all_sync(0xffffffffu, ok)) {
         q_fail(sm, a, 2);
         break;
       }
       tc_fence_after();
       const uint32_t d = tmem + uint32_t(acc.st) * 256;
-      uint32_t more = 0;  // adds to the sums from the second MMA on
-      for (int k = w.k0; k < w.k1; ++k) {
-        if (!q_wait(&sm.full[r.st], r.ph, sm)) {
+      const int n = __shfl_sync(0xffffffffu, w.k1 - w.k0, 0);
+      for (int k = 0; k < n; ++k) {
+        if (!__all_sync(0xffffffffu, q_wait(&sm.full[r.st], r.ph, sm))) {
           q_fail(sm, a, 3);
           stop = true;
           break;
         }
-        tc_fence_after();
         const uint64_t da = desc0 + uint32_t(r.st) * (kQStageBytes >> 4), db = da + (kQABytes >> 4);
+        if (issuer) {
 #pragma unroll
-        for (int kk = 0; kk < kQKb / 32; ++kk) {
-          tc_mma_i8_pair(d, da + kk * 2, db + kk * 2, idesc, more);
-          more = 1;
+          for (int kk = 0; kk < kQKb / 32; ++kk)
+            tc_mma_i8_pair(d, da + kk * 2, db + kk * 2, idesc, (k != 0 || kk != 0) ? 1u : 0u);
+          tc_commit_pair_mc(&sm.empty[r.st], 0x3);
         }
-        tc_commit_pair_mc(&sm.empty[r.st], 0x3);
+        __syncwarp();
         ++used;
         r.next(kQStages);
       }
       if (stop) break;
-      tc_commit_pair_mc(&sm.tfull[acc.st], 0x3);
+      if (issuer) tc_commit_pair_mc(&sm.tfull[acc.st], 0x3);
+      __syncwarp();
       acc.next(2);
     }
-    sm.used = used;
+    if (issuer) sm.used = used;
   } else if (warp >= kQEpi0) {
     // ---- epilogue: chunks of 32 rows, even ones by the first four warps
     QRing acc = {0, 0};
     const int quarter = warp & 3, sub = (warp - kQEpi0) >> 2;
     const uint32_t tempty0 = mapa_shared(smem_u32(&sm.tempty[0]), 0);
-    float* mine = xbuf + (sub * 4 + quarter) * 16 * 32;
-    const float* theirs = xbuf + (sub * 4 + (quarter ^ 2)) * 16 * 32;
-    float* xrow = xbuf + kQEpiWarps * 16 * 32 + (warp - kQEpi0) * 32;
+    float* mine = xbuf + (sub * 4 + quarter) * kQXFloats;
+    const float* theirs = xbuf + (sub * 4 + (quarter ^ 2)) * kQXFloats;
+    float* xrow = xbuf + kQEpiWarps * kQXFloats + (warp - kQEpi0) * 32;
     const int bar_id = 1 + sub * 2 + (quarter & 1);  // this warp and its gate or up partner
     for (QWalk w(s, split, tiles, pair, pairs); w.more(); w.next()) {
       const QTile t = q_tile(s, w.tile);
@@ -513,22 +552,47 @@ __global__ void __launch_bounds__(kQThreads, 1)
         if ((jc + 2) * 32 < t.rows) tmem_ld_32x32b_x32(d + uint32_t((jc + 2) * 32), v);
         if constexpr (GLU) {
           // The gate warp finishes rows 0..15 of the chunk, the up warp rows
-          // 16..31: each hands the other half over.
-          named_bar_sync(bar_id, 64);  // the last chunk's have been read
+          // 16..31: each hands the other half over, 16 values a lane at a
+          // stride of 20 (no bank conflicts in 16-byte accesses).
+          auto finish = [&](auto is_up) {
+            constexpr bool kUp = decltype(is_up)::value;
+            constexpr int kMine = kUp ? 16 : 0, kTheirs = 16 - kMine;
+            named_bar_sync(bar_id, 64);  // the last chunk's have been read
 #pragma unroll
-          for (int i = 0; i < 16; ++i) mine[i * 32 + lane] = up ? z[i] : z[16 + i];
-          named_bar_sync(bar_id, 64);
-          const int first = up ? 16 : 0;
+            for (int i = 0; i < 16; i += 4)
+              *reinterpret_cast<float4*>(mine + lane * 20 + i) =
+                  make_float4(z[kTheirs + i], z[kTheirs + i + 1], z[kTheirs + i + 2], z[kTheirs + i + 3]);
+            named_bar_sync(bar_id, 64);
 #pragma unroll
-          for (int i = 0; i < 16; ++i) {
-            const float o = theirs[i * 32 + lane];
-            const float h = up ? silu_mul(o, z[16 + i]) : silu_mul(z[i], o);
-            if (first + i < left && f < a.F) q_store(a, row + first + i, f, h);
-          }
+            for (int i = 0; i < 16; i += 4) {
+              const float4 o = *reinterpret_cast<const float4*>(theirs + lane * 20 + i);
+              const float ov[4] = {o.x, o.y, o.z, o.w};
+#pragma unroll
+              for (int j = 0; j < 4; ++j)
+                z[kMine + i + j] = kUp ? silu_mul(ov[j], z[kMine + i + j]) : silu_mul(z[kMine + i + j], ov[j]);
+            }
+            const int64_t at = (row + kMine) * a.F + f;
+            const int n = f < a.F ? left - kMine : 0;
+            if (a.out_f32) {
+              float* o = static_cast<float*>(a.out) + at;
+#pragma unroll
+              for (int i = 0; i < 16; ++i, o += a.F)
+                if (i < n) *o = z[kMine + i];
+            } else {
+              __nv_bfloat16* o = static_cast<__nv_bfloat16*>(a.out) + at;
+#pragma unroll
+              for (int i = 0; i < 16; ++i, o += a.F)
+                if (i < n) *o = __float2bfloat16_rn(z[kMine + i]);
+            }
+          };
+          if (up) finish(std::true_type{});
+          else finish(std::false_type{});
         } else if (a.out_f32) {
+          float* o = static_cast<float*>(a.out) + row * a.F + f;
+          const int n = f < a.F ? left : 0;
 #pragma unroll
-          for (int i = 0; i < 32; ++i)
-            if (i < left && f < a.F) static_cast<float*>(a.out)[(row + i) * a.F + f] = z[i];
+          for (int i = 0; i < 32; ++i, o += a.F)
+            if (i < n) *o = z[i];
         } else {
           // bf16, two rows to a word, through shared memory: a lane then
           // holds eight channels of two rows, 16 bytes each.
@@ -638,7 +702,7 @@ __global__ void __launch_bounds__(kQThreads, 1)
       }
     }
   }
-  if (leader && warp == 1 && lane == 0) {
+  if (leader && warp == 1 && elect_one()) {  // (the lane that issued the MMAs)
     tc_commit_pair(&sm.drain);
     const uint64_t until = globaltimer_ns() + kQBoundNs;
     while (!mbar_try_wait(&sm.drain, 0) && globaltimer_ns() < until) {
@@ -876,19 +940,20 @@ __global__ void __launch_bounds__(kQuantThreads)
   const int per = kQuantThreads / tpr, lr = threadIdx.x / tpr, c = threadIdx.x % tpr;
   const int64_t live = live_rows ? min(int64_t(max(*live_rows, 0)), rows) : rows;
   const int groups = K / 8;
+#pragma unroll 1
   for (int64_t base = int64_t(blockIdx.x) * per; base < live; base += int64_t(gridDim.x) * per) {
     const int64_t r = base + lr;
     const bool on = r < live;
     const In* src = x + (on ? (perm ? int64_t(perm[r]) : r) : 0) * K;
-    float v[VPT][8];
+    Raw8<In> v[VPT];
     uint32_t top = 0;
     if (on) {
 #pragma unroll
       for (int j = 0; j < VPT; ++j)
-        if (c + j * tpr < groups) load8(src + (c + j * tpr) * 8, v[j]);
+        if (c + j * tpr < groups) v[j].load(src + (c + j * tpr) * 8);
 #pragma unroll
       for (int j = 0; j < VPT; ++j)
-        if (c + j * tpr < groups) top = max(top, top8(v[j]));
+        if (c + j * tpr < groups) top = max(top, v[j].top());
       for (int g = c + VPT * tpr; g < groups; g += tpr) {
         float w[8];
         load8(src + g * 8, w);
@@ -910,7 +975,11 @@ __global__ void __launch_bounds__(kQuantThreads)
     auto put = [&](int g, float (&w)[8]) { *reinterpret_cast<uint2*>(dst + g * 8) = rs.round8(w); };
 #pragma unroll
     for (int j = 0; j < VPT; ++j)
-      if (c + j * tpr < groups) put(c + j * tpr, v[j]);
+      if (c + j * tpr < groups) {
+        float w[8];
+        v[j].values(w);
+        put(c + j * tpr, w);
+      }
     for (int g = c + VPT * tpr; g < groups; g += tpr) {
       float w[8];
       load8(src + g * 8, w);
