@@ -31,8 +31,9 @@
  *                               router included (utils.py:17-25, 28-75,
  *                               baseline.py:18-50 in one kernel)
  *   moe_quant_rows,             the expert products in 8-bit integers, beside
- *   moe_w8a8_gemm,              baseline.py:50's bf16 ones, and the top-k sum
- *   moe_weighted_sum            of their rows
+ *   moe_w8a8_gemm,              baseline.py:50's bf16 ones, the layer of a few
+ *   moe_w8a8_layer,             tokens in them, and the top-k sum of their rows
+ *   moe_weighted_sum
  *   moe_pack_compact,           the general (unbalanced) all-to-all that
  *   moe_ep_run_compact          alltoall_persistent_gemm.py:221-222 and
  *                               baseline.py:15-16 leave as stubs: unpadded
@@ -465,6 +466,39 @@ typedef struct moe_w8a8_params {
 int moe_w8a8_scratch_bytes(int64_t rows, int32_t K, int32_t N, int32_t experts, int32_t swiglu, int32_t with_x,
                            int32_t device, size_t* out);
 int moe_w8a8_gemm(const moe_w8a8_params* params, void* stream);
+
+/* The gated layer of a few tokens in 8 bits, two launches (two more for large
+ * H or ffn):
+ *   y[t, :] = sum over k of top_vals[t, k] * down_e(silu(gate_e(x_t)) * up_e(x_t)),
+ * e = top_idxs[t, k] - first_expert, with the products, quantisations and
+ * rules on ids of moe_w8a8_gemm, moe_quant_rows and moe_decode_layer; the sum
+ * is taken in fp32 in the order of the experts.  Requires T * K <=
+ * MOE_W8A8_LAYER_MAX_ROWS, hidden and ffn multiples of 16, T * hidden and
+ * T * K * ffn <= 98304, experts <= 1024; x, w13, w2 and scratch 16-byte
+ * aligned.  scratch: moe_w8a8_layer_scratch_bytes, as above. */
+#define MOE_W8A8_LAYER_MAX_ROWS 16
+typedef struct moe_w8a8_layer_params {
+  int64_t T;
+  int32_t hidden, ffn;
+  int32_t experts;         /* experts held here                              */
+  int32_t K;
+  int32_t first_expert;
+  int32_t ids_are_int64, vals_are_bf16;
+  int32_t reserved;
+  const void* x;           /* [T, hidden] bf16                               */
+  const void* w13;         /* [experts, 2*ffn, hidden] int8: gate, then up   */
+  const float* w13_scale;  /* [experts, 2*ffn]                               */
+  const void* w2;          /* [experts, hidden, ffn] int8                    */
+  const float* w2_scale;   /* [experts, hidden]                              */
+  const void* top_idxs;    /* [T, K]                                         */
+  const void* top_vals;    /* [T, K] fp32 or bf16                            */
+  void* y;                 /* [T, hidden] bf16                               */
+  void* scratch;
+  size_t scratch_bytes;
+} moe_w8a8_layer_params;
+
+int moe_w8a8_layer_scratch_bytes(int64_t T, int32_t hidden, int32_t ffn, int32_t experts, int32_t K, size_t* out);
+int moe_w8a8_layer(const moe_w8a8_layer_params* params, void* stream);
 
 /* y[t, :] = sum over k of top_vals[t, k] * rows[offsets[e] + slots[t, k], :],
  * e = top_idxs[t, k] - first_expert, in fp32 in the order of k, bf16 out; ids

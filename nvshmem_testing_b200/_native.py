@@ -27,7 +27,8 @@ EXPORTED = ["moe_ep_abi_version", "moe_ep_status_string", "moe_ep_num_sms", "moe
             "moe_ep_read_status", "moe_ep_run_noalloc", "moe_route_slots", "moe_ep_workspace_layout_ret",
             "moe_ep_run_combine", "moe_pack_compact", "moe_ep_run_compact", "moe_router", "moe_swiglu",
             "moe_ep_run_compact_swiglu", "moe_publish_i32", "moe_decode_scratch_bytes", "moe_decode_layer",
-            "moe_quant_rows", "moe_w8a8_scratch_bytes", "moe_w8a8_gemm", "moe_weighted_sum"]
+            "moe_quant_rows", "moe_w8a8_scratch_bytes", "moe_w8a8_gemm", "moe_weighted_sum",
+            "moe_w8a8_layer_scratch_bytes", "moe_w8a8_layer"]
 
 
 class MoeEpError(RuntimeError):
@@ -85,6 +86,18 @@ class W8A8Params(ctypes.Structure):
                 ("perm", ctypes.c_void_p), ("live_rows", ctypes.c_void_p)]
 
 
+class W8A8LayerParams(ctypes.Structure):
+    _fields_ = [("T", ctypes.c_int64), ("hidden", ctypes.c_int32), ("ffn", ctypes.c_int32),
+                ("experts", ctypes.c_int32), ("K", ctypes.c_int32), ("first_expert", ctypes.c_int32),
+                ("ids_are_int64", ctypes.c_int32), ("vals_are_bf16", ctypes.c_int32), ("reserved", ctypes.c_int32),
+                ("x", ctypes.c_void_p), ("w13", ctypes.c_void_p), ("w13_scale", ctypes.c_void_p),
+                ("w2", ctypes.c_void_p), ("w2_scale", ctypes.c_void_p), ("top_idxs", ctypes.c_void_p),
+                ("top_vals", ctypes.c_void_p), ("y", ctypes.c_void_p), ("scratch", ctypes.c_void_p),
+                ("scratch_bytes", ctypes.c_size_t)]
+
+
+W8A8_LAYER_MAX_ROWS = 16  # tokens times ids per token
+W8A8_LAYER_MAX_VALUES = 98304
 DECODE_MAX_TOKENS = 64
 DECODE_MAX_ROWS = 1024  # tokens times ids per token
 TRACE_WORDS = 24
@@ -140,6 +153,8 @@ def lib() -> ctypes.CDLL:
     L.moe_w8a8_gemm.argtypes = [P(W8A8Params), c_vp]
     L.moe_weighted_sum.argtypes = [c_vp, c_i32, c_vp, c_i32, c_i32, c_vp, c_i32, c_vp, c_vp, c_i64, c_i32, c_i32, c_i32,
                                    c_vp, c_vp]
+    L.moe_w8a8_layer_scratch_bytes.argtypes = [c_i64] + [c_i32] * 4 + [P(c_sz)]
+    L.moe_w8a8_layer.argtypes = [P(W8A8LayerParams), c_vp]
     L.moe_decode_scratch_bytes.argtypes = [c_i64] + [ctypes.c_int32] * 6 + [P(c_sz)]
     L.moe_decode_layer.argtypes = [P(DecodeParams), c_vp]
     for name in EXPORTED:

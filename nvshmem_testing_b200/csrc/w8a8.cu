@@ -92,10 +92,8 @@ __device__ __forceinline__ int quant_one(float x, float s, float half, float inv
 
 // Eight values.  x * inv is within 127 * 2^-24 < 1e-5 of the quotient, so its
 // rounding is the quotient's unless it lies nearer than that to a tie: only
-// then (bf16 rows: about 1 value in 1000, half the row's maximum, is one) the
-// exact form runs, behind a branch that the whole warp takes together so that
-// its instructions are not issued otherwise.  t's low byte is the integer in
-// two's complement.
+// then (bf16 rows: about 1 value in 500, half the row's maximum among them)
+// the exact form runs.  t's low byte is the integer in two's complement.
 __device__ __forceinline__ uint2 quant8(const float (&x)[8], float s, float inv, bool exact) {
   uint32_t t[8];
   float far = exact ? 1.f : 0.f;
@@ -105,7 +103,7 @@ __device__ __forceinline__ uint2 quant8(const float (&x)[8], float s, float inv,
     far = fmaxf(far, fabsf(fmaf(x[i], inv, kMagic - y)));
     t[i] = __float_as_uint(y);
   }
-  if (__any_sync(__activemask(), far > 0.49999f)) {
+  if (far > 0.49999f) {
     const float half = 0.5f * s;
 #pragma unroll
     for (int i = 0; i < 8; ++i) t[i] = uint32_t(quant_one(x[i], s, half, inv));
@@ -720,24 +718,31 @@ __global__ void __launch_bounds__(kQThreads, 1)
 
 // ---------------------------------------------------------------- a handful of rows
 // Up to kRwMaxRows rows (a decode step's): no tile to fill, so a warp takes a
-// channel (its gate and its up channel with SwiGLU) of up to four rows,
-// streams the channel's K contiguous bytes once, 16 per lane, against the
-// rows in shared memory with 4-way 8-bit dot products, and adds its lanes up.
-// No partial sums, barriers or tensor maps: the launch and one pass over the
-// weights.  Rows given in bf16 or fp32 are quantised by every CTA for itself
-// (four rows at most) behind the first loads of weights.
+// channel (its gate and its up channel with SwiGLU) of up to four rows of an
+// expert, streams the channel's K contiguous bytes once, 16 per lane, against
+// the rows in shared memory with 4-way 8-bit dot products, and adds its lanes
+// up.  No partial sums, barriers or tensor maps: the launch and one pass over
+// the weights (one row, 7168 x 4096: 16.4 us with the tiles above and a
+// launch for the quantisation, 7.4 us).  Rows given in bf16 or fp32 are
+// quantised by every CTA for itself, behind the first loads of weights, as
+// far as that takes less than a launch (kRwMaxFresh values).
+//
+// The gated layer of a few tokens is two such launches: gate and up channels
+// of every (token, expert) row, then (SUM) the down channels, a warp taking
+// one of all experts and adding their rows, weighted, to y.
 constexpr int kRwThreads = 512;
 constexpr int kRwMaxRows = 16;
-constexpr int kRwMaxFresh = 4;   // rows quantised here
-constexpr int kRwRows = 4;       // rows of a channel's pass
+constexpr int kRwMaxFresh = 32768;          // values quantised by every CTA
+constexpr int kRwRows = 4;                  // rows of a channel's pass
 constexpr uint32_t kRwMaxSmem = 96 * 1024;  // of rows: two CTAs per SM
 
 struct RwArgs {
-  int E, K, N, F, rows;
-  const int32_t* counts;
+  int E, K, N, F;
+  int rows;               // rows in memory
+  const int32_t* counts;  // [E] rows per expert, in order (null: all rows one expert's), unless ids
   const int8_t* xq;
   const float* xs;
-  const void* x;  // or null: xq and xs
+  const void* x;          // or null: xq and xs
   int x_f32;
   const int32_t* perm;
   const int32_t* live;
@@ -745,13 +750,21 @@ struct RwArgs {
   const float* ws;
   void* out;
   int out_f32;
+  // A layer of T tokens (ids != null).
+  const void* ids;
+  int ids64, first, T, topk;
+  const void* vals;       // SUM
+  int vals_bf16;
 };
 
 struct RwSmem {
   float scale[kRwMaxRows];
   uint32_t top[kRwThreads / 32];
+  int src[kRwMaxRows];     // a row's place in memory
+  int tok[kRwMaxRows];
+  float val[kRwMaxRows];
   int e[kRwMaxRows], r0[kRwMaxRows], n[kRwMaxRows];  // an expert's rows, four at a time
-  int chunks;
+  int rows, chunks;
 };
 
 __device__ __forceinline__ int dot16(uint4 a, uint4 b, int c) {
@@ -759,12 +772,6 @@ __device__ __forceinline__ int dot16(uint4 a, uint4 b, int c) {
   c = __dp4a(int(a.y), int(b.y), c);
   c = __dp4a(int(a.z), int(b.z), c);
   return __dp4a(int(a.w), int(b.w), c);
-}
-
-__device__ __forceinline__ void rw_store(const RwArgs& a, int row, int f, float v) {
-  const int64_t at = int64_t(row) * a.F + f;
-  if (a.out_f32) static_cast<float*>(a.out)[at] = v;
-  else static_cast<__nv_bfloat16*>(a.out)[at] = __float2bfloat16_rn(v);
 }
 
 // The loads of one round: kRwLoads vectors of 16 bytes per lane in all.
@@ -782,22 +789,31 @@ __device__ __forceinline__ void rw_load(const uint4* w, const uint4* w2, int v0,
   }
 }
 
+// One channel's sums over K for the rows of chunk c.  buf holds the first
+// round's loads and leaves with those of the next channel (null: none).
 template <bool GLU, int NR>
-__device__ __forceinline__ void rw_channel(const RwArgs& a, const RwSmem& sm, const uint4* rows, int c, int f,
-                                           const uint4* w, const uint4* w2, uint4 (&buf)[kRwLoads]) {
+__device__ __forceinline__ void rw_channel(const RwSmem& sm, const uint4* rows, int V, int c, const uint4* w,
+                                           const uint4* w2, const uint4* nw, const uint4* nw2,
+                                           uint4 (&buf)[kRwLoads], int (&s)[NR], int (&s2)[NR]) {
   constexpr int U = GLU ? kRwLoads / 2 : kRwLoads;
-  const int V = a.K / 16, lane = threadIdx.x & 31, r0 = sm.r0[c], last = sm.n[c] - 1;  // NR > n: the last row again
-  int s[NR] = {}, s2[NR] = {};
+  const int lane = threadIdx.x & 31, r0 = sm.r0[c], last = sm.n[c] - 1;  // NR > n: the last row again
+  const uint4* row[NR];
+#pragma unroll
+  for (int r = 0; r < NR; ++r) {
+    row[r] = rows + sm.src[r0 + min(r, last)] * V;
+    s[r] = s2[r] = 0;
+  }
 #pragma unroll 1
   for (int v0 = 0; v0 < V; v0 += 32 * U) {
     uint4 next[kRwLoads];
-    rw_load<GLU>(w, w2, v0 + 32 * U, V, lane, next);
+    const bool end = v0 + 32 * U >= V;
+    rw_load<GLU>(end ? nw : w, end ? nw2 : w2, end ? 0 : v0 + 32 * U, end && nw == nullptr ? 0 : V, lane, next);
 #pragma unroll
     for (int j = 0; j < U; ++j) {
       const int v = min(v0 + j * 32 + lane, V - 1);  // (past the end the weights are zeros)
 #pragma unroll
       for (int r = 0; r < NR; ++r) {
-        const uint4 x = rows[(r0 + min(r, last)) * V + v];
+        const uint4 x = row[r][v];
         s[r] = dot16(buf[j], x, s[r]);
         if constexpr (GLU) s2[r] = dot16(buf[U + j], x, s2[r]);
       }
@@ -805,34 +821,28 @@ __device__ __forceinline__ void rw_channel(const RwArgs& a, const RwSmem& sm, co
 #pragma unroll
     for (int j = 0; j < kRwLoads; ++j) buf[j] = next[j];
   }
-  const float* sw = a.ws + int64_t(sm.e[c]) * a.N + f;
-  const float g = sw[0], u = GLU ? sw[a.F] : 0.f;
 #pragma unroll
   for (int r = 0; r < NR; ++r) {
-    const int t = __reduce_add_sync(0xffffffffu, s[r]);
-    const int t2 = GLU ? __reduce_add_sync(0xffffffffu, s2[r]) : 0;
-    if (lane == r && r <= last) {
-      const float x = sm.scale[r0 + r];
-      const float z = float(t) * x * g;
-      rw_store(a, r0 + r, f, GLU ? silu_mul(z, float(t2) * x * u) : z);
-    }
+    s[r] = __reduce_add_sync(0xffffffffu, s[r]);
+    if constexpr (GLU) s2[r] = __reduce_add_sync(0xffffffffu, s2[r]);
   }
 }
 
 template <typename In>
-__device__ __forceinline__ void rw_quantize(const RwArgs& a, RwSmem& sm, unsigned char* rows) {
-  // All, half or a quarter of the warps for each of up to four rows.
-  const int per = a.rows == 1 ? kRwThreads : a.rows == 2 ? kRwThreads / 2 : kRwThreads / 4;
+__device__ __forceinline__ void rw_quantize(const RwArgs& a, RwSmem& sm, unsigned char* rows, int count) {
+  // The warps in equal groups, one for each row.
+  int per = kRwThreads;
+  while (per > 32 && per * count > kRwThreads) per /= 2;
   const int r = int(threadIdx.x) / per, c = int(threadIdx.x) % per, groups = a.K / 8;
-  const int live = a.live ? min(max(*a.live, 0), a.rows) : a.rows;
+  const int live = a.live ? min(max(*a.live, 0), count) : count;
   const bool on = r < live;
   const In* src = static_cast<const In*>(a.x) + int64_t(on ? (a.perm ? a.perm[r] : r) : 0) * a.K;
   uint32_t top = 0;
 #pragma unroll 4
   for (int g = c; g < groups && on; g += per) {
-    float v[8];
-    load8(src + g * 8, v);
-    top = max(top, top8(v));
+    Raw8<In> v;
+    v.load(src + g * 8);
+    top = max(top, v.top());
   }
   top = __reduce_max_sync(0xffffffffu, top);
   if ((threadIdx.x & 31) == 0) sm.top[threadIdx.x >> 5] = top;
@@ -849,63 +859,126 @@ __device__ __forceinline__ void rw_quantize(const RwArgs& a, RwSmem& sm, unsigne
   }
 }
 
-template <bool GLU>
-__global__ void __launch_bounds__(kRwThreads, 2) w8a8_rows_kernel(const RwArgs a) {
+// The table of rows and chunks, by one warp, from counts per expert.
+__device__ __forceinline__ void rw_table_counts(const RwArgs& a, RwSmem& sm, int lane) {
+  // Experts with rows, in order; counts that would pass the last row are cut.
+  int row = 0, chunks = 0;
+#pragma unroll 1
+  for (int e0 = 0; e0 < a.E && row < a.rows; e0 += 32) {
+    const int e = e0 + lane;
+    int c = e < a.E ? (a.counts ? min(max(a.counts[e], 0), a.rows) : a.rows) : 0;
+    int pre = c;
+#pragma unroll
+    for (int o = 1; o < 32; o <<= 1) {
+      const int v = __shfl_up_sync(0xffffffffu, pre, o);
+      if (lane >= o) pre += v;
+    }
+    const int begin = min(row + pre - c, a.rows);
+    c = min(row + pre, a.rows) - begin;
+    const int mine = (c + kRwRows - 1) / kRwRows;
+    int at = mine;
+#pragma unroll
+    for (int o = 1; o < 32; o <<= 1) {
+      const int v = __shfl_up_sync(0xffffffffu, at, o);
+      if (lane >= o) at += v;
+    }
+    for (int i = 0; i < mine; ++i) {
+      const int k = chunks + at - mine + i;
+      sm.e[k] = e;
+      sm.r0[k] = begin + i * kRwRows;
+      sm.n[k] = min(kRwRows, c - i * kRwRows);
+    }
+    row = min(row + __shfl_sync(0xffffffffu, pre, 31), a.rows);
+    chunks += __shfl_sync(0xffffffffu, at, 31);
+  }
+  if (lane < a.rows) sm.src[lane] = lane;
+  if (lane == 0) {
+    sm.chunks = chunks;
+    sm.rows = a.rows;
+  }
+}
+
+// The same from a layer's ids, sorted by expert, then token (T * topk <= 16
+// rows; an id repeated within a token's row counts once).
+template <bool SUM>
+__device__ __forceinline__ void rw_table_ids(const RwArgs& a, RwSmem& sm, int lane) {
+  const int n = a.T * a.topk, t = lane / a.topk;
+  long long e = -1;
+  if (lane < n)
+    e = (a.ids64 ? static_cast<const long long*>(a.ids)[lane] : static_cast<const int32_t*>(a.ids)[lane]) -
+        (long long)a.first;
+  const uint32_t none = 0xffffffffu;
+  const uint32_t key = lane < n && e >= 0 && e < a.E ? uint32_t(e) * 32 + uint32_t(t) : none;
+  const uint32_t same = __match_any_sync(0xffffffffu, key);
+  const bool on = key != none && (same & ((1u << lane) - 1)) == 0;
+  const uint32_t expert = on ? key >> 5 : none;
+  const uint32_t peers = __match_any_sync(0xffffffffu, expert);
+  // A row's rank among its expert's is that of its lane (tokens ascend with
+  // the lane); every fourth opens a chunk.
+  const int rank = __popc(peers & ((1u << lane) - 1));
+  const bool head = on && rank % kRwRows == 0;
+  const uint32_t hkey = head ? (expert * 32 + uint32_t(lane)) : none;
+  int row = 0, at = 0;
+#pragma unroll 4
+  for (int j = 0; j < kRwMaxRows; ++j) {
+    const uint32_t kj = __shfl_sync(0xffffffffu, on ? key : none, j);
+    const uint32_t hj = __shfl_sync(0xffffffffu, hkey, j);
+    row += on && kj < key;
+    at += head && hj < hkey;
+  }
+  if (on) {
+    sm.src[row] = SUM ? row : t;
+    sm.tok[row] = t;
+    if constexpr (SUM)
+      sm.val[row] = a.vals_bf16 ? __bfloat162float(static_cast<const __nv_bfloat16*>(a.vals)[lane])
+                                : static_cast<const float*>(a.vals)[lane];
+  }
+  if (head) {
+    sm.e[at] = int(expert);
+    sm.r0[at] = row;
+    sm.n[at] = min(kRwRows, __popc(peers) - rank);
+  }
+  const uint32_t ons = __ballot_sync(0xffffffffu, on), heads = __ballot_sync(0xffffffffu, head);
+  if (lane == 0) {
+    sm.rows = SUM ? __popc(ons) : a.T;
+    sm.chunks = __popc(heads);
+  }
+}
+
+template <bool GLU, bool SUM>
+__global__ void __launch_bounds__(kRwThreads, 2) w8a8_rows_kernel(const __grid_constant__ RwArgs a) {
   extern __shared__ __align__(16) unsigned char rw_rows[];
   __shared__ RwSmem sm;
   const int warp = int(threadIdx.x) >> 5, lane = threadIdx.x & 31;
   if (warp == 0) {
-    // Experts with rows, in order; counts that would pass the last row are cut.
-    int row = 0, chunks = 0;
-#pragma unroll 1
-    for (int e0 = 0; e0 < a.E && row < a.rows; e0 += 32) {
-      const int e = e0 + lane;
-      int c = e < a.E ? (a.counts ? min(max(a.counts[e], 0), a.rows) : a.rows) : 0;
-      int pre = c;
-#pragma unroll
-      for (int o = 1; o < 32; o <<= 1) {
-        const int v = __shfl_up_sync(0xffffffffu, pre, o);
-        if (lane >= o) pre += v;
-      }
-      const int begin = min(row + pre - c, a.rows);
-      c = min(row + pre, a.rows) - begin;
-      const int mine = (c + kRwRows - 1) / kRwRows;
-      int at = mine;
-#pragma unroll
-      for (int o = 1; o < 32; o <<= 1) {
-        const int v = __shfl_up_sync(0xffffffffu, at, o);
-        if (lane >= o) at += v;
-      }
-      for (int i = 0; i < mine; ++i) {
-        const int k = chunks + at - mine + i;
-        sm.e[k] = e;
-        sm.r0[k] = begin + i * kRwRows;
-        sm.n[k] = min(kRwRows, c - i * kRwRows);
-      }
-      row = min(row + __shfl_sync(0xffffffffu, pre, 31), a.rows);
-      chunks += __shfl_sync(0xffffffffu, at, 31);
-    }
-    if (lane == 0) sm.chunks = chunks;
+    if (a.ids != nullptr) rw_table_ids<SUM>(a, sm, lane);
+    else rw_table_counts(a, sm, lane);
   }
   __syncthreads();
-  const int V = a.K / 16, items = sm.chunks * a.F, warps = int(gridDim.x) * (kRwThreads / 32);
-  auto channel = [&](int item, int& c, int& f, const uint4*& w, const uint4*& w2) {
-    c = item / a.F;
-    f = item - c * a.F;
-    w = reinterpret_cast<const uint4*>(a.wq) + (int64_t(sm.e[c]) * a.N + f) * V;
-    w2 = w + int64_t(a.F) * V;
+  const int V = a.K / 16, warps = int(gridDim.x) * (kRwThreads / 32), chunks = sm.chunks;
+  // This warp's (chunk, channel) pairs: chunk by chunk, or (SUM) every chunk
+  // of a channel, then the next channel.
+  int c = 0, f = int(blockIdx.x) * (kRwThreads / 32) + warp;
+  auto settle = [&](int& cc, int& ff) {  // whether the pair exists; channels past a chunk's last go to the next chunk
+    if constexpr (!SUM) {
+      while (ff >= a.F && cc < chunks) {
+        ff -= a.F;
+        ++cc;
+      }
+    }
+    return cc < chunks && ff < a.F;
   };
-  int item = int(blockIdx.x) * (kRwThreads / 32) + warp;
-  int c = 0, f = 0;
-  const uint4 *w = nullptr, *w2 = nullptr;
+  auto weights = [&](int cc, int ff) {
+    return reinterpret_cast<const uint4*>(a.wq) + (int64_t(sm.e[cc]) * a.N + ff) * V;
+  };
   uint4 buf[kRwLoads];
-  if (item < items) {
-    channel(item, c, f, w, w2);
-    rw_load<GLU>(w, w2, 0, V, lane, buf);
-  }
+  bool more = settle(c, f);
+  const uint4* w = more ? weights(c, f) : nullptr;
+  const int64_t up = int64_t(a.F) * V;  // from a gate channel to its up channel
+  if (more) rw_load<GLU>(w, w + up, 0, V, lane, buf);
   if (a.x != nullptr) {
-    if (a.x_f32) rw_quantize<float>(a, sm, rw_rows);
-    else rw_quantize<__nv_bfloat16>(a, sm, rw_rows);
+    if (a.x_f32) rw_quantize<float>(a, sm, rw_rows, sm.rows);
+    else rw_quantize<__nv_bfloat16>(a, sm, rw_rows, sm.rows);
   } else {
     for (int i = threadIdx.x; i < a.rows * V; i += kRwThreads)
       reinterpret_cast<uint4*>(rw_rows)[i] = reinterpret_cast<const uint4*>(a.xq)[i];
@@ -913,16 +986,54 @@ __global__ void __launch_bounds__(kRwThreads, 2) w8a8_rows_kernel(const RwArgs a
   }
   __syncthreads();
   const uint4* rows = reinterpret_cast<const uint4*>(rw_rows);
-  while (item < items) {
-    const int n = sm.n[c];
-    if (n == 1) rw_channel<GLU, 1>(a, sm, rows, c, f, w, w2, buf);
-    else if (n == 2) rw_channel<GLU, 2>(a, sm, rows, c, f, w, w2, buf);
-    else rw_channel<GLU, 4>(a, sm, rows, c, f, w, w2, buf);
-    item += warps;
-    if (item < items) {
-      channel(item, c, f, w, w2);
-      rw_load<GLU>(w, w2, 0, V, lane, buf);
+  float y = 0.f;  // SUM: lane t's token
+  if (SUM && chunks == 0) {  // no token has an expert here
+    for (; f < a.F; f += warps)
+      if (lane < a.T) static_cast<__nv_bfloat16*>(a.out)[int64_t(lane) * a.F + f] = __float2bfloat16_rn(0.f);
+  }
+#pragma unroll 1
+  while (more) {
+    int nc = c, nf = f;
+    if (SUM && c + 1 < chunks) {
+      ++nc;
+    } else {
+      nf += warps;
+      if (SUM) nc = 0;
     }
+    more = settle(nc, nf);
+    const uint4* nw = more ? weights(nc, nf) : nullptr;
+    const float* sw = a.ws + int64_t(sm.e[c]) * a.N + f;
+    const float g = sw[0], u = GLU ? sw[a.F] : 0.f;
+    auto channel = [&](auto nr) {
+      constexpr int NR = decltype(nr)::value;
+      int s[NR], s2[NR];
+      rw_channel<GLU, NR>(sm, rows, V, c, w, w + up, nw, nw + up, buf, s, s2);
+      const int r0 = sm.r0[c], n = sm.n[c];
+#pragma unroll
+      for (int r = 0; r < NR; ++r) {
+        if (r >= n) break;
+        const float x = sm.scale[sm.src[r0 + r]], z = float(s[r]) * x * g;
+        if constexpr (SUM) {
+          if (lane == sm.tok[r0 + r]) y = fmaf(sm.val[r0 + r], z, y);
+        } else if (lane == r) {
+          const float v = GLU ? silu_mul(z, float(s2[r]) * x * u) : z;
+          const int64_t at = int64_t(r0 + r) * a.F + f;
+          if (a.out_f32) static_cast<float*>(a.out)[at] = v;
+          else static_cast<__nv_bfloat16*>(a.out)[at] = __float2bfloat16_rn(v);
+        }
+      }
+    };
+    const int n = sm.n[c];
+    if (n == 1) channel(std::integral_constant<int, 1>{});
+    else if (n == 2) channel(std::integral_constant<int, 2>{});
+    else channel(std::integral_constant<int, 4>{});
+    if (SUM && nf != f) {
+      if (lane < a.T) static_cast<__nv_bfloat16*>(a.out)[int64_t(lane) * a.F + f] = __float2bfloat16_rn(y);
+      y = 0.f;
+    }
+    c = nc;
+    f = nf;
+    w = nw;
   }
 }
 
@@ -1106,19 +1217,18 @@ int w8a8_pairs(int dev, int sms, cudaLaunchConfig_t cfg, int* out) {
 // The form for a handful of rows: they have to fit shared memory twice per SM.
 bool rows_form(int64_t rows, int K) { return rows <= kRwMaxRows && rows * K <= int64_t(kRwMaxSmem); }
 
-template <bool GLU>
-int launch_rows(const RwArgs& a, int dev, int sms, cudaStream_t stream) {
+template <bool GLU, bool SUM>
+int launch_rows(const RwArgs& a, int staged, int64_t items, int dev, int sms, cudaStream_t stream) {
   static std::atomic<bool> ready[kMaxDevices];
   if (dev < 0 || dev >= kMaxDevices) return kCudaErr;
   if (!ready[dev].load(std::memory_order_acquire)) {
-    if (cudaFuncSetAttribute(w8a8_rows_kernel<GLU>, cudaFuncAttributeMaxDynamicSharedMemorySize, int(kRwMaxSmem)) !=
-        cudaSuccess)
+    if (cudaFuncSetAttribute(w8a8_rows_kernel<GLU, SUM>, cudaFuncAttributeMaxDynamicSharedMemorySize,
+                             int(kRwMaxSmem)) != cudaSuccess)
       return kCudaErr;
     ready[dev].store(true, std::memory_order_release);
   }
-  const int64_t warps = int64_t(a.F) * std::min(a.rows, a.E);  // at least one chunk per expert with rows
-  const int64_t blocks = std::min<int64_t>((warps + kRwThreads / 32 - 1) / (kRwThreads / 32), 2 * int64_t(sms));
-  w8a8_rows_kernel<GLU><<<unsigned(blocks), kRwThreads, size_t(a.rows) * a.K, stream>>>(a);
+  const int64_t blocks = std::min<int64_t>((items + kRwThreads / 32 - 1) / (kRwThreads / 32), 2 * int64_t(sms));
+  w8a8_rows_kernel<GLU, SUM><<<unsigned(blocks), kRwThreads, size_t(staged) * a.K, stream>>>(a);
   return cudaGetLastError() == cudaSuccess ? kOk : kCudaErr;
 }
 
@@ -1180,7 +1290,7 @@ QScratch q_scratch(int64_t rows, int K, int N, bool glu, bool with_x, int sms) {
   QScratch q;
   q.few = rows_form(rows, K);
   q.split = !q.few && q_split(rows, N, glu ? N / 2 : N, glu, sms / 2);
-  q.rows_outside = with_x && !(q.few && rows <= kRwMaxFresh);
+  q.rows_outside = with_x && !(q.few && rows * K <= kRwMaxFresh);
   q.xq = q.split ? size_t(sms / 2) * 2 * kQSlotInts * 4 : 0;
   q.xs = q.xq + (q.rows_outside ? (size_t(rows) * K + 255) / 256 * 256 : 0);
   q.total = q.xs + (q.rows_outside ? size_t(rows) * 4 : 0);
@@ -1256,7 +1366,9 @@ extern "C" int moe_w8a8_gemm(const moe_w8a8_params* p, void* stream) {
     w.ws = p->ws;
     w.out = p->out;
     w.out_f32 = p->out_is_f32;
-    return glu ? launch_rows<true>(w, dev, sms, s) : launch_rows<false>(w, dev, sms, s);
+    const int64_t items = int64_t(a.F) * std::min(w.rows, a.E);  // at least one chunk per expert with rows
+    return glu ? launch_rows<true, false>(w, w.rows, items, dev, sms, s)
+               : launch_rows<false, false>(w, w.rows, items, dev, sms, s);
   }
   const bool split = sc.split;
   CUtensorMap tw;
@@ -1300,4 +1412,98 @@ extern "C" int moe_weighted_sum(const void* rows, int32_t rows_are_f32, const vo
   if (rows_are_f32) launch(static_cast<const float*>(rows));
   else launch(static_cast<const __nv_bfloat16*>(rows));
   return cudaGetLastError() == cudaSuccess ? kOk : kCudaErr;
+}
+
+namespace {
+// scratch of the layer of a few tokens: h, then what is quantised by launches
+// of its own.
+struct QLayerScratch {
+  bool x_outside, h_outside;
+  size_t xq, xs, hq, hs, total;
+};
+QLayerScratch q_layer_scratch(int64_t T, int H, int F, int K) {
+  QLayerScratch s;
+  s.x_outside = T * H > kRwMaxFresh;
+  s.h_outside = T * K * F > kRwMaxFresh;
+  const auto up = [](size_t v) { return (v + 255) / 256 * 256; };
+  s.xq = up(size_t(T) * K * F * 4);
+  s.xs = s.xq + (s.x_outside ? up(size_t(T) * H) : 0);
+  s.hq = s.xs + (s.x_outside ? 256 : 0);
+  s.hs = s.hq + (s.h_outside ? up(size_t(T) * K * F) : 0);
+  s.total = s.hs + (s.h_outside ? 256 : 0);
+  return s;
+}
+bool q_layer_ok(int64_t T, int32_t H, int32_t F, int32_t E, int32_t K) {
+  return T >= 0 && K >= 1 && T <= kRwMaxRows && T * K <= kRwMaxRows && H > 0 && H % 16 == 0 && F > 0 && F % 16 == 0 &&
+         E >= 1 && E <= kMaxExperts && T * H <= int64_t(kRwMaxSmem) && T * K * F <= int64_t(kRwMaxSmem);
+}
+}  // namespace
+
+extern "C" int moe_w8a8_layer_scratch_bytes(int64_t T, int32_t H, int32_t F, int32_t E, int32_t K, size_t* out) {
+  if (!out || !q_layer_ok(T, H, F, E, K)) return kBadArg;
+  *out = q_layer_scratch(T, H, F, K).total;
+  return kOk;
+}
+
+extern "C" int moe_w8a8_layer(const moe_w8a8_layer_params* p, void* stream) {
+  if (!p || !q_layer_ok(p->T, p->hidden, p->ffn, p->experts, p->K)) return kBadArg;
+  if (p->T == 0) return kOk;
+  if (!p->x || !p->w13 || !p->w13_scale || !p->w2 || !p->w2_scale || !p->top_idxs || !p->top_vals || !p->y ||
+      !p->scratch)
+    return kBadArg;
+  if (misaligned16(p->x) || misaligned16(p->w13) || misaligned16(p->w2) || misaligned16(p->scratch)) return kBadArg;
+  const int T = int(p->T), H = p->hidden, F = p->ffn, K = p->K;
+  const QLayerScratch sc = q_layer_scratch(T, H, F, K);
+  if (p->scratch_bytes < sc.total) return kBadArg;
+  int sms = 0, dev = 0;
+  if (sm_count(&sms, &dev) != kOk) return kCudaErr;
+  const cudaStream_t s = static_cast<cudaStream_t>(stream);
+  unsigned char* base = static_cast<unsigned char*>(p->scratch);
+  float* h = reinterpret_cast<float*>(base);
+  RwArgs a = {};
+  a.E = p->experts;
+  a.K = H;
+  a.N = 2 * F;
+  a.F = F;
+  a.rows = T;
+  a.wq = static_cast<const int8_t*>(p->w13);
+  a.ws = p->w13_scale;
+  a.out = h;
+  a.out_f32 = 1;
+  a.ids = p->top_idxs;
+  a.ids64 = p->ids_are_int64;
+  a.first = p->first_expert;
+  a.T = T;
+  a.topk = K;
+  a.vals = p->top_vals;
+  a.vals_bf16 = p->vals_are_bf16;
+  a.x = p->x;
+  if (sc.x_outside) {
+    int8_t* q = reinterpret_cast<int8_t*>(base + sc.xq);
+    float* scale = reinterpret_cast<float*>(base + sc.xs);
+    if (launch_quant<__nv_bfloat16>(p->x, T, H, nullptr, nullptr, q, scale, sms, s) != kOk) return kCudaErr;
+    a.x = nullptr;
+    a.xq = q;
+    a.xs = scale;
+  }
+  if (launch_rows<true, false>(a, T, int64_t(F) * std::min(T * K, a.E), dev, sms, s) != kOk) return kCudaErr;
+  // Rows of h that no id leads to were not written; they are not used either.
+  a.K = F;
+  a.N = a.F = H;
+  a.rows = T * K;
+  a.wq = static_cast<const int8_t*>(p->w2);
+  a.ws = p->w2_scale;
+  a.out = p->y;
+  a.out_f32 = 0;
+  a.x = h;
+  a.x_f32 = 1;
+  if (sc.h_outside) {
+    int8_t* q = reinterpret_cast<int8_t*>(base + sc.hq);
+    float* scale = reinterpret_cast<float*>(base + sc.hs);
+    if (launch_quant<float>(h, T * K, F, nullptr, nullptr, q, scale, sms, s) != kOk) return kCudaErr;
+    a.x = nullptr;
+    a.xq = q;
+    a.xs = scale;
+  }
+  return launch_rows<false, true>(a, T * K, H, dev, sms, s);
 }

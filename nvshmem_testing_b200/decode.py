@@ -27,7 +27,7 @@ from . import _native as N
 from . import utils
 
 
-def _check(x, w13, w2, out, status):
+def _check(x, w13, w2, first_expert, out, status):
     if x.dim() != 2 or w13.dim() != 3 or w2.dim() != 3:
         raise ValueError("x [T, H], w13 [El, H, 2F] and w2 [El, F, H] are required")
     T, H = x.shape
@@ -48,6 +48,8 @@ def _check(x, w13, w2, out, status):
     if out is not None and (tuple(out.shape) != (T, H) or out.dtype != torch.bfloat16 or out.device != x.device
                             or not out.is_contiguous()):
         raise ValueError(f"out must be a contiguous bfloat16 tensor of shape {(T, H)} on the tokens' device")
+    if not 0 <= first_expert < 1 << 31:
+        raise ValueError(f"first_expert = {first_expert} must be an expert's id")
     if status is not None and (status.dtype != torch.int32 or status.numel() != 1 or not status.is_pinned()):
         raise ValueError("status must be one pinned int32")
     return T, H, F, El
@@ -91,7 +93,7 @@ def moe_layer(x: torch.Tensor, top_idxs: torch.Tensor, top_vals: torch.Tensor, w
     first_expert: id of the first expert held here.  ``out`` optionally
     supplies y; ``status`` (one pinned int32) receives a device-side error
     word, if any."""
-    dims = _check(x, w13, w2, out, status)
+    dims = _check(x, w13, w2, first_expert, out, status)
     if top_idxs.dim() == 1:
         top_idxs = top_idxs[:, None]
     if top_vals.dim() == 1:
@@ -124,7 +126,7 @@ def routed_layer(x: torch.Tensor, router_w: torch.Tensor, topk: int, w13: torch.
     descending order, equal ones by ascending id, divided by their sum with
     ``renormalize``.  The other arguments are those of ``moe_layer``; w13 and
     w2 may hold a part of the E experts."""
-    dims = _check(x, w13, w2, out, status)
+    dims = _check(x, w13, w2, first_expert, out, status)
     T, H = dims[0], dims[1]
     if router_w.dim() != 2 or router_w.shape[0] != H:
         raise ValueError(f"router_w {tuple(router_w.shape)} does not match x {tuple(x.shape)}")

@@ -16,7 +16,8 @@ tensor-core rate.
   SwiGLU in its epilogue on request; ``linear`` — the dense form from bf16;
 * ``moe_layer`` — the gated layer on one rank's experts, the 8-bit sibling of
   ``combine.moe_layer`` over ``mlp``: route, gather and quantise, gate/up
-  product with SwiGLU, quantise, down product, weighted sum per token.
+  product with SwiGLU, quantise, down product, weighted sum per token (for a
+  few tokens two launches, which route, quantise and add for themselves).
 
 Nothing is read on the host and every call may be captured into a CUDA graph.
 """
@@ -115,6 +116,13 @@ def quantize_weights(w: torch.Tensor) -> QuantWeights:
 def _scratch_bytes(*sizes) -> int:
     need = ctypes.c_size_t()
     N.check(N.lib().moe_w8a8_scratch_bytes(*sizes, ctypes.byref(need)), "moe_w8a8_scratch_bytes")
+    return need.value
+
+
+@functools.lru_cache(maxsize=256)
+def _layer_scratch_bytes(*sizes) -> int:
+    need = ctypes.c_size_t()
+    N.check(N.lib().moe_w8a8_layer_scratch_bytes(*sizes, ctypes.byref(need)), "moe_w8a8_layer_scratch_bytes")
     return need.value
 
 
@@ -219,6 +227,8 @@ def moe_layer(x: torch.Tensor, top_idxs: torch.Tensor, top_vals: torch.Tensor, w
     _check_product(F, H, El, False)
     if status is not None and (status.dtype != torch.int32 or status.numel() != 1 or not status.is_pinned()):
         raise ValueError("status must be one pinned int32")
+    if not 0 <= first_expert < 1 << 31:
+        raise ValueError(f"first_expert = {first_expert} must be an expert's id")
     if top_idxs.dim() == 1:
         top_idxs = top_idxs[:, None]
     if top_vals.dim() == 1:
@@ -238,6 +248,18 @@ def moe_layer(x: torch.Tensor, top_idxs: torch.Tensor, top_vals: torch.Tensor, w
     if T == 0:
         return y
     ids, vals = top_idxs.contiguous(), top_vals.contiguous()
+    if T * K <= N.W8A8_LAYER_MAX_ROWS and max(T * H, T * K * F) <= N.W8A8_LAYER_MAX_VALUES:
+        # A few tokens: no routing, packing or sum of their own.
+        need = _layer_scratch_bytes(T, H, F, El, K)
+        scratch = torch.empty(need, dtype=torch.uint8, device=x.device)
+        x = x.contiguous()
+        p = N.W8A8LayerParams(T, H, F, El, K, first_expert, ids.dtype == torch.int64, vals.dtype == torch.bfloat16, 0,
+                              x.data_ptr(), w13.q.data_ptr(), w13.scale.data_ptr(), w2.q.data_ptr(),
+                              w2.scale.data_ptr(), ids.data_ptr(), vals.data_ptr(), y.data_ptr(), scratch.data_ptr(),
+                              need)
+        with utils.on_device(x.device) as stream:
+            N.check(N.lib().moe_w8a8_layer(ctypes.byref(p), stream), "moe_w8a8_layer")
+        return y
     with utils.on_device(x.device) as stream:
         r = utils.route(ids if first_expert == 0 else ids - first_expert, El, with_slots=True)
         n, live = T * K, r.offsets[El:]

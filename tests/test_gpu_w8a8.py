@@ -268,6 +268,15 @@ def layer_ref(x, ids, vals, w13, w2, first):
 LAYERS = [
     # T, H, El, E, first, K, F
     (1, 64, 4, 4, 0, 1, 32),
+    (1, 7168, 12, 12, 0, 8, 2048),
+    (1, 512, 6, 12, 3, 16, 176),
+    (1, 2048, 3, 3, 0, 2, 24576),     # h quantised by a launch of its own
+    (2, 24576, 4, 4, 0, 2, 64),       # x, too
+    (4, 336, 3, 3, 0, 3, 144),
+    (5, 256, 2, 2, 0, 2, 128),
+    (8, 1040, 2, 2, 0, 2, 96),
+    (16, 256, 2, 4, 1, 1, 80),
+    (17, 256, 2, 4, 1, 1, 80),
     (3, 144, 8, 8, 0, 2, 112),
     (40, 256, 8, 32, 16, 6, 208),
     (65, 512, 16, 16, 0, 4, 384),
@@ -281,7 +290,7 @@ def test_layer(T, H, El, E, first, K, F):
     x = torch.randn(T, H, generator=g, device="cuda").to(torch.bfloat16)
     w13 = w8a8.quantize_weights(0.05 * torch.randn(El, H, 2 * F, generator=g, device="cuda"))
     w2 = w8a8.quantize_weights(0.05 * torch.randn(El, F, H, generator=g, device="cuda"))
-    ids = torch.rand(T, E, generator=g, device="cuda").topk(K, dim=-1).indices
+    ids = torch.rand(T, max(E, K), generator=g, device="cuda").topk(K, dim=-1).indices
     vals = torch.randn(T, K, generator=g, device="cuda").softmax(-1)
     if K > 1:
         ids[0, 1] = ids[0, 0]        # repeated
