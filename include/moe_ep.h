@@ -387,7 +387,7 @@ int moe_ep_run_compact_swiglu(const moe_ep_run_params* params, int64_t send_rows
  * top_idxs and top_vals (fp32), divided by their sum with `renormalize`.
  * Requires T <= MOE_DECODE_MAX_TOKENS, T * K <= 1024, K <= 32, hidden and ffn
  * multiples of 8, hidden <= 32768, experts and router_experts <= 1024,
- * router_experts a multiple of 4; x, w13, w2 and scratch 16-byte aligned.
+ * router_experts a multiple of 4; x, w13, w2, y and scratch 16-byte aligned.
  * scratch: moe_decode_scratch_bytes of device memory, not initialised, for
  * this call alone until it has finished.  Launched cooperatively (one CTA per
  * SM), so calls on several streams run one after another. */
@@ -476,7 +476,7 @@ int moe_w8a8_gemm(const moe_w8a8_params* params, void* stream);
  * MOE_W8A8_LAYER_MAX_ROWS, hidden and ffn multiples of 16, T * hidden and
  * T * K * ffn <= 98304, experts <= 1024; x, w13, w2 and scratch 16-byte
  * aligned.  scratch: moe_w8a8_layer_scratch_bytes, as above. */
-#define MOE_W8A8_LAYER_MAX_ROWS 16
+#define MOE_W8A8_LAYER_MAX_ROWS 32
 typedef struct moe_w8a8_layer_params {
   int64_t T;
   int32_t hidden, ffn;

@@ -96,7 +96,7 @@ class W8A8LayerParams(ctypes.Structure):
                 ("scratch_bytes", ctypes.c_size_t)]
 
 
-W8A8_LAYER_MAX_ROWS = 16  # tokens times ids per token
+W8A8_LAYER_MAX_ROWS = 32  # tokens times ids per token
 W8A8_LAYER_MAX_VALUES = 98304
 DECODE_MAX_TOKENS = 64
 DECODE_MAX_ROWS = 1024  # tokens times ids per token

@@ -1150,7 +1150,9 @@ extern "C" int moe_decode_layer(const moe_decode_params* p, void* stream) {
   if (p->router_w && Er < 4) return kBadArg;
   if (p->T == 0) return kOk;
   if (!p->x || !p->w13 || !p->w2 || !p->y || !p->top_idxs || !p->top_vals || !p->scratch) return kBadArg;
-  if (misaligned(p->x) || misaligned(p->w13) || misaligned(p->w2) || misaligned(p->scratch)) return kBadArg;
+  if (misaligned(p->x) || misaligned(p->w13) || misaligned(p->w2) || misaligned(p->y) ||
+      misaligned(p->scratch))
+    return kBadArg;
   if (p->router_w && ((reinterpret_cast<uintptr_t>(p->router_w) & 3) || p->vals_are_bf16)) return kBadArg;
   if (!driver().ok) return kCudaErr;
   int dev = 0, sms = 0;

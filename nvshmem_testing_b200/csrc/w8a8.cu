@@ -731,8 +731,9 @@ __global__ void __launch_bounds__(kQThreads, 1)
 // of every (token, expert) row, then (SUM) the down channels, a warp taking
 // one of all experts and adding their rows, weighted, to y.
 constexpr int kRwThreads = 512;
-constexpr int kRwMaxRows = 16;
-constexpr int kRwMaxFresh = 32768;          // values quantised by every CTA
+constexpr int kRwMaxRows = 32;
+constexpr int kRwMaxFresh = 32768;          // values quantised by every CTA,
+constexpr int kRwMaxFreshRows = 16;         // in rows of at least a warp each
 constexpr int kRwRows = 4;                  // rows of a channel's pass
 constexpr uint32_t kRwMaxSmem = 96 * 1024;  // of rows: two CTAs per SM
 
@@ -898,7 +899,7 @@ __device__ __forceinline__ void rw_table_counts(const RwArgs& a, RwSmem& sm, int
   }
 }
 
-// The same from a layer's ids, sorted by expert, then token (T * topk <= 16
+// The same from a layer's ids, sorted by expert, then token (T * topk <= 32
 // rows; an id repeated within a token's row counts once).
 template <bool SUM>
 __device__ __forceinline__ void rw_table_ids(const RwArgs& a, RwSmem& sm, int lane) {
@@ -1215,6 +1216,7 @@ int w8a8_pairs(int dev, int sms, cudaLaunchConfig_t cfg, int* out) {
 }
 
 // The form for a handful of rows: they have to fit shared memory twice per SM.
+bool fresh(int64_t rows, int K) { return rows <= kRwMaxFreshRows && rows * K <= kRwMaxFresh; }
 bool rows_form(int64_t rows, int K) { return rows <= kRwMaxRows && rows * K <= int64_t(kRwMaxSmem); }
 
 template <bool GLU, bool SUM>
@@ -1290,7 +1292,7 @@ QScratch q_scratch(int64_t rows, int K, int N, bool glu, bool with_x, int sms) {
   QScratch q;
   q.few = rows_form(rows, K);
   q.split = !q.few && q_split(rows, N, glu ? N / 2 : N, glu, sms / 2);
-  q.rows_outside = with_x && !(q.few && rows * K <= kRwMaxFresh);
+  q.rows_outside = with_x && !(q.few && fresh(rows, K));
   q.xq = q.split ? size_t(sms / 2) * 2 * kQSlotInts * 4 : 0;
   q.xs = q.xq + (q.rows_outside ? (size_t(rows) * K + 255) / 256 * 256 : 0);
   q.total = q.xs + (q.rows_outside ? size_t(rows) * 4 : 0);
@@ -1423,8 +1425,8 @@ struct QLayerScratch {
 };
 QLayerScratch q_layer_scratch(int64_t T, int H, int F, int K) {
   QLayerScratch s;
-  s.x_outside = T * H > kRwMaxFresh;
-  s.h_outside = T * K * F > kRwMaxFresh;
+  s.x_outside = !fresh(T, H);
+  s.h_outside = !fresh(T * K, F);
   const auto up = [](size_t v) { return (v + 255) / 256 * 256; };
   s.xq = up(size_t(T) * K * F * 4);
   s.xs = s.xq + (s.x_outside ? up(size_t(T) * H) : 0);

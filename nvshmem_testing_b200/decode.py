@@ -27,32 +27,40 @@ from . import _native as N
 from . import utils
 
 
-def _check(x, w13, w2, first_expert, out, status):
-    if x.dim() != 2 or w13.dim() != 3 or w2.dim() != 3:
+@functools.lru_cache(maxsize=512)  # a decode step repeats its shapes
+def _dims(x, w13, w2) -> tuple[int, int, int, int]:
+    if len(x) != 2 or len(w13) != 3 or len(w2) != 3:
         raise ValueError("x [T, H], w13 [El, H, 2F] and w2 [El, F, H] are required")
-    T, H = x.shape
-    El, _, F2 = w13.shape
+    T, H = x
+    El, F2 = w13[0], w13[2]
     F = F2 // 2
-    if w13.shape[1] != H or F2 % 2 or tuple(w2.shape) != (El, F, H):
-        raise ValueError(f"x {tuple(x.shape)}, w13 {tuple(w13.shape)} and w2 {tuple(w2.shape)} do not form an MLP")
-    if H % 8 or F % 8 or H == 0 or F == 0:
-        raise ValueError(f"H = {H} and F = {F} must be positive multiples of 8")
+    if w13[1] != H or F2 % 2 or tuple(w2) != (El, F, H):
+        raise ValueError(f"x {tuple(x)}, w13 {tuple(w13)} and w2 {tuple(w2)} do not form an MLP")
+    if H % 8 or F % 8 or not 0 < H <= 32768 or F == 0:
+        raise ValueError(f"H = {H} and F = {F} must be positive multiples of 8, H 32768 at most")
+    if not 1 <= El <= 1024:
+        raise ValueError(f"{El} experts: 1 to 1024")
+    if T > N.DECODE_MAX_TOKENS:
+        raise ValueError(f"{T} tokens: this form takes {N.DECODE_MAX_TOKENS} at most (mlp.moe_mlp has no limit)")
+    return T, H, F, El
+
+
+def _check(x, w13, w2, first_expert, out, status):
+    dims = _dims(x.shape, w13.shape, w2.shape)
     if not (x.dtype == w13.dtype == w2.dtype == torch.bfloat16):
         raise TypeError("x, w13 and w2 must be bfloat16")
     if not x.is_cuda or w13.device != x.device or w2.device != x.device:
         raise ValueError("x, w13 and w2 must be CUDA tensors on one device")
     if not w13.is_contiguous() or not w2.is_contiguous():
         raise ValueError("w13 and w2 must be contiguous")
-    if T > N.DECODE_MAX_TOKENS:
-        raise ValueError(f"{T} tokens: this form takes {N.DECODE_MAX_TOKENS} at most (mlp.moe_mlp has no limit)")
-    if out is not None and (tuple(out.shape) != (T, H) or out.dtype != torch.bfloat16 or out.device != x.device
+    if out is not None and (out.shape != x.shape or out.dtype != torch.bfloat16 or out.device != x.device
                             or not out.is_contiguous()):
-        raise ValueError(f"out must be a contiguous bfloat16 tensor of shape {(T, H)} on the tokens' device")
+        raise ValueError(f"out must be a contiguous bfloat16 tensor of shape {tuple(x.shape)} on the tokens' device")
     if not 0 <= first_expert < 1 << 31:
         raise ValueError(f"first_expert = {first_expert} must be an expert's id")
     if status is not None and (status.dtype != torch.int32 or status.numel() != 1 or not status.is_pinned()):
         raise ValueError("status must be one pinned int32")
-    return T, H, F, El
+    return dims
 
 
 @functools.lru_cache(maxsize=256)

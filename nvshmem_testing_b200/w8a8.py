@@ -40,15 +40,25 @@ class QuantWeights:
     scale: torch.Tensor
 
 
-def _check_weights(w: QuantWeights, name: str) -> tuple[int, int, int]:
-    if w.q.dim() != 3 or tuple(w.scale.shape) != tuple(w.q.shape[:2]):
-        raise ValueError(f"{name}: q [El, N, K] and scale [El, N] are required, "
-                         f"got {tuple(w.q.shape)} and {tuple(w.scale.shape)}")
-    if w.q.dtype != torch.int8 or w.scale.dtype != torch.float32:
+# Checks of shapes are remembered (a decode step repeats them); the error of a
+# failed one is raised anew each time.
+@functools.lru_cache(maxsize=512)
+def _weights_dims(q, scale, name: str) -> tuple[int, int, int]:
+    if len(q) != 3 or scale != q[:2]:
+        raise ValueError(f"{name}: q [El, N, K] and scale [El, N] are required, got {tuple(q)} and {tuple(scale)}")
+    return tuple(q)
+
+
+def _check_weights(w: QuantWeights, name: str, device) -> tuple[int, int, int]:
+    q, scale = w.q, w.scale
+    dims = _weights_dims(q.shape, scale.shape, name)
+    if q.dtype != torch.int8 or scale.dtype != torch.float32:
         raise TypeError(f"{name}: q must be int8 and scale float32")
-    if not w.q.is_contiguous() or not w.scale.is_contiguous():
+    if not q.is_contiguous() or not scale.is_contiguous():
         raise ValueError(f"{name}: q and scale must be contiguous")
-    return tuple(w.q.shape)
+    if q.device != device or scale.device != device:
+        raise ValueError(f"{name}: q and scale must be on {device}")
+    return dims
 
 
 def _check_product(K: int, Nw: int, El: int, swiglu: bool):
@@ -56,14 +66,16 @@ def _check_product(K: int, Nw: int, El: int, swiglu: bool):
         raise ValueError(f"K = {K} must be a multiple of 16, 131056 at most")
     if Nw % (16 if swiglu else 8) or Nw == 0:
         raise ValueError(f"{Nw} channels: a multiple of {16 if swiglu else 8} is needed")
-    if El > 1024:
-        raise ValueError(f"{El} experts: 1024 at most")
+    if not 1 <= El <= 1024:
+        raise ValueError(f"{El} experts: 1 to 1024")
 
 
 def _on_gpu(device, **tensors):
+    if device.type != "cuda":
+        raise ValueError(f"CUDA tensors are required, not {device}")
     for name, t in tensors.items():
-        if t is not None and (not t.is_cuda or t.device != device):
-            raise ValueError(f"{name} must be a CUDA tensor on {device}")
+        if t is not None and t.device != device:
+            raise ValueError(f"{name} must be on {device}")
 
 
 def quantize_rows(x: torch.Tensor, perm: torch.Tensor | None = None,
@@ -85,7 +97,7 @@ def quantize_rows(x: torch.Tensor, perm: torch.Tensor | None = None,
         raise TypeError("perm must be a contiguous int32 vector")
     if live_rows is not None and (live_rows.dtype != torch.int32 or live_rows.numel() != 1):
         raise TypeError("live_rows must be one int32")
-    _on_gpu(x.device, x=x, perm=perm, live_rows=live_rows)
+    _on_gpu(x.device, perm=perm, live_rows=live_rows)
     rows = x.shape[0] if perm is None else perm.shape[0]
     x = x.contiguous()
     q = torch.empty((rows, K), dtype=torch.int8, device=x.device)
@@ -104,7 +116,7 @@ def quantize_weights(w: torch.Tensor) -> QuantWeights:
     if w.dim() != 3:
         raise ValueError("w [El, K, N] is required")
     El, K, Nout = w.shape
-    _on_gpu(w.device, w=w)
+    _on_gpu(w.device)
     q = torch.empty((El, Nout, K), dtype=torch.int8, device=w.device)
     scale = torch.empty((El, Nout), dtype=torch.float32, device=w.device)
     for e in range(El):
@@ -119,13 +131,6 @@ def _scratch_bytes(*sizes) -> int:
     return need.value
 
 
-@functools.lru_cache(maxsize=256)
-def _layer_scratch_bytes(*sizes) -> int:
-    need = ctypes.c_size_t()
-    N.check(N.lib().moe_w8a8_layer_scratch_bytes(*sizes, ctypes.byref(need)), "moe_w8a8_layer_scratch_bytes")
-    return need.value
-
-
 def grouped_gemm(xq: torch.Tensor, xs: torch.Tensor, w: QuantWeights, counts: torch.Tensor | None = None, *,
                  swiglu: bool = False, out_dtype=torch.bfloat16, out: torch.Tensor | None = None,
                  status: torch.Tensor | None = None) -> torch.Tensor:
@@ -137,7 +142,7 @@ def grouped_gemm(xq: torch.Tensor, xs: torch.Tensor, w: QuantWeights, counts: to
     [N/2, N) and ``out [rows, N/2] = silu(gate) * up``.  Rows behind the last
     expert's are left as they were (``out`` supplies the buffer).
     ``out_dtype`` is bfloat16 or float32."""
-    El, Nw, K = _check_weights(w, "w")
+    El, Nw, K = _check_weights(w, "w", xq.device)
     if xq.dim() != 2 or xq.shape[1] != K or tuple(xs.shape) != (xq.shape[0],):
         raise ValueError(f"xq {tuple(xq.shape)} and xs {tuple(xs.shape)} do not match w {tuple(w.q.shape)}")
     if xq.dtype != torch.int8 or xs.dtype != torch.float32:
@@ -157,7 +162,7 @@ def grouped_gemm(xq: torch.Tensor, xs: torch.Tensor, w: QuantWeights, counts: to
         raise ValueError(f"out must be a contiguous {out_dtype} tensor of shape {(rows, cols)}")
     if status is not None and (status.dtype != torch.int32 or status.numel() != 1 or not status.is_pinned()):
         raise ValueError("status must be one pinned int32")
-    _on_gpu(xq.device, xq=xq, xs=xs, q=w.q, scale=w.scale, counts=counts, out=out)
+    _on_gpu(xq.device, xs=xs, counts=counts, out=out)
     if rows == 0:
         return out
     with utils.on_device(xq.device) as stream:
@@ -170,10 +175,11 @@ def _gemm(xq, xs, x, w, counts, perm, live_rows, rows, K, Nw, El, swiglu, out, s
     """The checked call, for quantised rows (xq, xs) or rows x that are still
     to be."""
     need = _scratch_bytes(rows, K, Nw, El, int(swiglu), int(x is not None), out.device.index)
-    scratch = torch.empty(need, dtype=torch.uint8, device=out.device).data_ptr() if need else None
+    scratch = torch.empty(need, dtype=torch.uint8, device=out.device) if need else None
     p = N.W8A8Params(rows, K, Nw, El, swiglu, out.dtype == torch.float32, x is not None and x.dtype == torch.float32,
                      None if xq is None else xq.data_ptr(), None if xs is None else xs.data_ptr(), w.q.data_ptr(),
-                     w.scale.data_ptr(), None if counts is None else counts.data_ptr(), out.data_ptr(), scratch, need,
+                     w.scale.data_ptr(), None if counts is None else counts.data_ptr(), out.data_ptr(),
+                     None if scratch is None else scratch.data_ptr(), need,
                      None if status is None else status.data_ptr(), None if x is None else x.data_ptr(),
                      None if perm is None else perm.data_ptr(), None if live_rows is None else live_rows.data_ptr())
     N.check(N.lib().moe_w8a8_gemm(ctypes.byref(p), stream), "moe_w8a8_gemm")
@@ -182,7 +188,7 @@ def _gemm(xq, xs, x, w, counts, perm, live_rows, rows, K, Nw, El, swiglu, out, s
 def linear(x: torch.Tensor, w: QuantWeights, *, out_dtype=torch.bfloat16) -> torch.Tensor:
     """``x [rows, K] @ w`` for one weight matrix (w.q [1, N, K]): quantises the
     rows and multiplies."""
-    El, Nw, K = _check_weights(w, "w")
+    El, Nw, K = _check_weights(w, "w", x.device)
     if El != 1:
         raise ValueError(f"one weight matrix [1, N, K] is required, got {tuple(w.q.shape)}")
     if x.dim() != 2 or x.shape[1] != K or x.dtype not in (torch.bfloat16, torch.float32):
@@ -190,13 +196,39 @@ def linear(x: torch.Tensor, w: QuantWeights, *, out_dtype=torch.bfloat16) -> tor
     _check_product(K, Nw, El, False)
     if out_dtype not in (torch.bfloat16, torch.float32):
         raise TypeError("out_dtype must be bfloat16 or float32")
-    _on_gpu(x.device, x=x, q=w.q, scale=w.scale)
+    _on_gpu(x.device)
     rows = x.shape[0]
     out = torch.empty((rows, Nw), dtype=out_dtype, device=x.device)
     if rows:
         with utils.on_device(x.device) as stream:
             _gemm(None, None, x.contiguous(), w, None, None, None, rows, K, Nw, 1, False, out, None, stream)
     return out
+
+
+@functools.lru_cache(maxsize=512)
+def _layer_dims(x, ids, vals, q13, q2) -> tuple[int, int, int | None]:
+    """(T, ids per token, scratch of the form for a few tokens or None)."""
+    El, F2, H = q13
+    F = F2 // 2
+    if F2 % 2 or tuple(q2) != (El, H, F):
+        raise ValueError(f"w13 {tuple(q13)} and w2 {tuple(q2)} do not form an MLP")
+    if len(x) != 2 or x[1] != H:
+        raise ValueError(f"x {tuple(x)} does not match w13 {tuple(q13)}")
+    if H % 16 or F % 16:
+        raise ValueError(f"H = {H} and F = {F} must be multiples of 16")
+    _check_product(H, F2, El, True)
+    _check_product(F, H, El, False)
+    T = x[0]
+    if len(ids) != 2 or ids[0] != T or vals != ids:
+        raise ValueError(f"top_idxs {tuple(ids)} and top_vals {tuple(vals)} must be [T, K]")
+    K = ids[1]
+    if not 1 <= K <= 32:
+        raise ValueError(f"{K} ids per token: 1 to 32")
+    if T * K > N.W8A8_LAYER_MAX_ROWS or max(T * H, T * K * F) > N.W8A8_LAYER_MAX_VALUES:
+        return T, K, None
+    need = ctypes.c_size_t()
+    N.check(N.lib().moe_w8a8_layer_scratch_bytes(T, H, F, El, K, ctypes.byref(need)), "moe_w8a8_layer_scratch_bytes")
+    return T, K, need.value
 
 
 def moe_layer(x: torch.Tensor, top_idxs: torch.Tensor, top_vals: torch.Tensor, w13: QuantWeights, w2: QuantWeights,
@@ -212,45 +244,31 @@ def moe_layer(x: torch.Tensor, top_idxs: torch.Tensor, top_vals: torch.Tensor, w
     x [T, H] bf16, top_idxs [T, K] int32/int64, top_vals [T, K] float32 or
     bfloat16; w13.q [El, 2F, H] (gate channels [0, F), up after them) and w2.q
     [El, H, F].  H and F multiples of 16."""
-    El, F2, H = _check_weights(w13, "w13")
+    dev = x.device
+    El, F2, H = _check_weights(w13, "w13", dev)
+    _check_weights(w2, "w2", dev)
     F = F2 // 2
-    _check_weights(w2, "w2")
-    if F2 % 2 or tuple(w2.q.shape) != (El, H, F):
-        raise ValueError(f"w13 {tuple(w13.q.shape)} and w2 {tuple(w2.q.shape)} do not form an MLP")
-    if x.dim() != 2 or x.shape[1] != H:
-        raise ValueError(f"x {tuple(x.shape)} does not match w13 {tuple(w13.q.shape)}")
-    if x.dtype != torch.bfloat16:
-        raise TypeError("x must be bfloat16")
-    if H % 16 or F % 16:
-        raise ValueError(f"H = {H} and F = {F} must be multiples of 16")
-    _check_product(H, F2, El, True)
-    _check_product(F, H, El, False)
-    if status is not None and (status.dtype != torch.int32 or status.numel() != 1 or not status.is_pinned()):
-        raise ValueError("status must be one pinned int32")
-    if not 0 <= first_expert < 1 << 31:
-        raise ValueError(f"first_expert = {first_expert} must be an expert's id")
     if top_idxs.dim() == 1:
         top_idxs = top_idxs[:, None]
     if top_vals.dim() == 1:
         top_vals = top_vals[:, None]
-    T = x.shape[0]
-    if top_idxs.dim() != 2 or top_idxs.shape[0] != T or top_vals.shape != top_idxs.shape:
-        raise ValueError(f"top_idxs {tuple(top_idxs.shape)} and top_vals {tuple(top_vals.shape)} must be [T, K]")
+    T, K, need = _layer_dims(x.shape, top_idxs.shape, top_vals.shape, w13.q.shape, w2.q.shape)
+    if x.dtype != torch.bfloat16:
+        raise TypeError("x must be bfloat16")
     if top_idxs.dtype not in (torch.int32, torch.int64):
         raise TypeError("top_idxs must be int32 or int64")
     if top_vals.dtype not in (torch.float32, torch.bfloat16):
         raise TypeError("top_vals must be float32 or bfloat16")
-    K = top_idxs.shape[1]
-    if not 1 <= K <= 32:
-        raise ValueError(f"{K} ids per token: 1 to 32")
-    _on_gpu(x.device, x=x, top_idxs=top_idxs, top_vals=top_vals, w13=w13.q, w2=w2.q)
+    if status is not None and (status.dtype != torch.int32 or status.numel() != 1 or not status.is_pinned()):
+        raise ValueError("status must be one pinned int32")
+    if not 0 <= first_expert < 1 << 31:
+        raise ValueError(f"first_expert = {first_expert} must be an expert's id")
+    _on_gpu(dev, top_idxs=top_idxs, top_vals=top_vals)
     y = torch.empty((T, H), dtype=torch.bfloat16, device=x.device)
     if T == 0:
         return y
     ids, vals = top_idxs.contiguous(), top_vals.contiguous()
-    if T * K <= N.W8A8_LAYER_MAX_ROWS and max(T * H, T * K * F) <= N.W8A8_LAYER_MAX_VALUES:
-        # A few tokens: no routing, packing or sum of their own.
-        need = _layer_scratch_bytes(T, H, F, El, K)
+    if need is not None:  # a few tokens: no routing, packing or sum of their own
         scratch = torch.empty(need, dtype=torch.uint8, device=x.device)
         x = x.contiguous()
         p = N.W8A8LayerParams(T, H, F, El, K, first_expert, ids.dtype == torch.int64, vals.dtype == torch.bfloat16, 0,

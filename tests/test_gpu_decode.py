@@ -11,6 +11,7 @@ leave a relative error of at most sqrt(2/3) * 2^-8 < 2^-8 in the 2-norm."""
 import pytest
 import torch
 
+from nvshmem_testing_b200 import _native as N
 from nvshmem_testing_b200 import decode
 
 pytestmark = pytest.mark.gpu
@@ -172,6 +173,27 @@ def test_strides_and_given_output():
     y = decode.moe_layer(wide[:, ::2], idt.t(), vals.t().contiguous().t(), w13, w2, out=rows[1:8])
     assert torch.equal(y, ref)
     assert bool((rows[0] == 5).all()) and bool((rows[8] == 5).all())
+
+
+def test_misaligned_and_misplaced_tensors_are_refused():
+    x, ids, vals, w13, w2 = make(4, 128, 4, 2, 64, 1)
+    flat = torch.zeros(4 * 128 + 8, dtype=torch.bfloat16, device="cuda")
+    odd = flat[1:1 + 4 * 128].view(4, 128)  # contiguous, 2 bytes off
+    with pytest.raises(N.MoeEpError):
+        decode.moe_layer(odd, ids, vals, w13, w2)
+    with pytest.raises(N.MoeEpError):
+        decode.moe_layer(x, ids, vals, w13, w2, out=odd)
+    for bad in (dict(w13=w13.cpu()), dict(w2=w2.transpose(1, 2)), dict(top_vals=vals.cpu()), dict(first_expert=-1),
+                dict(first_expert=1 << 31), dict(top_vals=vals.half()), dict(top_idxs=ids.float()),
+                dict(top_idxs=ids[:3]), dict(out=x[:, :64])):
+        with pytest.raises((ValueError, TypeError)):
+            decode.moe_layer(**{**dict(x=x, top_idxs=ids, top_vals=vals, w13=w13, w2=w2), **bad})
+    with pytest.raises(ValueError):
+        decode.moe_layer(x.repeat(20, 1), ids.repeat(20, 1), vals.repeat(20, 1), w13, w2)  # 80 tokens
+    rw = torch.zeros(128, 8, dtype=torch.bfloat16, device="cuda")
+    for k, r in ((0, rw), (9, rw), (2, rw[:, :6]), (2, rw[:64]), (2, rw.cpu())):
+        with pytest.raises(ValueError):
+            decode.routed_layer(x, r, k, w13, w2)
 
 
 def test_captured_and_replayed_beside_eager_calls():

@@ -131,6 +131,8 @@ PRODUCTS = [
     (1040, 328, [2, 0, 4, 1, 5, 0, 4]),
     (6128, 256, [4, 0, 0, 12]),
     (6160, 256, [16]),
+    (2048, 136, [9, 0, 14, 9]),
+    (3088, 136, [5, 0, 14, 13]),
     (256, 4096, [1500, 2000, 1300]),   # whole tiles
     (512, 1536, [4090, 3841]),
 ]
@@ -277,6 +279,9 @@ LAYERS = [
     (8, 1040, 2, 2, 0, 2, 96),
     (16, 256, 2, 4, 1, 1, 80),
     (17, 256, 2, 4, 1, 1, 80),
+    (4, 2048, 20, 20, 0, 8, 1408),
+    (32, 272, 3, 5, 1, 1, 112),
+    (33, 272, 3, 5, 1, 1, 112),
     (3, 144, 8, 8, 0, 2, 112),
     (40, 256, 8, 32, 16, 6, 208),
     (65, 512, 16, 16, 0, 4, 384),
@@ -307,6 +312,31 @@ def test_layer(T, H, El, E, first, K, F):
         assert torch.equal(y, w8a8.moe_layer(x, i, v, w13, w2, first_expert=first))
     if K > 1 and T > 2:
         assert not y[1].any()
+
+
+def test_misaligned_and_misplaced_tensors_are_refused():
+    xq, xs, wq, ws = make(5, 64, 32, 2, 1)
+    cd = torch.tensor([2, 3], dtype=torch.int32, device="cuda")
+    w = w8a8.QuantWeights(wq, ws)
+    flat = torch.zeros(5 * 64 + 16, dtype=torch.int8, device="cuda")
+    with pytest.raises(N.MoeEpError):
+        w8a8.grouped_gemm(flat[1:1 + 5 * 64].view(5, 64), xs, w, cd)
+    for bad in (w8a8.QuantWeights(wq, ws.cpu()), w8a8.QuantWeights(wq.cpu(), ws),
+                w8a8.QuantWeights(wq.transpose(1, 2).contiguous().transpose(1, 2), ws)):
+        with pytest.raises(ValueError):
+            w8a8.grouped_gemm(xq, xs, bad, cd)
+    with pytest.raises(ValueError):
+        w8a8.grouped_gemm(xq, xs.cpu(), w, cd)
+    with pytest.raises(ValueError):
+        w8a8.grouped_gemm(xq, xs, w, cd.cpu())
+    x = torch.zeros(3, 64, dtype=torch.bfloat16, device="cuda")
+    ids, vals = torch.zeros(3, 1, dtype=torch.int64, device="cuda"), torch.ones(3, 1, device="cuda")
+    w2 = w8a8.QuantWeights(torch.zeros(2, 64, 16, dtype=torch.int8, device="cuda"), torch.ones(2, 64, device="cuda"))
+    w8a8.moe_layer(x, ids, vals, w, w2)
+    for bad in (dict(w2=w8a8.QuantWeights(w2.q, w2.scale.cpu())), dict(top_vals=vals.cpu()), dict(first_expert=-1),
+                dict(top_idxs=ids[:2]), dict(x=x[:, :32]), dict(top_vals=vals.double())):
+        with pytest.raises((ValueError, TypeError)):
+            w8a8.moe_layer(**{**dict(x=x, top_idxs=ids, top_vals=vals, w13=w, w2=w2), **bad})
 
 
 def test_layer_captured_and_on_streams():
