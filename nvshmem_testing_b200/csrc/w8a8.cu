@@ -777,26 +777,27 @@ __device__ __forceinline__ int dot16(uint4 a, uint4 b, int c) {
 
 // The loads of one round: kRwLoads vectors of 16 bytes per lane in all.
 constexpr int kRwLoads = 4;
-template <bool GLU>
+template <bool DUAL>
 __device__ __forceinline__ void rw_load(const uint4* w, const uint4* w2, int v0, int V, int lane,
                                         uint4 (&buf)[kRwLoads]) {
-  constexpr int U = GLU ? kRwLoads / 2 : kRwLoads;
+  constexpr int U = DUAL ? kRwLoads / 2 : kRwLoads;
 #pragma unroll
   for (int j = 0; j < U; ++j) {
     const int v = v0 + j * 32 + lane;
     const bool in = v < V;
     buf[j] = in ? ld_nc_v4(w + v) : make_uint4(0, 0, 0, 0);
-    if constexpr (GLU) buf[U + j] = in ? ld_nc_v4(w2 + v) : make_uint4(0, 0, 0, 0);
+    if constexpr (DUAL) buf[U + j] = in ? ld_nc_v4(w2 + v) : make_uint4(0, 0, 0, 0);
   }
 }
 
-// One channel's sums over K for the rows of chunk c.  buf holds the first
-// round's loads and leaves with those of the next channel (null: none).
-template <bool GLU, int NR>
+// One channel's (DUAL: two channels') sums over K for the rows of chunk c.
+// buf holds the first round's loads and leaves with those of the next channel
+// (null: none).
+template <bool DUAL, int NR>
 __device__ __forceinline__ void rw_channel(const RwSmem& sm, const uint4* rows, int V, int c, const uint4* w,
                                            const uint4* w2, const uint4* nw, const uint4* nw2,
                                            uint4 (&buf)[kRwLoads], int (&s)[NR], int (&s2)[NR]) {
-  constexpr int U = GLU ? kRwLoads / 2 : kRwLoads;
+  constexpr int U = DUAL ? kRwLoads / 2 : kRwLoads;
   const int lane = threadIdx.x & 31, r0 = sm.r0[c], last = sm.n[c] - 1;  // NR > n: the last row again
   const uint4* row[NR];
 #pragma unroll
@@ -808,7 +809,7 @@ __device__ __forceinline__ void rw_channel(const RwSmem& sm, const uint4* rows, 
   for (int v0 = 0; v0 < V; v0 += 32 * U) {
     uint4 next[kRwLoads];
     const bool end = v0 + 32 * U >= V;
-    rw_load<GLU>(end ? nw : w, end ? nw2 : w2, end ? 0 : v0 + 32 * U, end && nw == nullptr ? 0 : V, lane, next);
+    rw_load<DUAL>(end ? nw : w, end ? nw2 : w2, end ? 0 : v0 + 32 * U, end && nw == nullptr ? 0 : V, lane, next);
 #pragma unroll
     for (int j = 0; j < U; ++j) {
       const int v = min(v0 + j * 32 + lane, V - 1);  // (past the end the weights are zeros)
@@ -816,7 +817,7 @@ __device__ __forceinline__ void rw_channel(const RwSmem& sm, const uint4* rows, 
       for (int r = 0; r < NR; ++r) {
         const uint4 x = row[r][v];
         s[r] = dot16(buf[j], x, s[r]);
-        if constexpr (GLU) s2[r] = dot16(buf[U + j], x, s2[r]);
+        if constexpr (DUAL) s2[r] = dot16(buf[U + j], x, s2[r]);
       }
     }
 #pragma unroll
@@ -825,7 +826,7 @@ __device__ __forceinline__ void rw_channel(const RwSmem& sm, const uint4* rows, 
 #pragma unroll
   for (int r = 0; r < NR; ++r) {
     s[r] = __reduce_add_sync(0xffffffffu, s[r]);
-    if constexpr (GLU) s2[r] = __reduce_add_sync(0xffffffffu, s2[r]);
+    if constexpr (DUAL) s2[r] = __reduce_add_sync(0xffffffffu, s2[r]);
   }
 }
 
@@ -946,8 +947,12 @@ __device__ __forceinline__ void rw_table_ids(const RwArgs& a, RwSmem& sm, int la
   }
 }
 
-template <bool GLU, bool SUM>
+// PAIR: a warp takes two neighbouring channels at a time (two up to a row of
+// the table; F even), so that a row's values are read from shared memory once
+// for both.
+template <bool GLU, bool SUM, bool PAIR>
 __global__ void __launch_bounds__(kRwThreads, 2) w8a8_rows_kernel(const __grid_constant__ RwArgs a) {
+  constexpr bool DUAL = GLU || PAIR;
   extern __shared__ __align__(16) unsigned char rw_rows[];
   __shared__ RwSmem sm;
   const int warp = int(threadIdx.x) >> 5, lane = threadIdx.x & 31;
@@ -957,26 +962,27 @@ __global__ void __launch_bounds__(kRwThreads, 2) w8a8_rows_kernel(const __grid_c
   }
   __syncthreads();
   const int V = a.K / 16, warps = int(gridDim.x) * (kRwThreads / 32), chunks = sm.chunks;
+  const int cols = PAIR ? a.F / 2 : a.F;
   // This warp's (chunk, channel) pairs: chunk by chunk, or (SUM) every chunk
   // of a channel, then the next channel.
   int c = 0, f = int(blockIdx.x) * (kRwThreads / 32) + warp;
   auto settle = [&](int& cc, int& ff) {  // whether the pair exists; channels past a chunk's last go to the next chunk
     if constexpr (!SUM) {
-      while (ff >= a.F && cc < chunks) {
-        ff -= a.F;
+      while (ff >= cols && cc < chunks) {
+        ff -= cols;
         ++cc;
       }
     }
-    return cc < chunks && ff < a.F;
+    return cc < chunks && ff < cols;
   };
   auto weights = [&](int cc, int ff) {
-    return reinterpret_cast<const uint4*>(a.wq) + (int64_t(sm.e[cc]) * a.N + ff) * V;
+    return reinterpret_cast<const uint4*>(a.wq) + (int64_t(sm.e[cc]) * a.N + (PAIR ? 2 * ff : ff)) * V;
   };
   uint4 buf[kRwLoads];
   bool more = settle(c, f);
   const uint4* w = more ? weights(c, f) : nullptr;
-  const int64_t up = int64_t(a.F) * V;  // from a gate channel to its up channel
-  if (more) rw_load<GLU>(w, w + up, 0, V, lane, buf);
+  const int64_t second = GLU ? int64_t(a.F) * V : V;  // to the up channel, or the pair's other one
+  if (more) rw_load<DUAL>(w, w + second, 0, V, lane, buf);
   if (a.x != nullptr) {
     if (a.x_f32) rw_quantize<float>(a, sm, rw_rows, sm.rows);
     else rw_quantize<__nv_bfloat16>(a, sm, rw_rows, sm.rows);
@@ -987,10 +993,22 @@ __global__ void __launch_bounds__(kRwThreads, 2) w8a8_rows_kernel(const __grid_c
   }
   __syncthreads();
   const uint4* rows = reinterpret_cast<const uint4*>(rw_rows);
-  float y = 0.f;  // SUM: lane t's token
+  auto store = [&](int row, int ff, float v, float v2) {  // one value, or a pair's two
+    const int64_t at = int64_t(row) * a.F + (PAIR ? 2 * ff : ff);
+    if (a.out_f32) {
+      float* o = static_cast<float*>(a.out) + at;
+      if constexpr (PAIR) *reinterpret_cast<float2*>(o) = make_float2(v, v2);
+      else *o = v;
+    } else {
+      __nv_bfloat16* o = static_cast<__nv_bfloat16*>(a.out) + at;
+      if constexpr (PAIR) *reinterpret_cast<__nv_bfloat162*>(o) = __floats2bfloat162_rn(v, v2);
+      else *o = __float2bfloat16_rn(v);
+    }
+  };
+  float y = 0.f, y2 = 0.f;  // SUM: lane t's token
   if (SUM && chunks == 0) {  // no token has an expert here
-    for (; f < a.F; f += warps)
-      if (lane < a.T) static_cast<__nv_bfloat16*>(a.out)[int64_t(lane) * a.F + f] = __float2bfloat16_rn(0.f);
+    for (; f < cols; f += warps)
+      if (lane < a.T) store(lane, f, 0.f, 0.f);
   }
 #pragma unroll 1
   while (more) {
@@ -1003,24 +1021,24 @@ __global__ void __launch_bounds__(kRwThreads, 2) w8a8_rows_kernel(const __grid_c
     }
     more = settle(nc, nf);
     const uint4* nw = more ? weights(nc, nf) : nullptr;
-    const float* sw = a.ws + int64_t(sm.e[c]) * a.N + f;
-    const float g = sw[0], u = GLU ? sw[a.F] : 0.f;
+    const float* sw = a.ws + int64_t(sm.e[c]) * a.N + (PAIR ? 2 * f : f);
+    const float g = sw[0], u = DUAL ? sw[GLU ? a.F : 1] : 0.f;
     auto channel = [&](auto nr) {
       constexpr int NR = decltype(nr)::value;
       int s[NR], s2[NR];
-      rw_channel<GLU, NR>(sm, rows, V, c, w, w + up, nw, nw + up, buf, s, s2);
+      rw_channel<DUAL, NR>(sm, rows, V, c, w, w + second, nw, nw + second, buf, s, s2);
       const int r0 = sm.r0[c], n = sm.n[c];
 #pragma unroll
       for (int r = 0; r < NR; ++r) {
         if (r >= n) break;
-        const float x = sm.scale[sm.src[r0 + r]], z = float(s[r]) * x * g;
+        const float x = sm.scale[sm.src[r0 + r]], z = float(s[r]) * x * g, z2 = float(s2[r]) * x * u;
         if constexpr (SUM) {
-          if (lane == sm.tok[r0 + r]) y = fmaf(sm.val[r0 + r], z, y);
+          if (lane == sm.tok[r0 + r]) {
+            y = fmaf(sm.val[r0 + r], z, y);
+            if constexpr (PAIR) y2 = fmaf(sm.val[r0 + r], z2, y2);
+          }
         } else if (lane == r) {
-          const float v = GLU ? silu_mul(z, float(s2[r]) * x * u) : z;
-          const int64_t at = int64_t(r0 + r) * a.F + f;
-          if (a.out_f32) static_cast<float*>(a.out)[at] = v;
-          else static_cast<__nv_bfloat16*>(a.out)[at] = __float2bfloat16_rn(v);
+          store(r0 + r, f, GLU ? silu_mul(z, z2) : z, z2);
         }
       }
     };
@@ -1029,8 +1047,8 @@ __global__ void __launch_bounds__(kRwThreads, 2) w8a8_rows_kernel(const __grid_c
     else if (n == 2) channel(std::integral_constant<int, 2>{});
     else channel(std::integral_constant<int, 4>{});
     if (SUM && nf != f) {
-      if (lane < a.T) static_cast<__nv_bfloat16*>(a.out)[int64_t(lane) * a.F + f] = __float2bfloat16_rn(y);
-      y = 0.f;
+      if (lane < a.T) store(lane, f, y, y2);
+      y = y2 = 0.f;
     }
     c = nc;
     f = nf;
@@ -1215,23 +1233,40 @@ int w8a8_pairs(int dev, int sms, cudaLaunchConfig_t cfg, int* out) {
   return kOk;
 }
 
-// The form for a handful of rows: they have to fit shared memory twice per SM.
+// The form for a handful of rows: they have to fit shared memory twice per SM,
+// and an expert's to be taken in one pass as a rule (21 rows over 8 experts of
+// 14336 x 4096: 87.7 us against 80.5 with the tiles; 16 rows 55.9 against
+// 56.1; 32 over 64 experts of 2816 x 2048: 29.7 against 36.3; one expert of
+// 4096 x 7168 with 4 rows 10.7 against 13.1, with 6 rows 14.7 against 13.4).
+bool one_pass(int64_t rows, int E) { return rows <= kRwRows || rows <= 2 * int64_t(E); }
 bool fresh(int64_t rows, int K) { return rows <= kRwMaxFreshRows && rows * K <= kRwMaxFresh; }
-bool rows_form(int64_t rows, int K) { return rows <= kRwMaxRows && rows * K <= int64_t(kRwMaxSmem); }
+bool rows_form(int64_t rows, int K, int E) {
+  return rows <= kRwMaxRows && rows * K <= int64_t(kRwMaxSmem) && one_pass(rows, E);
+}
 
-template <bool GLU, bool SUM>
-int launch_rows(const RwArgs& a, int staged, int64_t items, int dev, int sms, cudaStream_t stream) {
+template <bool GLU, bool SUM, bool PAIR>
+int launch_rows_as(const RwArgs& a, int staged, int64_t items, int dev, int sms, cudaStream_t stream) {
   static std::atomic<bool> ready[kMaxDevices];
   if (dev < 0 || dev >= kMaxDevices) return kCudaErr;
   if (!ready[dev].load(std::memory_order_acquire)) {
-    if (cudaFuncSetAttribute(w8a8_rows_kernel<GLU, SUM>, cudaFuncAttributeMaxDynamicSharedMemorySize,
+    if (cudaFuncSetAttribute(w8a8_rows_kernel<GLU, SUM, PAIR>, cudaFuncAttributeMaxDynamicSharedMemorySize,
                              int(kRwMaxSmem)) != cudaSuccess)
       return kCudaErr;
     ready[dev].store(true, std::memory_order_release);
   }
   const int64_t blocks = std::min<int64_t>((items + kRwThreads / 32 - 1) / (kRwThreads / 32), 2 * int64_t(sms));
-  w8a8_rows_kernel<GLU, SUM><<<unsigned(blocks), kRwThreads, size_t(staged) * a.K, stream>>>(a);
+  w8a8_rows_kernel<GLU, SUM, PAIR><<<unsigned(blocks), kRwThreads, size_t(staged) * a.K, stream>>>(a);
   return cudaGetLastError() == cudaSuccess ? kOk : kCudaErr;
+}
+template <bool GLU, bool SUM>
+int launch_rows(const RwArgs& a, int staged, int64_t items, int dev, int sms, cudaStream_t stream) {
+  if constexpr (!GLU) {
+    // Pairs of channels where rows share an expert and they still occupy
+    // every warp: with several rows the shared memory reads bound the form.
+    if (staged > 1 && items / 2 >= 2 * int64_t(sms) * (kRwThreads / 32))
+      return launch_rows_as<GLU, SUM, true>(a, staged, items / 2, dev, sms, stream);
+  }
+  return launch_rows_as<GLU, SUM, false>(a, staged, items, dev, sms, stream);
 }
 
 template <bool GLU, bool SPLIT>
@@ -1288,9 +1323,9 @@ struct QScratch {
   bool few, split, rows_outside;
   size_t xq, xs, total;
 };
-QScratch q_scratch(int64_t rows, int K, int N, bool glu, bool with_x, int sms) {
+QScratch q_scratch(int64_t rows, int K, int N, int E, bool glu, bool with_x, int sms) {
   QScratch q;
-  q.few = rows_form(rows, K);
+  q.few = rows_form(rows, K, E);
   q.split = !q.few && q_split(rows, N, glu ? N / 2 : N, glu, sms / 2);
   q.rows_outside = with_x && !(q.few && fresh(rows, K));
   q.xq = q.split ? size_t(sms / 2) * 2 * kQSlotInts * 4 : 0;
@@ -1305,7 +1340,7 @@ extern "C" int moe_w8a8_scratch_bytes(int64_t rows, int32_t K, int32_t N, int32_
   if (!out || !q_sizes_ok(rows, K, N, E, swiglu)) return kBadArg;
   int sms = 0;
   if (cudaDeviceGetAttribute(&sms, cudaDevAttrMultiProcessorCount, device) != cudaSuccess) return kCudaErr;
-  *out = q_scratch(rows, K, N, swiglu != 0, with_x != 0, sms).total;
+  *out = q_scratch(rows, K, N, E, swiglu != 0, with_x != 0, sms).total;
   return kOk;
 }
 
@@ -1321,7 +1356,7 @@ extern "C" int moe_w8a8_gemm(const moe_w8a8_params* p, void* stream) {
   int sms = 0, dev = 0;
   if (sm_count(&sms, &dev) != kOk) return kCudaErr;
   const bool glu = p->swiglu != 0;
-  const QScratch sc = q_scratch(p->rows, p->K, p->N, glu, p->x != nullptr, sms);
+  const QScratch sc = q_scratch(p->rows, p->K, p->N, p->experts, glu, p->x != nullptr, sms);
   unsigned char* scratch = static_cast<unsigned char*>(p->scratch);
   if (sc.total > 0 && (!scratch || p->scratch_bytes < sc.total)) return kBadArg;
   const int8_t* xq = static_cast<const int8_t*>(p->xq);

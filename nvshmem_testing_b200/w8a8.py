@@ -224,7 +224,10 @@ def _layer_dims(x, ids, vals, q13, q2) -> tuple[int, int, int | None]:
     K = ids[1]
     if not 1 <= K <= 32:
         raise ValueError(f"{K} ids per token: 1 to 32")
-    if T * K > N.W8A8_LAYER_MAX_ROWS or max(T * H, T * K * F) > N.W8A8_LAYER_MAX_VALUES:
+    # Few rows per expert (four tokens at most, or two per expert on average);
+    # T = 0 returns before it matters.
+    if (T == 0 or T * K > N.W8A8_LAYER_MAX_ROWS or max(T * H, T * K * F) > N.W8A8_LAYER_MAX_VALUES
+            or (T > 4 and T * K > 2 * El)):
         return T, K, None
     need = ctypes.c_size_t()
     N.check(N.lib().moe_w8a8_layer_scratch_bytes(T, H, F, El, K, ctypes.byref(need)), "moe_w8a8_layer_scratch_bytes")

@@ -132,7 +132,8 @@ PRODUCTS = [
     (6128, 256, [4, 0, 0, 12]),
     (6160, 256, [16]),
     (2048, 136, [9, 0, 14, 9]),
-    (3088, 136, [5, 0, 14, 13]),
+    (3088, 136, [5, 0, 14, 13] + [0] * 12),
+    (1040, 4096, [1, 4, 3, 2, 0, 7]),
     (256, 4096, [1500, 2000, 1300]),   # whole tiles
     (512, 1536, [4090, 3841]),
 ]
@@ -277,10 +278,10 @@ LAYERS = [
     (4, 336, 3, 3, 0, 3, 144),
     (5, 256, 2, 2, 0, 2, 128),
     (8, 1040, 2, 2, 0, 2, 96),
-    (16, 256, 2, 4, 1, 1, 80),
+    (16, 256, 8, 10, 1, 1, 80),
     (17, 256, 2, 4, 1, 1, 80),
     (4, 2048, 20, 20, 0, 8, 1408),
-    (32, 272, 3, 5, 1, 1, 112),
+    (32, 272, 16, 20, 1, 1, 112),
     (33, 272, 3, 5, 1, 1, 112),
     (3, 144, 8, 8, 0, 2, 112),
     (40, 256, 8, 32, 16, 6, 208),
