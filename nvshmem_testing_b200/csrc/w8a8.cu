@@ -76,8 +76,8 @@ struct QRowMaps {
 };
 
 // ---------------------------------------------------------------- quantisation of one row
-// Rounds x / s half to even, exactly: |x / s| <= 127.5, inv = 1 / s rounded.
-// t holds the nearest integer of x * inv (within one of the answer) in its
+// Rounds x / s half to even, exactly: |x / s| <= 127.5, inv is 1 / s within
+// 2^-23.  t holds the nearest integer of x * inv (within one of the answer) in its
 // low mantissa bits; the remainder x - q*s fits fp32.
 constexpr float kMagic = 12582912.f;  // 1.5 * 2^23
 __device__ __forceinline__ int quant_one(float x, float s, float half, float inv) {
@@ -90,26 +90,29 @@ __device__ __forceinline__ int quant_one(float x, float s, float half, float inv
   return max(-127, min(127, q));
 }
 
-// Eight values.  x * inv is within 127 * 2^-24 < 1e-5 of the quotient, so its
-// rounding is the quotient's unless it lies nearer than that to a tie: only
+// Values by fours and eights.  inv and the product are each off by 2^-23 of
+// themselves at most, so x * inv is within 127 * 2^-22 < 4e-5 of the quotient
+// and its rounding is the quotient's unless that lies nearer to a tie: only
 // then (bf16 rows: about 1 value in 500, half the row's maximum among them)
 // the exact form runs.  t's low byte is the integer in two's complement.
-__device__ __forceinline__ uint2 quant8(const float (&x)[8], float s, float inv, bool exact) {
-  uint32_t t[8];
+__device__ __forceinline__ uint32_t quant4(const float* x, float s, float inv, bool exact) {
+  uint32_t t[4];
   float far = exact ? 1.f : 0.f;
 #pragma unroll
-  for (int i = 0; i < 8; ++i) {
+  for (int i = 0; i < 4; ++i) {
     const float y = fmaf(x[i], inv, kMagic);
     far = fmaxf(far, fabsf(fmaf(x[i], inv, kMagic - y)));
     t[i] = __float_as_uint(y);
   }
-  if (far > 0.49999f) {
+  if (far > 0.49995f) {
     const float half = 0.5f * s;
 #pragma unroll
-    for (int i = 0; i < 8; ++i) t[i] = uint32_t(quant_one(x[i], s, half, inv));
+    for (int i = 0; i < 4; ++i) t[i] = uint32_t(quant_one(x[i], s, half, inv));
   }
-  return make_uint2(__byte_perm(__byte_perm(t[0], t[1], 0x0040), __byte_perm(t[2], t[3], 0x0040), 0x5410),
-                    __byte_perm(__byte_perm(t[4], t[5], 0x0040), __byte_perm(t[6], t[7], 0x0040), 0x5410));
+  return __byte_perm(__byte_perm(t[0], t[1], 0x0040), __byte_perm(t[2], t[3], 0x0040), 0x5410);
+}
+__device__ __forceinline__ uint2 quant8(const float (&x)[8], float s, float inv, bool exact) {
+  return make_uint2(quant4(x, s, inv, exact), quant4(x + 4, s, inv, exact));
 }
 
 __device__ __forceinline__ void load8(const __nv_bfloat16* p, float (&v)[8]) {
@@ -142,7 +145,7 @@ struct RowScale {
     tiny = scale < 0x1p-90f;
     up = tiny ? 0x1p100f : 1.f;
     s = zero ? 1.f : scale * up;
-    inv = 1.f / s;
+    inv = __fdividef(1.f, s);
   }
   __device__ __forceinline__ uint2 round8(float (&w)[8]) const {
     if (zero) return make_uint2(0u, 0u);
@@ -154,7 +157,30 @@ struct RowScale {
   }
 };
 
-// Eight values as they lie in memory, and their largest magnitude's fp32 bits.
+// The largest magnitude of values as they come, NaN above infinity.
+template <typename In>
+struct RowTop;
+template <>
+struct RowTop<__nv_bfloat16> {
+  __nv_bfloat162 m = __floats2bfloat162_rn(0.f, 0.f);
+  __device__ __forceinline__ void add(uint32_t w) {
+    m = __hmax2_nan(m, __habs2(*reinterpret_cast<const __nv_bfloat162*>(&w)));
+  }
+  __device__ __forceinline__ uint32_t bits() const {
+    const uint32_t w = *reinterpret_cast<const uint32_t*>(&m);
+    return max(w << 16, w & 0xffff0000u);
+  }
+};
+template <>
+struct RowTop<float> {
+  float m = 0.f;
+  __device__ __forceinline__ void add(uint32_t w) {
+    asm("max.NaN.f32 %0, %0, %1;" : "+f"(m) : "f"(fabsf(__uint_as_float(w))));
+  }
+  __device__ __forceinline__ uint32_t bits() const { return __float_as_uint(m); }
+};
+
+// Eight values as they lie in memory.
 template <typename In>
 struct Raw8 {
   uint4 r[sizeof(In) / 2];
@@ -162,18 +188,14 @@ struct Raw8 {
 #pragma unroll
     for (int i = 0; i < int(sizeof(In) / 2); ++i) r[i] = ld_nc_v4(reinterpret_cast<const uint4*>(p) + i);
   }
-  __device__ __forceinline__ uint32_t top() const {
-    uint32_t t = 0;
+  __device__ __forceinline__ void top(RowTop<In>& t) const {
 #pragma unroll
     for (int i = 0; i < int(sizeof(In) / 2); ++i) {
-      const uint32_t w[4] = {r[i].x, r[i].y, r[i].z, r[i].w};
-#pragma unroll
-      for (int j = 0; j < 4; ++j) {
-        if constexpr (sizeof(In) == 2) t = max(t, max(w[j] & 0x7fff0000u, (w[j] << 16) & 0x7fffffffu));
-        else t = max(t, w[j] & 0x7fffffffu);
-      }
+      t.add(r[i].x);
+      t.add(r[i].y);
+      t.add(r[i].z);
+      t.add(r[i].w);
     }
-    return t;
   }
   __device__ __forceinline__ void values(float (&v)[8]) const {
 #pragma unroll
@@ -191,13 +213,6 @@ struct Raw8 {
     }
   }
 };
-
-__device__ __forceinline__ uint32_t top8(const float (&v)[8]) {
-  uint32_t top = 0;
-#pragma unroll
-  for (int i = 0; i < 8; ++i) top = max(top, __float_as_uint(v[i]) & 0x7fffffffu);
-  return top;
-}
 
 struct alignas(16) QSmem {
   uint64_t full[kQStages];   // leader: both CTAs' bytes
@@ -839,14 +854,14 @@ __device__ __forceinline__ void rw_quantize(const RwArgs& a, RwSmem& sm, unsigne
   const int live = a.live ? min(max(*a.live, 0), count) : count;
   const bool on = r < live;
   const In* src = static_cast<const In*>(a.x) + int64_t(on ? (a.perm ? a.perm[r] : r) : 0) * a.K;
-  uint32_t top = 0;
+  RowTop<In> seen;
 #pragma unroll 4
   for (int g = c; g < groups && on; g += per) {
     Raw8<In> v;
     v.load(src + g * 8);
-    top = max(top, v.top());
+    v.top(seen);
   }
-  top = __reduce_max_sync(0xffffffffu, top);
+  uint32_t top = __reduce_max_sync(0xffffffffu, seen.bits());
   if ((threadIdx.x & 31) == 0) sm.top[threadIdx.x >> 5] = top;
   __syncthreads();
 #pragma unroll 4
@@ -855,8 +870,10 @@ __device__ __forceinline__ void rw_quantize(const RwArgs& a, RwSmem& sm, unsigne
   if (c == 0 && on) sm.scale[r] = rs.scale;
 #pragma unroll 1
   for (int g = c; g < groups && on; g += per) {
+    Raw8<In> raw;
+    raw.load(src + g * 8);
     float v[8];
-    load8(src + g * 8, v);
+    raw.values(v);
     *reinterpret_cast<uint2*>(rows + r * a.K + g * 8) = rs.round8(v);
   }
 }
@@ -1076,21 +1093,22 @@ __global__ void __launch_bounds__(kQuantThreads)
     const bool on = r < live;
     const In* src = x + (on ? (perm ? int64_t(perm[r]) : r) : 0) * K;
     Raw8<In> v[VPT];
-    uint32_t top = 0;
+    RowTop<In> seen;
     if (on) {
 #pragma unroll
       for (int j = 0; j < VPT; ++j)
         if (c + j * tpr < groups) v[j].load(src + (c + j * tpr) * 8);
 #pragma unroll
       for (int j = 0; j < VPT; ++j)
-        if (c + j * tpr < groups) top = max(top, v[j].top());
+        if (c + j * tpr < groups) v[j].top(seen);
+#pragma unroll 1
       for (int g = c + VPT * tpr; g < groups; g += tpr) {
-        float w[8];
-        load8(src + g * 8, w);
-        top = max(top, top8(w));
+        Raw8<In> w;
+        w.load(src + g * 8);
+        w.top(seen);
       }
     }
-    top = __reduce_max_sync(0xffffffffu, top);
+    uint32_t top = __reduce_max_sync(0xffffffffu, seen.bits());
     if (tpr > 32) {
       __syncthreads();  // the last round's maxima have been read
       if ((threadIdx.x & 31) == 0) top_s[threadIdx.x >> 5] = top;
@@ -1110,9 +1128,12 @@ __global__ void __launch_bounds__(kQuantThreads)
         v[j].values(w);
         put(c + j * tpr, w);
       }
+#pragma unroll 1
     for (int g = c + VPT * tpr; g < groups; g += tpr) {
+      Raw8<In> raw;
+      raw.load(src + g * 8);
       float w[8];
-      load8(src + g * 8, w);
+      raw.values(w);
       put(g, w);
     }
   }
