@@ -69,7 +69,6 @@ struct DecArgs {
   int stages;
   uint32_t stage_bytes, scratch_bytes;
   int maxact;                // min(E, T * K)
-  int w2_atoms;              // w2 described in atoms of 64 features (H % 64 == 0)
   const __nv_bfloat16* x;
   const void* ids;
   const void* vals;
@@ -132,6 +131,16 @@ __device__ __noinline__ void dec_fail(DecSmem& sm, const DecArgs& a, int detail)
 __device__ __forceinline__ int share_lo(uint32_t units, uint32_t g, uint32_t c) { return int(units * c / g); }
 __device__ __forceinline__ int share_owner(uint32_t units, uint32_t g, uint32_t u) {
   return int(((u + 1) * g - 1) / units);
+}
+
+__device__ __forceinline__ float silu_mul(float g, float u) { return g / (1.f + expf(-g)) * u; }
+
+// Adds the values of the lane `o` away to this lane's (the same sum in both).
+__device__ __forceinline__ void add_xor(float4& v, int o) {
+  v.x += __shfl_xor_sync(0xffffffffu, v.x, o);
+  v.y += __shfl_xor_sync(0xffffffffu, v.y, o);
+  v.z += __shfl_xor_sync(0xffffffffu, v.z, o);
+  v.w += __shfl_xor_sync(0xffffffffu, v.w, o);
 }
 
 // The sum of parts lo..hi in order, `at(q)` giving part q's address: eight
@@ -594,6 +603,7 @@ struct Ring {
 
 __global__ void __launch_bounds__(kDecThreads, 1)
     decode_kernel(const __grid_constant__ CUtensorMap tm_w13, const __grid_constant__ CUtensorMap tm_w2,
+                  const __grid_constant__ CUtensorMap tm_w2e,
                   const __grid_constant__ CUtensorMap tm_x, const __grid_constant__ CUtensorMap tm_h,
                   const __grid_constant__ DecArgs a) {
   extern __shared__ unsigned char dec_dyn[];
@@ -689,7 +699,11 @@ __global__ void __launch_bounds__(kDecThreads, 1)
       p.chunks = rest / p.cz;
     }
     p.fixed = p.units - p.chunks * p.cz;
-    p.g = min(G, p.fixed);
+    // Short lists: a part costs the one who adds a tile's up about a fifth of
+    // the time of a unit, so about sqrt(tile / 5) units a CTA at least.
+    int least = 1;
+    while (5 * (least + 1) * (least + 1) <= tile && least < 8) ++least;
+    p.g = min(G, max(p.fixed / least, min(p.fixed, 1)));
     const bool on = int(blockIdx.x) < p.g;
     p.lo = on ? share_lo(p.fixed, p.g, blockIdx.x) : 0;
     p.hi = on ? share_lo(p.fixed, p.g, blockIdx.x + 1) : 0;
@@ -752,16 +766,21 @@ __global__ void __launch_bounds__(kDecThreads, 1)
     unsigned char* dst = stage + uint32_t(lr.st) * a.stage_bytes;
     const int e = tb.act_e[c.ai];
     if constexpr (PASS == 1) {
+      // Two boxes of 64 gate and the 64 up features (one of all four atoms
+      // was no faster).
       mbar_arrive_expect_tx(full, kDecABytes + uint32_t(a.NB) * 128);
       tma_load_4d_hint(&tm_w13, full, dst, c.ft * 128, c.k * 64, 0, e, once);
       tma_load_4d_hint(&tm_w13, full, dst + 16384, c.ft * 128 + 64, c.k * 64, 0, e, once);
     } else {
+      // One box of four atoms of 64 features; a tile whose last atom is a part
+      // of one atom by atom, clipped at the row's end.
       mbar_arrive_expect_tx(full, kDecABytes + uint32_t((act_rows(c.ai) + 15) >> 4) * 2048);
-      if (a.w2_atoms) {
+      if (c.ft * 4 + 4 <= a.H / 64) {
         tma_load_4d_hint(&tm_w2, full, dst, 0, c.k * 64, c.ft * 4, e, once);
       } else {
+#pragma unroll 1
         for (int g = 0; g < 4; ++g)
-          tma_load_3d_hint(&tm_w2, full, dst + g * 8192, c.ft * 256 + g * 64, c.k * 64, e, once);
+          tma_load_3d_hint(&tm_w2e, full, dst + g * 8192, c.ft * 256 + g * 64, c.k * 64, e, once);
       }
     }
     sm.fills[lr.st] += 1;
@@ -921,7 +940,7 @@ __global__ void __launch_bounds__(kDecThreads, 1)
             if (j >= n) break;
             const float gv = __uint_as_float(g[q]), uv = __uint_as_float(w[q]);
             if (whole) {
-              if (f < a.F) a.hs[size_t(r0 + j) * a.F + f] = __float2bfloat16_rn(gv / (1.f + expf(-gv)) * uv);
+              if (f < a.F) a.hs[size_t(r0 + j) * a.F + f] = __float2bfloat16_rn(silu_mul(gv, uv));
             } else {
               mine[j * 256 + fl] = gv;
               mine[j * 256 + 128 + fl] = uv;
@@ -935,13 +954,33 @@ __global__ void __launch_bounds__(kDecThreads, 1)
           named_bar_sync(kBarEpi, kDecEpiWarps * 32);
           if (etid == 0) sm.last = atom_add_acq_rel(&a.ctr[c0], 1u) == uint32_t(c1 - c0);
           named_bar_sync(kBarEpi, kDecEpiWarps * 32);
-          if (sm.last && f < a.F) {
+          if (sm.last) {
+            // Four gate or up features a thread, neighbours the same ones;
+            // many parts: four such pairs, a quarter of the parts each.
+            const int np = c1 - c0 + 1, quarters = np > 6 ? 4 : 1, lanes = 2 * quarters;
+            const int upper = lane & 1, qt = quarters == 4 ? (lane >> 1) & 3 : 0;
 #pragma unroll 1
-            for (int j = sub; j < n; j += 2) {
-              const int at = j * 256 + fl;
-              const float gv = sum_parts<float>(c0, c1, [&](int q) { return slot(q, q == c0 ? 1 : 0) + at; });
-              const float uv = sum_parts<float>(c0, c1, [&](int q) { return slot(q, q == c0 ? 1 : 0) + at + 128; });
-              a.hs[size_t(r0 + j) * a.F + f] = __float2bfloat16_rn(gv / (1.f + expf(-gv)) * uv);
+            for (int i0 = (etid & ~31) / lanes; i0 < n * 32; i0 += kDecEpiWarps * 32 / lanes) {
+              const int i = i0 + lane / lanes, j = i >> 5, l4 = (i & 31) * 4, f4 = c.ft * 128 + l4;
+              float4 v = make_float4(0.f, 0.f, 0.f, 0.f);
+              if (j < n)
+                v = sum_parts<float4>(c0 + np * qt / quarters, c0 + np * (qt + 1) / quarters - 1, [&](int q) {
+                  return reinterpret_cast<const float4*>(slot(q, q == c0 ? 1 : 0) + j * 256 + upper * 128 + l4);
+                });
+              if (quarters == 4) {
+                add_xor(v, 2);
+                add_xor(v, 4);
+              }
+              float4 w;
+              w.x = __shfl_xor_sync(0xffffffffu, v.x, 1);
+              w.y = __shfl_xor_sync(0xffffffffu, v.y, 1);
+              w.z = __shfl_xor_sync(0xffffffffu, v.z, 1);
+              w.w = __shfl_xor_sync(0xffffffffu, v.w, 1);
+              if (j < n && upper == 0 && qt == 0 && f4 < a.F) {
+                __nv_bfloat162* o = reinterpret_cast<__nv_bfloat162*>(a.hs + size_t(r0 + j) * a.F + f4);
+                o[0] = __floats2bfloat162_rn(silu_mul(v.x, w.x), silu_mul(v.y, w.y));
+                o[1] = __floats2bfloat162_rn(silu_mul(v.z, w.z), silu_mul(v.w, w.w));
+              }
             }
           }
         }
@@ -1019,12 +1058,7 @@ __global__ void __launch_bounds__(kDecThreads, 1)
         return reinterpret_cast<const float4*>(slot(q, q == c0 ? 1 : 0) + t * 256 + fl);
       });
 #pragma unroll
-      for (int o = 1; o < 4; o <<= 1) {
-        v.x += __shfl_xor_sync(0xffffffffu, v.x, o);
-        v.y += __shfl_xor_sync(0xffffffffu, v.y, o);
-        v.z += __shfl_xor_sync(0xffffffffu, v.z, o);
-        v.w += __shfl_xor_sync(0xffffffffu, v.w, o);
-      }
+      for (int o = 1; o < 4; o <<= 1) add_xor(v, o);
       if (split && f < a.H && qt == 0) {
         __nv_bfloat162* o = reinterpret_cast<__nv_bfloat162*>(a.y + size_t(t) * a.H + f);
         o[0] = __floats2bfloat162_rn(v.x, v.y);
@@ -1209,24 +1243,26 @@ extern "C" int moe_decode_layer(const moe_decode_params* p, void* stream) {
   a.eparts = Er % 32 == 0 && sms >= 8 && (H / (sms / 4) + 1) * xrow <= room ? 4 : 1;
   if (Er && (H / (sms / a.eparts) + 1) * xrow > room) return kBadArg;
 
-  CUtensorMap m13, m2, mx, mh;
+  CUtensorMap m13, m2, m2e, mx, mh;
   {
     const cuuint64_t dims[4] = {cuuint64_t(F), cuuint64_t(H), 2, cuuint64_t(E)};
     const cuuint64_t str[3] = {cuuint64_t(F) * 4, cuuint64_t(F) * 2, cuuint64_t(H) * F * 4};
     const cuuint32_t box[4] = {64, 64, 2, 1};
     if (encode(&m13, 4, p->w13, dims, str, box)) return kCudaErr;
   }
-  a.w2_atoms = H % 64 == 0;
-  if (a.w2_atoms) {
-    const cuuint64_t dims[4] = {64, cuuint64_t(F), cuuint64_t(H / 64), cuuint64_t(E)};
+  {
+    // Whole atoms of 64 features (at least one is described; a row shorter
+    // than one is never read through it).
+    const cuuint64_t dims[4] = {64, cuuint64_t(F), cuuint64_t(H < 64 ? 1 : H / 64), cuuint64_t(E)};
     const cuuint64_t str[3] = {cuuint64_t(H) * 2, 128, cuuint64_t(H) * F * 2};
     const cuuint32_t box[4] = {64, 64, 4, 1};
     if (encode(&m2, 4, p->w2, dims, str, box)) return kCudaErr;
-  } else {
+  }
+  {
     const cuuint64_t dims[3] = {cuuint64_t(H), cuuint64_t(F), cuuint64_t(E)};
     const cuuint64_t str[2] = {cuuint64_t(H) * 2, cuuint64_t(H) * F * 2};
     const cuuint32_t box[3] = {64, 64, 1};
-    if (encode(&m2, 3, p->w2, dims, str, box)) return kCudaErr;
+    if (encode(&m2e, 3, p->w2, dims, str, box)) return kCudaErr;
   }
   {
     const cuuint64_t dims[2] = {cuuint64_t(H), cuuint64_t(T)};
@@ -1259,5 +1295,5 @@ extern "C" int moe_decode_layer(const moe_decode_params* p, void* stream) {
   at[0].val.cooperative = 1;
   cfg.attrs = at;
   cfg.numAttrs = 1;
-  return cudaLaunchKernelEx(&cfg, decode_kernel, m13, m2, mx, mh, a) == cudaSuccess ? kOk : kCudaErr;
+  return cudaLaunchKernelEx(&cfg, decode_kernel, m13, m2, m2e, mx, mh, a) == cudaSuccess ? kOk : kCudaErr;
 }

@@ -426,9 +426,15 @@ __global__ void __launch_bounds__(kQThreads, 1)
   tc_fence_after();
   const uint32_t tmem = __shfl_sync(0xffffffffu, sm.tmem_base, 0);
   const int tiles = s.tpre[a.E] * s.FT;
-  // (The host launches the form with a grid barrier where the rows alone
-  // leave it open; ragged experts may make enough tiles all the same.)
-  const bool split = SPLIT && tiles < kQWaves * pairs;
+  // Splitting saves the last round's idle pairs and costs a barrier and the
+  // parts' way through memory: about 12 stages, and one for every 8 rows of a
+  // tile.  (The host launches the form with a grid barrier where the rows
+  // alone leave it open; ragged experts may make enough tiles all the same.)
+  bool split = false;
+  if (SPLIT && tiles > 0 && tiles < kQWaves * pairs) {
+    const int rounds = (tiles + pairs - 1) / pairs, mean = s.off[a.E] / s.tpre[a.E];
+    split = rounds * s.kb > tiles * s.kb / pairs + 12 + mean / 8;
+  }
 
   if (warp == 0 && lane == 0) {
     // ---- loads: each CTA its 128 channels and half of the tile's rows, all
