@@ -910,6 +910,29 @@ __global__ void __launch_bounds__(kDecThreads, 1)
     eseg.next(2);
   };
 
+  // A short list with many rows per expert: the parts of its few tiles are
+  // too much for one CTA each (56 rows of 20 parts: 64 us), so the grid adds
+  // them up, behind a barrier of its own.
+  const bool spread = nact > 0 && int(tb.act_off[nact]) >= 12 * nact && p1.units < 16 * G;
+  auto join1 = [&](const Pass& p) {
+    const int warps = kDecThreads / 32;
+#pragma unroll 1
+    for (int i = int(blockIdx.x) * warps + warp; i < nact * p.nt * kDecMaxT; i += G * warps) {
+      const int tile = i / kDecMaxT, j = i % kDecMaxT, ai = tile / p.nt, l4 = lane * 4;
+      const int c0 = p.part_of(tile * p.kb), c1 = p.part_of(tile * p.kb + p.kb - 1);
+      const int f = (tile - ai * p.nt) * 128 + l4;
+      if (j >= act_rows(ai) || c0 == c1) continue;
+      auto at = [&](int q) { return reinterpret_cast<const float4*>(slot(q, q == c0 ? 1 : 0) + j * 256 + l4); };
+      const float4 g = sum_parts<float4>(c0, c1, at);
+      const float4 u = sum_parts<float4>(c0, c1, [&](int q) { return at(q) + 32; });
+      if (f < a.F) {
+        __nv_bfloat162* o = reinterpret_cast<__nv_bfloat162*>(a.hs + size_t(tb.act_off[ai] + j) * a.F + f);
+        o[0] = __floats2bfloat162_rn(silu_mul(g.x, u.x), silu_mul(g.y, u.y));
+        o[1] = __floats2bfloat162_rn(silu_mul(g.z, u.z), silu_mul(g.w, u.w));
+      }
+    }
+  };
+
   auto epilogue1 = [&](const Pass& p) {
     first_run(eruns, p);
     do {
@@ -948,7 +971,7 @@ __global__ void __launch_bounds__(kDecThreads, 1)
           }
         }
         seg_done();
-        if (!whole) {
+        if (!whole && !spread) {
           // The part whose ticket is the tile's last adds them all up.
           const int c0 = p.part_of(tile0), c1 = p.part_of(tile0 + p.kb - 1);
           named_bar_sync(kBarEpi, kDecEpiWarps * 32);
@@ -1079,6 +1102,10 @@ __global__ void __launch_bounds__(kDecThreads, 1)
   __syncwarp();
   if (threadIdx.x == 0 && !*reinterpret_cast<volatile int*>(&sm.err)) preload(Pass2{}, p2);
   __syncwarp();
+  if (spread) {
+    grid.sync();
+    join1(p1);
+  }
   fence_proxy_async_global();  // h, written by threads, is read by the TMA
   grid.sync();
   if (!*reinterpret_cast<volatile int*>(&sm.err)) {

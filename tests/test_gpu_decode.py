@@ -83,6 +83,8 @@ SIZES = [
     (64, 1024, 32, 8, 256),
     (64, 256, 64, 16, 128),
     (64, 320, 1, 1, 1000),
+    (56, 5000, 4, 4, 216),
+    (40, 1032, 3, 3, 520),
 ]
 
 
