@@ -25,8 +25,11 @@
 // experts of 352 MB: 410 -> 392 us; 705 MB in all: no gain).  A tile that ends
 // up in several parts is summed from fp32 partials in the order of the list,
 // so results depend neither on timing nor on who did what: in pass 1 by the
-// last of its CTAs (few parts, few rows), in pass 2, where 256 features may
-// be spread over all CTAs, by the whole grid after another barrier.
+// last of its CTAs (few parts, few rows; otherwise by the grid), in pass 2,
+// where 256 features may be spread over all CTAs, by the grid after another
+// barrier.  The grid barriers are cooperative groups': the launch guarantees
+// that all CTAs are resident, every wait of a CTA's own is bounded, and after
+// an error a CTA skips work, not barriers.
 // The weights' first stages of a pass are requested before the barrier in
 // front of it; only the token rows wait for it.
 #include <cooperative_groups.h>

@@ -19,7 +19,9 @@
 // products wait for the weights' bytes alone.  Then the list of (tile, 128 of
 // K) units is split evenly over the pairs at any k, the partial sums go to
 // scratch and, behind a grid barrier, are added and scaled.  Integer sums do
-// not depend on the split.
+// not depend on the split.  (The barrier is cooperative groups', under a
+// cooperative launch; every other wait is bounded, and after an error a CTA
+// skips work, not the barrier.)
 //
 // Quantisation (quant_rows_kernel).  scale = absmax * (1/127) in fp32, q = the
 // exact quotient x / scale rounded half to even: the product with the

@@ -9,7 +9,7 @@ import pytest
 import torch
 
 from nvshmem_testing_b200 import _native as N
-from nvshmem_testing_b200 import utils, w8a8
+from nvshmem_testing_b200 import decode, utils, w8a8
 
 pytestmark = pytest.mark.gpu
 
@@ -367,6 +367,44 @@ def test_layer_captured_and_on_streams():
         eager = w8a8.moe_layer(x, ids, vals, w13, w2)
         torch.cuda.synchronize()
         assert torch.equal(outs[0], eager) and torch.equal(outs[1], eager)
+
+
+@pytest.mark.parametrize("T", [1, 6, 40])
+def test_a_decode_step_with_both_operators(T):
+    """As a model would run them, in one captured step: the bf16 layer routes
+    its tokens, the 8-bit layer of the next block follows the same routing,
+    a dense 8-bit projection comes last."""
+    g = torch.Generator(device="cuda").manual_seed(T)
+    H, E, K, F, Nn = 512, 16, 4, 256, 264
+    x = torch.randn(T, H, generator=g, device="cuda").to(torch.bfloat16)
+    rw = (torch.randn(H, E, generator=g, device="cuda") / H ** 0.5).to(torch.bfloat16)
+    w13 = (0.05 * torch.randn(E, H, 2 * F, generator=g, device="cuda")).to(torch.bfloat16)
+    w2 = (0.05 * torch.randn(E, F, H, generator=g, device="cuda")).to(torch.bfloat16)
+    q13, q2 = w8a8.quantize_weights(w13), w8a8.quantize_weights(w2)
+    head = w8a8.quantize_weights(torch.randn(1, H, Nn, generator=g, device="cuda"))
+
+    def step():
+        y, vals, ids = decode.routed_layer(x, rw, K, w13, w2, renormalize=True)
+        z = w8a8.moe_layer(y, ids, vals, q13, q2)
+        return y, vals, ids, z, w8a8.linear(z, head)
+
+    step()
+    torch.cuda.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        out = step()
+    for _ in range(2):
+        x.copy_(torch.randn(T, H, generator=g, device="cuda"))
+        graph.replay()
+        torch.cuda.synchronize()
+        y, vals, ids, z, logits = out
+        for a, b in zip(out, step()):
+            assert torch.equal(a, b)
+        ref, tol = layer_ref(y, ids, vals, q13, q2, 0)
+        assert bool(((z.double() - ref).abs() <= tol).all())
+        q, s = quant_ref(z)
+        ref = product_ref(q, s, head.q, head.scale, [T])
+        assert bool(((logits.double() - ref).abs() <= ref.abs() * (HALF + 2.0 ** -20)).all())
 
 
 def test_weighted_sum_uses_the_routing():
