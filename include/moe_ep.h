@@ -467,16 +467,15 @@ int moe_w8a8_scratch_bytes(int64_t rows, int32_t K, int32_t N, int32_t experts, 
                            int32_t device, size_t* out);
 int moe_w8a8_gemm(const moe_w8a8_params* params, void* stream);
 
-/* The gated layer of a few tokens in 8 bits, two launches (two more for large
- * H or ffn):
+/* The gated layer in 8 bits:
  *   y[t, :] = sum over k of top_vals[t, k] * down_e(silu(gate_e(x_t)) * up_e(x_t)),
  * e = top_idxs[t, k] - first_expert, with the products, quantisations and
  * rules on ids of moe_w8a8_gemm, moe_quant_rows and moe_decode_layer; the sum
- * is taken in fp32 in the order of the experts.  Requires T * K <=
- * MOE_W8A8_LAYER_MAX_ROWS, hidden and ffn multiples of 16, T * hidden and
- * T * K * ffn <= 98304, experts <= 1024; x, w13, w2 and scratch 16-byte
- * aligned.  scratch: moe_w8a8_layer_scratch_bytes, as above. */
-#define MOE_W8A8_LAYER_MAX_ROWS 32
+ * is taken in fp32 in the order of k, or of the experts with few rows.  A few
+ * tokens take two launches (two more for large hidden or ffn), others six.
+ * Requires hidden and ffn multiples of 16 within moe_w8a8_gemm's K, K <= 32,
+ * experts <= 1024; x, w13, w2, y and scratch 16-byte aligned.  scratch:
+ * moe_w8a8_layer_scratch_bytes, as above. */
 typedef struct moe_w8a8_layer_params {
   int64_t T;
   int32_t hidden, ffn;
@@ -495,9 +494,11 @@ typedef struct moe_w8a8_layer_params {
   void* y;                 /* [T, hidden] bf16                               */
   void* scratch;
   size_t scratch_bytes;
+  int32_t* status_host;    /* optional mapped pinned word for device errors  */
 } moe_w8a8_layer_params;
 
-int moe_w8a8_layer_scratch_bytes(int64_t T, int32_t hidden, int32_t ffn, int32_t experts, int32_t K, size_t* out);
+int moe_w8a8_layer_scratch_bytes(int64_t T, int32_t hidden, int32_t ffn, int32_t experts, int32_t K, int32_t device,
+                                 size_t* out);
 int moe_w8a8_layer(const moe_w8a8_layer_params* params, void* stream);
 
 /* y[t, :] = sum over k of top_vals[t, k] * rows[offsets[e] + slots[t, k], :],

@@ -93,11 +93,9 @@ class W8A8LayerParams(ctypes.Structure):
                 ("x", ctypes.c_void_p), ("w13", ctypes.c_void_p), ("w13_scale", ctypes.c_void_p),
                 ("w2", ctypes.c_void_p), ("w2_scale", ctypes.c_void_p), ("top_idxs", ctypes.c_void_p),
                 ("top_vals", ctypes.c_void_p), ("y", ctypes.c_void_p), ("scratch", ctypes.c_void_p),
-                ("scratch_bytes", ctypes.c_size_t)]
+                ("scratch_bytes", ctypes.c_size_t), ("status_host", ctypes.c_void_p)]
 
 
-W8A8_LAYER_MAX_ROWS = 32  # tokens times ids per token
-W8A8_LAYER_MAX_VALUES = 98304
 DECODE_MAX_TOKENS = 64
 DECODE_MAX_ROWS = 1024  # tokens times ids per token
 TRACE_WORDS = 24
@@ -153,7 +151,7 @@ def lib() -> ctypes.CDLL:
     L.moe_w8a8_gemm.argtypes = [P(W8A8Params), c_vp]
     L.moe_weighted_sum.argtypes = [c_vp, c_i32, c_vp, c_i32, c_i32, c_vp, c_i32, c_vp, c_vp, c_i64, c_i32, c_i32, c_i32,
                                    c_vp, c_vp]
-    L.moe_w8a8_layer_scratch_bytes.argtypes = [c_i64] + [c_i32] * 4 + [P(c_sz)]
+    L.moe_w8a8_layer_scratch_bytes.argtypes = [c_i64] + [c_i32] * 5 + [P(c_sz)]
     L.moe_w8a8_layer.argtypes = [P(W8A8LayerParams), c_vp]
     L.moe_decode_scratch_bytes.argtypes = [c_i64] + [ctypes.c_int32] * 6 + [P(c_sz)]
     L.moe_decode_layer.argtypes = [P(DecodeParams), c_vp]

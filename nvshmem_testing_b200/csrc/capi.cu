@@ -40,7 +40,7 @@ int moe_route(const void* top_idxs, int ids_are_int64, int64_t T, int K, int E, 
       (T > 0 && !perm))
     return kBadArg;
   if (T * int64_t(K) >= (int64_t(1) << 31)) return kBadArg;
-  return launch_route(top_idxs, ids_are_int64, T, K, E, counts, offsets, perm, nullptr, max_count,
+  return launch_route(top_idxs, ids_are_int64, T, K, 0, E, counts, offsets, perm, nullptr, max_count,
                       static_cast<cudaStream_t>(stream));
 }
 
@@ -50,7 +50,7 @@ int moe_route_slots(const void* top_idxs, int ids_are_int64, int64_t T, int K, i
       !counts || !offsets || !max_count)
     return kBadArg;
   if (T * int64_t(K) >= (int64_t(1) << 31)) return kBadArg;
-  return launch_route(top_idxs, ids_are_int64, T, K, E, counts, offsets, perm, slots, max_count,
+  return launch_route(top_idxs, ids_are_int64, T, K, 0, E, counts, offsets, perm, slots, max_count,
                       static_cast<cudaStream_t>(stream));
 }
 

@@ -36,8 +36,9 @@ constexpr int kMaxRouteK = 32;     // routing kernel: ids per token (top-k width
 
 // ---- routing (route.cu)
 size_t route_smem_bytes(int E);
-int launch_route(const void* ids, int ids_are_int64, int64_t T, int K, int E, int32_t* counts, int32_t* offsets,
-                 int32_t* perm, int32_t* slots, int32_t* max_count, cudaStream_t stream);
+// Ids count from `first`: those outside [first, first + E) are skipped.
+int launch_route(const void* ids, int ids_are_int64, int64_t T, int K, int first, int E, int32_t* counts,
+                 int32_t* offsets, int32_t* perm, int32_t* slots, int32_t* max_count, cudaStream_t stream);
 // Words at the workspace's off_local (never accessed by peers).
 struct LocalWords {
   uint32_t push_ctr[2];

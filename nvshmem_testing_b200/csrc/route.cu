@@ -26,9 +26,9 @@ constexpr int kRouteThreads = 512;        // one token per thread per chunk
 constexpr int kRouteWords = kRouteThreads / 32;
 
 template <typename IdT>
-__device__ __forceinline__ int load_id(const IdT* ids, int64_t i, int E) {
+__device__ __forceinline__ int load_id(const IdT* ids, int64_t i, int first, int E) {
   const long long v = static_cast<long long>(ids[i]);
-  return (v >= 0 && v < E) ? static_cast<int>(v) : -1;
+  return (v >= first && v < (long long)first + E) ? static_cast<int>(v - first) : -1;
 }
 
 __device__ __forceinline__ uint32_t ld_shared_cluster_u32(uint32_t addr_cluster) {
@@ -71,7 +71,7 @@ __device__ int block_exclusive_scan(int v, int* warp_sums, int* total) {
 // experts touch consecutive banks.
 template <typename IdT>
 __global__ void __launch_bounds__(kRouteThreads, 1)
-    route_kernel(const IdT* __restrict__ ids, int64_t T, int K, int E, int32_t* __restrict__ counts,
+    route_kernel(const IdT* __restrict__ ids, int64_t T, int K, int first, int E, int32_t* __restrict__ counts,
                  int32_t* __restrict__ offsets, int32_t* __restrict__ perm, int32_t* __restrict__ slots,
                  int32_t* __restrict__ max_count) {
   extern __shared__ __align__(16) unsigned char smem_raw[];
@@ -97,7 +97,7 @@ __global__ void __launch_bounds__(kRouteThreads, 1)
     const IdT* row = ids + t * K;
     int seen[kMaxRouteK];
     for (int k = 0; k < K; ++k) {
-      const int e = load_id(row, k, E);
+      const int e = load_id(row, k, first, E);
       bool dup = false;
       for (int j = 0; j < k; ++j) dup |= (seen[j] == e);
       seen[k] = e;
@@ -165,7 +165,7 @@ __global__ void __launch_bounds__(kRouteThreads, 1)
     if (t < t_end) {
       const IdT* row = ids + t * K;
       for (int k = 0; k < K; ++k) {
-        const int e = load_id(row, k, E);
+        const int e = load_id(row, k, first, E);
         seen[k] = e;
         if (e >= 0) atomicOr(&bits[size_t(w) * E + e], 1u << b);
       }
@@ -256,7 +256,7 @@ int launch_publish_i32(const int32_t* src, int64_t n, int32_t* dst, cudaStream_t
 size_t route_smem_bytes(int E) { return size_t(E) * (4 * 4 + 4 * kRouteWords + 2 * kRouteWords); }
 
 template <typename IdT>
-static int launch_route_t(const IdT* ids, int64_t T, int K, int E, int32_t* counts, int32_t* offsets, int32_t* perm,
+static int launch_route_t(const IdT* ids, int64_t T, int K, int first, int E, int32_t* counts, int32_t* offsets, int32_t* perm,
                           int32_t* slots, int32_t* max_count, cudaStream_t stream) {
   const size_t smem = route_smem_bytes(E);
   if (cudaFuncSetAttribute(route_kernel<IdT>, cudaFuncAttributeMaxDynamicSharedMemorySize, int(smem)) != cudaSuccess)
@@ -273,17 +273,19 @@ static int launch_route_t(const IdT* ids, int64_t T, int K, int E, int32_t* coun
   cfg.stream = stream;
   cfg.attrs = attr;
   cfg.numAttrs = 1;
-  if (cudaLaunchKernelEx(&cfg, route_kernel<IdT>, ids, T, K, E, counts, offsets, perm, slots, max_count) !=
+  if (cudaLaunchKernelEx(&cfg, route_kernel<IdT>, ids, T, K, first, E, counts, offsets, perm, slots, max_count) !=
       cudaSuccess)
     return kCudaErr;
   return cudaGetLastError() == cudaSuccess ? kOk : kCudaErr;
 }
 
-int launch_route(const void* ids, int ids_are_int64, int64_t T, int K, int E, int32_t* counts, int32_t* offsets,
-                 int32_t* perm, int32_t* slots, int32_t* max_count, cudaStream_t stream) {
+int launch_route(const void* ids, int ids_are_int64, int64_t T, int K, int first, int E, int32_t* counts,
+                 int32_t* offsets, int32_t* perm, int32_t* slots, int32_t* max_count, cudaStream_t stream) {
   if (ids_are_int64)
-    return launch_route_t(static_cast<const long long*>(ids), T, K, E, counts, offsets, perm, slots, max_count, stream);
-  return launch_route_t(static_cast<const int32_t*>(ids), T, K, E, counts, offsets, perm, slots, max_count, stream);
+    return launch_route_t(static_cast<const long long*>(ids), T, K, first, E, counts, offsets, perm, slots, max_count,
+                          stream);
+  return launch_route_t(static_cast<const int32_t*>(ids), T, K, first, E, counts, offsets, perm, slots, max_count,
+                        stream);
 }
 
 int launch_pack_padded(const void* tokens, int64_t H, int elem_bytes, const int32_t* counts, const int32_t* offsets,

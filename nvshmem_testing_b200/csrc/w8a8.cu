@@ -1481,48 +1481,128 @@ extern "C" int moe_weighted_sum(const void* rows, int32_t rows_are_f32, const vo
 }
 
 namespace {
-// scratch of the layer of a few tokens: h, then what is quantised by launches
-// of its own.
-struct QLayerScratch {
+size_t up256(size_t v) { return (v + 255) / 256 * 256; }
+
+// The layer of a few tokens: where each expert has few rows (four tokens, or
+// two rows per expert on average) the rows kernel finds them itself and sums
+// them; its scratch is h, then what is quantised by launches of its own.
+bool q_layer_few(int64_t T, int H, int F, int E, int K) {
+  return T * K <= kRwMaxRows && T * H <= int64_t(kRwMaxSmem) && T * K * F <= int64_t(kRwMaxSmem) &&
+         (T <= kRwRows || T * K <= 2 * int64_t(E));
+}
+struct QFewScratch {
   bool x_outside, h_outside;
   size_t xq, xs, hq, hs, total;
 };
-QLayerScratch q_layer_scratch(int64_t T, int H, int F, int K) {
-  QLayerScratch s;
+QFewScratch q_few_scratch(int64_t T, int H, int F, int K) {
+  QFewScratch s;
   s.x_outside = !fresh(T, H);
   s.h_outside = !fresh(T * K, F);
-  const auto up = [](size_t v) { return (v + 255) / 256 * 256; };
-  s.xq = up(size_t(T) * K * F * 4);
-  s.xs = s.xq + (s.x_outside ? up(size_t(T) * H) : 0);
+  s.xq = up256(size_t(T) * K * F * 4);
+  s.xs = s.xq + (s.x_outside ? up256(size_t(T) * H) : 0);
   s.hq = s.xs + (s.x_outside ? 256 : 0);
-  s.hs = s.hq + (s.h_outside ? up(size_t(T) * K * F) : 0);
+  s.hs = s.hq + (s.h_outside ? up256(size_t(T) * K * F) : 0);
   s.total = s.hs + (s.h_outside ? 256 : 0);
   return s;
 }
+// Else: the routing's vectors, h, the second product's rows, and what either
+// product needs (the second after the first).
+struct QManyScratch {
+  size_t offsets, max_count, perm, slots, h, rows, product, total;
+};
+QManyScratch q_many_scratch(int64_t T, int H, int F, int E, int K, int sms) {
+  const int64_t n = T * K;
+  QManyScratch s;
+  s.offsets = up256(size_t(E) * 4);
+  s.max_count = s.offsets + up256(size_t(E + 1) * 4);
+  s.perm = s.max_count + 256;
+  s.slots = s.perm + up256(size_t(n) * 4);
+  s.h = s.slots + up256(size_t(n) * 4);
+  s.rows = s.h + up256(size_t(n) * F * 4);
+  s.product = s.rows + up256(size_t(n) * H * 4);
+  s.total = s.product + std::max(q_scratch(n, H, 2 * F, E, true, true, sms).total,
+                                 q_scratch(n, F, H, E, false, true, sms).total);
+  return s;
+}
 bool q_layer_ok(int64_t T, int32_t H, int32_t F, int32_t E, int32_t K) {
-  return T >= 0 && K >= 1 && T <= kRwMaxRows && T * K <= kRwMaxRows && H > 0 && H % 16 == 0 && F > 0 && F % 16 == 0 &&
-         E >= 1 && E <= kMaxExperts && T * H <= int64_t(kRwMaxSmem) && T * K * F <= int64_t(kRwMaxSmem);
+  return T >= 0 && T <= (int64_t(1) << 30) && K >= 1 && K <= kMaxRouteK && H > 0 && H % 16 == 0 && F > 0 &&
+         F % 16 == 0 && F <= kQMaxK && q_sizes_ok(T * K, H, 2 * F, E, 1) && q_sizes_ok(T * K, F, H, E, 0);
+}
+
+// Routing, the two products with h in fp32 between them, and the sum of fp32
+// rows: y is rounded once, as where no sum is split.
+int q_layer_many(const moe_w8a8_layer_params* p, int sms, void* stream) {
+  const int H = p->hidden, F = p->ffn, E = p->experts;
+  const int64_t n = p->T * p->K;
+  const QManyScratch sc = q_many_scratch(p->T, H, F, E, p->K, sms);
+  if (p->scratch_bytes < sc.total) return kBadArg;
+  unsigned char* base = static_cast<unsigned char*>(p->scratch);
+  int32_t* counts = reinterpret_cast<int32_t*>(base);
+  int32_t* offsets = reinterpret_cast<int32_t*>(base + sc.offsets);
+  int32_t* perm = reinterpret_cast<int32_t*>(base + sc.perm);
+  int32_t* slots = reinterpret_cast<int32_t*>(base + sc.slots);
+  int rc = launch_route(p->top_idxs, p->ids_are_int64, p->T, p->K, p->first_expert, E, counts, offsets, perm, slots,
+                        reinterpret_cast<int32_t*>(base + sc.max_count), static_cast<cudaStream_t>(stream));
+  if (rc != kOk) return rc;
+  moe_w8a8_params g = {};
+  g.rows = n;
+  g.experts = E;
+  g.counts = counts;
+  g.live_rows = offsets + E;
+  g.scratch = base + sc.product;
+  g.scratch_bytes = sc.total - sc.product;
+  g.status_host = p->status_host;
+  g.out_is_f32 = 1;
+  g.K = H;
+  g.N = 2 * F;
+  g.swiglu = 1;
+  g.wq = p->w13;
+  g.ws = p->w13_scale;
+  g.x = p->x;
+  g.perm = perm;
+  g.out = base + sc.h;
+  rc = moe_w8a8_gemm(&g, stream);
+  if (rc != kOk) return rc;
+  g.K = F;
+  g.N = H;
+  g.swiglu = 0;
+  g.wq = p->w2;
+  g.ws = p->w2_scale;
+  g.x = base + sc.h;
+  g.x_is_f32 = 1;
+  g.perm = nullptr;
+  g.out = base + sc.rows;
+  rc = moe_w8a8_gemm(&g, stream);
+  if (rc != kOk) return rc;
+  return moe_weighted_sum(base + sc.rows, 1, p->top_idxs, p->ids_are_int64, p->first_expert, p->top_vals,
+                          p->vals_are_bf16, slots, offsets, p->T, p->K, H, E, p->y, stream);
 }
 }  // namespace
 
-extern "C" int moe_w8a8_layer_scratch_bytes(int64_t T, int32_t H, int32_t F, int32_t E, int32_t K, size_t* out) {
+extern "C" int moe_w8a8_layer_scratch_bytes(int64_t T, int32_t H, int32_t F, int32_t E, int32_t K, int32_t device,
+                                            size_t* out) {
   if (!out || !q_layer_ok(T, H, F, E, K)) return kBadArg;
-  *out = q_layer_scratch(T, H, F, K).total;
+  int sms = 0;
+  if (cudaDeviceGetAttribute(&sms, cudaDevAttrMultiProcessorCount, device) != cudaSuccess) return kCudaErr;
+  *out = q_layer_few(T, H, F, E, K) ? q_few_scratch(T, H, F, K).total : q_many_scratch(T, H, F, E, K, sms).total;
   return kOk;
 }
 
 extern "C" int moe_w8a8_layer(const moe_w8a8_layer_params* p, void* stream) {
-  if (!p || !q_layer_ok(p->T, p->hidden, p->ffn, p->experts, p->K)) return kBadArg;
+  if (!p || !q_layer_ok(p->T, p->hidden, p->ffn, p->experts, p->K) || p->first_expert < 0) return kBadArg;
   if (p->T == 0) return kOk;
   if (!p->x || !p->w13 || !p->w13_scale || !p->w2 || !p->w2_scale || !p->top_idxs || !p->top_vals || !p->y ||
       !p->scratch)
     return kBadArg;
-  if (misaligned16(p->x) || misaligned16(p->w13) || misaligned16(p->w2) || misaligned16(p->scratch)) return kBadArg;
-  const int T = int(p->T), H = p->hidden, F = p->ffn, K = p->K;
-  const QLayerScratch sc = q_layer_scratch(T, H, F, K);
-  if (p->scratch_bytes < sc.total) return kBadArg;
+  if (misaligned16(p->x) || misaligned16(p->w13) || misaligned16(p->w2) || misaligned16(p->y) ||
+      misaligned16(p->scratch))
+    return kBadArg;
   int sms = 0, dev = 0;
   if (sm_count(&sms, &dev) != kOk) return kCudaErr;
+  if (!q_layer_few(p->T, p->hidden, p->ffn, p->experts, p->K)) return q_layer_many(p, sms, stream);
+  const int T = int(p->T), H = p->hidden, F = p->ffn, K = p->K;
+  const QFewScratch sc = q_few_scratch(T, H, F, K);
+  if (p->scratch_bytes < sc.total) return kBadArg;
   const cudaStream_t s = static_cast<cudaStream_t>(stream);
   unsigned char* base = static_cast<unsigned char*>(p->scratch);
   float* h = reinterpret_cast<float*>(base);

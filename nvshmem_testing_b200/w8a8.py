@@ -166,12 +166,11 @@ def grouped_gemm(xq: torch.Tensor, xs: torch.Tensor, w: QuantWeights, counts: to
     if rows == 0:
         return out
     with utils.on_device(xq.device) as stream:
-        _gemm(xq.contiguous(), xs.contiguous(), None, w, counts, None, None, rows, K, Nw, El, swiglu, out, status,
-              stream)
+        _gemm(xq.contiguous(), xs.contiguous(), None, w, counts, rows, K, Nw, El, swiglu, out, status, stream)
     return out
 
 
-def _gemm(xq, xs, x, w, counts, perm, live_rows, rows, K, Nw, El, swiglu, out, status, stream):
+def _gemm(xq, xs, x, w, counts, rows, K, Nw, El, swiglu, out, status, stream):
     """The checked call, for quantised rows (xq, xs) or rows x that are still
     to be."""
     need = _scratch_bytes(rows, K, Nw, El, int(swiglu), int(x is not None), out.device.index)
@@ -180,8 +179,7 @@ def _gemm(xq, xs, x, w, counts, perm, live_rows, rows, K, Nw, El, swiglu, out, s
                      None if xq is None else xq.data_ptr(), None if xs is None else xs.data_ptr(), w.q.data_ptr(),
                      w.scale.data_ptr(), None if counts is None else counts.data_ptr(), out.data_ptr(),
                      None if scratch is None else scratch.data_ptr(), need,
-                     None if status is None else status.data_ptr(), None if x is None else x.data_ptr(),
-                     None if perm is None else perm.data_ptr(), None if live_rows is None else live_rows.data_ptr())
+                     None if status is None else status.data_ptr(), None if x is None else x.data_ptr(), None, None)
     N.check(N.lib().moe_w8a8_gemm(ctypes.byref(p), stream), "moe_w8a8_gemm")
 
 
@@ -201,13 +199,13 @@ def linear(x: torch.Tensor, w: QuantWeights, *, out_dtype=torch.bfloat16) -> tor
     out = torch.empty((rows, Nw), dtype=out_dtype, device=x.device)
     if rows:
         with utils.on_device(x.device) as stream:
-            _gemm(None, None, x.contiguous(), w, None, None, None, rows, K, Nw, 1, False, out, None, stream)
+            _gemm(None, None, x.contiguous(), w, None, rows, K, Nw, 1, False, out, None, stream)
     return out
 
 
 @functools.lru_cache(maxsize=512)
-def _layer_dims(x, ids, vals, q13, q2) -> tuple[int, int, int | None]:
-    """(T, ids per token, scratch of the form for a few tokens or None)."""
+def _layer_dims(x, ids, vals, q13, q2) -> tuple[int, int]:
+    """(T, ids per token)."""
     El, F2, H = q13
     F = F2 // 2
     if F2 % 2 or tuple(q2) != (El, H, F):
@@ -224,14 +222,14 @@ def _layer_dims(x, ids, vals, q13, q2) -> tuple[int, int, int | None]:
     K = ids[1]
     if not 1 <= K <= 32:
         raise ValueError(f"{K} ids per token: 1 to 32")
-    # Few rows per expert (four tokens at most, or two per expert on average);
-    # T = 0 returns before it matters.
-    if (T == 0 or T * K > N.W8A8_LAYER_MAX_ROWS or max(T * H, T * K * F) > N.W8A8_LAYER_MAX_VALUES
-            or (T > 4 and T * K > 2 * El)):
-        return T, K, None
+    return T, K
+
+
+@functools.lru_cache(maxsize=256)
+def _layer_scratch_bytes(*sizes) -> int:
     need = ctypes.c_size_t()
-    N.check(N.lib().moe_w8a8_layer_scratch_bytes(T, H, F, El, K, ctypes.byref(need)), "moe_w8a8_layer_scratch_bytes")
-    return T, K, need.value
+    N.check(N.lib().moe_w8a8_layer_scratch_bytes(*sizes, ctypes.byref(need)), "moe_w8a8_layer_scratch_bytes")
+    return need.value
 
 
 def moe_layer(x: torch.Tensor, top_idxs: torch.Tensor, top_vals: torch.Tensor, w13: QuantWeights, w2: QuantWeights,
@@ -255,7 +253,7 @@ def moe_layer(x: torch.Tensor, top_idxs: torch.Tensor, top_vals: torch.Tensor, w
         top_idxs = top_idxs[:, None]
     if top_vals.dim() == 1:
         top_vals = top_vals[:, None]
-    T, K, need = _layer_dims(x.shape, top_idxs.shape, top_vals.shape, w13.q.shape, w2.q.shape)
+    T, K = _layer_dims(x.shape, top_idxs.shape, top_vals.shape, w13.q.shape, w2.q.shape)
     if x.dtype != torch.bfloat16:
         raise TypeError("x must be bfloat16")
     if top_idxs.dtype not in (torch.int32, torch.int64):
@@ -271,26 +269,13 @@ def moe_layer(x: torch.Tensor, top_idxs: torch.Tensor, top_vals: torch.Tensor, w
     if T == 0:
         return y
     ids, vals = top_idxs.contiguous(), top_vals.contiguous()
-    if need is not None:  # a few tokens: no routing, packing or sum of their own
-        scratch = torch.empty(need, dtype=torch.uint8, device=x.device)
-        x = x.contiguous()
-        p = N.W8A8LayerParams(T, H, F, El, K, first_expert, ids.dtype == torch.int64, vals.dtype == torch.bfloat16, 0,
-                              x.data_ptr(), w13.q.data_ptr(), w13.scale.data_ptr(), w2.q.data_ptr(),
-                              w2.scale.data_ptr(), ids.data_ptr(), vals.data_ptr(), y.data_ptr(), scratch.data_ptr(),
-                              need)
-        with utils.on_device(x.device) as stream:
-            N.check(N.lib().moe_w8a8_layer(ctypes.byref(p), stream), "moe_w8a8_layer")
-        return y
-    with utils.on_device(x.device) as stream:
-        r = utils.route(ids if first_expert == 0 else ids - first_expert, El, with_slots=True)
-        n, live = T * K, r.offsets[El:]
-        h = torch.empty((n, F), dtype=torch.float32, device=x.device)
-        _gemm(None, None, x.contiguous(), w13, r.counts, r.perm, live, n, H, F2, El, True, h, status, stream)
-        # fp32 rows: y is rounded once, like a layer that never splits its sum
-        rows = torch.empty((n, H), dtype=torch.float32, device=x.device)
-        _gemm(None, None, h, w2, r.counts, None, live, n, F, H, El, False, rows, status, stream)
-        N.check(N.lib().moe_weighted_sum(rows.data_ptr(), 1, ids.data_ptr(), ids.dtype == torch.int64, first_expert,
-                                         vals.data_ptr(), vals.dtype == torch.bfloat16, r.slots.data_ptr(),
-                                         r.offsets.data_ptr(), T, K, H, El, y.data_ptr(), stream),
-                "moe_weighted_sum")
+    x = x.contiguous()
+    need = _layer_scratch_bytes(T, H, F, El, K, dev.index)
+    scratch = torch.empty(need, dtype=torch.uint8, device=dev)
+    p = N.W8A8LayerParams(T, H, F, El, K, first_expert, ids.dtype == torch.int64, vals.dtype == torch.bfloat16, 0,
+                          x.data_ptr(), w13.q.data_ptr(), w13.scale.data_ptr(), w2.q.data_ptr(),
+                          w2.scale.data_ptr(), ids.data_ptr(), vals.data_ptr(), y.data_ptr(), scratch.data_ptr(),
+                          need, None if status is None else status.data_ptr())
+    with utils.on_device(dev) as stream:
+        N.check(N.lib().moe_w8a8_layer(ctypes.byref(p), stream), "moe_w8a8_layer")
     return y
