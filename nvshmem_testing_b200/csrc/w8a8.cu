@@ -1082,17 +1082,15 @@ __global__ void __launch_bounds__(kRwThreads, 2) w8a8_rows_kernel(const __grid_c
 }
 
 // ---------------------------------------------------------------- quantisation
-constexpr int kQuantThreads = 256;
-
 // TPR threads per row, each VPT groups of eight values in registers; rows
 // longer than that are read again for the rounding.
-template <typename In, int VPT>
-__global__ void __launch_bounds__(kQuantThreads)
+template <typename In, int VPT, int THREADS>
+__global__ void __launch_bounds__(THREADS)
     quant_rows_kernel(const In* __restrict__ x, int64_t rows, int K, const int32_t* __restrict__ perm,
                       const int32_t* __restrict__ live_rows, int tpr, int8_t* __restrict__ q,
                       float* __restrict__ scale) {
-  __shared__ uint32_t top_s[kQuantThreads / 32];
-  const int per = kQuantThreads / tpr, lr = threadIdx.x / tpr, c = threadIdx.x % tpr;
+  __shared__ uint32_t top_s[THREADS / 32];
+  const int per = THREADS / tpr, lr = threadIdx.x / tpr, c = threadIdx.x % tpr;
   const int64_t live = live_rows ? min(int64_t(max(*live_rows, 0)), rows) : rows;
   const int groups = K / 8;
 #pragma unroll 1
@@ -1150,19 +1148,23 @@ __global__ void __launch_bounds__(kQuantThreads)
 template <typename In>
 int launch_quant(const void* x, int64_t rows, int K, const int32_t* perm, const int32_t* live, void* q, float* scale,
                  int sms, cudaStream_t stream) {
-  // The fewest threads per row that leave each at most four groups of eight.
-  int tpr = 32;
-  while (tpr < kQuantThreads && K / 8 > 4 * tpr) tpr *= 2;
-  const int per = kQuantThreads / tpr, vpt = (K / 8 + tpr - 1) / tpr;
-  const int64_t blocks = std::min<int64_t>((rows + per - 1) / per, int64_t(sms) * 8);
   const In* xi = static_cast<const In*>(x);
   int8_t* qi = static_cast<int8_t*>(q);
-  const unsigned g = unsigned(blocks);
-  // (Eight groups where even all threads leave more: 16384 values.)
-  if (vpt <= 1) quant_rows_kernel<In, 1><<<g, kQuantThreads, 0, stream>>>(xi, rows, K, perm, live, tpr, qi, scale);
-  else if (vpt <= 2) quant_rows_kernel<In, 2><<<g, kQuantThreads, 0, stream>>>(xi, rows, K, perm, live, tpr, qi, scale);
-  else if (vpt <= 4) quant_rows_kernel<In, 4><<<g, kQuantThreads, 0, stream>>>(xi, rows, K, perm, live, tpr, qi, scale);
-  else quant_rows_kernel<In, 8><<<g, kQuantThreads, 0, stream>>>(xi, rows, K, perm, live, tpr, qi, scale);
+  // The fewest threads per row that leave each at most four groups of eight,
+  // in CTAs of 256, or of 512 for fp32 rows that need them (8192 x 14336: 98
+  // us, 104 with eight groups in each of 256 threads; bf16 95 and 76 us, so
+  // there the smaller CTAs stay).
+  constexpr int kMost = sizeof(In) == 4 ? 512 : 256;
+  int tpr = 32;
+  while (tpr < kMost && K / 8 > 4 * tpr) tpr *= 2;
+  const int vpt = (K / 8 + tpr - 1) / tpr, per = tpr < 256 ? 256 / tpr : 1;
+  const unsigned g = unsigned(std::min<int64_t>((rows + per - 1) / per, int64_t(sms) * 8));
+  if (vpt <= 1) quant_rows_kernel<In, 1, 256><<<g, 256, 0, stream>>>(xi, rows, K, perm, live, tpr, qi, scale);
+  else if (vpt <= 2) quant_rows_kernel<In, 2, 256><<<g, 256, 0, stream>>>(xi, rows, K, perm, live, tpr, qi, scale);
+  else if (tpr <= 256 && vpt <= 4)
+    quant_rows_kernel<In, 4, 256><<<g, 256, 0, stream>>>(xi, rows, K, perm, live, tpr, qi, scale);
+  else  // kMost threads per row
+    quant_rows_kernel<In, 2048 / kMost, kMost><<<g, kMost, 0, stream>>>(xi, rows, K, perm, live, tpr, qi, scale);
   return cudaGetLastError() == cudaSuccess ? kOk : kCudaErr;
 }
 
