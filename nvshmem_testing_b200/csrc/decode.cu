@@ -22,7 +22,8 @@
 // or tiles.  SMs do not get the same bandwidth, though (those of the fuller
 // GPCs up to 14 % less, always the same ones), so of a long list the last
 // eighth is left in small chunks for whoever is done first (7 tokens, 8
-// experts of 352 MB: 410 -> 392 us; 705 MB in all: no gain).  A tile that ends
+// experts of 352 MB: 410 -> 392 us; 705 MB in all: no gain), and more where
+// the rows' alignment sets the SMs further apart.  A tile that ends
 // up in several parts is summed from fp32 partials in the order of the list,
 // so results depend neither on timing nor on who did what: in pass 1 by the
 // last of its CTAs (few parts, few rows; otherwise by the grid), in pass 2,
@@ -61,7 +62,6 @@ constexpr uint32_t kDecABytes = 256 * 64 * 2;     // 256 features x 64 K
 constexpr uint32_t kDecMaxSmem = 226 * 1024;      // dynamic; under 1 KB is static
 constexpr int kDecTokChunk = 8;                   // router: tokens whose logits a thread sums at a time
 constexpr int kDecMaxChunks = 640;                // handed out as CTAs get done
-constexpr int kDecChunkTokens = 32;               // most tokens of a call that uses them (partials grow with T)
 constexpr int kDecRunSlots = 16;                  // > stages + 2 accumulators: runs under way in a CTA
 constexpr uint64_t kDecBoundNs = 2000000000ull;   // bug guard on every pipeline wait
 constexpr int kBarEpi = 1;
@@ -537,6 +537,16 @@ __device__ void dec_router_topk(const DecArgs& a, unsigned char* stage, unsigned
   }
 }
 
+__host__ __device__ inline bool ragged_rows(int n) { return n % 64 != 0; }
+
+// The most chunks of a pass.  Their sums grow with the tokens: above 32 only
+// ragged rows are worth them, and fewer (64 tokens: all would take 100 MB of
+// scratch; 7168 x 2048, 64 experts: 781 us with, 756 without; 33 tokens,
+// F 1000: 128 and 142).
+__host__ __device__ inline int max_chunks(int T, bool ragged) {
+  return T <= 32 ? kDecMaxChunks : ragged ? kDecMaxChunks / 2 : 0;
+}
+
 // One pass: its units in order.  The first `fixed` are shared out evenly, the
 // rest lies in `chunks` chunks of `cz`; a CTA's share and every chunk is a
 // part.
@@ -688,7 +698,7 @@ __global__ void __launch_bounds__(kDecThreads, 1)
   const int nact = sm.nact;
   const int G = gridDim.x;
 
-  auto make_pass = [&](int tiles, int tile, int kb, int nt) {
+  auto make_pass = [&](int tiles, int tile, int kb, int nt, bool ragged) {
     Pass p;
     p.units = tiles * tile;
     p.tile = tile;
@@ -696,9 +706,15 @@ __global__ void __launch_bounds__(kDecThreads, 1)
     p.nt = nt;
     p.chunks = 0;
     p.cz = 1;
-    if (a.T <= kDecChunkTokens && p.units >= 128 * G) {  // shorter lists: the chunks' sums cost more than they gain
-      const int rest = p.units / 8;
-      p.cz = max(16, (rest + kDecMaxChunks - 1) / kDecMaxChunks);
+    // Shorter lists: the chunks' sums cost more than they gain.  Rows of w13
+    // that are no multiple of 128 bytes set the SMs further apart (18 tokens,
+    // F 728: shares of pass 1 done after 70 to 107 us), so there a third is
+    // dealt out, in smaller chunks and from shorter lists on (88 us); it gains
+    // nothing in pass 2, whose pieces of a row are twice as long.
+    const int most = max_chunks(a.T, ragged);
+    if (most > 0 && p.units >= (ragged ? 32 : 128) * G) {
+      const int rest = p.units / (ragged ? 3 : 8);
+      p.cz = max(ragged ? 8 : 16, (rest + most - 1) / most);
       p.chunks = rest / p.cz;
     }
     p.fixed = p.units - p.chunks * p.cz;
@@ -714,8 +730,8 @@ __global__ void __launch_bounds__(kDecThreads, 1)
   };
   const int kb1 = (a.H + 63) / 64, nt1 = (a.F + 127) / 128;
   const int kb2 = (a.F + 63) / 64, nt2 = (a.H + 255) / 256;
-  const Pass p1 = make_pass(nact * nt1, kb1, kb1, nt1);
-  const Pass p2 = make_pass(nact > 0 ? nt2 : 0, nact * kb2, kb2, nt2);
+  const Pass p1 = make_pass(nact * nt1, kb1, kb1, nt1, ragged_rows(a.F));
+  const Pass p2 = make_pass(nact > 0 ? nt2 : 0, nact * kb2, kb2, nt2, false);
   // The runs of units that a CTA does in a pass: its share, then chunks until
   // none is left.  One thread takes them and the other roles follow through
   // a ring in shared memory; `n` counts a role's chunks over both passes.
@@ -1184,7 +1200,7 @@ DecScratch dec_scratch(int T, int K, int F, int Er, int sms) {
   DecScratch s;
   s.hs = 0;
   s.part = up256(size_t(T) * K * F * 2);
-  const size_t parts = size_t(sms) + (T <= kDecChunkTokens ? kDecMaxChunks : 0);
+  const size_t parts = size_t(sms) + max_chunks(T, ragged_rows(F));
   s.ctr = s.part + up256(2 * parts * T * 256 * 4);
   s.lpart = s.ctr + up256((size_t(sms) + kDecMaxChunks + 2) * 4);
   s.total = s.lpart + up256(size_t(sms) * T * Er * 4);

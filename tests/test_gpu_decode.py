@@ -108,6 +108,18 @@ def test_long_lists(T, H, E, K, F):
         assert torch.equal(y, decode.moe_layer(x, ids, vals, w13, w2))
 
 
+@pytest.mark.parametrize("T,H,E,K,F", [(18, 4360, 32, 3, 728), (9, 32768, 8, 2, 136), (32, 2056, 64, 4, 264),
+                                       (33, 4352, 32, 3, 728), (1, 4096, 40, 32, 744)])
+def test_long_lists_of_odd_rows(T, H, E, K, F):
+    """Rows of w13 that are no multiple of 128 bytes: chunks from shorter lists
+    on, many to a tile (33 tokens: fewer and larger ones)."""
+    x, ids, vals, w13, w2 = make(T, H, E, K, F, T, scale=0.02)
+    y = decode.moe_layer(x, ids, vals, w13, w2)
+    check(y, x, ids, vals, w13, w2)
+    for _ in range(3):
+        assert torch.equal(y, decode.moe_layer(x, ids, vals, w13, w2))
+
+
 @pytest.mark.parametrize("ids_dtype", [torch.int32, torch.int64])
 @pytest.mark.parametrize("vals_dtype", [torch.float32, torch.bfloat16])
 def test_types(ids_dtype, vals_dtype):
