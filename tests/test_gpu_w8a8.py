@@ -315,6 +315,24 @@ def test_layer(T, H, El, E, first, K, F):
         assert not y[1].any()
 
 
+@pytest.mark.parametrize("T", [3, 40])
+@pytest.mark.parametrize("dt", [torch.int32, torch.int64])
+@pytest.mark.parametrize("first", [0, 5, 2 ** 31 - 3])
+def test_layer_ids_at_the_types_ends(T, dt, first):
+    g = torch.Generator(device="cuda").manual_seed(T)
+    x = torch.randn(T, 64, generator=g, device="cuda").to(torch.bfloat16)
+    w13 = w8a8.quantize_weights(0.05 * torch.randn(3, 64, 64, generator=g, device="cuda"))
+    w2 = w8a8.quantize_weights(0.05 * torch.randn(3, 32, 64, generator=g, device="cuda"))
+    ends = torch.iinfo(dt)
+    ids = torch.tensor([ends.min, ends.max, first - 1, first, first + 1, -first], device="cuda").clamp(
+        ends.min, ends.max).to(dt).expand(T, 6).contiguous()
+    ids[1:] = ids[1:].roll(1, 1)
+    vals = torch.rand(T, 6, generator=g, device="cuda")
+    y = w8a8.moe_layer(x, ids, vals, w13, w2, first_expert=first)
+    ref, tol = layer_ref(x, ids, vals, w13, w2, first)
+    assert bool(((y.double() - ref).abs() <= tol).all())
+
+
 def test_misaligned_and_misplaced_tensors_are_refused():
     xq, xs, wq, ws = make(5, 64, 32, 2, 1)
     cd = torch.tensor([2, 3], dtype=torch.int32, device="cuda")
