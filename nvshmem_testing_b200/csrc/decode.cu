@@ -41,6 +41,7 @@
 #include <climits>
 #include <type_traits>
 
+#include "decode_parts.h"
 #include "moe_ep.h"
 #include "moe_ep_internal.h"
 #include "ptx.cuh"
@@ -61,7 +62,6 @@ constexpr int kDecMaxStages = 8;
 constexpr uint32_t kDecABytes = 256 * 64 * 2;     // 256 features x 64 K
 constexpr uint32_t kDecMaxSmem = 226 * 1024;      // dynamic; under 1 KB is static
 constexpr int kDecTokChunk = 8;                   // router: tokens whose logits a thread sums at a time
-constexpr int kDecMaxChunks = 640;                // handed out as CTAs get done
 constexpr int kDecRunSlots = 16;                  // > stages + 2 accumulators: runs under way in a CTA
 constexpr uint64_t kDecBoundNs = 2000000000ull;   // bug guard on every pipeline wait
 constexpr int kBarEpi = 1;
@@ -127,13 +127,6 @@ __device__ __forceinline__ bool dec_wait(uint64_t* bar, uint32_t parity, DecSmem
 __device__ __noinline__ void dec_fail(DecSmem& sm, const DecArgs& a, int detail) {
   if (atomicExch(&sm.err, 1) == 0 && a.status_host)
     *reinterpret_cast<volatile int32_t*>(a.status_host) = int32_t(status_word(kTimeout, kSitePipe, detail));
-}
-
-// Share of CTA c of `units`, and the CTA a unit belongs to (g CTAs, g <= units;
-// units * g < 2^32).
-__device__ __forceinline__ int share_lo(uint32_t units, uint32_t g, uint32_t c) { return int(units * c / g); }
-__device__ __forceinline__ int share_owner(uint32_t units, uint32_t g, uint32_t u) {
-  return int(((u + 1) * g - 1) / units);
 }
 
 __device__ __forceinline__ float silu_mul(float g, float u) { return g / (1.f + expf(-g)) * u; }
@@ -537,34 +530,6 @@ __device__ void dec_router_topk(const DecArgs& a, unsigned char* stage, unsigned
   }
 }
 
-__host__ __device__ inline bool ragged_rows(int n) { return n % 64 != 0; }
-
-// The most chunks of a pass.  Their sums grow with the tokens: above 32 only
-// ragged rows are worth them, and fewer (64 tokens: all would take 100 MB of
-// scratch; 7168 x 2048, 64 experts: 781 us with, 756 without; 33 tokens,
-// F 1000: 128 and 142).
-__host__ __device__ inline int max_chunks(int T, bool ragged) {
-  return T <= 32 ? kDecMaxChunks : ragged ? kDecMaxChunks / 2 : 0;
-}
-
-// One pass: its units in order.  The first `fixed` are shared out evenly, the
-// rest lies in `chunks` chunks of `cz`; a CTA's share and every chunk is a
-// part.
-// Pass 1: expert by expert, its tiles of 128 features of F, each over H.
-// Pass 2: tile by tile of 256 features of H, each over the experts' F.
-struct Pass {
-  int units;     // of all CTAs
-  int tile;      // units of one tile (the units whose sums belong together)
-  int kb;        // units of one expert's K
-  int nt;        // tiles per expert (pass 1), tiles (pass 2)
-  int g;         // CTAs that have a share
-  int fixed, chunks, cz;
-  int lo, hi;    // this CTA's share
-  __device__ __forceinline__ int part_of(int u) const {
-    return u < fixed ? share_owner(uint32_t(fixed), uint32_t(g), uint32_t(u)) : g + (u - fixed) / cz;
-  }
-};
-
 // A position in a pass, moved on by additions: the loads and the MMAs each
 // run in one thread, whose integer divisions (two per unit and more) took
 // longer than a unit's share of the memory bandwidth.
@@ -698,40 +663,10 @@ __global__ void __launch_bounds__(kDecThreads, 1)
   const int nact = sm.nact;
   const int G = gridDim.x;
 
-  auto make_pass = [&](int tiles, int tile, int kb, int nt, bool ragged) {
-    Pass p;
-    p.units = tiles * tile;
-    p.tile = tile;
-    p.kb = kb;
-    p.nt = nt;
-    p.chunks = 0;
-    p.cz = 1;
-    // Shorter lists: the chunks' sums cost more than they gain.  Rows of w13
-    // that are no multiple of 128 bytes set the SMs further apart (18 tokens,
-    // F 728: shares of pass 1 done after 70 to 107 us), so there a third is
-    // dealt out, in smaller chunks and from shorter lists on (88 us); it gains
-    // nothing in pass 2, whose pieces of a row are twice as long.
-    const int most = max_chunks(a.T, ragged);
-    if (most > 0 && p.units >= (ragged ? 32 : 128) * G) {
-      const int rest = p.units / (ragged ? 3 : 8);
-      p.cz = max(ragged ? 8 : 16, (rest + most - 1) / most);
-      p.chunks = rest / p.cz;
-    }
-    p.fixed = p.units - p.chunks * p.cz;
-    // Short lists: a part costs the one who adds a tile's up about a fifth of
-    // the time of a unit, so about sqrt(tile / 5) units a CTA at least.
-    int least = 1;
-    while (5 * (least + 1) * (least + 1) <= tile && least < 8) ++least;
-    p.g = min(G, max(p.fixed / least, min(p.fixed, 1)));
-    const bool on = int(blockIdx.x) < p.g;
-    p.lo = on ? share_lo(p.fixed, p.g, blockIdx.x) : 0;
-    p.hi = on ? share_lo(p.fixed, p.g, blockIdx.x + 1) : 0;
-    return p;
-  };
   const int kb1 = (a.H + 63) / 64, nt1 = (a.F + 127) / 128;
   const int kb2 = (a.F + 63) / 64, nt2 = (a.H + 255) / 256;
-  const Pass p1 = make_pass(nact * nt1, kb1, kb1, nt1, ragged_rows(a.F));
-  const Pass p2 = make_pass(nact > 0 ? nt2 : 0, nact * kb2, kb2, nt2, false);
+  const Pass p1 = make_pass(a.T, G, blockIdx.x, nact * nt1, kb1, kb1, nt1, ragged_rows(a.F));
+  const Pass p2 = make_pass(a.T, G, blockIdx.x, nact > 0 ? nt2 : 0, nact * kb2, kb2, nt2, false);
   // The runs of units that a CTA does in a pass: its share, then chunks until
   // none is left.  One thread takes them and the other roles follow through
   // a ring in shared memory; `n` counts a role's chunks over both passes.

@@ -1,5 +1,7 @@
 """Argument checks of the one-kernel layer, which need no GPU."""
 import ctypes
+import subprocess
+from pathlib import Path
 
 import pytest
 import torch
@@ -65,3 +67,13 @@ def test_c_entry_refuses_before_any_device_call():
     assert lib.moe_decode_layer(ctypes.byref(p), None) == N.BAD_ARG
     p.x, p.T = at, 0
     assert lib.moe_decode_layer(ctypes.byref(p), None) == N.OK  # nothing to do
+
+
+def test_every_unit_belongs_to_one_part(tmp_path):
+    """The kernel's division of its work, an empty rank's included, on the host."""
+    exe = tmp_path / "check"
+    here = Path(__file__).resolve().parent
+    subprocess.run(["g++", "-std=c++17", "-O1", "-I", str(here.parent / "nvshmem_testing_b200" / "csrc"),
+                    str(here / "native" / "decode_parts_check.cpp"), "-o", str(exe)], check=True)
+    done = subprocess.run([str(exe)], capture_output=True, text=True)
+    assert done.returncode == 0, f"status {done.returncode}: {done.stdout}"

@@ -159,6 +159,20 @@ def test_no_expert_here_and_no_token():
     assert decode.moe_layer(x[:0], ids[:0], vals[:0], w13, w2).shape == (0, 128)
 
 
+@pytest.mark.parametrize("T,H,F", [(1, 64, 72), (5, 7168, 256), (40, 1032, 520), (64, 4096, 728)])
+def test_an_empty_rank(T, H, F):
+    """No token has an expert here: every row is written, and zero."""
+    x, ids, vals, w13, w2 = make(T, H, 3, 2, F, T)
+    status = torch.zeros(1, dtype=torch.int32, pin_memory=True)
+    rw = torch.randn(H, 8, device="cuda").to(torch.bfloat16)
+    for _ in range(3):
+        out = torch.full_like(x, float("nan"))
+        decode.moe_layer(x, ids, vals, w13, w2, first_expert=3, out=out, status=status)
+        routed = decode.routed_layer(x, rw, 2, w13, w2, first_expert=8, status=status)[0]
+        torch.cuda.synchronize()
+        assert bool((out == 0).all()) and bool((routed == 0).all()) and int(status[0]) == 0
+
+
 def test_a_token_is_touched_by_its_own_experts_only():
     """Non-finite tokens and experts stay with the rows that use them."""
     x, ids, vals, w13, w2 = make(8, 192, 4, 1, 96, 21)
