@@ -62,7 +62,6 @@ constexpr int kDecMaxStages = 8;
 constexpr uint32_t kDecABytes = 256 * 64 * 2;     // 256 features x 64 K
 constexpr uint32_t kDecMaxSmem = 226 * 1024;      // dynamic; under 1 KB is static
 constexpr int kDecTokChunk = 8;                   // router: tokens whose logits a thread sums at a time
-constexpr int kDecRunSlots = 16;                  // > stages + 2 accumulators: runs under way in a CTA
 constexpr uint64_t kDecBoundNs = 2000000000ull;   // bug guard on every pipeline wait
 constexpr int kBarEpi = 1;
 
@@ -667,25 +666,6 @@ __global__ void __launch_bounds__(kDecThreads, 1)
   const int kb2 = (a.F + 63) / 64, nt2 = (a.H + 255) / 256;
   const Pass p1 = make_pass(a.T, G, blockIdx.x, nact * nt1, kb1, kb1, nt1, ragged_rows(a.F));
   const Pass p2 = make_pass(a.T, G, blockIdx.x, nact > 0 ? nt2 : 0, nact * kb2, kb2, nt2, false);
-  // The runs of units that a CTA does in a pass: its share, then chunks until
-  // none is left.  One thread takes them and the other roles follow through
-  // a ring in shared memory; `n` counts a role's chunks over both passes.
-  struct Runs {
-    int n;          // chunks seen by this role
-    int lo, hi;     // current run
-    int part;
-  };
-  auto first_run = [&](Runs& r, const Pass& p) {
-    r.lo = p.lo;
-    r.hi = p.hi;
-    r.part = blockIdx.x;
-  };
-  auto set_run = [&](Runs& r, const Pass& p, int chunk) {
-    r.lo = p.fixed + chunk * p.cz;
-    r.hi = r.lo + p.cz;
-    r.part = p.g + chunk;
-    return chunk >= 0;
-  };
   auto take_run = [&](Runs& r, const Pass& p, int pass) {
     if (p.chunks == 0) return false;
     int chunk = int(atomicAdd(&a.ctr[G + kDecMaxChunks + pass - 1], 1u));
@@ -695,11 +675,10 @@ __global__ void __launch_bounds__(kDecThreads, 1)
     ++r.n;
     return set_run(r, p, chunk);
   };
-  auto follow_run = [&](Runs& r, const Pass& p) {
-    if (p.chunks == 0 || !dec_wait(&sm.run[r.n % kDecRunSlots], (r.n / kDecRunSlots) & 1, sm)) return false;
-    const int chunk = *reinterpret_cast<volatile int*>(&sm.chunk[r.n % kDecRunSlots]);
-    ++r.n;
-    return set_run(r, p, chunk);
+  auto next_chunk = [&](Runs& r, const Pass& p) {
+    return follow_run(
+        r, p, [&](int slot, uint32_t parity) { return dec_wait(&sm.run[slot], parity, sm); },
+        [&](int slot) { return *reinterpret_cast<volatile int*>(&sm.chunk[slot]); }, [&] { dec_fail(sm, a, 6); });
   };
   auto act_rows = [&](int ai) { return int(tb.act_off[ai + 1]) - int(tb.act_off[ai]); };
 
@@ -767,7 +746,7 @@ __global__ void __launch_bounds__(kDecThreads, 1)
   auto produce = [&](auto pass, const Pass& p) {
     constexpr int PASS = decltype(pass)::value;
     Runs& r = lruns;
-    first_run(r, p);
+    first_run(r, p, blockIdx.x);
     do {
       Cursor c = cursor_at<PASS>(p, nact, r.lo);
       for (int u = r.lo; u < r.hi; ++u) {
@@ -795,7 +774,7 @@ __global__ void __launch_bounds__(kDecThreads, 1)
     // pass 2: four groups of 64 features in order.
     constexpr uint32_t half = PASS == 1 ? 8192 : 16384, group = PASS == 1 ? 16384 : 8192;
     Runs& r = mruns;
-    first_run(r, p);
+    first_run(r, p, blockIdx.x);
     do {
       Cursor c = cursor_at<PASS>(p, nact, r.lo);
       bool begin = true;
@@ -834,7 +813,7 @@ __global__ void __launch_bounds__(kDecThreads, 1)
         }
         cursor_next<PASS>(c, p, nact);
       }
-    } while (follow_run(r, p));
+    } while (next_chunk(r, p));
   };
 
   // ---- epilogue (8 warps: lane quarter = 32 features of 128; two warps each)
@@ -849,7 +828,7 @@ __global__ void __launch_bounds__(kDecThreads, 1)
   Runs eruns = {0, 0, 0, 0};
   // Every epilogue warp follows the same runs.
   auto next_run = [&](const Pass& p) {
-    const bool more = follow_run(eruns, p);
+    const bool more = next_chunk(eruns, p);
     return p.chunks != 0 && named_bar_and(kBarEpi, kDecEpiWarps * 32, more);
   };
   auto seg_full = [&](int site) {
@@ -888,7 +867,7 @@ __global__ void __launch_bounds__(kDecThreads, 1)
   };
 
   auto epilogue1 = [&](const Pass& p) {
-    first_run(eruns, p);
+    first_run(eruns, p, blockIdx.x);
     do {
       Cursor c = cursor_at<1>(p, nact, eruns.lo);
       for (int u = eruns.lo; u < eruns.hi;) {
@@ -969,7 +948,7 @@ __global__ void __launch_bounds__(kDecThreads, 1)
 
   auto epilogue2 = [&](const Pass& p) {
     const int fl = sub * 128 + quarter * 32 + lane;  // feature within the tile: this thread's alone
-    first_run(eruns, p);
+    first_run(eruns, p, blockIdx.x);
     do {
       Cursor c = cursor_at<2>(p, nact, eruns.lo);
       for (int u = eruns.lo; u < eruns.hi;) {

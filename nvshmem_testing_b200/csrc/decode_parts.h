@@ -12,6 +12,7 @@
 namespace moe {
 
 constexpr int kDecMaxChunks = 640;  // handed out as CTAs get done
+constexpr int kDecRunSlots = 16;    // > stages + 2 accumulators: runs under way in a CTA
 
 // Share of CTA c of `units`, and the CTA a unit belongs to (g CTAs, g <= units;
 // units * g < 2^32).
@@ -76,6 +77,39 @@ MOE_HD Pass make_pass(int T, int G, int cta, int tiles, int tile, int kb, int nt
   p.lo = on ? share_lo(uint32_t(p.fixed), uint32_t(p.g), uint32_t(cta)) : 0;
   p.hi = on ? share_lo(uint32_t(p.fixed), uint32_t(p.g), uint32_t(cta) + 1) : 0;
   return p;
+}
+
+// The runs of units that a CTA does in a pass: its share, then chunks until
+// none is left.  One thread takes them and the other roles follow through a
+// ring of kDecRunSlots; `n` counts a role's chunks over both passes.
+struct Runs {
+  int n;       // chunks seen by this role
+  int lo, hi;  // current run
+  int part;
+};
+MOE_HD void first_run(Runs& r, const Pass& p, int cta) {
+  r.lo = p.lo;
+  r.hi = p.hi;
+  r.part = cta;
+}
+MOE_HD bool set_run(Runs& r, const Pass& p, int chunk) {  // chunk -1: the end
+  r.lo = p.fixed + chunk * p.cz;
+  r.hi = r.lo + p.cz;
+  r.part = p.g + chunk;
+  return chunk >= 0;
+}
+// The next run that the taker left in the ring: wait(slot, parity) waits for
+// it, chunk(slot) reads it.  A wait that gives up is an error, not the end.
+template <typename Wait, typename Chunk, typename Fail>
+MOE_HD bool follow_run(Runs& r, const Pass& p, Wait wait, Chunk chunk, Fail fail) {
+  if (p.chunks == 0) return false;
+  const int slot = r.n % kDecRunSlots;
+  if (!wait(slot, uint32_t(r.n / kDecRunSlots) & 1)) {
+    fail();
+    return false;
+  }
+  ++r.n;
+  return set_run(r, p, chunk(slot));
 }
 
 }  // namespace moe

@@ -50,7 +50,34 @@ static void check(int T, int G, int H, int F, int nact) {
   }
 }
 
+// A role follows the taker's chunks through the ring to the end marker; a
+// chunk that does not come in time is reported.
+static void check_runs() {
+  const int H = 4096, F = 728, nact = 64, G = 148, cta = 5;
+  const Pass p = make_pass(7, G, cta, nact * ((F + 127) / 128), H / 64, H / 64, (F + 127) / 128, true);
+  CHECK(p.chunks > 2 * kDecRunSlots, "%d chunks", p.chunks);
+  for (int given : {p.chunks, 3, 0}) {
+    for (bool end : {true, false}) {
+      Runs r = {0, 0, 0, 0};
+      int waits = 0, fails = 0, seen = 0;
+      const auto wait = [&](int slot, uint32_t parity) {
+        CHECK(slot == waits % kDecRunSlots && parity == uint32_t(waits / kDecRunSlots & 1), "wait %d", waits);
+        return waits++ < given + (end ? 1 : 0);
+      };
+      first_run(r, p, cta);
+      CHECK(r.lo == p.lo && r.hi == p.hi && r.part == cta, "first run");
+      while (follow_run(r, p, wait, [&](int) { return seen < given ? seen : -1; }, [&] { ++fails; })) {
+        CHECK(r.lo == p.fixed + seen * p.cz && r.part == p.part_of(r.lo) && r.part == p.part_of(r.hi - 1), "chunk %d", seen);
+        ++seen;
+      }
+      CHECK(seen == given, "%d of %d chunks", seen, given);
+      CHECK(fails == (end ? 0 : 1), "%d failures reported, end marker %d", fails, int(end));
+    }
+  }
+}
+
 int main() {
+  check_runs();
   const int Ts[] = {1, 7, 32, 33, 64}, Hs[] = {8, 64, 1344, 7168, 32768}, Fs[] = {8, 64, 728, 1408, 14336};
   for (int T : Ts)
     for (int H : Hs)
