@@ -439,9 +439,9 @@ int moe_quant_rows(const void* x, int32_t x_is_f32, int64_t rows, int32_t K, con
  * behind the sum of the counts are left as they were; counts beyond `rows`
  * are cut.  counts == NULL: one expert for all rows.
  * Requires K % 16 == 0, K <= 131056, N % 8 == 0 (16 with swiglu), experts <=
- * 1024; xq, wq, ws, out, x and scratch 16-byte aligned.  scratch:
- * moe_w8a8_scratch_bytes of device memory (may be 0), not initialised, for
- * this call alone until it has finished.
+ * 1024; xq, wq, out, x and scratch 16-byte aligned, the scales 4-byte.
+ * scratch: moe_w8a8_scratch_bytes of device memory (may be 0), not
+ * initialised, for this call alone until it has finished.
  * With x the rows are quantised first, as moe_quant_rows does (x_is_f32,
  * perm, live_rows); xq and xs are then not used. */
 typedef struct moe_w8a8_params {
@@ -474,8 +474,8 @@ int moe_w8a8_gemm(const moe_w8a8_params* params, void* stream);
  * is taken in fp32 in the order of k, or of the experts with few rows.  A few
  * tokens take two launches (two more for large hidden or ffn), others six.
  * Requires hidden and ffn multiples of 16 within moe_w8a8_gemm's K, K <= 32,
- * experts <= 1024; x, w13, w2, y and scratch 16-byte aligned.  scratch:
- * moe_w8a8_layer_scratch_bytes, as above. */
+ * experts <= 1024; x, w13, w2, y and scratch 16-byte aligned, the scales
+ * 4-byte.  scratch: moe_w8a8_layer_scratch_bytes, as above. */
 typedef struct moe_w8a8_layer_params {
   int64_t T;
   int32_t hidden, ffn;

@@ -346,6 +346,9 @@ __device__ __forceinline__ void q_store4(const QArgs& a, int64_t row, int f, flo
   }
 }
 
+// Four neighbouring scales (they are aligned like floats only).
+__device__ __forceinline__ float4 scales4(const float* p) { return make_float4(p[0], p[1], p[2], p[3]); }
+
 // The quotient within 2 steps of 2^-24 (0 where exp(-g) overflows).
 __device__ __forceinline__ float silu_mul(float g, float u) { return __fdividef(g, 1.f + expf(-g)) * u; }
 
@@ -685,8 +688,7 @@ __global__ void __launch_bounds__(kQThreads, 1)
             const int at = j * 64 + (c >> 4) * 32 + (c & 15), f = t.f * 128 + c * 4;
             const int4 g4 = sum4(at), u4 = sum4(at + 16);
             if (f < a.F) {
-              const float4 sg = *reinterpret_cast<const float4*>(sw + f);
-              const float4 su = *reinterpret_cast<const float4*>(sw + a.F + f);
+              const float4 sg = scales4(sw + f), su = scales4(sw + a.F + f);
               q_store4(a, t.r0 + j, f, silu_mul(float(g4.x) * xv * sg.x, float(u4.x) * xv * su.x),
                        silu_mul(float(g4.y) * xv * sg.y, float(u4.y) * xv * su.y),
                        silu_mul(float(g4.z) * xv * sg.z, float(u4.z) * xv * su.z),
@@ -696,7 +698,7 @@ __global__ void __launch_bounds__(kQThreads, 1)
             const int f = t.f * 256 + c * 4;
             const int4 z = sum4(j * 64 + c);
             if (f < a.N) {
-              const float4 s4 = *reinterpret_cast<const float4*>(sw + f);
+              const float4 s4 = scales4(sw + f);
               q_store4(a, t.r0 + j, f, float(z.x) * xv * s4.x, float(z.y) * xv * s4.y, float(z.z) * xv * s4.z,
                        float(z.w) * xv * s4.w);
             }
@@ -1215,6 +1217,7 @@ int sm_count(int* sms, int* device = nullptr) {
 }
 
 bool misaligned16(const void* p) { return (reinterpret_cast<uintptr_t>(p) & 15) != 0; }
+bool misaligned4(const void* p) { return (reinterpret_cast<uintptr_t>(p) & 3) != 0; }
 
 size_t q_smem_bytes(int E) {
   return 1024 + size_t(kQStages) * kQStageBytes + kQXBytes + sizeof(QSmem) + size_t(E + 1) * 8;
@@ -1380,8 +1383,8 @@ extern "C" int moe_w8a8_gemm(const moe_w8a8_params* p, void* stream) {
   if (p->rows == 0) return kOk;
   if ((!p->x && (!p->xq || !p->xs)) || !p->wq || !p->ws || !p->out || (!p->counts && p->experts != 1)) return kBadArg;
   if (misaligned16(p->x)) return kBadArg;
-  if (misaligned16(p->xq) || misaligned16(p->wq) || misaligned16(p->ws) || misaligned16(p->out) ||
-      misaligned16(p->scratch))
+  if (misaligned16(p->xq) || misaligned16(p->wq) || misaligned16(p->out) || misaligned16(p->scratch) ||
+      misaligned4(p->xs) || misaligned4(p->ws))
     return kBadArg;
   if (!driver().ok) return kCudaErr;
   int sms = 0, dev = 0;
@@ -1597,7 +1600,7 @@ extern "C" int moe_w8a8_layer(const moe_w8a8_layer_params* p, void* stream) {
       !p->scratch)
     return kBadArg;
   if (misaligned16(p->x) || misaligned16(p->w13) || misaligned16(p->w2) || misaligned16(p->y) ||
-      misaligned16(p->scratch))
+      misaligned16(p->scratch) || misaligned4(p->w13_scale) || misaligned4(p->w2_scale))
     return kBadArg;
   int sms = 0, dev = 0;
   if (sm_count(&sms, &dev) != kOk) return kCudaErr;

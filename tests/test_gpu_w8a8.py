@@ -358,6 +358,34 @@ def test_misaligned_and_misplaced_tensors_are_refused():
             w8a8.moe_layer(**{**dict(x=x, top_idxs=ids, top_vals=vals, w13=w, w2=w2), **bad})
 
 
+@pytest.mark.parametrize("T", [2, 40])
+def test_scales_at_any_float(T):
+    """Scales need no more than a float's alignment, for any number of tokens."""
+    g = torch.Generator(device="cuda").manual_seed(T)
+    El, H, K, F = 3, 256, 2, 128
+    x = torch.randn(T, H, generator=g, device="cuda").to(torch.bfloat16)
+    w13 = w8a8.quantize_weights(0.05 * torch.randn(El, H, 2 * F, generator=g, device="cuda"))
+    w2 = w8a8.quantize_weights(0.05 * torch.randn(El, F, H, generator=g, device="cuda"))
+
+    def odd(w):
+        flat = torch.zeros(w.scale.numel() + 1, device="cuda")
+        flat[1:] = w.scale.flatten()
+        return w8a8.QuantWeights(w.q, flat[1:].view(w.scale.shape))
+
+    assert odd(w13).scale.data_ptr() % 16 == 4
+    ids = torch.rand(T, El, generator=g, device="cuda").topk(K, dim=-1).indices
+    vals = torch.rand(T, K, generator=g, device="cuda")
+    y = w8a8.moe_layer(x, ids, vals, w13, w2)
+    assert torch.equal(w8a8.moe_layer(x, ids, vals, odd(w13), odd(w2)), y)
+    for rows, counts in ((5, [2, 0, 3]), (330, [200, 0, 130]), (9000, [4000, 2000, 3000])):
+        xq = torch.randint(-127, 128, (rows, H), generator=g, device="cuda", dtype=torch.int8)
+        xs = torch.rand(rows + 1, generator=g, device="cuda")
+        cd = torch.tensor(counts, dtype=torch.int32, device="cuda")
+        for glu in (False, True):
+            ref = w8a8.grouped_gemm(xq, xs[1:].clone(), w13, cd, swiglu=glu)
+            assert torch.equal(w8a8.grouped_gemm(xq, xs[1:], odd(w13), cd, swiglu=glu), ref)
+
+
 def test_layer_captured_and_on_streams():
     g = torch.Generator(device="cuda").manual_seed(6)
     T, H, E, K, F = 24, 256, 8, 2, 128

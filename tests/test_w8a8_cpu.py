@@ -74,3 +74,21 @@ def test_c_entries_refuse_before_any_device_call():
     assert lib.moe_weighted_sum(None, 0, None, 1, 0, None, 0, None, None, 4, 2, 64, 2, None, None) == N.BAD_ARG
     assert lib.moe_weighted_sum(None, 0, None, 1, 0, None, 0, None, None, 4, 33, 64, 2, None, None) == N.BAD_ARG
     assert lib.moe_weighted_sum(None, 0, None, 1, 0, None, 0, None, None, 0, 2, 64, 2, None, None) == N.OK
+
+
+def test_c_entries_refuse_scales_that_are_no_floats():
+    buf = ctypes.create_string_buffer(64)
+    at = (ctypes.addressof(buf) + 15) // 16 * 16
+    lib = N.lib()
+    for bad in ("xs", "ws"):
+        p = N.W8A8Params()
+        p.rows, p.K, p.N, p.experts = 4, 64, 64, 1
+        for f in ("xq", "xs", "wq", "ws", "out", "scratch"):
+            setattr(p, f, at + 2 * (f == bad))
+        assert lib.moe_w8a8_gemm(ctypes.byref(p), None) == N.BAD_ARG
+    for bad in ("w13_scale", "w2_scale"):
+        p = N.W8A8LayerParams()
+        p.T, p.hidden, p.ffn, p.experts, p.K = 4, 64, 64, 2, 1
+        for f in ("x", "w13", "w13_scale", "w2", "w2_scale", "top_idxs", "top_vals", "y", "scratch"):
+            setattr(p, f, at + 2 * (f == bad))
+        assert lib.moe_w8a8_layer(ctypes.byref(p), None) == N.BAD_ARG
