@@ -78,6 +78,11 @@ def _on_gpu(device, **tensors):
             raise ValueError(f"{name} must be on {device}")
 
 
+def _check_status(status):
+    if status is not None and (status.dtype != torch.int32 or status.numel() != 1 or not status.is_pinned()):
+        raise ValueError("status must be one pinned int32")
+
+
 def quantize_rows(x: torch.Tensor, perm: torch.Tensor | None = None,
                   live_rows: torch.Tensor | None = None) -> tuple[torch.Tensor, torch.Tensor]:
     """``(q [rows, K] int8, scale [rows] float32)`` of x [n, K], bf16 or fp32.
@@ -141,7 +146,8 @@ def grouped_gemm(xq: torch.Tensor, xs: torch.Tensor, w: QuantWeights, counts: to
     multiple of 16.  With ``swiglu`` w's channels are gate [0, N/2) and up
     [N/2, N) and ``out [rows, N/2] = silu(gate) * up``.  Rows behind the last
     expert's are left as they were (``out`` supplies the buffer).
-    ``out_dtype`` is bfloat16 or float32."""
+    ``out_dtype`` is bfloat16 or float32; ``status`` (one pinned int32)
+    receives a device-side error word, if any."""
     El, Nw, K = _check_weights(w, "w", xq.device)
     if xq.dim() != 2 or xq.shape[1] != K or tuple(xs.shape) != (xq.shape[0],):
         raise ValueError(f"xq {tuple(xq.shape)} and xs {tuple(xs.shape)} do not match w {tuple(w.q.shape)}")
@@ -160,8 +166,7 @@ def grouped_gemm(xq: torch.Tensor, xs: torch.Tensor, w: QuantWeights, counts: to
         out = torch.empty((rows, cols), dtype=out_dtype, device=xq.device)
     elif tuple(out.shape) != (rows, cols) or out.dtype != out_dtype or not out.is_contiguous():
         raise ValueError(f"out must be a contiguous {out_dtype} tensor of shape {(rows, cols)}")
-    if status is not None and (status.dtype != torch.int32 or status.numel() != 1 or not status.is_pinned()):
-        raise ValueError("status must be one pinned int32")
+    _check_status(status)
     _on_gpu(xq.device, xs=xs, counts=counts, out=out)
     if rows == 0:
         return out
@@ -183,9 +188,10 @@ def _gemm(xq, xs, x, w, counts, rows, K, Nw, El, swiglu, out, status, stream):
     N.check(N.lib().moe_w8a8_gemm(ctypes.byref(p), stream), "moe_w8a8_gemm")
 
 
-def linear(x: torch.Tensor, w: QuantWeights, *, out_dtype=torch.bfloat16) -> torch.Tensor:
+def linear(x: torch.Tensor, w: QuantWeights, *, out_dtype=torch.bfloat16,
+           status: torch.Tensor | None = None) -> torch.Tensor:
     """``x [rows, K] @ w`` for one weight matrix (w.q [1, N, K]): quantises the
-    rows and multiplies."""
+    rows and multiplies.  ``status`` is grouped_gemm's."""
     El, Nw, K = _check_weights(w, "w", x.device)
     if El != 1:
         raise ValueError(f"one weight matrix [1, N, K] is required, got {tuple(w.q.shape)}")
@@ -194,12 +200,13 @@ def linear(x: torch.Tensor, w: QuantWeights, *, out_dtype=torch.bfloat16) -> tor
     _check_product(K, Nw, El, False)
     if out_dtype not in (torch.bfloat16, torch.float32):
         raise TypeError("out_dtype must be bfloat16 or float32")
+    _check_status(status)
     _on_gpu(x.device)
     rows = x.shape[0]
     out = torch.empty((rows, Nw), dtype=out_dtype, device=x.device)
     if rows:
         with utils.on_device(x.device) as stream:
-            _gemm(None, None, x.contiguous(), w, None, rows, K, Nw, 1, False, out, None, stream)
+            _gemm(None, None, x.contiguous(), w, None, rows, K, Nw, 1, False, out, status, stream)
     return out
 
 
@@ -244,7 +251,7 @@ def moe_layer(x: torch.Tensor, top_idxs: torch.Tensor, top_vals: torch.Tensor, w
 
     x [T, H] bf16, top_idxs [T, K] int32/int64, top_vals [T, K] float32 or
     bfloat16; w13.q [El, 2F, H] (gate channels [0, F), up after them) and w2.q
-    [El, H, F].  H and F multiples of 16."""
+    [El, H, F].  H and F multiples of 16.  ``status`` is grouped_gemm's."""
     dev = x.device
     El, F2, H = _check_weights(w13, "w13", dev)
     _check_weights(w2, "w2", dev)
@@ -260,8 +267,7 @@ def moe_layer(x: torch.Tensor, top_idxs: torch.Tensor, top_vals: torch.Tensor, w
         raise TypeError("top_idxs must be int32 or int64")
     if top_vals.dtype not in (torch.float32, torch.bfloat16):
         raise TypeError("top_vals must be float32 or bfloat16")
-    if status is not None and (status.dtype != torch.int32 or status.numel() != 1 or not status.is_pinned()):
-        raise ValueError("status must be one pinned int32")
+    _check_status(status)
     if not 0 <= first_expert < 1 << 31:
         raise ValueError(f"first_expert = {first_expert} must be an expert's id")
     _on_gpu(dev, top_idxs=top_idxs, top_vals=top_vals)

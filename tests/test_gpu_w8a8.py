@@ -453,6 +453,18 @@ def test_a_decode_step_with_both_operators(T):
         assert bool(((logits.double() - ref).abs() <= ref.abs() * (HALF + 2.0 ** -20)).all())
 
 
+@pytest.mark.parametrize("rows", [1, 20, 600])
+def test_status_word_stays_clear(rows):
+    g = torch.Generator(device="cuda").manual_seed(rows)
+    x = torch.randn(rows, 256, generator=g, device="cuda").to(torch.bfloat16)
+    w = w8a8.quantize_weights(torch.randn(1, 256, 512, generator=g, device="cuda"))
+    status = torch.zeros(1, dtype=torch.int32, pin_memory=True)
+    assert torch.equal(w8a8.linear(x, w, status=status), w8a8.linear(x, w))
+    w8a8.grouped_gemm(*w8a8.quantize_rows(x), w, status=status)
+    torch.cuda.synchronize()
+    assert int(status[0]) == 0
+
+
 def test_weighted_sum_uses_the_routing():
     g = torch.Generator(device="cuda").manual_seed(8)
     T, E, K, H = 50, 6, 3, 72

@@ -92,3 +92,14 @@ def test_c_entries_refuse_scales_that_are_no_floats():
         for f in ("x", "w13", "w13_scale", "w2", "w2_scale", "top_idxs", "top_vals", "y", "scratch"):
             setattr(p, f, at + 2 * (f == bad))
         assert lib.moe_w8a8_layer(ctypes.byref(p), None) == N.BAD_ARG
+
+
+@pytest.mark.parametrize("status", [torch.zeros(1), torch.zeros(2, dtype=torch.int32), torch.zeros(1, dtype=torch.int32)])
+def test_every_product_takes_a_pinned_status_word(status):
+    x = torch.zeros(2, 64, dtype=torch.bfloat16)
+    for call in (lambda: w8a8.linear(x, weights(E=1), status=status),
+                 lambda: w8a8.grouped_gemm(*rows(), weights(), C, status=status),
+                 lambda: w8a8.moe_layer(x, torch.zeros(2, 1, dtype=torch.int64), torch.zeros(2, 1), weights(Nn=32),
+                                        weights(Nn=64, K=16), status=status)):
+        with pytest.raises(ValueError, match="status"):
+            call()
