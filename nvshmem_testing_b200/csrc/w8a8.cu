@@ -349,8 +349,12 @@ __device__ __forceinline__ void q_store4(const QArgs& a, int64_t row, int f, flo
 // Four neighbouring scales (they are aligned like floats only).
 __device__ __forceinline__ float4 scales4(const float* p) { return make_float4(p[0], p[1], p[2], p[3]); }
 
-// The quotient within 2 steps of 2^-24 (0 where exp(-g) overflows).
-__device__ __forceinline__ float silu_mul(float g, float u) { return __fdividef(g, 1.f + expf(-g)) * u; }
+// The quotient within 2 steps of 2^-24 (0 where exp(-g) overflows).  Both
+// sides are taken by 8: the fast division gives 0 for every divisor above
+// 2^126, gates under -87.3, whose silu a large u brings back.
+__device__ __forceinline__ float silu_mul(float g, float u) {
+  return __fdividef(0.125f * g, fmaf(0.125f, expf(-g), 0.125f)) * u;
+}
 
 template <bool GLU, bool SPLIT>
 __global__ void __launch_bounds__(kQThreads, 1)

@@ -162,6 +162,26 @@ def test_products(K, Nn, counts, swiglu):
         assert torch.equal(out, w8a8.grouped_gemm(xq, xs, w, cd, swiglu=swiglu, out_dtype=dt))
 
 
+@pytest.mark.parametrize("rows,K", [(1, 16), (40, 16), (40, 8192), (9000, 16)])
+def test_swiglu_of_far_gates(rows, K):
+    """silu's values are far below 1 at gates of -80 to -88, not zero: a large
+    up value brings them back."""
+    gates = torch.arange(80, 88.7, 0.1, device="cuda")
+    Nn = 2 * ((gates.numel() + 7) // 8 * 8)
+    ws = torch.full((1, Nn), 1e30, device="cuda")
+    ws[0, :Nn // 2] = -1.0
+    ws[0, :gates.numel()] = -gates
+    wq = torch.zeros(1, Nn, K, dtype=torch.int8, device="cuda")
+    wq[..., 0] = 1
+    xq = torch.zeros(rows, K, dtype=torch.int8, device="cuda")
+    xq[:, 0] = 1
+    out = w8a8.grouped_gemm(xq, torch.ones(rows, device="cuda"), w8a8.QuantWeights(wq, ws), swiglu=True,
+                            out_dtype=torch.float32)
+    a = ws[0].double()
+    ref = a[:Nn // 2] * torch.sigmoid(a[:Nn // 2]) * a[Nn // 2:]
+    assert bool(((out.double() - ref).abs() <= ref.abs() * 2.0 ** -20).all())
+
+
 def test_many_experts_mostly_empty():
     counts = [0] * 1024
     for e in (0, 5, 511, 512, 1000, 1023):
