@@ -335,6 +335,47 @@ def test_router_with_non_finite_tokens():
     assert bool(((ids >= 0) & (ids < E)).all()) and bool(y[2].isnan().all())
 
 
+@pytest.mark.parametrize("E", [16, 200])  # both ways to find the largest
+@pytest.mark.parametrize("T", [1, 7])
+@pytest.mark.parametrize("renormalize", [False, True])
+def test_router_with_infinite_logits(T, E, renormalize):
+    """Logits of minus infinity have weight 0 and come last, by id; plus
+    infinity comes first and leaves no softmax (NaN weights, valid ids), as
+    the softmax's definition has it; a token's row concerns itself only."""
+    H, K, F = 256, 6, 64
+    x, _, _, w13, w2 = make(T, H, 4, 1, F, E)
+    x = x.abs() + 1
+    rw = (0.1 * torch.randn(H, E, generator=torch.Generator(device="cuda").manual_seed(E), device="cuda")).to(
+        torch.bfloat16)
+    finite = [3, 5, 11, E - 2]
+    low = torch.full_like(rw, float("-inf"))
+    low[:, finite] = rw[:, finite]
+    y, vals, ids = decode.routed_layer(x, low, K, w13, w2, renormalize=renormalize)
+    logits = x.double() @ low.double()
+    prob = torch.softmax(logits, -1)  # of the four finite ones
+    for t in range(T):
+        assert sorted(ids[t, :4].tolist()) == sorted(finite)
+        assert ids[t, 4:].tolist() == [0, 1]  # of the rest the lowest ids
+    # fp32 logits (each off by `slack` at most), expf, the sum and the division
+    slack = (x.double().abs() @ rw.double().abs()).amax() * (H + 4) * 2.0 ** -24
+    rel = torch.expm1(4 * slack) + (E + K + 16) * 2.0 ** -23
+    assert bool(((vals.double() - prob.gather(1, ids)).abs() <= prob.gather(1, ids) * rel).all())
+    check(y, x, ids, vals, w13, w2)
+    high = rw.clone()
+    high[:, E // 2] = float("inf")
+    y, vals, ids = decode.routed_layer(x, high, K, w13, w2, renormalize=renormalize)
+    assert bool((ids[:, 0] == E // 2).all()) and bool(vals.isnan().all())
+    assert bool(((ids >= 0) & (ids < E)).all()) and all(len(set(r)) == K for r in ids.tolist())
+    if T > 1:  # one token's infinity
+        x2 = x.clone()
+        x2[2, 9] = float("inf")
+        ref = decode.routed_layer(x, rw, K, w13, w2, renormalize=renormalize)
+        got = decode.routed_layer(x2, rw, K, w13, w2, renormalize=renormalize)
+        keep = [t for t in range(T) if t != 2]
+        assert all(torch.equal(a[keep], b[keep]) for a, b in zip(got, ref))
+        assert bool(((got[2] >= 0) & (got[2] < E)).all()) and bool(got[1][2].isnan().all())
+
+
 def test_status_word_stays_clear():
     x, ids, vals, w13, w2 = make(4, 128, 4, 2, 64, 6)
     status = torch.zeros(1, dtype=torch.int32, pin_memory=True)
