@@ -335,6 +335,46 @@ def test_layer(T, H, El, E, first, K, F):
         assert not y[1].any()
 
 
+MIXED = [
+    # T, H, El, E, first, K, F
+    (4, 4096, 8, 16, 4, 2, 14336),    # gate and up by rows, gathered and quantised in place; down by tiles
+    (1, 2048, 64, 64, 0, 8, 16384),   # the same, every row live
+    (4, 2048, 32, 32, 0, 8, 4096),    # gathered and quantised by a launch of its own, multiplied by rows
+    (4, 32768, 4, 6, 1, 2, 128),      # gate and up by tiles; down by rows, h quantised in place
+    (24, 4112, 12, 14, 1, 1, 2048),   # the same, h quantised by a launch of its own
+]
+
+
+@pytest.mark.parametrize("none", [False, True])
+@pytest.mark.parametrize("T,H,El,E,first,K,F", MIXED)
+def test_layer_of_both_forms(T, H, El, E, first, K, F, none):
+    """Sizes at which one product of the layer takes the form for a few rows
+    and the other one tiles, with rows for experts elsewhere (the live rows
+    end before the last) and without any live row."""
+    g = torch.Generator(device="cuda").manual_seed(T + F)
+
+    def weights(Nn, K8):
+        q = torch.randint(-127, 128, (El, Nn, K8), generator=g, device="cuda", dtype=torch.int8)
+        return w8a8.QuantWeights(q, (0.5 + torch.rand(El, Nn, generator=g, device="cuda")) * 2.0 ** -11)
+
+    w13, w2 = weights(2 * F, H), weights(H, F)
+    x = torch.randn(T, H, generator=g, device="cuda").to(torch.bfloat16)
+    ids = torch.rand(T, E, generator=g, device="cuda").topk(K, dim=-1).indices
+    vals = torch.randn(T, K, generator=g, device="cuda").softmax(-1)
+    if none:
+        ids += first + El
+    elif El < E:
+        ids[-1, 0] = first + El
+    y = w8a8.moe_layer(x, ids, vals, w13, w2, first_expert=first)
+    if none:
+        assert not y.any()
+        return
+    ref, tol = layer_ref(x, ids, vals, w13, w2, first)
+    err = (y.double() - ref).abs()
+    assert bool((err <= tol).all()), f"{int((err > tol).sum())} of {err.numel()}, worst {float((err / tol).max()):.2f}x"
+    assert torch.equal(y, w8a8.moe_layer(x, ids, vals, w13, w2, first_expert=first))
+
+
 @pytest.mark.parametrize("T", [3, 40])
 @pytest.mark.parametrize("dt", [torch.int32, torch.int64])
 @pytest.mark.parametrize("first", [0, 5, 2 ** 31 - 3])
@@ -433,6 +473,36 @@ def test_layer_captured_and_on_streams():
         eager = w8a8.moe_layer(x, ids, vals, w13, w2)
         torch.cuda.synchronize()
         assert torch.equal(outs[0], eager) and torch.equal(outs[1], eager)
+
+
+def test_kernels_with_grid_barriers_side_by_side():
+    """The decode layer, an 8-bit product split over K and one of whole tiles
+    on three streams at once: each has the result that it has alone."""
+    g = torch.Generator(device="cuda").manual_seed(11)
+    T, H, E, K, F = 20, 1024, 16, 4, 512
+    x = torch.randn(T, H, generator=g, device="cuda").to(torch.bfloat16)
+    w13 = (0.05 * torch.randn(E, H, 2 * F, generator=g, device="cuda")).to(torch.bfloat16)
+    w2 = (0.05 * torch.randn(E, F, H, generator=g, device="cuda")).to(torch.bfloat16)
+    ids = torch.rand(T, E, generator=g, device="cuda").topk(K, dim=-1).indices
+    vals = torch.rand(T, K, generator=g, device="cuda")
+    split = make(100, 7168, 512, 2, 12)     # two tiles of rows, two of channels: shares of K
+    whole = make(9000, 512, 4096, 1, 13)    # enough tiles for every SM
+    counts = torch.tensor([61, 39], dtype=torch.int32, device="cuda")
+    calls = [lambda: decode.moe_layer(x, ids, vals, w13, w2),
+             lambda: w8a8.grouped_gemm(*split[:2], w8a8.QuantWeights(*split[2:]), counts),
+             lambda: w8a8.grouped_gemm(*whole[:2], w8a8.QuantWeights(*whole[2:]))]
+    want = [c() for c in calls]
+    streams = [torch.cuda.Stream() for _ in calls]
+    torch.cuda.synchronize()
+    for _ in range(8):
+        got = [[] for _ in calls]
+        for _ in range(3):
+            for c, s, o in zip(calls, streams, got):
+                with torch.cuda.stream(s):
+                    o.append(c())
+        torch.cuda.synchronize()
+        for w, o in zip(want, got):
+            assert all(torch.equal(a, w) for a in o)
 
 
 @pytest.mark.parametrize("T", [1, 6, 40])
