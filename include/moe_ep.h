@@ -380,7 +380,9 @@ int moe_ep_run_compact_swiglu(const moe_ep_run_params* params, int64_t send_rows
  * row, so that ranks holding parts of the experts add their y's.
  *   w13 [experts, hidden, 2*ffn] bf16: gate columns [0, ffn), up after them
  *   w2  [experts, ffn, hidden] bf16
- * Sums are fp32; silu(gate) * up is rounded once to bf16 and y once.
+ * Sums are fp32; silu(gate) * up enters the second product as the sum of two
+ * bf16 values (off by 2^-16 of itself at most; so an infinite weight of w2
+ * may leave NaN in its column) and y is rounded once.
  * With router_w ([hidden, router_experts] bf16; NULL: none) the call also
  * chooses the experts: logits = x @ router_w kept in fp32, softmax over
  * router_experts, the K largest (equal logits: lowest id first), written to

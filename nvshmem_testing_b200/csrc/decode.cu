@@ -11,12 +11,19 @@
 //   pass 1  units (active expert, 128 features of F, 64 of H): the gate and
 //           the up block (2 x 128 features) are the MMA A operand
 //           (tcgen05, M = 128 each, feature-contiguous as stored), all T
-//           tokens the B operand; h = silu(gate) * up is written, in bf16,
-//           for the tokens that chose the expert only.
+//           tokens the B operand; h = silu(gate) * up is written for the
+//           tokens that chose the expert only.
 //   pass 2  units (256 features of H, active expert, 64 of F): the rows of
 //           h of one expert are B; the epilogue adds v * D to an fp32 sum
 //           per token and feature in shared memory, so that the experts'
 //           outputs meet without leaving the CTA.
+// h passes as two bf16 values, its rounding and what that leaves: beside bf16
+// weights the MMA takes bf16 only, and one value alone would double the
+// squared error of the result (2-norm 0.0023; with two 0.0017, the rounding
+// of y).  An expert's n rows and their n remainders lie next to each other,
+// so that up to eight rows per expert are one 16-row block as before (one
+// token, 64 experts: 35.6 -> 35.9 us; 48 tokens over 16 experts: 68.9 -> 69.9;
+// 64 rows in each of four experts: 80.5 -> 83).
 // Each pass splits its list of 32 KB units evenly over the CTAs, at any k:
 // every SM streams the same number of bytes whatever the number of experts
 // or tiles.  SMs do not get the same bandwidth, though (those of the fuller
@@ -68,6 +75,7 @@ constexpr int kBarEpi = 1;
 struct DecArgs {
   int T, H, F, E, K, first;  // E: experts held here
   int NB;                    // T rounded to 16: B rows and MMA N of pass 1
+  int NB2;                   // 2 * T rounded to 16: the most of pass 2
   int stages;
   uint32_t stage_bytes, scratch_bytes;
   int maxact;                // min(E, T * K)
@@ -75,7 +83,7 @@ struct DecArgs {
   const void* ids;
   const void* vals;
   int ids64, vals_bf16;
-  __nv_bfloat16* hs;         // [T*K][F]
+  __nv_bfloat16* hs;         // [2*T*K][F]: an expert's n rows, then their remainders
   float* part;               // [2 * (grid + kDecMaxChunks)][T][256]
   uint32_t* ctr;             // [grid + kDecMaxChunks] tickets of pass 1's split tiles, [2] chunks handed out
   __nv_bfloat16* y;
@@ -129,6 +137,32 @@ __device__ __noinline__ void dec_fail(DecSmem& sm, const DecArgs& a, int detail)
 }
 
 __device__ __forceinline__ float silu_mul(float g, float u) { return g / (1.f + expf(-g)) * u; }
+
+// h as the sum of two bf16 values: its rounding, and what that leaves (nothing
+// where it left the finite numbers).
+__device__ __forceinline__ __nv_bfloat16 rest_of(float h, __nv_bfloat16 hi) {
+  const float r = h - __bfloat162float(hi);
+  return __float2bfloat16_rn(fabsf(r) < INFINITY ? r : 0.f);
+}
+__device__ __forceinline__ void store_h(__nv_bfloat16* at, size_t to_rest, float h) {
+  const __nv_bfloat16 hi = __float2bfloat16_rn(h);
+  at[0] = hi;
+  at[to_rest] = rest_of(h, hi);
+}
+__device__ __forceinline__ void store_h4(__nv_bfloat16* at, size_t to_rest, float4 g, float4 u) {
+  const float h[4] = {silu_mul(g.x, u.x), silu_mul(g.y, u.y), silu_mul(g.z, u.z), silu_mul(g.w, u.w)};
+  __nv_bfloat16 hi[4], lo[4];
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    hi[i] = __float2bfloat16_rn(h[i]);
+    lo[i] = rest_of(h[i], hi[i]);
+  }
+#pragma unroll
+  for (int i = 0; i < 4; i += 2) {
+    *reinterpret_cast<__nv_bfloat162*>(at + i) = __nv_bfloat162(hi[i], hi[i + 1]);
+    *reinterpret_cast<__nv_bfloat162*>(at + to_rest + i) = __nv_bfloat162(lo[i], lo[i + 1]);
+  }
+}
 
 // Adds the values of the lane `o` away to this lane's (the same sum in both).
 __device__ __forceinline__ void add_xor(float4& v, int o) {
@@ -620,7 +654,7 @@ __global__ void __launch_bounds__(kDecThreads, 1)
     prefetch_tensormap(&tm_w2);
     prefetch_tensormap(&tm_h);
   }
-  const uint32_t tmem_cols = a.NB <= 16 ? 64 : a.NB <= 32 ? 128 : 256;
+  const uint32_t tmem_cols = a.NB2 <= 16 ? 64 : a.NB2 <= 32 ? 128 : a.NB2 <= 64 ? 256 : 512;
   if (warp == 1) {
     __syncwarp();
     tmem_alloc(&sm.tmem_base, tmem_cols);
@@ -681,6 +715,7 @@ __global__ void __launch_bounds__(kDecThreads, 1)
         [&](int slot) { return *reinterpret_cast<volatile int*>(&sm.chunk[slot]); }, [&] { dec_fail(sm, a, 6); });
   };
   auto act_rows = [&](int ai) { return int(tb.act_off[ai + 1]) - int(tb.act_off[ai]); };
+  auto blocks2 = [&](int ai) { return (2 * act_rows(ai) + 15) >> 4; };  // of 16 B rows in pass 2
 
   // ---- loads (one thread)
   Ring lr = {0, 0};  // next stage to fill
@@ -707,7 +742,7 @@ __global__ void __launch_bounds__(kDecThreads, 1)
     } else {
       // One box of four atoms of 64 features; a tile whose last atom is a part
       // of one atom by atom, clipped at the row's end.
-      mbar_arrive_expect_tx(full, kDecABytes + uint32_t((act_rows(c.ai) + 15) >> 4) * 2048);
+      mbar_arrive_expect_tx(full, kDecABytes + uint32_t(blocks2(c.ai)) * 2048);
       if (c.ft * 4 + 4 <= a.H / 64) {
         tma_load_4d_hint(&tm_w2, full, dst, 0, c.k * 64, c.ft * 4, e, once);
       } else {
@@ -727,7 +762,7 @@ __global__ void __launch_bounds__(kDecThreads, 1)
     if constexpr (PASS == 1) {
       tma_load_2d(&tm_x, full, dst, c.k * 64, 0);
     } else {
-      const int r0 = tb.act_off[c.ai], nb = (act_rows(c.ai) + 15) >> 4;
+      const int r0 = 2 * tb.act_off[c.ai], nb = blocks2(c.ai);
       for (int b = 0; b < nb; ++b) tma_load_2d(&tm_h, full, dst + b * 2048, c.k * 64, r0 + b * 16);
     }
   };
@@ -785,7 +820,7 @@ __global__ void __launch_bounds__(kDecThreads, 1)
             dec_fail(sm, a, 2);
             return;
           }
-          const int n = PASS == 1 ? a.NB : (act_rows(c.ai) + 15) / 16 * 16;
+          const int n = PASS == 1 ? a.NB : blocks2(c.ai) * 16;
           idesc = make_idesc_mn(/*bf16*/ 1, 128, uint32_t(n), /*A MN-major*/ 1, /*B K-major*/ 0);
         }
         if (!dec_wait(&sm.full[mr.st], mr.ph, sm)) {
@@ -794,14 +829,14 @@ __global__ void __launch_bounds__(kDecThreads, 1)
         }
         tc_fence_after();
         const uint32_t aa = smem_u32(stage + uint32_t(mr.st) * a.stage_bytes), ba = aa + kDecABytes;
-        const uint32_t d = tmem + uint32_t(mseg.st) * 2 * uint32_t(a.NB);
+        const uint32_t d = tmem + uint32_t(mseg.st) * 2 * uint32_t(a.NB2);
 #pragma unroll
         for (int kk = 0; kk < 4; ++kk) {
           const uint64_t bd = smem_desc_sw128(ba + kk * 32, 16, 1024);
 #pragma unroll
           for (int h = 0; h < 2; ++h) {
             const uint64_t ad = smem_desc_sw128(aa + h * half + kk * 2048, group, 1024);
-            tc_mma_f16(d + h * uint32_t(a.NB), ad, bd, idesc, (!begin || kk != 0) ? 1u : 0u);
+            tc_mma_f16(d + h * uint32_t(a.NB2), ad, bd, idesc, (!begin || kk != 0) ? 1u : 0u);
           }
         }
         tc_commit(&sm.empty[mr.st]);
@@ -859,9 +894,7 @@ __global__ void __launch_bounds__(kDecThreads, 1)
       const float4 g = sum_parts<float4>(c0, c1, at);
       const float4 u = sum_parts<float4>(c0, c1, [&](int q) { return at(q) + 32; });
       if (f < a.F) {
-        __nv_bfloat162* o = reinterpret_cast<__nv_bfloat162*>(a.hs + size_t(tb.act_off[ai] + j) * a.F + f);
-        o[0] = __floats2bfloat162_rn(silu_mul(g.x, u.x), silu_mul(g.y, u.y));
-        o[1] = __floats2bfloat162_rn(silu_mul(g.z, u.z), silu_mul(g.w, u.w));
+        store_h4(a.hs + size_t(2 * tb.act_off[ai] + j) * a.F + f, size_t(act_rows(ai)) * a.F, g, u);
       }
     }
   };
@@ -878,7 +911,7 @@ __global__ void __launch_bounds__(kDecThreads, 1)
         const int n = act_rows(c.ai), r0 = tb.act_off[c.ai];
         const int fl = quarter * 32 + lane;              // feature within the tile
         const int f = c.ft * 128 + fl;
-        const uint32_t d = tlane + uint32_t(eseg.st) * 2 * uint32_t(a.NB);
+        const uint32_t d = tlane + uint32_t(eseg.st) * 2 * uint32_t(a.NB2);
         float* mine = slot(eruns.part, c.k == 0 ? 1 : 0);
         for (int j0 = sub; j0 < n; j0 += 8) {
           uint32_t g[4], w[4];
@@ -887,7 +920,7 @@ __global__ void __launch_bounds__(kDecThreads, 1)
             if (j0 + 2 * q < n) {
               const uint32_t t = tb.tok[r0 + j0 + 2 * q];
               g[q] = tmem_ld_32x32b_x1(d + t);
-              w[q] = tmem_ld_32x32b_x1(d + uint32_t(a.NB) + t);
+              w[q] = tmem_ld_32x32b_x1(d + uint32_t(a.NB2) + t);
             }
           tmem_ld_wait();
 #pragma unroll
@@ -896,7 +929,7 @@ __global__ void __launch_bounds__(kDecThreads, 1)
             if (j >= n) break;
             const float gv = __uint_as_float(g[q]), uv = __uint_as_float(w[q]);
             if (whole) {
-              if (f < a.F) a.hs[size_t(r0 + j) * a.F + f] = __float2bfloat16_rn(silu_mul(gv, uv));
+              if (f < a.F) store_h(a.hs + size_t(2 * r0 + j) * a.F + f, size_t(n) * a.F, silu_mul(gv, uv));
             } else {
               mine[j * 256 + fl] = gv;
               mine[j * 256 + 128 + fl] = uv;
@@ -933,9 +966,7 @@ __global__ void __launch_bounds__(kDecThreads, 1)
               w.z = __shfl_xor_sync(0xffffffffu, v.z, 1);
               w.w = __shfl_xor_sync(0xffffffffu, v.w, 1);
               if (j < n && upper == 0 && qt == 0 && f4 < a.F) {
-                __nv_bfloat162* o = reinterpret_cast<__nv_bfloat162*>(a.hs + size_t(r0 + j) * a.F + f4);
-                o[0] = __floats2bfloat162_rn(silu_mul(v.x, w.x), silu_mul(v.y, w.y));
-                o[1] = __floats2bfloat162_rn(silu_mul(v.z, w.z), silu_mul(v.w, w.w));
+                store_h4(a.hs + size_t(2 * r0 + j) * a.F + f4, size_t(n) * a.F, v, w);
               }
             }
           }
@@ -961,18 +992,21 @@ __global__ void __launch_bounds__(kDecThreads, 1)
           if (!seg_full(5)) return;
           tc_fence_after();
           const int n = act_rows(c.ai), r0 = tb.act_off[c.ai];
-          const uint32_t d = tlane + (uint32_t(eseg.st) * 2 + uint32_t(sub)) * uint32_t(a.NB);
+          const uint32_t d = tlane + (uint32_t(eseg.st) * 2 + uint32_t(sub)) * uint32_t(a.NB2);
           for (int j0 = 0; j0 < n; j0 += 4) {
-            uint32_t v[4];
+            uint32_t v[4], w[4];  // the products of h's two parts
 #pragma unroll
             for (int q = 0; q < 4; ++q)
-              if (j0 + q < n) v[q] = tmem_ld_32x32b_x1(d + uint32_t(j0 + q));
+              if (j0 + q < n) {
+                v[q] = tmem_ld_32x32b_x1(d + uint32_t(j0 + q));
+                w[q] = tmem_ld_32x32b_x1(d + uint32_t(n + j0 + q));
+              }
             tmem_ld_wait();
 #pragma unroll
             for (int q = 0; q < 4; ++q) {
               if (j0 + q >= n) break;
               float* s = &acc[int(tb.tok[r0 + j0 + q]) * 256 + fl];
-              *s = fmaf(tb.val[r0 + j0 + q], __uint_as_float(v[q]), *s);
+              *s = fmaf(tb.val[r0 + j0 + q], __uint_as_float(v[q]) + __uint_as_float(w[q]), *s);
             }
           }
           seg_done();
@@ -1113,7 +1147,7 @@ size_t up256(size_t v) { return (v + 255) / 256 * 256; }
 DecScratch dec_scratch(int T, int K, int F, int Er, int sms) {
   DecScratch s;
   s.hs = 0;
-  s.part = up256(size_t(T) * K * F * 2);
+  s.part = up256(size_t(T) * K * F * 4);
   const size_t parts = size_t(sms) + max_chunks(T, ragged_rows(F));
   s.ctr = s.part + up256(2 * parts * T * 256 * 4);
   s.lpart = s.ctr + up256((size_t(sms) + kDecMaxChunks + 2) * 4);
@@ -1175,6 +1209,7 @@ extern "C" int moe_decode_layer(const moe_decode_params* p, void* stream) {
   a.K = K;
   a.first = p->first_expert;
   a.NB = (T + 15) / 16 * 16;
+  a.NB2 = (2 * T + 15) / 16 * 16;
   a.x = static_cast<const __nv_bfloat16*>(p->x);
   a.ids = p->top_idxs;
   a.vals = p->top_vals;
@@ -1192,7 +1227,7 @@ extern "C" int moe_decode_layer(const moe_decode_params* p, void* stream) {
   a.out_ids = p->top_idxs;
   a.out_vals = static_cast<float*>(p->top_vals);
   a.maxact = E < T * K ? E : T * K;
-  a.stage_bytes = kDecABytes + uint32_t(a.NB) * 128;
+  a.stage_bytes = kDecABytes + uint32_t(a.NB2) * 128;
   // Pass 2's sums [T][256] and, before them, the masks and offsets of the
   // routing tables and one token's logits.
   uint32_t scratch = uint32_t(T) * 1024;
@@ -1241,7 +1276,7 @@ extern "C" int moe_decode_layer(const moe_decode_params* p, void* stream) {
     if (encode(&mx, 2, p->x, dims, str, box, H * 2)) return kCudaErr;
   }
   {
-    const cuuint64_t dims[2] = {cuuint64_t(F), cuuint64_t(T) * K};
+    const cuuint64_t dims[2] = {cuuint64_t(F), cuuint64_t(2 * T) * K};
     const cuuint64_t str[1] = {cuuint64_t(F) * 2};
     const cuuint32_t box[2] = {64, 16};
     if (encode(&mh, 2, a.hs, dims, str, box, F * 2)) return kCudaErr;

@@ -13,8 +13,9 @@ router, utils.py:28-75 and baseline.py:18-50 for routing and products).
 with e = ids[t, k] - first_expert.  Ids outside the experts held here are
 skipped and a token without any gets a zero row: a rank that holds experts
 [first_expert, first_expert + El) of a replicated batch computes its part of
-the sum, and the ranks' parts add up.  Nothing is read on the host, and a
-call may be captured into a CUDA graph.
+the sum, and the ranks' parts add up.  Sums are fp32, silu(gate) * up keeps 16
+bits between the products, and y is rounded once.  Nothing is read on the
+host, and a call may be captured into a CUDA graph.
 """
 from __future__ import annotations
 

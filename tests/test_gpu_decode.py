@@ -120,6 +120,42 @@ def test_long_lists_of_odd_rows(T, H, E, K, F):
         assert torch.equal(y, decode.moe_layer(x, ids, vals, w13, w2))
 
 
+@pytest.mark.parametrize("T,H,E,K,F", [(1, 64, 4, 2, 64), (3, 64, 4, 2, 64), (9, 72, 3, 3, 136), (40, 64, 2, 2, 64),
+                                       (56, 1024, 4, 4, 72), (64, 1024, 32, 8, 64)])
+def test_h_keeps_its_bits(T, H, E, K, F):
+    """h = silu(gate) * up as two bf16 values: the second's rounding is half a
+    step of what the first one's left, 2^-16 of h.  Beside it the terms of
+    `reference`: fp32 sums of both products (twice as many terms in the
+    second), y's rounding."""
+    x, ids, vals, w13, w2 = make(T, H, E, K, F, T + F)
+    y = decode.moe_layer(x, ids, vals, w13, w2).double()
+    a = torch.einsum("th,ehf->etf", x.double(), w13.double())
+    da = torch.einsum("th,ehf->etf", x.double().abs(), w13.double().abs()) * H * 2.0 ** -23
+    g, u, dg, du = a[..., :F], a[..., F:], da[..., :F], da[..., F:]
+    s = g * torch.sigmoid(g)
+    h = s * u
+    dh = 1.1 * dg * u.abs() + (s.abs() + 1.1 * dg) * du + h.abs() * (2.0 ** -16 + 2.0 ** -20)
+    coef = torch.zeros(T, E, dtype=torch.float64, device="cuda").scatter_(1, ids, vals.double())
+    ref = torch.einsum("te,eth->th", coef, h @ w2.double())
+    tol = torch.einsum("te,eth->th", coef, (dh + (h.abs() + dh) * (2 * F + 4) * 2.0 ** -23) @ w2.double().abs())
+    err = (y - ref).abs()
+    tol = tol + (ref.abs() + tol) * HALF
+    assert bool((err <= tol).all()), f"{int((err > tol).sum())} of {err.numel()} beyond the bound, worst {float((err / tol).max()):.2f}x"
+
+
+def test_h_beyond_the_types_range():
+    """h above bf16's largest number goes on as infinity, not as NaN."""
+    x = torch.full((3, 8), 1.0, dtype=torch.bfloat16, device="cuda")
+    w13 = torch.zeros(1, 8, 32, dtype=torch.bfloat16, device="cuda")
+    w13[0, :, 0], w13[0, :, 16] = 1e19, 1e19    # h = 6.4e39 at one feature
+    w13[0, :, 1], w13[0, :, 17] = 0.25, 0.5     # and an ordinary one
+    w2 = torch.zeros(1, 16, 8, dtype=torch.bfloat16, device="cuda")
+    w2[0, 0, 3], w2[0, 1, 5] = -2.0, 1.0
+    ids, vals = torch.zeros(3, 1, dtype=torch.int64, device="cuda"), torch.ones(3, 1, device="cuda")
+    y = decode.moe_layer(x, ids, vals, w13, w2)
+    assert y[:, 3].tolist() == [-float("inf")] * 3
+
+
 @pytest.mark.parametrize("ids_dtype", [torch.int32, torch.int64])
 @pytest.mark.parametrize("vals_dtype", [torch.float32, torch.bfloat16])
 def test_types(ids_dtype, vals_dtype):
