@@ -389,7 +389,8 @@ int moe_ep_run_compact_swiglu(const moe_ep_run_params* params, int64_t send_rows
  * top_idxs and top_vals (fp32), divided by their sum with `renormalize`.
  * Requires T <= MOE_DECODE_MAX_TOKENS, T * K <= 1024, K <= 32, hidden and ffn
  * multiples of 8, hidden <= 32768, experts and router_experts <= 1024,
- * router_experts a multiple of 4; x, w13, w2, y and scratch 16-byte aligned.
+ * router_experts a multiple of 4; x, w13, w2, y and scratch 16-byte aligned,
+ * router_w 4-byte.
  * scratch: moe_decode_scratch_bytes of device memory, not initialised, for
  * this call alone until it has finished.  Launched cooperatively (one CTA per
  * SM), so calls on several streams run one after another. */
@@ -428,7 +429,7 @@ int moe_decode_layer(const moe_decode_params* params, void* stream);
  * src(r) = perm[r] (the dispatch order of moe_route), or r without perm.
  * A row of zeros has scale 0 and zeros; a row with an infinity or a NaN has a
  * NaN scale and zeros, so that its products are NaN.  x is bf16 or
- * (x_is_f32) fp32, 16-byte aligned, K % 8 == 0.  live_rows (device, optional):
+ * (x_is_f32) fp32, 16-byte aligned, q 8-byte aligned, K % 8 == 0.  live_rows (device, optional):
  * rows from *live_rows on are left as they were. */
 int moe_quant_rows(const void* x, int32_t x_is_f32, int64_t rows, int32_t K, const int32_t* perm,
                    const int32_t* live_rows, void* q, float* scale, void* stream);

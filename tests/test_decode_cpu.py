@@ -77,3 +77,14 @@ def test_every_unit_belongs_to_one_part(tmp_path):
                     str(here / "native" / "decode_parts_check.cpp"), "-o", str(exe)], check=True)
     done = subprocess.run([str(exe)], capture_output=True, text=True)
     assert done.returncode == 0, f"status {done.returncode}: {done.stdout}"
+
+
+def test_c_entry_refuses_a_misaligned_router():
+    buf = ctypes.create_string_buffer(64)
+    at = (ctypes.addressof(buf) + 15) // 16 * 16
+    p = N.DecodeParams()
+    p.T, p.hidden, p.ffn, p.experts, p.K, p.router_experts = 4, 64, 64, 4, 2, 4
+    for f in ("x", "w13", "w2", "y", "top_idxs", "top_vals", "scratch"):
+        setattr(p, f, at)
+    p.router_w = at + 2
+    assert N.lib().moe_decode_layer(ctypes.byref(p), None) == N.BAD_ARG
