@@ -429,8 +429,8 @@ int moe_decode_layer(const moe_decode_params* params, void* stream);
  * src(r) = perm[r] (the dispatch order of moe_route), or r without perm.
  * A row of zeros has scale 0 and zeros; a row with an infinity or a NaN has a
  * NaN scale and zeros, so that its products are NaN.  x is bf16 or
- * (x_is_f32) fp32, 16-byte aligned, q 8-byte aligned, K % 8 == 0.  live_rows (device, optional):
- * rows from *live_rows on are left as they were. */
+ * (x_is_f32) fp32, 16-byte aligned, q 8-byte aligned, K % 8 == 0.  live_rows
+ * (device, optional): rows from *live_rows on are left as they were. */
 int moe_quant_rows(const void* x, int32_t x_is_f32, int64_t rows, int32_t K, const int32_t* perm,
                    const int32_t* live_rows, void* q, float* scale, void* stream);
 
